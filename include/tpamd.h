@@ -424,6 +424,37 @@ int tpamd_linear_w8_add(const void *x_dev, const void *wq_dev, const void *scale
                         int64_t n_out, const void *bias_dev, const void *addend_dev, void *y_dev, void *copy_dev, int64_t M, int64_t N,
                         int64_t K, int64_t ldx, int64_t ldw, int64_t ld_wout, int64_t ldadd, int64_t ldy, int dtype, int act, void *stream);
 
+/* ---- both operands in 8 bits ---------------------------------------------------------------------------------------------------------
+ * Not part of the reference (its README points to LLM.int8 notebooks); defined here in closed form.
+ *
+ * Rows in 8 bits with a scale each: a = max over the row of |x|, q = round_half_even(127 x / a) of the exact quotient, scale = a / 127 (fp32); scale = 1 and codes of
+ * 0 where no value of the row is 2^-100 or more; scale = NaN and codes of 0 where the row holds an infinity or NaN. x [rows, D] in `dtype` (BF16 or F16), q int8 [rows, D],
+ * scale fp32 [rows]; elements between rows in ldx, ldq, the bytes between D and ldq are left alone. Any length and alignment; rows of up to 16384 elements, a multiple
+ * of 8, on 16-byte boundaries (q: 8) are read once. Outputs overlap no input. */
+int tpamd_quantize_rows(const void *x_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldq, int dtype, void *stream);
+/* y = scale * q, rounded to `dtype` (BF16, F16 or F32). */
+int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, void *y_dev, int64_t rows, int64_t D, int64_t ldq, int64_t ldy, int dtype, void *stream);
+/* The RMS norm of tpamd_rms_norm (run by every rank's wrapped modules, src/tensor_parallel/wrapper.py:69-72) with its rows in 8 bits: w x rsqrt(mean(x^2) + eps) quantised as
+ * above without being rounded to `dtype` in between. The codes are those of w x (products of two 16-bit values, exact in fp32), the scale takes the row's factor. */
+int tpamd_rms_norm_q8(const void *x_dev, const void *w_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldq, float eps, int dtype, void *stream);
+/* The same of sum = r + x (rounded to `dtype` and stored), as tpamd_add_rms_norm. */
+int tpamd_add_rms_norm_q8(const void *x_dev, const void *r_dev, const void *w_dev, void *sum_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldr,
+                          int64_t ldsum, int64_t ldq, float eps, int dtype, void *stream);
+
+/* Shard Linears of 8-bit rows: y[m,n] = act(xscale[m] * wscale[n] * sum_k x[m,k] * w[n,k] + bias[n]), x int8 [M,K], w int8 [N,K], scales fp32, y and bias in `dtype` (BF16 or
+ * F16). The sum is exact in int32 (K up to 131071, TPAMD_ERR_UNSUPPORTED beyond), so results do not depend on how it is taken; everything behind it in fp32, rounded
+ * once. Any shape, pitch and alignment is accepted. */
+int tpamd_linear_a8(const void *x_dev, const void *xscale_dev, const void *w_dev, const void *wscale_dev, const void *bias_dev, void *y_dev, int64_t M, int64_t N, int64_t K,
+                    int64_t ldx, int64_t ldw, int64_t ldy, int dtype, int act, void *stream);
+/* Followed by one step of the partial-sum reduction, y = round_dtype(round_dtype(...) + addend), as tpamd_linear_add; with copy_dev (may be NULL) every result is stored there
+ * too (leading dimension ldy), as tpamd_linear_add_copy. addend_dev may be y_dev or copy_dev (then ldadd must equal ldy). */
+int tpamd_linear_a8_add(const void *x_dev, const void *xscale_dev, const void *w_dev, const void *wscale_dev, const void *bias_dev, const void *addend_dev, void *y_dev, void *copy_dev,
+                        int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldadd, int64_t ldy, int dtype, int act, void *stream);
+/* The gate/up pair of a SiLU-gated MLP shard in one pass over x: h = silu(g) * u with g, u the two Linears of 8-bit rows, all in fp32 behind the exact sums, rounded once
+ * (tpamd_swiglu_up rounds g, u, silu(g) and the product as four separate operations of 16-bit tensors would). */
+int tpamd_swiglu_up_a8(const void *x_dev, const void *xscale_dev, const void *wg_dev, const void *gscale_dev, const void *wu_dev, const void *uscale_dev, void *h_dev, int64_t M,
+                       int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

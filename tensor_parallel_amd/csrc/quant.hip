@@ -1,0 +1,327 @@
+// Rows of an activation in 8 bits with a scale each, on their own or behind an RMS norm (with or without the residual's addition), and the way back.
+//
+//   p = x, or t w of the norm's input t (round(r + x) with a residual);  a = max |p| over the row
+//   codes  round_half_even(127 p / a)     scale  a f / 127, f = 1 or rsqrt(mean t^2 + eps)
+// The norm's factor is the same for a whole row, so it is in the scale alone: a row's codes do not depend on how its squares are summed, the maximum is found in
+// the pass that sums them, and one meeting of the block serves both.
+// A code is the integer nearest to the exact quotient: in rows of 16-bit values many quotients lie on a half (a value of half the largest is 63.5), which a product with a
+// rounded 127 / a would put on either side. What the product leaves within 2^-13 of a half (its error is below 127 * 3 * 2^-24) is compared with the
+// half in 64 bits, where 2 * 127 p and (2 l + 1) a are exact; p is exact in fp32 (two 16-bit significands).
+// A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
+//
+// Bound: at a few rows by the latency of a launch, else by HBM (x, r read once; sum and codes written once).
+#include "common.h"
+
+namespace tpamd {
+namespace {
+
+struct QuantParams {
+    const char *x, *w, *r;
+    char *s, *q;
+    float *scale;
+    int64_t ldx, ldr, lds, ldq;  // elements between rows
+    int D;
+    float eps;
+};
+
+// What a row has in common: its scale, 127 / a, and a (0: codes of 0).
+struct RowCode {
+    float scale, inv, most;
+};
+__device__ __forceinline__ RowCode row_code(uint32_t most_bits, float factor) {
+    RowCode c;
+    c.most = __uint_as_float(most_bits);
+    if (most_bits >= 0x7f800000u) {  // an infinity or NaN: the integer maximum keeps both
+        c.scale = __uint_as_float(0x7fc00000u);
+        c.most = 0.f;
+    } else if (c.most < 0x1p-100f) {
+        c.scale = 1.f;
+        c.most = 0.f;
+    } else {
+        c.scale = c.most * factor / 127.f;
+    }
+    c.inv = c.most != 0.f ? 127.f / c.most : 0.f;
+    return c;
+}
+__device__ __forceinline__ int code_of(float p, const RowCode &c) {
+    const float t = p * c.inv;
+    float n = rintf(t);
+    if (fabsf(t - n) > 0.5f - 0x1p-13f) {
+        const float low = floorf(t);
+        const double twice = 254.0 * static_cast<double>(p), half = (2.0 * low + 1.0) * static_cast<double>(c.most);
+        n = twice > half || (twice == half && (static_cast<int>(low) & 1)) ? low + 1.f : low;
+    }
+    return c.most != 0.f ? static_cast<int>(n) : 0;
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Sum and maximum over the block, the same in every thread. `part`: two words for each wavefront.
+template <int WAVES>
+__device__ __forceinline__ void block_sum_max(float &sum, uint32_t &most, uint2 *part) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        sum += __shfl_xor(sum, d);
+        const uint32_t other = __shfl_xor(most, d);
+        most = most > other ? most : other;
+    }
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_uint2(__float_as_uint(sum), most);
+        __syncthreads();
+        sum = 0.f;
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            const uint2 v = part[i];
+            sum += __uint_as_float(v.x);
+            most = most > v.y ? most : v.y;
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b) { return add_packed2<DT>(a, b); }
+
+// Rows of D elements, D a multiple of 8 and at most 64 * WAVES * CH * 8, every row of x, r, s on a 16-byte boundary and of q on an 8-byte one. A block holds its row in registers.
+template <int DT, int WAVES, int CH, bool NORM, bool ADD>
+__global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
+    constexpr int T = 64 * WAVES;
+    __shared__ uint2 part[WAVES];
+    const int64_t row = blockIdx.x;
+    const uint4 *x = reinterpret_cast<const uint4 *>(p.x + row * p.ldx * 2);
+    const uint4 *w = reinterpret_cast<const uint4 *>(p.w);
+    const int n = p.D / 8;
+    uint4 v[CH], wv[NORM ? CH : 1];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = threadIdx.x + c * T;
+        v[c] = i < n ? x[i] : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (NORM) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = threadIdx.x + c * T;
+            wv[c] = i < n ? w[i] : make_uint4(0, 0, 0, 0);
+        }
+    }
+    if constexpr (ADD) {
+        const uint4 *r = reinterpret_cast<const uint4 *>(p.r + row * p.ldr * 2);
+        uint4 *s = reinterpret_cast<uint4 *>(p.s + row * p.lds * 2);
+        uint4 rv[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = threadIdx.x + c * T;
+            rv[c] = i < n ? r[i] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = threadIdx.x + c * T;
+            v[c] = make_uint4(add2<DT>(rv[c].x, v[c].x), add2<DT>(rv[c].y, v[c].y), add2<DT>(rv[c].z, v[c].z), add2<DT>(rv[c].w, v[c].w));
+            if (i < n) s[i] = v[c];
+        }
+    }
+    float f[CH][8], sum = 0.f;
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const uint32_t u[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+        const uint32_t g[4] = {wv[NORM ? c : 0].x, wv[NORM ? c : 0].y, wv[NORM ? c : 0].z, wv[NORM ? c : 0].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float a = lo_half_to_f32<DT>(u[j]), b = hi_half_to_f32<DT>(u[j]);
+            if constexpr (NORM) {
+                sum = fmaf(a, a, fmaf(b, b, sum));
+                a *= lo_half_to_f32<DT>(g[j]);
+                b *= hi_half_to_f32<DT>(g[j]);
+            }
+            f[c][2 * j] = a;
+            f[c][2 * j + 1] = b;
+            most = max(most, max(abs_bits(a), abs_bits(b)));
+        }
+    }
+    block_sum_max<WAVES>(sum, most, part);
+    const RowCode code = row_code(most, NORM ? rsqrtf(sum / static_cast<float>(p.D) + p.eps) : 1.f);
+    if (threadIdx.x == 0) p.scale[row] = code.scale;
+    uint2 *q = reinterpret_cast<uint2 *>(p.q + row * p.ldq);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = threadIdx.x + c * T;
+        if (i >= n) continue;
+        uint32_t o[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j >> 2] |= static_cast<uint32_t>(code_of(f[c][j], code) & 0xff) << (8 * (j & 3));
+        q[i] = make_uint2(o[0], o[1]);
+    }
+}
+
+// Any length and alignment: element loads, x (ADD: the stored sum, by the thread that stored it) read twice.
+template <int DT, bool NORM, bool ADD>
+__global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
+    __shared__ uint2 part[4];
+    const int64_t row = blockIdx.x;
+    const uint16_t *x = reinterpret_cast<const uint16_t *>(p.x) + row * p.ldx, *w = reinterpret_cast<const uint16_t *>(p.w);
+    const uint16_t *r = reinterpret_cast<const uint16_t *>(p.r) + row * p.ldr;
+    uint16_t *s = reinterpret_cast<uint16_t *>(p.s) + row * p.lds;
+    float sum = 0.f;
+    uint32_t most = 0;
+    for (int i = threadIdx.x; i < p.D; i += 256) {
+        float a = half_to_f32<DT>(x[i]);
+        if constexpr (ADD) {
+            s[i] = f32_to_half<DT>(half_to_f32<DT>(r[i]) + a);
+            a = half_to_f32<DT>(s[i]);
+        }
+        sum = fmaf(a, a, sum);
+        if constexpr (NORM) a *= half_to_f32<DT>(w[i]);
+        most = max(most, abs_bits(a));
+    }
+    block_sum_max<4>(sum, most, part);
+    const RowCode code = row_code(most, NORM ? rsqrtf(sum / static_cast<float>(p.D) + p.eps) : 1.f);
+    if (threadIdx.x == 0) p.scale[row] = code.scale;
+    for (int i = threadIdx.x; i < p.D; i += 256) {
+        const float a = half_to_f32<DT>(ADD ? s[i] : x[i]);
+        p.q[row * p.ldq + i] = static_cast<char>(code_of(NORM ? a * half_to_f32<DT>(w[i]) : a, code));
+    }
+}
+
+template <int DT, bool NORM, bool ADD>
+void launch_rows(const QuantParams &p, int64_t rows, bool vec, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(rows));
+    const int n = p.D / 8;  // 16-byte chunks per row
+    if (!vec) hipLaunchKernelGGL((quantize_any_kernel<DT, NORM, ADD>), grid, dim3(256), 0, s, p);
+    else if (n <= 64) hipLaunchKernelGGL((quantize_kernel<DT, 1, 1, NORM, ADD>), grid, dim3(64), 0, s, p);
+    else if (n <= 256) hipLaunchKernelGGL((quantize_kernel<DT, 4, 1, NORM, ADD>), grid, dim3(256), 0, s, p);
+    else if (n <= 512) hipLaunchKernelGGL((quantize_kernel<DT, 8, 1, NORM, ADD>), grid, dim3(512), 0, s, p);
+    else if (n <= 1024) hipLaunchKernelGGL((quantize_kernel<DT, 8, 2, NORM, ADD>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((quantize_kernel<DT, 16, 2, NORM, ADD>), grid, dim3(1024), 0, s, p);
+}
+
+// A launch has at most 2^32 - 1 threads; further rows go into further launches.
+constexpr int64_t ROWS_PER_LAUNCH = 1ll << 20;
+
+template <int DT, bool NORM, bool ADD>
+int launch(QuantParams p, int64_t rows, bool vec, hipStream_t s) {
+    for (; rows > 0; rows -= ROWS_PER_LAUNCH) {
+        launch_rows<DT, NORM, ADD>(p, rows < ROWS_PER_LAUNCH ? rows : ROWS_PER_LAUNCH, vec, s);
+        TPAMD_HIP(hipGetLastError());
+        p.x += ROWS_PER_LAUNCH * p.ldx * 2;
+        p.q += ROWS_PER_LAUNCH * p.ldq;
+        p.scale += ROWS_PER_LAUNCH;
+        if constexpr (ADD) {
+            p.r += ROWS_PER_LAUNCH * p.ldr * 2;
+            p.s += ROWS_PER_LAUNCH * p.lds * 2;
+        }
+    }
+    return TPAMD_OK;
+}
+
+template <bool NORM, bool ADD>
+int quantize_entry(const char *who, const QuantParams &p, int64_t rows, int64_t D, int dtype, void *stream) {
+    TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 31), "%s: dimension negative or over 2^31 (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
+    TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16, "%s: rows of bfloat16 or float16 are quantised, not dtype %d", who, dtype);
+    if (rows == 0) return TPAMD_OK;
+    TPAMD_REQUIRE(p.scale != nullptr && (D == 0 || (p.x != nullptr && p.q != nullptr && (!NORM || p.w != nullptr) && (!ADD || (p.r != nullptr && p.s != nullptr)))),
+                  "%s: null pointer", who);
+    TPAMD_REQUIRE(p.ldx >= D && p.ldq >= D && (!ADD || (p.ldr >= D && p.lds >= D)), "%s: leading dimension smaller than the row (ldx=%lld ldr=%lld lds=%lld ldq=%lld)", who,
+                  (long long)p.ldx, (long long)p.ldr, (long long)p.lds, (long long)p.ldq);
+    TPAMD_REQUIRE(aligned(p.x, 2) && aligned(p.w, 2) && aligned(p.r, 2) && aligned(p.s, 2) && aligned(p.scale, 4), "%s: a pointer is not aligned to its type", who);
+    const bool vec = D > 0 && D % 8 == 0 && D <= 16384 && aligned(p.x, 16) && p.ldx % 8 == 0 && aligned(p.q, 8) && p.ldq % 8 == 0 && (!NORM || aligned(p.w, 16)) &&
+                     (!ADD || (aligned(p.r, 16) && p.ldr % 8 == 0 && aligned(p.s, 16) && p.lds % 8 == 0));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == TPAMD_BF16 ? launch<TPAMD_BF16, NORM, ADD>(p, rows, vec, s) : launch<TPAMD_F16, NORM, ADD>(p, rows, vec, s);
+}
+
+// A product as an fp32 value of its own: the compiler would otherwise make one instruction of it and its conversion to fp16, which rounds once where the packed conversion behind
+// the product rounds twice, and a row's bits would depend on its alignment.
+__device__ __forceinline__ float product(float a, float b) {
+    float v = a * b;
+    asm("" : "+v"(v));
+    return v;
+}
+
+// y = q * scale in fp32, rounded to the dtype: blockIdx.y takes every gridDim.y-th row, a thread 16 codes of it (VEC: rows of q on 16-byte, of y on 16-byte boundaries, D a multiple of 16).
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void dequantize_kernel(const char *q, const float *scale, char *y, int64_t rows, int D, int64_t ldq, int64_t ldy) {
+    const int i = (blockIdx.x * 256 + threadIdx.x) * (VEC ? 16 : 1);
+    if (i >= D) return;
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        const float f = scale[row];
+        if constexpr (VEC) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(q + row * ldq + i);
+            const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = product(static_cast<float>(static_cast<int8_t>(a[j] >> (8 * e))), f);
+                if constexpr (DT == TPAMD_F32)
+                    reinterpret_cast<float4 *>(y + (row * ldy + i) * 4)[j] = make_float4(v[0], v[1], v[2], v[3]);
+                else
+                    reinterpret_cast<uint2 *>(y + (row * ldy + i) * 2)[j] = make_uint2(pack2_half<DT>(v[0], v[1]), pack2_half<DT>(v[2], v[3]));
+            }
+        } else {
+            const float v = product(static_cast<float>(static_cast<int8_t>(q[row * ldq + i])), f);
+            if constexpr (DT == TPAMD_F32) reinterpret_cast<float *>(y)[row * ldy + i] = v;
+            else reinterpret_cast<uint16_t *>(y)[row * ldy + i] = f32_to_half<DT>(v);
+        }
+    }
+}
+
+template <int DT>
+void launch_dequantize(const char *q, const float *scale, char *y, int64_t rows, int D, int64_t ldq, int64_t ldy, bool vec, hipStream_t s) {
+    const unsigned columns = static_cast<unsigned>((static_cast<int64_t>(D) + (vec ? 4095 : 255)) / (vec ? 4096 : 256));
+    // rows in turn once 2^22 blocks are out
+    const int64_t most = (1 << 22) / columns > 0 ? (1 << 22) / columns : 1;
+    const int64_t by = rows < 65535 ? rows : 65535;
+    const dim3 grid(columns, static_cast<unsigned>(by < most ? by : most));
+    if (vec) hipLaunchKernelGGL((dequantize_kernel<DT, true>), grid, dim3(256), 0, s, q, scale, y, rows, D, ldq, ldy);
+    else hipLaunchKernelGGL((dequantize_kernel<DT, false>), grid, dim3(256), 0, s, q, scale, y, rows, D, ldq, ldy);
+}
+
+}  // namespace
+}  // namespace tpamd
+
+using namespace tpamd;
+
+extern "C" int tpamd_quantize_rows(const void *x_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldq, int dtype, void *stream) {
+    QuantParams p{};
+    p.x = static_cast<const char *>(x_dev); p.q = static_cast<char *>(q_dev); p.scale = static_cast<float *>(scale_dev);
+    p.ldx = ldx; p.ldq = ldq; p.D = static_cast<int>(D);
+    return quantize_entry<false, false>("tpamd_quantize_rows", p, rows, D, dtype, stream);
+}
+
+extern "C" int tpamd_rms_norm_q8(const void *x_dev, const void *w_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldq, float eps, int dtype,
+                                 void *stream) {
+    QuantParams p{};
+    p.x = static_cast<const char *>(x_dev); p.w = static_cast<const char *>(w_dev); p.q = static_cast<char *>(q_dev); p.scale = static_cast<float *>(scale_dev);
+    p.ldx = ldx; p.ldq = ldq; p.D = static_cast<int>(D); p.eps = eps;
+    return quantize_entry<true, false>("tpamd_rms_norm_q8", p, rows, D, dtype, stream);
+}
+
+extern "C" int tpamd_add_rms_norm_q8(const void *x_dev, const void *r_dev, const void *w_dev, void *sum_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx,
+                                     int64_t ldr, int64_t ldsum, int64_t ldq, float eps, int dtype, void *stream) {
+    QuantParams p{};
+    p.x = static_cast<const char *>(x_dev); p.r = static_cast<const char *>(r_dev); p.w = static_cast<const char *>(w_dev);
+    p.s = static_cast<char *>(sum_dev); p.q = static_cast<char *>(q_dev); p.scale = static_cast<float *>(scale_dev);
+    p.ldx = ldx; p.ldr = ldr; p.lds = ldsum; p.ldq = ldq; p.D = static_cast<int>(D); p.eps = eps;
+    return quantize_entry<true, true>("tpamd_add_rms_norm_q8", p, rows, D, dtype, stream);
+}
+
+extern "C" int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, void *y_dev, int64_t rows, int64_t D, int64_t ldq, int64_t ldy, int dtype, void *stream) {
+    const char *who = "tpamd_dequantize_rows";
+    TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 31), "%s: dimension negative or over 2^31 (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
+    TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16 || dtype == TPAMD_F32, "%s: unknown dtype %d", who, dtype);
+    if (rows == 0 || D == 0) return TPAMD_OK;
+    TPAMD_REQUIRE(q_dev != nullptr && scale_dev != nullptr && y_dev != nullptr, "%s: null pointer", who);
+    TPAMD_REQUIRE(ldq >= D && ldy >= D, "%s: leading dimension smaller than the row (ldq=%lld ldy=%lld)", who, (long long)ldq, (long long)ldy);
+    TPAMD_REQUIRE(aligned(scale_dev, 4) && aligned(y_dev, dtype == TPAMD_F32 ? 4 : 2), "%s: a pointer is not aligned to its type", who);
+    const char *q = static_cast<const char *>(q_dev);
+    const float *scale = static_cast<const float *>(scale_dev);
+    char *y = static_cast<char *>(y_dev);
+    const bool vec = D % 16 == 0 && aligned(q, 16) && ldq % 16 == 0 && aligned(y, 16) && ldy % (dtype == TPAMD_F32 ? 4 : 8) == 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int d = static_cast<int>(D);
+    if (dtype == TPAMD_BF16) launch_dequantize<TPAMD_BF16>(q, scale, y, rows, d, ldq, ldy, vec, s);
+    else if (dtype == TPAMD_F16) launch_dequantize<TPAMD_F16>(q, scale, y, rows, d, ldq, ldy, vec, s);
+    else launch_dequantize<TPAMD_F32>(q, scale, y, rows, d, ldq, ldy, vec, s);
+    TPAMD_HIP(hipGetLastError());
+    return TPAMD_OK;
+}

@@ -11,13 +11,21 @@ module on a HIP device) into `ShardLinearW8`, whose forward is `tpamd_linear_w8`
   y        = x . (Wq * scale[:,None])^T  +  x[:, O] . W[:, O]^T  (+ bias)
 
 The quantiser runs on the device with torch's elementwise ops (it runs once per weight); the Linear itself runs on the
-library's kernels only. A quantised Linear no longer has a `weight`: `save_tensor_parallel`, which rebuilds the full
+library's kernels only.
+
+With both operands in 8 bits (`QuantizedRows`, `quantize_activations`, `rms_norm`, `add_rms_norm`, `linear`, `swiglu_up`) the rows of an activation have a scale each too:
+
+  a        = max |p| over the row, p = x, or w x of an RMS norm's input x (its factor f = rsqrt(mean(x^2) + eps) is in the scale alone; else f = 1)
+  codes    = round_half_even(127 p / a) of the exact quotient          scale = a f / 127      (zeros: 1.0; an infinity or NaN: NaN, and codes of 0)
+  linear   = act(scale[m] wscale[n] (codes . Wq^T) + bias), the product exact in 32-bit integers, rounded once (a partial sum of other ranks is added to the rounded value)
+
+A quantised Linear no longer has a `weight`: `save_tensor_parallel`, which rebuilds the full
 weights of the original model from the shards, refuses a model that holds one; its shards can be saved as they are.
 """
 from __future__ import annotations
 
 import functools
-from typing import Callable, Mapping, Optional, Sequence, Tuple, Union
+from typing import Callable, Mapping, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import nn
@@ -61,6 +69,52 @@ def quantize_rows(w: torch.Tensor, outlier_cols: Optional[torch.Tensor] = None) 
         scale[r0:r0 + 4096] = sc
     q[:, ~keep] = 0
     return q, scale, cols.to(torch.int32), w.detach()[:, cols].contiguous()
+
+
+class QuantizedRows(NamedTuple):
+    """Rows of an activation in 8 bits: `scale` * `codes` stand for rows of `dtype`, which is what Linears of them return."""
+
+    codes: torch.Tensor  # int8 [..., K]
+    scale: torch.Tensor  # float32 [...]
+    dtype: torch.dtype
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """scale * codes, in `dtype` (the rows' own by default)."""
+        return _guard(_native.dequantize_rows(self.codes, self.scale, self.dtype if dtype is None else dtype), self.scale)
+
+
+def quantize_activations(x: torch.Tensor) -> QuantizedRows:
+    """The rows of x (bfloat16 or float16, on a HIP device) in 8 bits, by the definition in the module docstring. Inference only, as everything here: a
+    backward pass through the rows' scales, or what Linears make of them, raises."""
+    codes, scale = _native.quantize_rows(x.detach())
+    return QuantizedRows(codes, _guard(scale, x), x.dtype)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> QuantizedRows:
+    """The RMS norm of x's rows in 8 bits, in one launch: weight * x * rsqrt(mean(x^2) + eps), not rounded in between."""
+    codes, scale = _native.rms_norm_q8(x.detach(), weight.detach(), eps)
+    return QuantizedRows(codes, _guard(scale, x, weight), x.dtype)
+
+
+def add_rms_norm(r: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float) -> Tuple[torch.Tensor, QuantizedRows]:
+    """(r + x, the RMS norm of that sum in 8 bits), in one launch: a residual stream and the input of the Linears behind its norm."""
+    total, codes, scale = _native.add_rms_norm_q8(r.detach(), x.detach(), weight.detach(), eps)
+    return _guard(total, r, x), QuantizedRows(codes, _guard(scale, r, x, weight), x.dtype)
+
+
+def linear(rows: QuantizedRows, wq: torch.Tensor, wscale: torch.Tensor, bias: Optional[torch.Tensor] = None, *, gelu: bool = False,
+           addend: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A Linear of 8-bit rows on int8 weights [N, K] with a float32 scale for each output (`quantize_rows` without outlier columns makes both), in the rows' dtype. `addend`: other ranks' partial
+    sum, added to the rounded result. K is at most 131071 (the sum fits 32 bits)."""
+    y = _native.linear_a8(rows.codes, rows.scale.detach(), wq, wscale.detach(), None if bias is None else bias.detach(), rows.dtype, _native.ACT_GELU if gelu else _native.ACT_NONE,
+                          None if addend is None else addend.detach())
+    return _guard(y, rows.scale, wscale, bias, addend)
+
+
+def swiglu_up(rows: QuantizedRows, gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor) -> torch.Tensor:
+    """silu(g) * u of the Linears g and u of 8-bit rows (as in `linear`, no bias), in one launch and rounded once."""
+    h = _native.swiglu_up_a8(rows.codes, rows.scale.detach(), gate, gate_scale.detach(), up, up_scale.detach(), rows.dtype)
+    return _guard(h, rows.scale, gate_scale, up_scale)
 
 
 # From 65 to this many rows a Linear neither meets its peer nor hands a sum over: the host sets the pace of an eager prompt there, and the reduction kernel's launch costs it
