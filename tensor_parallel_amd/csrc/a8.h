@@ -18,19 +18,36 @@ struct A8Params {
 
 constexpr int64_t A8_MAX_K = 131071;   // 128 * 128 * K < 2^31
 
+// An fp32 value of its own: products, sums and conversions to fp16 would otherwise become one instruction that rounds once in some kernels and not in others, and a
+// row's bits would depend on the kernel that its batch selects.
+__device__ __forceinline__ float a8_value(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // From a sum to the value before it is rounded: in fp32 behind the exact sum (the int32 is rounded to 24 bits, 2^-24 of it).
-__device__ __forceinline__ float a8_scaled(int sum, float sx, float sw) { return static_cast<float>(sum) * sw * sx; }
+__device__ __forceinline__ float a8_scaled(int sum, float sx, float sw) { return a8_value(static_cast<float>(sum) * sw * sx); }
+__device__ __forceinline__ float a8_linear(float v, float bias, int act) {
+    v = a8_value(v + bias);
+    return act == TPAMD_ACT_GELU ? a8_value(gelu_erf(v)) : v;
+}
 
 // SiLU(g) u, rounded once by the caller: both factors stay in fp32 (the 16-bit pair rounds g, u, SiLU(g) and the product as its four separate operations would;
 // here no 16-bit operation is stood in for, and one rounding is 2.3 times closer to the definition).
-__device__ __forceinline__ float a8_gated(float g, float u) { return silu_f32(g) * u; }
+__device__ __forceinline__ float a8_gated(float g, float u) { return a8_value(a8_value(silu_f32(g)) * u); }
 
-// Rounded to the outputs' dtype as an fp32 value of its own: a product and its conversion to fp16 may otherwise become one instruction that rounds once, in some kernels and not in
-// others, and a row's bits would depend on the kernel that its batch selects.
 template <int DT>
-__device__ __forceinline__ uint16_t a8_round(float v) {
-    asm("" : "+v"(v));
-    return f32_to_half<DT>(v);
+__device__ __forceinline__ uint16_t a8_round(float v) { return f32_to_half<DT>(v); }
+template <int DT>
+__device__ __forceinline__ uint32_t a8_round2(float a, float b) { return pack2_half<DT>(a, b); }
+
+// Where the fast kernels take operands: pieces of 16 codes in the rows of x and w, rows within reach of 32-bit offsets.
+static inline bool a8_fast(const A8Params &p) {
+    return p.K >= 16 && p.K % 16 == 0 && p.ldx % 16 == 0 && p.ldw % 16 == 0 && p.ldx < (1ll << 22) && p.ldw < (1ll << 22) && aligned(p.x, 16) && aligned(p.w, 16) && aligned(p.w2, 16);
 }
+// gemm_a8.hip: tiles of 32 * tmx x-rows by 32 * tnx w-rows (a pair: 16 * tnx columns), K in at most `splits` ranges. stream_a8.hip: up to 64 rows on one block per CU. Operands of a8_fast.
+int gemm_a8(const A8Params &p, bool pair, int dtype, int tmx, int tnx, int splits, hipStream_t s);
+bool stream_a8_takes(const A8Params &p, bool pair, int cus);
+int stream_a8(const A8Params &p, bool pair, int dtype, int cus, hipStream_t s);
 
 }  // namespace tpamd

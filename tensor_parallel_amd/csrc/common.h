@@ -53,6 +53,8 @@ struct Tuning {
     int skinny_max_m;        // TPAMD_SKINNY_MAX_M: most rows of a single 16-bit matrix that go to the weight-streaming kernels (16 to 64; unset: by shape)
     int skinny_xlds;         // TPAMD_SKINNY_XLDS: 0 = gated pair at 4-16 rows through the older kernels
     int gemv_rows;           // TPAMD_GEMV_ROWS: wavefronts per block of the unrolled M <= 3 kernel (4, 8, 16); 0 = the general kernel, -1 = the MFMA kernels
+    int a8_tile;             // TPAMD_A8_TILE: products of two 8-bit operands on tiles of 1000 * rows + columns, at any number of rows
+    int a8_splits;           // TPAMD_A8_SPLITS: their ranges of K
     int stream;              // TPAMD_STREAM: 0 = no launch on stream_kernel and stream_w8_kernel, 1 = every launch that they take
     int attn_decode;         // TPAMD_ATTN_DECODE: 0 = one new position per sequence through the general attention kernel, 1 = every such call that attention_decode_kernel takes
     int attn_splits;         // TPAMD_ATTN_SPLITS: key-range splits of the attention kernel

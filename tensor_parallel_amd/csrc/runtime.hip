@@ -36,6 +36,8 @@ Tuning read_tuning() {
     t.skinny_xlds = env_int("TPAMD_SKINNY_XLDS");
     t.skinny_max_m = env_int("TPAMD_SKINNY_MAX_M");
     t.gemv_rows = env_int("TPAMD_GEMV_ROWS");
+    t.a8_tile = env_int("TPAMD_A8_TILE");
+    t.a8_splits = env_int("TPAMD_A8_SPLITS");
     t.stream = env_int("TPAMD_STREAM");
     t.attn_decode = env_int("TPAMD_ATTN_DECODE");
     t.attn_splits = env_int("TPAMD_ATTN_SPLITS");

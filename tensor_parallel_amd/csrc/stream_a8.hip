@@ -1,0 +1,203 @@
+#include "a8.h"
+#include "gemm_tile.h"
+#include "stream_model.h"
+
+namespace tpamd {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int SA_NW = 4;        // wavefronts per block
+constexpr int SA_LDS_KB = 160;  // one block per CU
+constexpr int SA_DEPTH = 4;     // most stages
+
+// stream_a8_kernel: products of up to 64 rows of 8-bit codes on one block per CU, cut and staged as stream_kernel cuts and stages 16-bit ones (stream.hip): a block owns an even share of the
+// columns and all of K, its wavefronts contiguous quarters of K, 128 elements (bytes) of NR weight rows (a pair: gate rows, then up rows) and XR rows of x at a time through rings of their own in
+// LDS, filled by loads that go straight there; the wavefronts' sums meet in LDS. K ends in a multiple of 16: the pieces of x behind it are asked for outside the descriptor's range, which
+// gives zeros.
+template <int DT, bool PAIR, int NR, int XR, int D>
+__global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
+    constexpr int NT = (NR + 15) / 16, MT = (XR + 15) / 16, KK = 2;
+    constexpr int RP = 8, PITCH = 128;  // rows per load, bytes of a staged row
+    constexpr int NB = NR / RP, XB = XR / RP, L = NB + XB, STAGE = L * 1024, RING = D * STAGE;
+    constexpr int UP = PAIR ? NR / 2 : 0;
+    static_assert(NR % RP == 0 && XR % RP == 0 && UP % RP == 0, "whole loads");
+    static_assert(SA_NW * RING <= SA_LDS_KB * 1024 && D >= 2 && (D - 1) * L < 64, "LDS, and the count in s_waitcnt");
+    static_assert(NT * MT * 1024 <= RING, "the partial sums take the place of the stages");
+    constexpr int XLAST = XR - (MT - 1) * 16;  // staged rows of the last 16 of x: the lanes of the others read these again
+    static_assert(NT * 16 * PITCH <= STAGE && NB * 1024 + ((MT - 1) * 16 + XLAST) * PITCH <= STAGE && (XLAST & (XLAST - 1)) == 0, "fragments are read inside their stage");
+    extern __shared__ __align__(16) char smem[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, lq = lane >> 4, rb = lane >> 3;
+    const int n0 = static_cast<int>(static_cast<int64_t>(p.N) * blockIdx.x / gridDim.x);
+    const int cols = static_cast<int>(static_cast<int64_t>(p.N) * (blockIdx.x + 1) / gridDim.x) - n0;
+    const int KU = (p.K + 127) / 128, pieces = (p.K - (KU - 1) * 128) / 16;
+    const int first = KU * wave / SA_NW, units = KU * (wave + 1) / SA_NW - first;
+    // blocks start at different places of long rows: they would otherwise ask for the same columns of all rows at one time, which the memory channels answer unevenly
+    const int skew = units >= 32 ? static_cast<int>(((blockIdx.x >> 3) * 5 + (blockIdx.x & 7) * 3) % static_cast<unsigned>(units)) : 0;
+    const uint32_t ldw = static_cast<uint32_t>(p.ldw), ldx = static_cast<uint32_t>(p.ldx);
+    uint32_t w_off[NB], x_off[XB], behind[2];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int row = j * RP + rb, r = row - (PAIR && j >= NB / 2 ? UP : 0);
+        w_off[j] = static_cast<uint32_t>(r < cols ? r : cols - 1) * ldw + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < XB; ++j) {
+        const int row = j * RP + rb;
+        x_off[j] = static_cast<uint32_t>(row < p.M ? row : p.M - 1) * ldx + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) behind[h] = static_cast<int>((lane & 7) ^ ((h * 4 + (rb >> 1)) & 7)) >= pieces ? 0x80000000u : 0u;
+    const uint32_t w_extent = static_cast<uint32_t>(cols - 1) * ldw + static_cast<uint32_t>(p.K);
+    const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + static_cast<int64_t>(n0) * ldw, w_extent);
+    const __amdgpu_buffer_rsrc_t w2_rsrc = PAIR ? make_rsrc(p.w2 + static_cast<int64_t>(n0) * ldw, w_extent) : w_rsrc;
+    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(p.x, static_cast<uint32_t>(p.M - 1) * ldx + static_cast<uint32_t>(p.K));
+    char *ring = smem + wave * RING;
+    auto load = [&](int stage_off, int i) __attribute__((always_inline)) {  // unit number i of this wavefront (the last one again behind it)
+        const int t = skew + (i < units ? i : units > 0 ? units - 1 : 0);
+        const int u = first + (t < units || t == 0 ? t : t - units);
+        unrolled<NB>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(PAIR && j >= NB / 2 ? w2_rsrc : w_rsrc, (lds_void *)(ring + stage_off + j * 1024), 16, static_cast<int>(w_off[j]), u * PITCH, 0, 2);
+        });
+        unrolled<XB>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            buffer_load16_to_lds(x_rsrc, x_off[j] | (u == KU - 1 ? behind[j & 1] : 0u), u * PITCH, ring + stage_off + (NB + j) * 1024);
+        });
+    };
+
+    i32x4 acc[NT][MT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int a = 0; a < MT; ++a) acc[b][a] = i32x4{0, 0, 0, 0};
+
+    unrolled<D>([&](auto sc) { load(decltype(sc)::value * STAGE, decltype(sc)::value); });
+    const uint32_t rd = lds_addr_of(ring) + l16 * PITCH;
+    const uint32_t rd_last = lds_addr_of(ring) + (l16 & (XLAST - 1)) * PITCH;
+    uint32_t kk_off[KK];
+#pragma unroll
+    for (int k = 0; k < KK; ++k) kk_off[k] = static_cast<uint32_t>(((k * 4 + lq) ^ (l16 >> 1)) * 16);
+    int stage_off = 0;
+    for (int i = 0; i < units; ++i) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * L) : "memory");
+        u32x4 wq[KK][NT], xq[KK][MT];
+        unrolled<KK>([&](auto hc) {
+            constexpr int h = decltype(hc)::value;
+            const uint32_t at = rd + stage_off + kk_off[h], at_last = rd_last + stage_off + kk_off[h];
+            unrolled<NT>([&](auto bc) { wq[h][decltype(bc)::value] = lds_read16<decltype(bc)::value * 16 * PITCH>(at); });
+            unrolled<MT>([&](auto ac) { xq[h][decltype(ac)::value] = lds_read16<NB * 1024 + decltype(ac)::value * 16 * PITCH>(decltype(ac)::value == MT - 1 ? at_last : at); });
+        });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        unrolled<KK>([&](auto hc) {
+            constexpr int h = decltype(hc)::value;
+            unrolled<NT>([&](auto bc) { already_landed(wq[h][decltype(bc)::value]); });
+            unrolled<MT>([&](auto ac) { already_landed(xq[h][decltype(ac)::value]); });
+        });
+        load(stage_off, i + D);
+#pragma unroll
+        for (int h = 0; h < KK; ++h)
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+                    acc[b][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wq[h][b]), __builtin_bit_cast(i32x4, xq[h][a]), acc[b][a], 0, 0, 0);
+        stage_off = stage_off + STAGE == RING ? 0 : stage_off + STAGE;
+    }
+    // every load into the stages has landed before the partial sums take their place
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    i32x4 *red = reinterpret_cast<i32x4 *>(smem);
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int a = 0; a < MT; ++a) red[(wave * NT * MT + b * MT + a) * 64 + lane] = acc[b][a];
+    __syncthreads();
+    const int *sums = reinterpret_cast<const int *>(smem);
+    auto total = [&](int row, int m) __attribute__((always_inline)) {
+        const int at = (((row >> 4) * MT + (m >> 4)) * 64 + ((row & 15) >> 2) * 16 + (m & 15)) * 4 + (row & 3);
+        int s = 0;
+#pragma unroll
+        for (int v = 0; v < SA_NW; ++v) s += sums[v * NT * MT * 256 + at];
+        return s;
+    };
+    for (int e = tid; e < cols * p.M; e += SA_NW * 64) {
+        const int m = e / cols, c = e - m * cols, n = n0 + c;
+        const float sx = p.sx[m];
+        const float v = a8_scaled(total(c, m), sx, p.sw[n]);
+        uint16_t out;
+        if constexpr (PAIR) {
+            out = a8_round<DT>(a8_gated(v, a8_scaled(total(c + UP, m), sx, p.sw2[n])));
+        } else {
+            out = a8_round<DT>(a8_linear(v, p.bias != nullptr ? half_to_f32<DT>(reinterpret_cast<const uint16_t *>(p.bias)[n]) : 0.f, p.act));
+            if (p.addend != nullptr) out = f32_to_half<DT>(half_to_f32<DT>(out) + half_to_f32<DT>(reinterpret_cast<const uint16_t *>(p.addend)[m * p.ldadd + n]));
+        }
+        uint16_t *y = reinterpret_cast<uint16_t *>(p.y) + m * p.ldy + n;
+        *y = out;
+        if (!PAIR && p.copy != 0) *reinterpret_cast<uint16_t *>(reinterpret_cast<char *>(y) + p.copy) = out;
+    }
+}
+
+template <int DT, bool PAIR, int NR, int XR>
+int launch_nr(const A8Params &p, int blocks, hipStream_t s) {
+    constexpr int L = (NR + XR) / 8, DM = SA_LDS_KB / SA_NW / L, D = DM < SA_DEPTH ? DM : SA_DEPTH;
+    static_assert(D >= 2, "LDS");
+    constexpr int LDS = SA_NW * D * L * 1024;
+    auto kern = stream_a8_kernel<DT, PAIR, NR, XR, D>;
+    static thread_local int configured_dev = -1;  // per instantiation and host thread
+    int dev = 0;
+    TPAMD_HIP(hipGetDevice(&dev));
+    if (configured_dev != dev) {
+        TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        configured_dev = dev;
+    }
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(SA_NW * 64), LDS, s, p);
+    TPAMD_HIP(hipGetLastError());
+    return TPAMD_OK;
+}
+
+template <int DT, bool PAIR, int XR>
+int launch_xr(const A8Params &p, int nr, int blocks, hipStream_t s) {
+#define SA_ROWS(n) case n: return launch_nr<DT, PAIR, n, XR>(p, blocks, s)
+    switch (nr) {
+        SA_ROWS(32);
+        SA_ROWS(48);
+        SA_ROWS(64);
+        SA_ROWS(80);
+        SA_ROWS(96);
+    }
+    if constexpr (!PAIR) {
+        switch (nr) {
+            SA_ROWS(16);
+            SA_ROWS(24);
+        }
+    }
+#undef SA_ROWS
+    set_error("a8: no kernel of %d rows", nr);
+    return TPAMD_ERR_UNSUPPORTED;
+}
+
+template <int DT, bool PAIR>
+int launch_m(const A8Params &p, int nr, int blocks, hipStream_t s) {
+    if (p.M <= 8) return launch_xr<DT, PAIR, 8>(p, nr, blocks, s);
+    if (p.M <= 16) return launch_xr<DT, PAIR, 16>(p, nr, blocks, s);
+    if (p.M <= 24) return launch_xr<DT, PAIR, 24>(p, nr, blocks, s);
+    if (p.M <= 32) return launch_xr<DT, PAIR, 32>(p, nr, blocks, s);
+    if (p.M <= 48) return launch_xr<DT, PAIR, 48>(p, nr, blocks, s);
+    return launch_xr<DT, PAIR, 64>(p, nr, blocks, s);
+}
+
+}  // namespace
+
+bool stream_a8_takes(const A8Params &p, bool pair, int cus) { return p.M <= 64 && stream_cut(p.N, 1, pair, false, cus).groups > 0; }
+
+int stream_a8(const A8Params &p, bool pair, int dtype, int cus, hipStream_t s) {
+    const StreamCut cut = stream_cut(p.N, 1, pair, false, cus);
+    TPAMD_REQUIRE(cut.groups > 0, "a8: no cut of %d columns", p.N);
+    if (dtype == TPAMD_BF16) return pair ? launch_m<TPAMD_BF16, true>(p, cut.rows, cut.blocks, s) : launch_m<TPAMD_BF16, false>(p, cut.rows, cut.blocks, s);
+    return pair ? launch_m<TPAMD_F16, true>(p, cut.rows, cut.blocks, s) : launch_m<TPAMD_F16, false>(p, cut.rows, cut.blocks, s);
+}
+
+}  // namespace tpamd

@@ -200,3 +200,45 @@ def test_streams_graphs_and_gradients(m, n, k):
     rows = int8.QuantizedRows(x, sx, dtype)
     with pytest.raises(NotImplementedError):
         int8.linear(rows, w, sw, addend=addend.clone().requires_grad_()).sum().backward()
+
+
+TILES = [96128, 128128, 128192, 128256, 192192, 192256, 256192, 256256]
+
+
+@pytest.mark.parametrize("splits", [1, 3, 64])
+@pytest.mark.parametrize("tile", TILES)
+def test_every_tile(tile, splits, tune):
+    """Tiles that reach over the ends of rows and columns, K that ends inside a stage (one piece of 16, seven of them, none), fewer K tiles than stages or ranges."""
+    tune("TPAMD_A8_TILE", tile)
+    tune("TPAMD_A8_SPLITS", splits)
+    for m, n, k in [(1, 1, 16), (65, 50, 272), (130, 516, 384), (300, 1001, 1040), (515, 388, 2032), (256, 512, 4096)]:
+        check(m, n, k, torch.float16 if k % 128 else torch.bfloat16, low=-128)
+
+
+def test_a_tile_that_there_is_none_of(tune):
+    tune("TPAMD_A8_TILE", 64064)
+    x, sx, w, sw, *_ = operands(70, 64, 128, torch.float16)
+    with pytest.raises(_native.Unsupported, match="tile"):
+        _native.linear_a8(x, sx, w, sw, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("tile,splits", [(128128, 4), (256256, 2)])
+def test_ranges_of_k_under_capture_and_without_scratch_memory(tile, splits, tune):
+    """The ranges' sums lie in the stream's scratch buffer: a graph captured on a stream that has none takes the spare one, or all of K in a block; the same bits either way."""
+    tune("TPAMD_A8_TILE", tile)
+    x, sx, w, sw, u, su, *_ = operands(200, 640, 2048, torch.bfloat16)
+    want = _native.linear_a8(x, sx, w, sw), _native.swiglu_up_a8(x, sx, w, sw, u, su)
+    tune("TPAMD_A8_SPLITS", splits)
+    graphs = []
+    for _ in range(3):
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream(DEV)
+        with torch.cuda.graph(graph, stream=stream):
+            graphs.append((graph, (_native.linear_a8(x, sx, w, sw), _native.swiglu_up_a8(x, sx, w, sw, u, su)), stream))
+    for _ in range(3):
+        for graph, got, _ in graphs:
+            graph.replay()
+            assert torch.equal(_native.linear_a8(x, sx, w, sw), want[0])
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for *_, stream in graphs:
+        _native.release_scratch(DEV, stream.cuda_stream)
