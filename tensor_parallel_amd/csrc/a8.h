@@ -4,7 +4,7 @@
 
 namespace tpamd {
 
-// y[m][n] = act(s_x[m] s_w[n] sum_k x[m][k] w[n][k] + bias[n]) (+ addend), or the gated pair; sums exact in int32.
+// y[m][n] = act((s_x[m] s_w[n]) sum_k x[m][k] w[n][k] + bias[n]) (+ addend), or the gated pair; sums exact in int32.
 struct A8Params {
     const char *x, *w, *w2;            // codes: rows, weights (pair: gate), up weights
     const float *sx, *sw, *sw2;        // a scale for each row, column
@@ -25,12 +25,9 @@ __device__ __forceinline__ float a8_value(float v) {
     return v;
 }
 
-// From a sum to the value before it is rounded: in fp32 behind the exact sum (the int32 is rounded to 24 bits, 2^-24 of it).
-__device__ __forceinline__ float a8_scaled(int sum, float sx, float sw) { return a8_value(static_cast<float>(sum) * sw * sx); }
-__device__ __forceinline__ float a8_linear(float v, float bias, int act) {
-    v = a8_value(v + bias);
-    return act == TPAMD_ACT_GELU ? a8_value(gelu_erf(v)) : v;
-}
+// From a sum to the value before it is rounded, in fp32: the sum converted (24 bits of it), times the product of the scales, and the bias in the same operation.
+__device__ __forceinline__ float a8_linear(int sum, float sx, float sw, float bias) { return a8_value(fmaf(static_cast<float>(sum), a8_value(sx * sw), bias)); }
+__device__ __forceinline__ float a8_act(float v, int act) { return act == TPAMD_ACT_GELU ? a8_value(gelu_erf(v)) : v; }
 
 // SiLU(g) u, rounded once by the caller: both factors stay in fp32 (the 16-bit pair rounds g, u, SiLU(g) and the product as its four separate operations would;
 // here no 16-bit operation is stood in for, and one rounding is 2.3 times closer to the definition).
@@ -45,9 +42,10 @@ __device__ __forceinline__ uint32_t a8_round2(float a, float b) { return pack2_h
 static inline bool a8_fast(const A8Params &p) {
     return p.K >= 16 && p.K % 16 == 0 && p.ldx % 16 == 0 && p.ldw % 16 == 0 && p.ldx < (1ll << 22) && p.ldw < (1ll << 22) && aligned(p.x, 16) && aligned(p.w, 16) && aligned(p.w2, 16);
 }
-// gemm_a8.hip: tiles of 32 * tmx x-rows by 32 * tnx w-rows (a pair: 16 * tnx columns), K in at most `splits` ranges. stream_a8.hip: up to 64 rows on one block per CU. Operands of a8_fast.
-int gemm_a8(const A8Params &p, bool pair, int dtype, int tmx, int tnx, int splits, hipStream_t s);
+// gemm_a8.hip: tiles of 64 * tm x-rows by 64 * tn w-rows (a pair: 32 * tn columns), K in at most `splits` ranges. stream_a8.hip: up to 64 rows on one block per CU. Operands of a8_fast.
+int gemm_a8(const A8Params &p, bool pair, int dtype, int tm, int tn, int splits, hipStream_t s);
 bool stream_a8_takes(const A8Params &p, bool pair, int cus);
+float stream_a8_us(const A8Params &p, bool pair, int cus);  // predicted
 int stream_a8(const A8Params &p, bool pair, int dtype, int cus, hipStream_t s);
 
 }  // namespace tpamd

@@ -1,4 +1,5 @@
 #include "a8.h"
+#include "a8_model.h"
 
 namespace tpamd {
 namespace {
@@ -46,12 +47,11 @@ __global__ __launch_bounds__(256) void gemm_a8_any_kernel(A8Params p) {
         for (int b = 0; b < 4; ++b) {
             const int64_t n = n0 + tx + 16 * b;
             if (n >= p.N) continue;
-            const float v = a8_scaled(acc[0][a][b], sx, p.sw[n]);
             uint16_t out;
             if constexpr (PAIR) {
-                out = a8_round<DT>(a8_gated(v, a8_scaled(acc[1][a][b], sx, p.sw2[n])));
+                out = a8_round<DT>(a8_gated(a8_linear(acc[0][a][b], sx, p.sw[n], 0.f), a8_linear(acc[1][a][b], sx, p.sw2[n], 0.f)));
             } else {
-                out = a8_round<DT>(a8_linear(v, p.bias != nullptr ? half_to_f32<DT>(reinterpret_cast<const uint16_t *>(p.bias)[n]) : 0.f, p.act));
+                out = a8_round<DT>(a8_act(a8_linear(acc[0][a][b], sx, p.sw[n], p.bias != nullptr ? half_to_f32<DT>(reinterpret_cast<const uint16_t *>(p.bias)[n]) : 0.f), p.act));
                 if (p.addend != nullptr)
                     out = f32_to_half<DT>(half_to_f32<DT>(out) + half_to_f32<DT>(reinterpret_cast<const uint16_t *>(p.addend)[m * p.ldadd + n]));
             }
@@ -73,21 +73,19 @@ int launch_any(const A8Params &p, int dtype, hipStream_t s) {
     return TPAMD_OK;
 }
 
-// Up to 64 rows are streamed through one block per CU, more of them take tiles: the largest that the launch fills the device with, else K in ranges.
 int a8_dispatch(const A8Params &p, bool pair, int dtype, hipStream_t s) {
     int dev = 0, cus = 256;
     TPAMD_HIP(hipGetDevice(&dev));
     if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
     if (a8_fast(p)) {
         const Tuning &t = tuning();
-        if (t.a8_tile == TUNE_UNSET && stream_a8_takes(p, pair, cus)) return stream_a8(p, pair, dtype, cus, s);
-        int tmx = 8, tnx = 8, splits = 1;
-        if (t.a8_tile != TUNE_UNSET) {
-            tmx = t.a8_tile / 1000 / 32;
-            tnx = t.a8_tile % 1000 / 32;
-        }
-        if (t.a8_splits != TUNE_UNSET) splits = t.a8_splits < 1 ? 1 : t.a8_splits;
-        return gemm_a8(p, pair, dtype, tmx, tnx, splits, s);
+        const bool stream = t.stream != 0 && t.a8_tile == TUNE_UNSET && stream_a8_takes(p, pair, cus);
+        if (stream && t.stream == 1) return stream_a8(p, pair, dtype, cus, s);
+        A8Choice tile = a8_choose(pair, p.M, p.N, p.K, cus, static_cast<int64_t>(scratch_reserve(cus)));
+        if (stream && stream_a8_us(p, pair, cus) <= tile.us) return stream_a8(p, pair, dtype, cus, s);
+        if (t.a8_tile != TUNE_UNSET) tile = {t.a8_tile / 1000 / 64, t.a8_tile % 1000 / 64, 1, 0.f};
+        if (t.a8_splits != TUNE_UNSET) tile.ranges = t.a8_splits < 1 ? 1 : t.a8_splits;
+        return gemm_a8(p, pair, dtype, tile.tm, tile.tn, tile.ranges, s);
     }
     return pair ? launch_any<true>(p, dtype, s) : launch_any<false>(p, dtype, s);
 }

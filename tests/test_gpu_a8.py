@@ -202,7 +202,7 @@ def test_streams_graphs_and_gradients(m, n, k):
         int8.linear(rows, w, sw, addend=addend.clone().requires_grad_()).sum().backward()
 
 
-TILES = [96128, 128128, 128192, 128256, 192192, 192256, 256192, 256256]
+TILES = [64128, 128128, 128192, 192192, 192256, 256256]
 
 
 @pytest.mark.parametrize("splits", [1, 3, 64])
