@@ -1220,136 +1220,171 @@ def linear_w8_sum_ranks(calls: Sequence[tuple]) -> Optional[list]:
     return [y.view(*x.shape[:-1], y.shape[1]) for _, y in keep]
 
 
-def _code_rows(x: torch.Tensor, what: str) -> tuple:
-    """x as a matrix of contiguous rows, and the tensors that its codes and scales go to."""
-    require_device(x, what)
-    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
+# Rows in 8 bits and their products: calls of a few microseconds on the device, whose host side is kept short (one look at a tensor's shape and device, no views of contiguous ones).
+_HALF_CODES = {torch.bfloat16: BF16, torch.float16: F16}
+_device_of_thread = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(what: str, call, index: int, *args) -> None:
+    """call(*args, stream) on HIP device `index`."""
+    prev = _device_of_thread()
+    if prev == index:
+        rc = call(*args, _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream)
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = call(*args, _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream)
+        finally:
+            torch.cuda.set_device(prev)
+    if rc != 0:
+        _check(rc, what)
+
+
+def _flat_rows(t: torch.Tensor, shape: torch.Size) -> tuple:
+    """t as rows one after another (its memory, where it is that already), the number of rows and the elements between them."""
+    D = shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // D if D else math.prod(shape[:-1]), D or 1
+    if D == 0:
+        return t, math.prod(shape[:-1]), 1
+    t = _as_2d(t)
+    return t, t.shape[0], _ld(t)
+
+
+def _half_code(x: torch.Tensor, what: str) -> int:
+    if not x.is_cuda:
+        require_device(x, what)
+    code = _HALF_CODES.get(x.dtype)
+    if code is None:
         raise TypeError(f"{what}: rows of bfloat16 or float16 are quantised, got {x.dtype}")
     if x.dim() == 0:
         raise ValueError(f"{what}: a row has at least one axis")
-    D = x.shape[-1]
-    x2 = x if x.dim() == 2 and x.is_contiguous() else _as_2d(x) if D else x.reshape(math.prod(x.shape[:-1]), 0)
-    return x2, torch.empty(x.shape, dtype=torch.int8, device=x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    return code
 
 
 def quantize_rows(x: torch.Tensor) -> tuple:
     """(codes int8, scale fp32 [...]) of the rows of x: code = the integer nearest to 127 x / max |x| of the row (ties to even), scale = max |x| / 127; 1 for a row of
     zeros, NaN (and codes of 0) for one with an infinity or NaN."""
-    x2, q, scale_ = _code_rows(x, "quantize_rows")
-    M, D = x2.shape
-    with _on_device(x.device):
-        _check(lib().tpamd_quantize_rows(x2.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, _ld(x2), max(D, 1), dtype_code(x.dtype), current_stream_ptr(x.device)),
-               "tpamd_quantize_rows")
+    code, shape = _half_code(x, "quantize_rows"), x.shape
+    x2, M, ldx = _flat_rows(x, shape)
+    q, scale_ = torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    D = shape[-1]
+    _launch("tpamd_quantize_rows", lib().tpamd_quantize_rows, x.get_device(), x2.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, D or 1, code)
     return q, scale_
 
 
-def dequantize_rows(q: torch.Tensor, scale_: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """scale * q, in `dtype`."""
-    require_device(q, "dequantize_rows")
-    _check_codes(q, scale_, "dequantize_rows")
-    y = torch.empty(q.shape, dtype=dtype, device=q.device)
-    if q.numel():
-        q2, s2 = _as_2d(q), scale_.contiguous()
-        with _on_device(q.device):
-            _check(lib().tpamd_dequantize_rows(q2.data_ptr(), s2.data_ptr(), y.data_ptr(), *q2.shape, _ld(q2), q2.shape[1], dtype_code(dtype), current_stream_ptr(q.device)),
-                   "tpamd_dequantize_rows")
-    return y
-
-
-def _check_codes(q: torch.Tensor, scale_: torch.Tensor, what: str) -> None:
-    if q.dtype is not torch.int8 or scale_.dtype is not torch.float32:
-        raise TypeError(f"{what}: codes must be int8 and their scales float32, got {q.dtype} and {scale_.dtype}")
-    if q.dim() == 0 or scale_.shape != q.shape[:-1] or scale_.device != q.device:
-        raise ValueError(f"{what}: codes {tuple(q.shape)} on {q.device} need scales {list(q.shape[:-1])} there, got {tuple(scale_.shape)} on {scale_.device}")
-
-
-def _check_norm_weight(x: torch.Tensor, w: torch.Tensor, what: str) -> None:
-    if w.dtype != x.dtype or w.device != x.device or w.dim() != 1 or x.shape[-1] != w.shape[0]:
+def _check_norm_weight(x: torch.Tensor, w: torch.Tensor, what: str) -> torch.Tensor:
+    if w.dtype is not x.dtype or w.get_device() != x.get_device() or w.dim() != 1 or x.shape[-1] != w.shape[0]:
         raise ValueError(f"{what}: x {tuple(x.shape)} {x.dtype} on {x.device} and w {tuple(w.shape)} {w.dtype} on {w.device} do not fit")
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float) -> tuple:
     """`quantize_rows` of w * x * rsqrt(mean(x^2) + eps), which is not rounded in between."""
-    x2, q, scale_ = _code_rows(x, "rms_norm_q8")
-    _check_norm_weight(x, w, "rms_norm_q8")
-    M, D = x2.shape
-    w = w.contiguous()
-    with _on_device(x.device):
-        _check(lib().tpamd_rms_norm_q8(x2.data_ptr(), w.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, _ld(x2), max(D, 1), float(eps), dtype_code(x.dtype),
-                                       current_stream_ptr(x.device)), "tpamd_rms_norm_q8")
+    code, shape = _half_code(x, "rms_norm_q8"), x.shape
+    w = _check_norm_weight(x, w, "rms_norm_q8")
+    x2, M, ldx = _flat_rows(x, shape)
+    q, scale_ = torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    D = shape[-1]
+    _launch("tpamd_rms_norm_q8", lib().tpamd_rms_norm_q8, x.get_device(), x2.data_ptr(), w.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, D or 1, eps, code)
     return q, scale_
 
 
 def add_rms_norm_q8(r: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float) -> tuple:
     """(r + x, codes, scale): `rms_norm_q8` of that (rounded) sum."""
-    x2, q, scale_ = _code_rows(x, "add_rms_norm_q8")
-    _check_norm_weight(x, w, "add_rms_norm_q8")
-    if r.shape != x.shape or r.dtype != x.dtype or r.device != x.device:
-        raise ValueError(f"add_rms_norm_q8: r {tuple(r.shape)} {r.dtype} on {r.device} and x {tuple(x.shape)} {x.dtype} on {x.device} do not fit")
-    M, D = x2.shape
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    r2, w = r if r.dim() == 2 and r.is_contiguous() else _as_2d(r) if D else x2, w.contiguous()
-    with _on_device(x.device):
-        _check(lib().tpamd_add_rms_norm_q8(x2.data_ptr(), r2.data_ptr(), w.data_ptr(), total.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, _ld(x2), _ld(r2), max(D, 1),
-                                           max(D, 1), float(eps), dtype_code(x.dtype), current_stream_ptr(x.device)), "tpamd_add_rms_norm_q8")
+    code, shape = _half_code(x, "add_rms_norm_q8"), x.shape
+    w = _check_norm_weight(x, w, "add_rms_norm_q8")
+    if r.shape != shape or r.dtype is not x.dtype or r.get_device() != x.get_device():
+        raise ValueError(f"add_rms_norm_q8: r {tuple(r.shape)} {r.dtype} on {r.device} and x {tuple(shape)} {x.dtype} on {x.device} do not fit")
+    x2, M, ldx = _flat_rows(x, shape)
+    r2, _, ldr = _flat_rows(r, shape)
+    total = torch.empty(shape, dtype=x.dtype, device=x.device)
+    q, scale_ = torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    D = shape[-1]
+    _launch("tpamd_add_rms_norm_q8", lib().tpamd_add_rms_norm_q8, x.get_device(), x2.data_ptr(), r2.data_ptr(), w.data_ptr(), total.data_ptr(), q.data_ptr(), scale_.data_ptr(),
+            M, D, ldx, ldr, D or 1, D or 1, eps, code)
     return total, q, scale_
 
 
-def _a8_operands(what: str, q: torch.Tensor, scale_: torch.Tensor, weights: Sequence[tuple], dtype: torch.dtype) -> tuple:
-    """The codes as a matrix, their scales, and each (wq, wscale), as the library takes them, and N."""
-    require_device(q, what)
-    _check_codes(q, scale_, what)
-    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+def _check_codes(q: torch.Tensor, scale_: torch.Tensor, what: str) -> torch.Size:
+    if q.dtype is not torch.int8 or scale_.dtype is not torch.float32:
+        raise TypeError(f"{what}: codes must be int8 and their scales float32, got {q.dtype} and {scale_.dtype}")
+    shape = q.shape
+    if len(shape) == 0 or scale_.shape != shape[:-1] or scale_.get_device() != q.get_device():
+        raise ValueError(f"{what}: codes {tuple(shape)} on {q.device} need scales {list(shape[:-1])} there, got {tuple(scale_.shape)} on {scale_.device}")
+    return shape
+
+
+def dequantize_rows(q: torch.Tensor, scale_: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """scale * q, in `dtype`."""
+    if not q.is_cuda:
+        require_device(q, "dequantize_rows")
+    shape = _check_codes(q, scale_, "dequantize_rows")
+    y = torch.empty(shape, dtype=dtype, device=q.device)
+    q2, M, ldq = _flat_rows(q, shape)
+    D = shape[-1]
+    _launch("tpamd_dequantize_rows", lib().tpamd_dequantize_rows, q.get_device(), q2.data_ptr(), (scale_ if scale_.is_contiguous() else scale_.contiguous()).data_ptr(), y.data_ptr(),
+            M, D, ldq, D or 1, dtype_code(dtype))
+    return y
+
+
+def _a8_weight(what: str, wq: torch.Tensor, ws: torch.Tensor, K: int, index: int) -> tuple:
+    """The weight's codes and scales as the library takes them, its columns and the elements between its rows."""
+    shape = _check_codes(wq, ws, what)
+    if len(shape) != 2 or shape[1] != K or wq.get_device() != index:
+        raise ValueError(f"{what}: rows of {K} codes on device {index} and weights {tuple(shape)} on {wq.device} do not fit")
+    w2, _, ldw = _flat_rows(wq, shape)
+    return w2, ws if ws.is_contiguous() else ws.contiguous(), shape[0], ldw
+
+
+def _a8_rows(what: str, q: torch.Tensor, scale_: torch.Tensor, dtype: torch.dtype) -> tuple:
+    if not q.is_cuda:
+        require_device(q, what)
+    shape = _check_codes(q, scale_, what)
+    code = _HALF_CODES.get(dtype)
+    if code is None:
         raise TypeError(f"{what}: results are bfloat16 or float16, got {dtype}")
-    K, out = q.shape[-1], []
-    for wq, ws in weights:
-        _check_codes(wq, ws, what)
-        if wq.dim() != 2 or wq.shape[1] != K or wq.shape != weights[0][0].shape or wq.device != q.device:
-            raise ValueError(f"{what}: rows of {K} codes on {q.device} and weights {[tuple(w.shape) for w, _ in weights]} on {wq.device} do not fit")
-        out.append((wq if wq.is_contiguous() else _as_2d(wq) if K else wq, ws.contiguous()))
-    q2 = q if q.dim() == 2 and q.is_contiguous() else _as_2d(q) if K else q.reshape(math.prod(q.shape[:-1]), 0)
-    return q2, scale_.contiguous(), out, weights[0][0].shape[0]
+    return (code, shape, scale_ if scale_.is_contiguous() else scale_.contiguous(), *_flat_rows(q, shape))
 
 
 def linear_a8(q: torch.Tensor, scale_: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
               act: int = ACT_NONE, addend: Optional[torch.Tensor] = None, copy: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act((scale q) . (wscale wq)^T + bias) of int8 codes q [..., K] and wq [N, K], in `dtype`. `addend` and `copy` as in `linear`."""
-    q2, s2, ((w2, ws),), N = _a8_operands("linear_a8", q, scale_, [(wq, wscale)], dtype)
-    M, K = q2.shape
+    code, shape, s2, q2, M, ldx = _a8_rows("linear_a8", q, scale_, dtype)
+    K, index = shape[-1], q.get_device()
+    w2, ws, N, ldw = _a8_weight("linear_a8", wq, wscale, K, index)
     if bias is not None:
-        if bias.shape != (N,) or bias.dtype is not dtype or bias.device != q.device:
+        if bias.shape != (N,) or bias.dtype is not dtype or bias.get_device() != index:
             raise ValueError(f"linear_a8: bias must have shape [{N}] and {dtype} and live on {q.device}")
         bias = bias.contiguous()
-    if addend is not None and (addend.dtype is not dtype or addend.device != q.device or addend.shape != (*q.shape[:-1], N)):
+    out_shape = (*shape[:-1], N)
+    if addend is not None and (addend.dtype is not dtype or addend.get_device() != index or addend.shape != out_shape):
         raise ValueError("linear_a8: addend must have the shape, dtype and device of the result")
-    if copy is not None and (addend is None or copy.dtype is not dtype or copy.device != q.device or copy.shape != addend.shape or not copy.is_contiguous()):
+    if copy is not None and (addend is None or copy.dtype is not dtype or copy.get_device() != index or copy.shape != out_shape or not copy.is_contiguous()):
         raise ValueError("linear_a8: copy goes with an addend and must be a contiguous tensor of the result's shape, dtype and device")
-    y = torch.empty((*q.shape[:-1], N), dtype=dtype, device=q.device)
-    if y.numel() == 0:
-        return y
-    head = (q2.data_ptr(), s2.data_ptr(), w2.data_ptr(), ws.data_ptr(), None if bias is None else bias.data_ptr())
-    with _on_device(q.device):
-        stream = current_stream_ptr(q.device)
-        if addend is None:
-            rc = lib().tpamd_linear_a8(*head, y.data_ptr(), M, N, K, _ld(q2), _ld(w2), N, dtype_code(dtype), act, stream)
-        else:
-            a2 = _as_2d(addend)
-            rc = lib().tpamd_linear_a8_add(*head, a2.data_ptr(), y.data_ptr(), None if copy is None else copy.data_ptr(), M, N, K, _ld(q2), _ld(w2), _ld(a2), N, dtype_code(dtype),
-                                           act, stream)
-    _check(rc, "tpamd_linear_a8")
+    y = torch.empty(out_shape, dtype=dtype, device=q.device)
+    if addend is None:
+        _launch("tpamd_linear_a8", lib().tpamd_linear_a8, index, q2.data_ptr(), s2.data_ptr(), w2.data_ptr(), ws.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+                M, N, K, ldx, ldw, N, code, act)
+    elif M and N:
+        a2, _, ldadd = _flat_rows(addend, addend.shape)
+        _launch("tpamd_linear_a8_add", lib().tpamd_linear_a8_add, index, q2.data_ptr(), s2.data_ptr(), w2.data_ptr(), ws.data_ptr(), None if bias is None else bias.data_ptr(),
+                a2.data_ptr(), y.data_ptr(), None if copy is None else copy.data_ptr(), M, N, K, ldx, ldw, ldadd, N, code, act)
     return y
 
 
 def swiglu_up_a8(q: torch.Tensor, scale_: torch.Tensor, gate: torch.Tensor, gscale: torch.Tensor, up: torch.Tensor, uscale: torch.Tensor,
                  dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """silu(g) * u of the two `linear_a8`s g and u of the rows, in `dtype`; not rounded in between."""
-    q2, s2, ((g2, gs), (u2, us)), N = _a8_operands("swiglu_up_a8", q, scale_, [(gate, gscale), (up, uscale)], dtype)
-    if _ld(g2) != _ld(u2):
-        g2, u2 = g2.contiguous(), u2.contiguous()
-    M, K = q2.shape
-    h = torch.empty((*q.shape[:-1], N), dtype=dtype, device=q.device)
-    if h.numel():
-        with _on_device(q.device):
-            _check(lib().tpamd_swiglu_up_a8(q2.data_ptr(), s2.data_ptr(), g2.data_ptr(), gs.data_ptr(), u2.data_ptr(), us.data_ptr(), h.data_ptr(), M, N, K, _ld(q2), _ld(g2), N,
-                                            dtype_code(dtype), current_stream_ptr(q.device)), "tpamd_swiglu_up_a8")
+    code, shape, s2, q2, M, ldx = _a8_rows("swiglu_up_a8", q, scale_, dtype)
+    K, index = shape[-1], q.get_device()
+    g2, gs, N, ldg = _a8_weight("swiglu_up_a8", gate, gscale, K, index)
+    u2, us, Nu, ldu = _a8_weight("swiglu_up_a8", up, uscale, K, index)
+    if N != Nu:
+        raise ValueError(f"swiglu_up_a8: {N} gate columns and {Nu} up columns")
+    if ldg != ldu:
+        g2, u2, ldg = g2.contiguous(), u2.contiguous(), K or 1
+    h = torch.empty((*shape[:-1], N), dtype=dtype, device=q.device)
+    _launch("tpamd_swiglu_up_a8", lib().tpamd_swiglu_up_a8, index, q2.data_ptr(), s2.data_ptr(), g2.data_ptr(), gs.data_ptr(), u2.data_ptr(), us.data_ptr(), h.data_ptr(),
+            M, N, K, ldx, ldg, N, code)
     return h

@@ -6,7 +6,7 @@
 // the pass that sums them, and one meeting of the block serves both.
 // A code is the integer nearest to the exact quotient: in rows of 16-bit values many quotients lie on a half (a value of half the largest is 63.5), which a product with a
 // rounded 127 / a would put on either side. What the product leaves within 2^-13 of a half (its error is below 127 * 3 * 2^-24) is compared with the
-// half in 64 bits, where 2 * 127 p and (2 l + 1) a are exact; p is exact in fp32 (two 16-bit significands).
+// half in 64 bits, where 2 * 127 p and (2 l + 1) a are exact; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
 // A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
 //
 // Bound: at a few rows by the latency of a launch, else by HBM (x, r read once; sum and codes written once).
@@ -43,15 +43,45 @@ __device__ __forceinline__ RowCode row_code(uint32_t most_bits, float factor) {
     c.inv = c.most != 0.f ? 127.f / c.most : 0.f;
     return c;
 }
+// p * inv rounded by an addition of 1.5 * 2^23, whose low byte is then the code, and how far that integer is from p * inv.
+constexpr float CODE_MAGIC = 12582912.f;
+__device__ __forceinline__ float code_bits(float p, float inv, float &off) {
+    const float m = fmaf(p, inv, CODE_MAGIC);
+    off = fmaf(p, inv, CODE_MAGIC - m);
+    return m;
+}
+constexpr float CODE_NEAR = 0.5f - 0x1p-13f;
+__device__ __forceinline__ float code_bits_exact(float p, const RowCode &c) {
+    const float low = floorf(p * c.inv);
+    const double twice = 254.0 * static_cast<double>(p), half = (2.0 * low + 1.0) * static_cast<double>(c.most);
+    return CODE_MAGIC + (twice > half || (twice == half && (static_cast<int>(low) & 1)) ? low + 1.f : low);
+}
 __device__ __forceinline__ int code_of(float p, const RowCode &c) {
-    const float t = p * c.inv;
-    float n = rintf(t);
-    if (fabsf(t - n) > 0.5f - 0x1p-13f) {
-        const float low = floorf(t);
-        const double twice = 254.0 * static_cast<double>(p), half = (2.0 * low + 1.0) * static_cast<double>(c.most);
-        n = twice > half || (twice == half && (static_cast<int>(low) & 1)) ? low + 1.f : low;
+    if (c.most == 0.f) return 0;
+    float off, m = code_bits(p, c.inv, off);
+    if (fabsf(off) > CODE_NEAR) m = code_bits_exact(p, c);
+    return static_cast<int8_t>(__float_as_uint(m));
+}
+// Eight codes; whether one of them lies near a half is asked once.
+__device__ __forceinline__ uint2 codes8(const float (&p)[8], const RowCode &c) {
+    float m[8], off[8], far = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[j] = code_bits(p[j], c.inv, off[j]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) far = fmaxf(far, fabsf(off[j]));
+    if (far > CODE_NEAR) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (fabsf(off[j]) > CODE_NEAR) m[j] = code_bits_exact(p[j], c);
     }
-    return c.most != 0.f ? static_cast<int>(n) : 0;
+    uint32_t o[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(m[4 * h + 1]), __float_as_uint(m[4 * h]), 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(m[4 * h + 3]), __float_as_uint(m[4 * h + 2]), 0x0c0c0400u);
+        o[h] = c.most != 0.f ? lo | hi << 16 : 0;
+    }
+    return make_uint2(o[0], o[1]);
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
@@ -77,9 +107,6 @@ __device__ __forceinline__ void block_sum_max(float &sum, uint32_t &most, uint2 
         }
     }
 }
-
-template <int DT>
-__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b) { return add_packed2<DT>(a, b); }
 
 // Rows of D elements, D a multiple of 8 and at most 64 * WAVES * CH * 8, every row of x, r, s on a 16-byte boundary and of q on an 8-byte one. A block holds its row in registers.
 template <int DT, int WAVES, int CH, bool NORM, bool ADD>
@@ -115,7 +142,7 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = threadIdx.x + c * T;
-            v[c] = make_uint4(add2<DT>(rv[c].x, v[c].x), add2<DT>(rv[c].y, v[c].y), add2<DT>(rv[c].z, v[c].z), add2<DT>(rv[c].w, v[c].w));
+            v[c] = make_uint4(add_packed2<DT>(rv[c].x, v[c].x), add_packed2<DT>(rv[c].y, v[c].y), add_packed2<DT>(rv[c].z, v[c].z), add_packed2<DT>(rv[c].w, v[c].w));
             if (i < n) s[i] = v[c];
         }
     }
@@ -146,10 +173,7 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
     for (int c = 0; c < CH; ++c) {
         const int i = threadIdx.x + c * T;
         if (i >= n) continue;
-        uint32_t o[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j >> 2] |= static_cast<uint32_t>(code_of(f[c][j], code) & 0xff) << (8 * (j & 3));
-        q[i] = make_uint2(o[0], o[1]);
+        q[i] = codes8(f[c], code);
     }
 }
 
@@ -182,12 +206,20 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
     }
 }
 
+// Without the addition, rows of a large launch are held by fewer wavefronts with four chunks a lane: more of them are under way on a CU. 4096 rows: quantised 5504 17.2 -> 16.1 us, 16384 39.2 -> 35.3,
+// norms of 5504 19.8 -> 17.3, of 16384 45.6 -> 39.3, of 8192 23.0 -> 22.2; at 1024 rows of 4096 it takes 6.4 -> 8.1, and with the addition 13.8 -> 15.1 at 2103.
+constexpr int64_t MANY_ROWS = 2048;
+
 template <int DT, bool NORM, bool ADD>
 void launch_rows(const QuantParams &p, int64_t rows, bool vec, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(rows));
     const int n = p.D / 8;  // 16-byte chunks per row
     if (!vec) hipLaunchKernelGGL((quantize_any_kernel<DT, NORM, ADD>), grid, dim3(256), 0, s, p);
     else if (n <= 64) hipLaunchKernelGGL((quantize_kernel<DT, 1, 1, NORM, ADD>), grid, dim3(64), 0, s, p);
+    else if (!ADD && rows >= MANY_ROWS && n <= 256) hipLaunchKernelGGL((quantize_kernel<DT, 1, 4, NORM, ADD>), grid, dim3(64), 0, s, p);
+    else if (!ADD && rows >= MANY_ROWS && n <= 512) hipLaunchKernelGGL((quantize_kernel<DT, 2, 4, NORM, ADD>), grid, dim3(128), 0, s, p);
+    else if (!ADD && rows >= MANY_ROWS && n <= 1024) hipLaunchKernelGGL((quantize_kernel<DT, 4, 4, NORM, ADD>), grid, dim3(256), 0, s, p);
+    else if (!ADD && rows >= MANY_ROWS) hipLaunchKernelGGL((quantize_kernel<DT, 8, 4, NORM, ADD>), grid, dim3(512), 0, s, p);
     else if (n <= 256) hipLaunchKernelGGL((quantize_kernel<DT, 4, 1, NORM, ADD>), grid, dim3(256), 0, s, p);
     else if (n <= 512) hipLaunchKernelGGL((quantize_kernel<DT, 8, 1, NORM, ADD>), grid, dim3(512), 0, s, p);
     else if (n <= 1024) hipLaunchKernelGGL((quantize_kernel<DT, 8, 2, NORM, ADD>), grid, dim3(512), 0, s, p);
@@ -237,37 +269,51 @@ __device__ __forceinline__ float product(float a, float b) {
     return v;
 }
 
-// y = q * scale in fp32, rounded to the dtype: blockIdx.y takes every gridDim.y-th row, a thread 16 codes of it (VEC: rows of q on 16-byte, of y on 16-byte boundaries, D a multiple of 16).
+// y = q * scale in fp32, rounded to the dtype: blockIdx.y takes every gridDim.y-th row; VEC (rows of q on boundaries of V, of y on 16 bytes, D a multiple of V): a thread
+// has V codes, 16 bytes of y, 256 V further on once more.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void dequantize_kernel(const char *q, const float *scale, char *y, int64_t rows, int D, int64_t ldq, int64_t ldy) {
-    const int i = (blockIdx.x * 256 + threadIdx.x) * (VEC ? 16 : 1);
-    if (i >= D) return;
+    constexpr int V = !VEC ? 1 : DT == TPAMD_F32 ? 4 : 8, U = VEC ? 2 : 1;
+    const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * (U * 256) + threadIdx.x) * V;
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float f = scale[row];
         if constexpr (VEC) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(q + row * ldq + i);
-            const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+            uint2 u[U];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = product(static_cast<float>(static_cast<int8_t>(a[j] >> (8 * e))), f);
-                if constexpr (DT == TPAMD_F32)
-                    reinterpret_cast<float4 *>(y + (row * ldy + i) * 4)[j] = make_float4(v[0], v[1], v[2], v[3]);
-                else
-                    reinterpret_cast<uint2 *>(y + (row * ldy + i) * 2)[j] = make_uint2(pack2_half<DT>(v[0], v[1]), pack2_half<DT>(v[2], v[3]));
+            for (int h = 0; h < U; ++h) {
+                const int64_t i = i0 + h * (256 * V);
+                u[h] = make_uint2(0, 0);
+                if (i < D) {
+                    if constexpr (V == 8) u[h] = *reinterpret_cast<const uint2 *>(q + row * ldq + i);
+                    else u[h].x = *reinterpret_cast<const uint32_t *>(q + row * ldq + i);
+                }
             }
-        } else {
-            const float v = product(static_cast<float>(static_cast<int8_t>(q[row * ldq + i])), f);
-            if constexpr (DT == TPAMD_F32) reinterpret_cast<float *>(y)[row * ldy + i] = v;
-            else reinterpret_cast<uint16_t *>(y)[row * ldy + i] = f32_to_half<DT>(v);
+#pragma unroll
+            for (int h = 0; h < U; ++h) {
+                const int64_t i = i0 + h * (256 * V);
+                if (i >= D) break;
+                const uint32_t a[2] = {u[h].x, u[h].y};
+                float v[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = product(static_cast<float>(static_cast<int8_t>(a[e >> 2] >> (8 * (e & 3)))), f);
+                if constexpr (DT == TPAMD_F32)
+                    *reinterpret_cast<float4 *>(y + (row * ldy + i) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                else
+                    *reinterpret_cast<uint4 *>(y + (row * ldy + i) * 2) =
+                        make_uint4(pack2_half<DT>(v[0], v[1]), pack2_half<DT>(v[2], v[3]), pack2_half<DT>(v[4], v[5]), pack2_half<DT>(v[6], v[7]));
+            }
+        } else if (i0 < D) {
+            const float v = product(static_cast<float>(static_cast<int8_t>(q[row * ldq + i0])), f);
+            if constexpr (DT == TPAMD_F32) reinterpret_cast<float *>(y)[row * ldy + i0] = v;
+            else reinterpret_cast<uint16_t *>(y)[row * ldy + i0] = f32_to_half<DT>(v);
         }
     }
 }
 
 template <int DT>
 void launch_dequantize(const char *q, const float *scale, char *y, int64_t rows, int D, int64_t ldq, int64_t ldy, bool vec, hipStream_t s) {
-    const unsigned columns = static_cast<unsigned>((static_cast<int64_t>(D) + (vec ? 4095 : 255)) / (vec ? 4096 : 256));
+    const int64_t per = !vec ? 256 : DT == TPAMD_F32 ? 2048 : 4096;
+    const unsigned columns = static_cast<unsigned>((D + per - 1) / per);
     // rows in turn once 2^22 blocks are out
     const int64_t most = (1 << 22) / columns > 0 ? (1 << 22) / columns : 1;
     const int64_t by = rows < 65535 ? rows : 65535;
@@ -316,7 +362,8 @@ extern "C" int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, v
     const char *q = static_cast<const char *>(q_dev);
     const float *scale = static_cast<const float *>(scale_dev);
     char *y = static_cast<char *>(y_dev);
-    const bool vec = D % 16 == 0 && aligned(q, 16) && ldq % 16 == 0 && aligned(y, 16) && ldy % (dtype == TPAMD_F32 ? 4 : 8) == 0;
+    const int v = dtype == TPAMD_F32 ? 4 : 8;
+    const bool vec = D % v == 0 && aligned(q, v) && ldq % v == 0 && aligned(y, 16) && ldy % v == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int d = static_cast<int>(D);
     if (dtype == TPAMD_BF16) launch_dequantize<TPAMD_BF16>(q, scale, y, rows, d, ldq, ldy, vec, s);

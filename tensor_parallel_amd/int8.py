@@ -86,19 +86,19 @@ class QuantizedRows(NamedTuple):
 def quantize_activations(x: torch.Tensor) -> QuantizedRows:
     """The rows of x (bfloat16 or float16, on a HIP device) in 8 bits, by the definition in the module docstring. Inference only, as everything here: a
     backward pass through the rows' scales, or what Linears make of them, raises."""
-    codes, scale = _native.quantize_rows(x.detach())
+    codes, scale = _native.quantize_rows(x)
     return QuantizedRows(codes, _guard(scale, x), x.dtype)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> QuantizedRows:
     """The RMS norm of x's rows in 8 bits, in one launch: weight * x * rsqrt(mean(x^2) + eps), not rounded in between."""
-    codes, scale = _native.rms_norm_q8(x.detach(), weight.detach(), eps)
+    codes, scale = _native.rms_norm_q8(x, weight, eps)
     return QuantizedRows(codes, _guard(scale, x, weight), x.dtype)
 
 
 def add_rms_norm(r: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float) -> Tuple[torch.Tensor, QuantizedRows]:
     """(r + x, the RMS norm of that sum in 8 bits), in one launch: a residual stream and the input of the Linears behind its norm."""
-    total, codes, scale = _native.add_rms_norm_q8(r.detach(), x.detach(), weight.detach(), eps)
+    total, codes, scale = _native.add_rms_norm_q8(r, x, weight, eps)
     return _guard(total, r, x), QuantizedRows(codes, _guard(scale, r, x, weight), x.dtype)
 
 
@@ -106,15 +106,14 @@ def linear(rows: QuantizedRows, wq: torch.Tensor, wscale: torch.Tensor, bias: Op
            addend: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A Linear of 8-bit rows on int8 weights [N, K] with a float32 scale for each output (`quantize_rows` without outlier columns makes both), in the rows' dtype. `addend`: other ranks' partial
     sum, added to the rounded result. K is at most 131071 (the sum fits 32 bits)."""
-    y = _native.linear_a8(rows.codes, rows.scale.detach(), wq, wscale.detach(), None if bias is None else bias.detach(), rows.dtype, _native.ACT_GELU if gelu else _native.ACT_NONE,
-                          None if addend is None else addend.detach())
-    return _guard(y, rows.scale, wscale, bias, addend)
+    codes, scale, dtype = rows
+    return _guard(_native.linear_a8(codes, scale, wq, wscale, bias, dtype, _native.ACT_GELU if gelu else _native.ACT_NONE, addend), scale, wscale, bias, addend)
 
 
 def swiglu_up(rows: QuantizedRows, gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor) -> torch.Tensor:
     """silu(g) * u of the Linears g and u of 8-bit rows (as in `linear`, no bias), in one launch and rounded once."""
-    h = _native.swiglu_up_a8(rows.codes, rows.scale.detach(), gate, gate_scale.detach(), up, up_scale.detach(), rows.dtype)
-    return _guard(h, rows.scale, gate_scale, up_scale)
+    codes, scale, dtype = rows
+    return _guard(_native.swiglu_up_a8(codes, scale, gate, gate_scale, up, up_scale, dtype), scale, gate_scale, up_scale)
 
 
 # From 65 to this many rows a Linear neither meets its peer nor hands a sum over: the host sets the pace of an eager prompt there, and the reduction kernel's launch costs it

@@ -39,8 +39,10 @@ class _NoBackward(torch.autograd.Function):
 
 
 def _guard(out: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return _NoBackward.apply(out, *inputs)
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                return _NoBackward.apply(out, *inputs)
     return out
 
 
