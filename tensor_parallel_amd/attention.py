@@ -174,10 +174,13 @@ def _share_qkv_storage(module: torch.nn.Module) -> bool:
 
 
 def _project_qkv(self, hidden_states: torch.Tensor, D: int):
-    """q, k, v as [B, S, heads, D]: one call on the shared weight matrix when the three Linears still are views of it."""
-    from .shard_modules import ShardLinear, _guard
+    """q, k, v as [B, S, heads, D]: one call on the shared weight matrix when the three Linears still are views of it; Linears of 8-bit rows on rows that are
+    quantised once."""
+    from .shard_modules import ShardLinear, _guard, _has_a8
 
     B, S, _ = hidden_states.shape
+    if _has_a8(self, ("q_proj", "k_proj", "v_proj")) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
+        hidden_states = self.q_proj.rows_of(hidden_states)
     shared = self.__dict__.get("_tp_qkv")
     if shared is not None:
         w, b = shared
@@ -246,23 +249,38 @@ def _attend_on_cache(q, k, v, cos, sin, layer, static, scale, layer_idx: int) ->
     return out.reshape(B, S, Hq, D)
 
 
-def _fused_rotary_forward(self, hidden_states: torch.Tensor, position_embeddings=None, attention_mask=None, past_key_values=None,
-                          **kwargs):
-    own = type(self).forward
-    D = getattr(self, "head_dim", None)
-    layer = static = None
-    no_padding = self.__dict__.get("_tp_no_padding", False)  # the caller's word: masks are the causal pattern and nothing else
+def _caches_for(self, hidden_states, position_embeddings, attention_mask, past_key_values, kwargs) -> tuple:
+    """(growing layer, static layer) of the cache that the fused forward would work on; (None, None) where the module's own runs."""
     usable = (position_embeddings is not None and past_key_values is not None and not self.training
               and hidden_states.dim() == 3 and hidden_states.device.type == "cuda"
-              and hidden_states.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
+              and hidden_states.dtype in (torch.bfloat16, torch.float16) and getattr(self, "head_dim", None) in (64, 128)
               and not kwargs.get("output_attentions") and getattr(self, "is_causal", True))
+    no_padding = self.__dict__.get("_tp_no_padding", False)  # the caller's word: masks are the causal pattern and nothing else
+    layer = static = None
     if usable and (attention_mask is None or no_padding):
         layer = _cache_layer(past_key_values, self.layer_idx)
         if layer is None and no_padding:  # a static cache always comes with a materialised mask
             static = _static_layer(past_key_values, self.layer_idx)
+    return layer, static
+
+
+def takes_rows(module: torch.nn.Module, forward, hidden_states: torch.Tensor, kwargs: dict) -> bool:
+    """Whether a fused attention module would take this call, and only project the hidden states, by Linears of 8-bit rows."""
+    if forward is not _fused_rotary_forward or any(module._modules[name].dtype != hidden_states.dtype for name in ("q_proj", "k_proj", "v_proj")):
+        return False
+    more = dict(kwargs)
+    return _caches_for(module, hidden_states, more.pop("position_embeddings", None), more.pop("attention_mask", None), more.pop("past_key_values", None), more) != (None, None)
+
+
+def _fused_rotary_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+    # (hidden_states may be `QuantizedRows`, where takes_rows has said that this forward takes the call)
+    layer, static = _caches_for(self, hidden_states, position_embeddings, attention_mask, past_key_values, kwargs)
     if layer is None and static is None:
-        return own(self, hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
-                   past_key_values=past_key_values, **kwargs)
+        if not isinstance(hidden_states, torch.Tensor):
+            hidden_states = hidden_states.dequantize()
+        return type(self).forward(self, hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
+                                  past_key_values=past_key_values, **kwargs)
+    D = self.head_dim
     B, S, _ = hidden_states.shape
     q, k, v = _project_qkv(self, hidden_states, D)
     cos, sin = position_embeddings

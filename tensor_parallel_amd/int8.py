@@ -25,6 +25,7 @@ weights of the original model from the shards, refuses a model that holds one; i
 from __future__ import annotations
 
 import functools
+import types
 from typing import Callable, Mapping, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -77,6 +78,17 @@ class QuantizedRows(NamedTuple):
     codes: torch.Tensor  # int8 [..., K]
     scale: torch.Tensor  # float32 [...]
     dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dim(self) -> int:
+        return self.codes.dim()
 
     def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """scale * codes, in `dtype` (the rows' own by default)."""
@@ -169,6 +181,53 @@ class ShardLinearW8(nn.Module):
                 f"outlier_columns={self.outlier_idx.numel()}, dtype={self.dtype}")
 
 
+class ShardLinearA8(nn.Module):
+    """A Linear of 8-bit rows: weights int8 with a float32 scale for each output, the input's rows quantised by the forward (`quantize_activations`) unless they come as
+    `QuantizedRows`; the product is `tpamd_linear_a8`. Inference only."""
+
+    def __init__(self, wq: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor], dtype: torch.dtype):
+        super().__init__()
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"ShardLinearA8: activations must be bfloat16 or float16, got {dtype}")
+        self.out_features, self.in_features = wq.shape
+        if self.in_features > MAX_A8_FEATURES:
+            raise ValueError(f"ShardLinearA8: sums of {self.in_features} products of 8-bit codes may not fit 32 bits (at most {MAX_A8_FEATURES} do)")
+        self.dtype = dtype
+        self.register_buffer("wq", wq.contiguous())
+        self.register_buffer("scale", scale.contiguous())
+        self.register_buffer("bias", None if bias is None else bias.detach().to(dtype).contiguous())
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "ShardLinearA8":
+        """Quantise a [out, in] weight that lives on a HIP device."""
+        if weight.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"ShardLinearA8: the weight must be bfloat16 or float16, got {weight.dtype}")
+        if weight.dim() == 2 and weight.shape[1] > MAX_A8_FEATURES:
+            raise ValueError(f"ShardLinearA8: sums of {weight.shape[1]} products of 8-bit codes may not fit 32 bits (at most {MAX_A8_FEATURES} do)")
+        wq, scale, _, _ = quantize_rows(weight)
+        return cls(wq, scale, bias, weight.dtype)
+
+    def rows_of(self, input: Union[torch.Tensor, QuantizedRows]) -> QuantizedRows:  # noqa: A002
+        if input.dtype != self.dtype:
+            raise TypeError(f"ShardLinearA8: the input is {input.dtype}, the Linear was quantised for {self.dtype}")
+        return input if type(input) is QuantizedRows else quantize_activations(input)
+
+    def forward(self, input: Union[torch.Tensor, QuantizedRows]) -> torch.Tensor:  # noqa: A002
+        return self._product(input, _native.ACT_NONE)
+
+    def _product(self, input: Union[torch.Tensor, QuantizedRows], act: int) -> torch.Tensor:  # noqa: A002
+        rows = self.rows_of(input)
+        alone = functools.partial(_native.linear_a8, rows.codes, rows.scale, self.wq, self.scale, self.bias, self.dtype, act)
+        return product_in_context(self, rows, self.out_features, (rows.scale,), alone, alone, None, learned=False)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, dtype={self.dtype}"
+
+
+shard_modules.LINEAR_A8 = ShardLinearA8
+MAX_A8_FEATURES = 131071  # 128 * 128 * in_features < 2^31
+
+
 def _outliers_of(choice: OutlierChoice, name: str, module: nn.Module) -> Optional[Sequence[int]]:
     if choice is None:
         return None
@@ -178,27 +237,38 @@ def _outliers_of(choice: OutlierChoice, name: str, module: nn.Module) -> Optiona
 
 
 def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
-                      skip: Callable[[str, nn.Module], bool] = lambda name, m: False) -> int:
+                      skip: Callable[[str, nn.Module], bool] = lambda name, m: False, activations: bool = False) -> int:
     """Replace, in place, every 16-bit `nn.Linear` (and transformers `Conv1D`) under `module` whose weight lives on a HIP
     device by a `ShardLinearW8`. `outlier_cols`: the outlier input columns per Linear, as a mapping from the Linear's name
     under `module` (as in `module.named_modules()`) or as a function of (name, Linear); none by default. `skip(name,
-    Linear)` keeps a Linear as it is (an output head, say). Returns how many were replaced."""
+    Linear)` keeps a Linear as it is (an output head, say). Returns how many were replaced.
+
+    `activations=True`: both operands in 8 bits (`ShardLinearA8`; no outlier columns). A SiLU-gated MLP block then quantises its input once for gate and up, which are one launch
+    (`swiglu_up`), a fused attention of the Llama pattern its input once for q, k and v, and a Llama decoder layer takes their inputs from the launches of its norms (`rms_norm`,
+    `add_rms_norm`) where nothing watches the norms."""
+    if activations and outlier_cols is not None:
+        raise ValueError("quantize_linears_: with 8-bit activations there are no outlier columns")
     replaced = 0
     for parent_name, parent in list(module.named_modules()):
         for child_name, child in list(parent.named_children()):
             name = f"{parent_name}.{child_name}" if parent_name else child_name
             conv1d = is_conv1d(child)
-            if not (isinstance(child, nn.Linear) or conv1d) or isinstance(child, ShardLinearW8):
+            if not (isinstance(child, nn.Linear) or conv1d):
                 continue
             w = child.weight
             if w.device.type != "cuda" or w.dtype not in (torch.bfloat16, torch.float16) or skip(name, child):
                 continue
             weight = w.detach().t() if conv1d else w.detach()  # Conv1D keeps [in, out]
-            new = ShardLinearW8.from_weight(weight, getattr(child, "bias", None), _outliers_of(outlier_cols, name, child))
+            if activations:
+                new = ShardLinearA8.from_weight(weight, getattr(child, "bias", None))
+            else:
+                new = ShardLinearW8.from_weight(weight, getattr(child, "bias", None), _outliers_of(outlier_cols, name, child))
             setattr(parent, child_name, new)
             replaced += 1
             # a SiLU-gated MLP block whose fused forward reads gate_proj.weight / up_proj.weight goes back to its own forward
             fused = parent.__dict__.get("forward")
             if getattr(fused, "__func__", None) in (shard_modules._gated_mlp_forward, shard_modules._gated_mlp_first_forward):
                 del parent.forward
+        if activations and shard_modules.is_gated_silu_a8_mlp(parent):
+            parent.forward = types.MethodType(shard_modules._gated_mlp_a8_first_forward, parent)
     return replaced

@@ -126,7 +126,7 @@ def hands_through(ctx, module: nn.Module) -> bool:
         return True
     own, cls = wrapped.__dict__.get("forward"), type(wrapped)
     if own is not None:
-        return getattr(own, "__func__", None) is _gated_mlp_forward and wrapped._modules.get("down_proj") is module
+        return getattr(own, "__func__", None) in (_gated_mlp_forward, _gated_mlp_a8_forward) and wrapped._modules.get("down_proj") is module
     last = "o_proj" if cls.forward is _llama_attention_forward else "dense_4h_to_h" if cls.forward is _falcon_mlp_forward else None
     return last is not None and cls._tp_base.forward is cls._tp_replaced and wrapped._modules.get(last) is module
 
@@ -261,7 +261,17 @@ def _llama_layer_forward(self, hidden_states: torch.Tensor, *args, **kwargs) -> 
             or norm._tp_base.forward is not norm._tp_replaced or "forward" in norm.__dict__ or _has_hooks(norm)
             or hooks._global_forward_hooks or hooks._global_forward_pre_hooks or torch.is_grad_enabled() or not _norm_kernel_takes(hidden_states, norm.weight)):
         return own(self, hidden_states, *args, **kwargs)
-    attended, _ = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **{**_LAYER_DEFAULTS, **kwargs})
+    kwargs = {**_LAYER_DEFAULTS, **kwargs}
+    first, own_dtypes = self.input_layernorm, hidden_states.dtype in (torch.bfloat16, torch.float16)
+    rows = None
+    if own_dtypes and takes_rows(self._modules.get("self_attn"), hidden_states, kwargs) and _plain_rms_norm(first, hidden_states):
+        rows = int8_rows().rms_norm(hidden_states, first.weight, first.variance_epsilon)
+    attended, _ = self.self_attn(hidden_states=first(hidden_states) if rows is None else rows, **kwargs)
+    if own_dtypes and takes_rows(self._modules.get("mlp")) and type(attended) is torch.Tensor and attended.dtype == hidden_states.dtype and attended.shape == hidden_states.shape \
+            and attended.get_device() == hidden_states.get_device():
+        total, rows = int8_rows().add_rms_norm(hidden_states, attended, norm.weight, norm.variance_epsilon)
+        out = self.mlp(rows)
+        return together.add(total, out) if type(out) is torch.Tensor else total + out
     if type(attended) is torch.Tensor and attended.dtype == hidden_states.dtype and attended.shape == hidden_states.shape and attended.get_device() == hidden_states.get_device():
         total, normed = together.add_rms_norm(hidden_states, attended, norm.weight, norm.variance_epsilon)
     else:
@@ -269,6 +279,53 @@ def _llama_layer_forward(self, hidden_states: torch.Tensor, *args, **kwargs) -> 
         normed = norm(total)
     out = self.mlp(normed)
     return together.add(total, out) if type(out) is torch.Tensor else total + out
+
+
+def _plain_rms_norm(norm: nn.Module, x: torch.Tensor) -> bool:
+    """Whether a norm is nothing but `tpamd_rms_norm` for x, as far as anybody can tell (the layer has looked at hooks on all modules and at gradients)."""
+    return getattr(type(norm), "forward", None) is _rms_norm_forward and norm._tp_base.forward is norm._tp_replaced and "forward" not in norm.__dict__ and not _has_hooks(norm) \
+        and _norm_kernel_takes(x, norm.weight)
+
+
+LINEAR_A8 = None  # int8.ShardLinearA8, which that module puts here
+
+
+def int8_rows():
+    from . import int8
+
+    return int8
+
+
+def takes_rows(module, hidden_states=None, kwargs=None) -> bool:
+    """Whether a block (wrapped by a rank's rules or not) of Linears with 8-bit rows may be handed `QuantizedRows` in the place of its input: a gated MLP, or, with the call's hidden
+    states and arguments, a fused attention that will project them and do nothing else with them. Not where rules or hooks are told of the input."""
+    if module is None:
+        return False
+    block = module._modules.get("tp_wrapped_module", module)
+    own = getattr(block.__dict__.get("forward"), "__func__", None)
+    if hidden_states is None:
+        if own is not _gated_mlp_a8_forward or not _has_a8(block, ("gate_proj", "up_proj", "down_proj")):
+            return False
+    else:
+        if own is None or not _has_a8(block, ("q_proj", "k_proj", "v_proj")):
+            return False
+        from .attention import takes_rows as attention_takes_rows
+
+        if not attention_takes_rows(block, own, hidden_states, kwargs):
+            return False
+    if _has_hooks(module) or block is not module and (
+            "forward" in module.__dict__ or _has_hooks(block) or any(isinstance(target, int) or target in ("hidden_states", "x") for target in module.input_actions or ())):
+        return False
+    return True
+
+
+def _has_a8(module: nn.Module, names: tuple) -> bool:
+    """Whether these children are Linears of 8-bit rows that nobody watches."""
+    for name in names:
+        part = module._modules.get(name)
+        if type(part) is not LINEAR_A8 or "forward" in part.__dict__ or _has_hooks(part):
+            return False
+    return True
 
 
 def is_llama_attention(module: nn.Module) -> bool:
@@ -337,13 +394,13 @@ def _falcon_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
     """The module's own forward on a few rows with the activation in the epilogue of an int8 Linear before it, on the sum in 32 bits: a recorded step of 16 rows through a
     Falcon-40B-shaped layer 287 -> 281 us. Both ranks' first Linears with the activation take 0.67-0.94 of what they and torch's two
     passes do at 1 to 64 rows (16384 x 8192 at 64: 97.0 -> 90.6 us). Over many rows the error functions at the end of each tile take longer than torch's pass over memory (1024 rows 1490 -> 1515)."""
-    from .int8 import ShardLinearW8
+    from .int8 import ShardLinearA8, ShardLinearW8
 
     own = self._tp_base.forward
     if x.dim() == 0 or x.numel() > together.W8_TOGETHER_ROWS * x.shape[-1]:
         return own(self, x)
     up, act, hooks = self._modules.get("dense_h_to_4h"), self._modules.get("act"), torch.nn.modules.module
-    if (own is not self._tp_replaced or type(up) is not ShardLinearW8 or not _native.plain_call(x) or "forward" in up.__dict__ or not _is_erf_gelu(act)
+    if (own is not self._tp_replaced or type(up) not in (ShardLinearW8, ShardLinearA8) or not _native.plain_call(x) or "forward" in up.__dict__ or not _is_erf_gelu(act)
             or hooks._global_forward_hooks or hooks._global_forward_pre_hooks or _has_hooks(up) or _has_hooks(act) or torch.is_grad_enabled() and x.requires_grad):
         return own(self, x)
     return self.dense_4h_to_h(up._product(x, _native.ACT_GELU))
@@ -474,6 +531,37 @@ def _gated_mlp_first_forward(self, x: torch.Tensor) -> torch.Tensor:
         same = False
     if same:
         self.forward = types.MethodType(_gated_mlp_forward, self)
+    return own
+
+
+def is_gated_silu_a8_mlp(module: nn.Module) -> bool:
+    """As is_gated_silu_mlp, of Linears with 8-bit rows."""
+    if "forward" in module.__dict__ or not _has_a8(module, ("gate_proj", "up_proj", "down_proj")):
+        return False
+    gate, up = module._modules["gate_proj"], module._modules["up_proj"]
+    return gate.bias is None and up.bias is None and gate.wq.shape == up.wq.shape and gate.dtype == up.dtype and \
+        _is_silu(module._modules.get("act_fn", module.__dict__.get("act_fn")))
+
+
+def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
+    """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch."""
+    gate, up, down = self.gate_proj, self.up_proj, self.down_proj
+    return down(int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))
+
+
+def _gated_mlp_a8_first_forward(self, x: torch.Tensor) -> torch.Tensor:
+    """First call, as of _gated_mlp_first_forward. The block's own forward rounds gate, up and their product to 16 bits, which moves hidden codes by a step of 127 here and there: the two are
+    a percent of the result's spread apart in the mean (single values up to 8), where another function would be as far off as the result is large."""
+    del self.forward  # the class's forward is visible again
+    own = type(self).forward(self, x)
+    try:
+        fused = _gated_mlp_a8_forward(self, x)
+        same = isinstance(own, torch.Tensor) and own.shape == fused.shape and bool(
+            (own.detach().float() - fused.detach().float()).square().sum() <= 0.05**2 * own.detach().float().square().sum())
+    except (TypeError, ValueError, RuntimeError):
+        same = False
+    if same:
+        self.forward = types.MethodType(_gated_mlp_a8_forward, self)
     return own
 
 
