@@ -11,24 +11,24 @@ struct A8Tile {
     int tm, tn, blocks_per_cu;
     float fixed, round, full, few, part, one, two, split, per_mb, per_range;
 };
-// Fitted to 300 shapes at 65-6144 rows, 1024-16384 columns, K 1024-11008, each tile with 1-12 ranges timed inside HIP graphs on rotated weights; the choice is 0.8 % off the best of them in the
-// geometric mean, 1.0 % on 200 others (worst 28 %). Without one of the tiles the best would be 1-4 % slower each.
+// Fitted to 400 shapes at 65-6144 rows, 1024-16384 columns, K 1024-11008, each tile with 1-12 ranges timed inside HIP graphs on rotated weights; the choice is 1.2 % off the best of them in the
+// geometric mean, 0.8 % on 200 others (worst 32 and 18 %). Without one of the tiles the best would be 1-4 % slower each.
 constexpr A8Tile A8_TILES[2][6] = {
     {
-        {1, 2, 2, 5.1, 1.3, 0.77, 0.21, 0.0, 0.42, 0.58, 2.4, 0.25, 0.13},
-        {2, 2, 1, 4.6, 2.1, 0.60, 0.31, 1.1, 0, 0, 2.7, 0.18, 0.10},
-        {2, 3, 1, 6.6, 2.8, 0.77, 0.39, 0.5, 0, 0, 2.1, 0.19, 0.12},
-        {3, 3, 1, 5.7, 3.5, 1.02, 0.51, 2.7, 0, 0, 1.3, 0.19, 0.04},
-        {3, 4, 1, 7.5, 1.7, 1.45, 0.80, 1.3, 0, 0, 0.7, 0.20, 0.02},
-        {4, 4, 1, 2.2, 9.2, 1.61, 0.92, 8.6, 0, 0, 0.0, 0.21, 0.00},
+        {1, 2, 2, 4.8, 0.9, 0.75, 0.25, 0.0, 0.44, 0.62, 2.1, 0.27, 0.22},
+        {2, 2, 1, 5.6, 1.8, 0.60, 0.36, 0.0, 0, 0, 2.4, 0.20, 0.17},
+        {2, 3, 1, 5.3, 2.6, 0.77, 0.45, 1.6, 0, 0, 1.9, 0.20, 0.20},
+        {3, 3, 1, 5.7, 3.1, 1.03, 0.55, 2.8, 0, 0, 1.0, 0.20, 0.09},
+        {3, 4, 1, 6.0, 2.1, 1.46, 0.86, 2.5, 0, 0, 0.7, 0.21, 0.08},
+        {4, 4, 1, 0.5, 9.7, 1.59, 1.00, 9.9, 0, 0, 0.0, 0.22, 0.00},
     },
     {
-        {1, 2, 2, 4.1, 1.3, 0.83, 0.19, 0.0, 0.49, 0.58, 3.3, 0.28, 0.00},
-        {2, 2, 1, 4.7, 2.0, 0.63, 0.34, 0.0, 0, 0, 3.5, 0.20, 0.02},
-        {2, 3, 1, 5.9, 2.3, 0.83, 0.44, 0.0, 0, 0, 3.4, 0.21, 0.02},
-        {3, 3, 1, 7.1, 3.1, 1.06, 0.53, 0.5, 0, 0, 2.8, 0.17, 0.00},
-        {3, 4, 1, 4.6, 2.6, 1.56, 0.84, 3.0, 0, 0, 2.5, 0.17, 0.00},
-        {4, 4, 1, 1.5, 7.7, 1.70, 0.95, 8.2, 0, 0, 1.7, 0.18, 0.00},
+        {1, 2, 2, 4.5, 1.4, 0.75, 0.25, 0.0, 0.46, 0.65, 2.5, 0.29, 0.00},
+        {2, 2, 1, 4.7, 1.9, 0.59, 0.36, 0.8, 0, 0, 2.9, 0.22, 0.00},
+        {2, 3, 1, 6.0, 3.0, 0.76, 0.45, 0.8, 0, 0, 2.6, 0.21, 0.00},
+        {3, 3, 1, 3.2, 4.0, 1.02, 0.59, 4.4, 0, 0, 2.2, 0.20, 0.00},
+        {3, 4, 1, 6.9, 2.3, 1.48, 0.93, 0.4, 0, 0, 2.0, 0.21, 0.00},
+        {4, 4, 1, 3.4, 7.3, 1.64, 1.03, 6.0, 0, 0, 0.8, 0.21, 0.00},
     },
 };
 inline float a8_tile_us(const A8Tile &t, bool pair, int64_t M, int64_t N, int64_t K, int ranges, int cus, float *mb) {
@@ -36,12 +36,14 @@ inline float a8_tile_us(const A8Tile &t, bool pair, int64_t M, int64_t N, int64_
     const int64_t all = (K + 127) / 128, kt = (all + ranges - 1) / ranges, splits = (all + kt - 1) / kt, blocks = tiles * splits;
     const int64_t round = static_cast<int64_t>(t.blocks_per_cu) * cus, rounds = blocks / round, rest = blocks % round;
     const float k = static_cast<float>(kt), part = static_cast<float>(rest) / static_cast<float>(cus);
-    float us = t.fixed + static_cast<float>(rounds) * (t.round + t.full * k);
+    float us = static_cast<float>(rounds) * (t.round + t.full * k);
     if (rest > 0) {
         float rate = t.few + (t.full - t.few) * part;
         if (t.blocks_per_cu == 2) rate = part <= 1.f ? t.few + (t.one - t.few) * part : t.two + (t.full - t.two) * (part - 1.f);
         us += t.part + rate * k;
     }
+    const float weights = static_cast<float>(N) * static_cast<float>(K) * (pair ? 2.f : 1.f) * (1.f / 4.8e6f);  // from memory, at what tiles of few rows read
+    us = t.fixed + (us > weights ? us : weights);
     *mb = static_cast<float>(blocks) * static_cast<float>(t.tm * t.tn) * (64 * 64 * 4 * 1e-6f);
     return splits > 1 ? us + t.split + t.per_mb * *mb + t.per_range * static_cast<float>(splits) : us;
 }

@@ -129,14 +129,13 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
     const int last_kt = KT_ALL - 1 - first;  // the K tile of this range that K ends in
     const int pieces = (p.K - (KT_ALL - 1) * A8_BK) / 16;
 
-    // ---- load addresses: rows past the end of an operand are clamped to its last one
+    // ---- load addresses: rows past the end of an operand lie outside the descriptors, whose extents are below 2^31
     const int rb = lane >> 3;
     uint32_t x_off[XL], w_off[WL], behind[2];
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
         const int row = (wave * XL + i) * 8 + rb;
-        const int r = m0 + row < p.M ? row : p.M - 1 - m0;
-        x_off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.ldx) + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+        x_off[i] = m0 + row < p.M ? static_cast<uint32_t>(row) * static_cast<uint32_t>(p.ldx) + ((lane & 7) ^ ((row >> 1) & 7)) * 16 : 0x80000000u;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)  // by whether the 8 rows of a load are an odd or an even eighth
@@ -145,8 +144,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
         const int row = (wave * WL + i) * 8 + rb, wr = MODE == MODE_SWIGLU ? (row >> 5) * 16 + (row & 15) : row;
-        const int r = n0 + wr < p.N ? wr : p.N - 1 - n0;
-        w_off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.ldw) + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+        w_off[i] = n0 + wr < p.N ? static_cast<uint32_t>(wr) * static_cast<uint32_t>(p.ldw) + ((lane & 7) ^ ((row >> 1) & 7)) * 16 : 0x80000000u;
     }
     const int x_rows = p.M - m0 < BM ? p.M - m0 : BM, w_rows = p.N - n0 < BN_OUT ? p.N - n0 : BN_OUT;
     const uint32_t w_extent = static_cast<uint32_t>(w_rows - 1) * static_cast<uint32_t>(p.ldw) + static_cast<uint32_t>(p.K);
@@ -154,13 +152,16 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
         make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx, static_cast<uint32_t>(x_rows - 1) * static_cast<uint32_t>(p.ldx) + static_cast<uint32_t>(p.K));
     const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw, w_extent);
     const __amdgpu_buffer_rsrc_t w2_rsrc = MODE == MODE_SWIGLU ? make_rsrc(p.w2 + static_cast<int64_t>(n0) * p.ldw, w_extent) : w_rsrc;
-    auto load = [&](auto ic, int kt, int stage_off) __attribute__((always_inline)) {  // load number ic of K tile kt of this range
+    // load number ic of K tile kt of this range; behind the last one the same count of loads from outside the descriptors (with the uniform offset inside their extents)
+    auto load = [&](auto ic, int kt, int stage_off) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
+        const uint32_t none = kt < KT ? 0u : 0x80000000u;
+        const int at = (first + (kt < KT ? kt : 0)) * A8_BK;
         if constexpr (i < XL) {
-            const uint32_t end = kt == last_kt ? behind[i & 1] : 0u;  // (XL is even)
-            buffer_load16_to_lds(x_rsrc, x_off[i] | end, (first + kt) * A8_BK, smem + stage_off + (wave * XL + i) * 1024);
+            const uint32_t end = kt == last_kt ? behind[i & 1] : none;  // (XL is even)
+            buffer_load16_to_lds(x_rsrc, x_off[i] | end, at, smem + stage_off + (wave * XL + i) * 1024);
         } else {
-            buffer_load16_to_lds(is_up(i - XL) ? w2_rsrc : w_rsrc, w_off[i - XL], (first + kt) * A8_BK, smem + stage_off + XREG + (wave * WL + i - XL) * 1024);
+            buffer_load16_to_lds(is_up(i - XL) ? w2_rsrc : w_rsrc, w_off[i - XL] | none, at, smem + stage_off + XREG + (wave * WL + i - XL) * 1024);
         }
     };
 
@@ -203,8 +204,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
     // ---- first stages: the second half of the last one is loaded in the first step
     unrolled<NS>([&](auto sc) {
         constexpr int s = decltype(sc)::value;
-        const int kt = s < KT ? s : KT - 1;
-        unrolled<(s < NS - 1 ? LPT : HALF)>([&](auto ic) { load(ic, kt, s * STAGE); });
+        unrolled<(s < NS - 1 ? LPT : HALF)>([&](auto ic) { load(ic, s, s * STAGE); });
     });
     if constexpr (!SPLIT) {
 #pragma unroll
@@ -216,8 +216,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
 
     int cur = 0, nxt = STAGE, old = (NS - 1) * STAGE;  // offsets of the stages of K tiles g, g + 1 and g + NS - 1
     for (int g = 0; g < KT; ++g) {
-        // past the end the last tile again, into stages nobody reads any more
-        const int k_old = g + NS - 1 < KT ? g + NS - 1 : KT - 1, k_cur = g + NS < KT ? g + NS : KT - 1;
+        const int k_old = g + NS - 1, k_cur = g + NS;
         unrolled<4>([&](auto sc) {
             constexpr int s = decltype(sc)::value, bar = s == 3 ? BAR : 0, slots = MF - bar, per = (READS + slots - 1) / slots;
             const uint32_t off = (s == 3 ? nxt : cur) + kk_off[(s + 1) & 3], xa = x_rd + off, wa = w_rd + off;

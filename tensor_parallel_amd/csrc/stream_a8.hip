@@ -41,12 +41,12 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
         const int row = j * RP + rb, r = row - (PAIR && j >= NB / 2 ? UP : 0);
-        w_off[j] = static_cast<uint32_t>(r < cols ? r : cols - 1) * ldw + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+        w_off[j] = r < cols ? static_cast<uint32_t>(r) * ldw + ((lane & 7) ^ ((row >> 1) & 7)) * 16 : 0x80000000u;
     }
 #pragma unroll
     for (int j = 0; j < XB; ++j) {
         const int row = j * RP + rb;
-        x_off[j] = static_cast<uint32_t>(row < p.M ? row : p.M - 1) * ldx + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+        x_off[j] = row < p.M ? static_cast<uint32_t>(row) * ldx + ((lane & 7) ^ ((row >> 1) & 7)) * 16 : 0x80000000u;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) behind[h] = static_cast<int>((lane & 7) ^ ((h * 4 + (rb >> 1)) & 7)) >= pieces ? 0x80000000u : 0u;
@@ -55,16 +55,17 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
     const __amdgpu_buffer_rsrc_t w2_rsrc = PAIR ? make_rsrc(p.w2 + static_cast<int64_t>(n0) * ldw, w_extent) : w_rsrc;
     const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(p.x, static_cast<uint32_t>(p.M - 1) * ldx + static_cast<uint32_t>(p.K));
     char *ring = smem + wave * RING;
-    auto load = [&](int stage_off, int i) __attribute__((always_inline)) {  // unit number i of this wavefront (the last one again behind it)
-        const int t = skew + (i < units ? i : units > 0 ? units - 1 : 0);
+    auto load = [&](int stage_off, int i) __attribute__((always_inline)) {  // unit number i of this wavefront; behind the last one the same count of loads from outside the descriptors
+        const int t = i < units ? skew + i : 0;  // (the wavefront-uniform offset stays inside the extents)
         const int u = first + (t < units || t == 0 ? t : t - units);
+        const uint32_t none = i < units ? 0u : 0x80000000u;
         unrolled<NB>([&](auto jc) {
             constexpr int j = decltype(jc)::value;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(PAIR && j >= NB / 2 ? w2_rsrc : w_rsrc, (lds_void *)(ring + stage_off + j * 1024), 16, static_cast<int>(w_off[j]), u * PITCH, 0, 2);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(PAIR && j >= NB / 2 ? w2_rsrc : w_rsrc, (lds_void *)(ring + stage_off + j * 1024), 16, static_cast<int>(w_off[j] | none), u * PITCH, 0, 2);
         });
         unrolled<XB>([&](auto jc) {
             constexpr int j = decltype(jc)::value;
-            buffer_load16_to_lds(x_rsrc, x_off[j] | (u == KU - 1 ? behind[j & 1] : 0u), u * PITCH, ring + stage_off + (NB + j) * 1024);
+            buffer_load16_to_lds(x_rsrc, x_off[j] | none | (u == KU - 1 ? behind[j & 1] : 0u), u * PITCH, ring + stage_off + (NB + j) * 1024);
         });
     };
 
@@ -192,12 +193,15 @@ int launch_m(const A8Params &p, int nr, int blocks, hipStream_t s) {
 
 bool stream_a8_takes(const A8Params &p, bool pair, int cus) { return p.M <= 64 && stream_cut(p.N, 1, pair, false, cus).groups > 0; }
 
-// Fitted to 150 shapes of 9-64 rows (within 15 % of them): a CU stages weights at 26 GB/s and x at 134 GB/s, in each turn of the blocks.
+// Fitted to 300 shapes of 1-64 rows (within 8 % of them in the mean, and of 150 others): each turn of the blocks costs 3.4 us, what it stages of weight rows (padded ones too) 0.010 us per KB,
+// of x 0.012, what it reads of memory 0.028 with every CU at it, and a thousand outputs 1.6.
 float stream_a8_us(const A8Params &p, bool pair, int cus) {
     const StreamCut cut = stream_cut(p.N, 1, pair, false, cus);
     const int xr = p.M <= 32 ? (p.M + 7) / 8 * 8 : p.M <= 48 ? 48 : 64;
-    const float k = static_cast<float>(p.K) * 1e-3f, outputs = static_cast<float>((p.N + cut.blocks - 1) / cut.blocks * (pair ? 2 : 1)) * static_cast<float>(p.M);
-    return 2.8f + static_cast<float>(cut.groups) * (0.73f + k * static_cast<float>(cut.rows) / 26.4f + k * static_cast<float>(xr) / 134.f + 0.0023f * outputs);
+    const float k = static_cast<float>(p.K) * 1e-3f, columns = static_cast<float>((p.N + cut.blocks - 1) / cut.blocks * (pair ? 2 : 1));
+    const float busy = cut.blocks < cus ? static_cast<float>(cut.blocks) / static_cast<float>(cus) : 1.f;
+    return static_cast<float>(cut.groups) *
+           (3.37f + k * (0.0101f * static_cast<float>(cut.rows) + 0.0118f * static_cast<float>(xr) + 0.028f * columns * busy) + 1.62e-3f * columns * static_cast<float>(p.M));
 }
 
 int stream_a8(const A8Params &p, bool pair, int dtype, int cus, hipStream_t s) {
