@@ -5,8 +5,8 @@
 // The norm's factor is the same for a whole row, so it is in the scale alone: a row's codes do not depend on how its squares are summed, the maximum is found in
 // the pass that sums them, and one meeting of the block serves both.
 // A code is the integer nearest to the exact quotient: in rows of 16-bit values many quotients lie on a half (a value of half the largest is 63.5), which a product with a
-// rounded 127 / a would put on either side. What the product leaves within 2^-13 of a half (its error is below 127 * 3 * 2^-24) is compared with the
-// half in 64 bits, where 2 * 127 p and (2 l + 1) a are exact; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
+// rounded 127 / a would put on either side. What the product leaves within 2^-15 of a half (its error is below 127 * 2 * 2^-24: one rounding each of 127 / a and of the product) is
+// compared with the half exactly; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
 // A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
 //
 // Bound: at a few rows by the latency of a launch, else by HBM (x, r read once; sum and codes written once).
@@ -50,16 +50,18 @@ __device__ __forceinline__ float code_bits(float p, float inv, float &off) {
     off = fmaf(p, inv, CODE_MAGIC - m);
     return m;
 }
-constexpr float CODE_NEAR = 0.5f - 0x1p-13f;
-__device__ __forceinline__ float code_bits_exact(float p, const RowCode &c) {
-    const float low = floorf(p * c.inv);
-    const double twice = 254.0 * static_cast<double>(p), half = (2.0 * low + 1.0) * static_cast<double>(c.most);
-    return CODE_MAGIC + (twice > half || (twice == half && (static_cast<int>(low) & 1)) ? low + 1.f : low);
+constexpr float CODE_NEAR = 0.5f - 0x1p-15f;
+// A quotient that near to h, `whole` + 1/2 or - 1/2 on the side of `off`: 127 p against h a, both divided by 256 against overflow. h a is t + low exactly; 127 p lies within 2^-13 a of it and both are
+// multiples of 2^-33 a, so their difference from t is exact as well. On a tie the rounding of h itself takes the even side.
+__device__ __forceinline__ float code_bits_exact(float p, float m, float off, float most) {
+    const float h = m - CODE_MAGIC + (off > 0.f ? 0.5f : -0.5f), a = most * 0x1p-8f;
+    const float t = h * a, low = fmaf(h, a, -t), d = fmaf(127.f, p * 0x1p-8f, -t);
+    return CODE_MAGIC + rintf(h + (d > low ? 0.25f : d < low ? -0.25f : 0.f));
 }
 __device__ __forceinline__ int code_of(float p, const RowCode &c) {
     if (c.most == 0.f) return 0;
     float off, m = code_bits(p, c.inv, off);
-    if (fabsf(off) > CODE_NEAR) m = code_bits_exact(p, c);
+    if (fabsf(off) > CODE_NEAR) m = code_bits_exact(p, m, off, c.most);
     return static_cast<int8_t>(__float_as_uint(m));
 }
 // Eight codes; whether one of them lies near a half is asked once.
@@ -71,8 +73,7 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const RowCode &c) {
     for (int j = 0; j < 8; ++j) far = fmaxf(far, fabsf(off[j]));
     if (far > CODE_NEAR) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (fabsf(off[j]) > CODE_NEAR) m[j] = code_bits_exact(p[j], c);
+        for (int j = 0; j < 8; ++j) m[j] = fabsf(off[j]) > CODE_NEAR ? code_bits_exact(p[j], m[j], off[j], c.most) : m[j];
     }
     uint32_t o[2];
 #pragma unroll
@@ -85,12 +86,12 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const RowCode &c) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// Sum and maximum over the block, the same in every thread. `part`: two words for each wavefront.
-template <int WAVES>
+// Sum (SUM) and maximum over the block, the same in every thread. `part`: two words for each wavefront.
+template <int WAVES, bool SUM>
 __device__ __forceinline__ void block_sum_max(float &sum, uint32_t &most, uint2 *part) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        sum += __shfl_xor(sum, d);
+        if constexpr (SUM) sum += __shfl_xor(sum, d);
         const uint32_t other = __shfl_xor(most, d);
         most = most > other ? most : other;
     }
@@ -102,7 +103,7 @@ __device__ __forceinline__ void block_sum_max(float &sum, uint32_t &most, uint2 
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) {
             const uint2 v = part[i];
-            sum += __uint_as_float(v.x);
+            if constexpr (SUM) sum += __uint_as_float(v.x);
             most = most > v.y ? most : v.y;
         }
     }
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
             most = max(most, max(abs_bits(a), abs_bits(b)));
         }
     }
-    block_sum_max<WAVES>(sum, most, part);
+    block_sum_max<WAVES, NORM>(sum, most, part);
     const RowCode code = row_code(most, NORM ? rsqrtf(sum / static_cast<float>(p.D) + p.eps) : 1.f);
     if (threadIdx.x == 0) p.scale[row] = code.scale;
     uint2 *q = reinterpret_cast<uint2 *>(p.q + row * p.ldq);
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
         if constexpr (NORM) a *= half_to_f32<DT>(w[i]);
         most = max(most, abs_bits(a));
     }
-    block_sum_max<4>(sum, most, part);
+    block_sum_max<4, NORM>(sum, most, part);
     const RowCode code = row_code(most, NORM ? rsqrtf(sum / static_cast<float>(p.D) + p.eps) : 1.f);
     if (threadIdx.x == 0) p.scale[row] = code.scale;
     for (int i = threadIdx.x; i < p.D; i += 256) {
