@@ -207,20 +207,26 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
     }
 }
 
-// Without the addition, rows of a large launch are held by fewer wavefronts with four chunks a lane: more of them are under way on a CU. 4096 rows: quantised 5504 17.2 -> 16.1 us, 16384 39.2 -> 35.3,
-// norms of 5504 19.8 -> 17.3, of 16384 45.6 -> 39.3, of 8192 23.0 -> 22.2; at 1024 rows of 4096 it takes 6.4 -> 8.1, and with the addition 13.8 -> 15.1 at 2103.
-constexpr int64_t MANY_ROWS = 2048;
+// Without the addition, rows of a large launch are held by fewer wavefronts with four chunks a lane: more rows are under way on a CU, and a row's meeting costs less. Quantised / normed, us:
+// 2103 x 4096 9.6 -> 9.0 / 10.9 -> 9.5, 4096 x 5504 16.4 -> 15.0 / 19.0 -> 16.3, 4096 x 16384 36.1 -> 34.1 / 42.4 -> 37.1, 1024 x 11008 10.9 -> 9.9 / 12.3 -> 11.0; smaller ones lose, 1024 x 4096
+// 6.1 -> 6.9, 2048 x 2048 6.0 -> 6.7, and with the addition 4096 x 8192 37.6 -> 38.7.
+constexpr int64_t MANY_VALUES = 1 << 23;
 
 template <int DT, bool NORM, bool ADD>
 void launch_rows(const QuantParams &p, int64_t rows, bool vec, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(rows));
     const int n = p.D / 8;  // 16-byte chunks per row
+    if constexpr (!ADD) {
+        if (vec && n > 64 && rows * p.D > MANY_VALUES) {
+            if (n <= 256) hipLaunchKernelGGL((quantize_kernel<DT, 1, 4, NORM, ADD>), grid, dim3(64), 0, s, p);
+            else if (n <= 512) hipLaunchKernelGGL((quantize_kernel<DT, 2, 4, NORM, ADD>), grid, dim3(128), 0, s, p);
+            else if (n <= 1024) hipLaunchKernelGGL((quantize_kernel<DT, 4, 4, NORM, ADD>), grid, dim3(256), 0, s, p);
+            else hipLaunchKernelGGL((quantize_kernel<DT, 8, 4, NORM, ADD>), grid, dim3(512), 0, s, p);
+            return;
+        }
+    }
     if (!vec) hipLaunchKernelGGL((quantize_any_kernel<DT, NORM, ADD>), grid, dim3(256), 0, s, p);
     else if (n <= 64) hipLaunchKernelGGL((quantize_kernel<DT, 1, 1, NORM, ADD>), grid, dim3(64), 0, s, p);
-    else if (!ADD && rows >= MANY_ROWS && n <= 256) hipLaunchKernelGGL((quantize_kernel<DT, 1, 4, NORM, ADD>), grid, dim3(64), 0, s, p);
-    else if (!ADD && rows >= MANY_ROWS && n <= 512) hipLaunchKernelGGL((quantize_kernel<DT, 2, 4, NORM, ADD>), grid, dim3(128), 0, s, p);
-    else if (!ADD && rows >= MANY_ROWS && n <= 1024) hipLaunchKernelGGL((quantize_kernel<DT, 4, 4, NORM, ADD>), grid, dim3(256), 0, s, p);
-    else if (!ADD && rows >= MANY_ROWS) hipLaunchKernelGGL((quantize_kernel<DT, 8, 4, NORM, ADD>), grid, dim3(512), 0, s, p);
     else if (n <= 256) hipLaunchKernelGGL((quantize_kernel<DT, 4, 1, NORM, ADD>), grid, dim3(256), 0, s, p);
     else if (n <= 512) hipLaunchKernelGGL((quantize_kernel<DT, 8, 1, NORM, ADD>), grid, dim3(512), 0, s, p);
     else if (n <= 1024) hipLaunchKernelGGL((quantize_kernel<DT, 8, 2, NORM, ADD>), grid, dim3(512), 0, s, p);
