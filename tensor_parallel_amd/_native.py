@@ -1267,7 +1267,7 @@ def quantize_rows(x: torch.Tensor) -> tuple:
     zeros, NaN (and codes of 0) for one with an infinity or NaN."""
     code, shape = _half_code(x, "quantize_rows"), x.shape
     x2, M, ldx = _flat_rows(x, shape)
-    q, scale_ = torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    q, scale_ = x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     D = shape[-1]
     _launch("tpamd_quantize_rows", lib().tpamd_quantize_rows, x.get_device(), x2.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, D or 1, code)
     return q, scale_
@@ -1284,7 +1284,7 @@ def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float) -> tuple:
     code, shape = _half_code(x, "rms_norm_q8"), x.shape
     w = _check_norm_weight(x, w, "rms_norm_q8")
     x2, M, ldx = _flat_rows(x, shape)
-    q, scale_ = torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    q, scale_ = x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     D = shape[-1]
     _launch("tpamd_rms_norm_q8", lib().tpamd_rms_norm_q8, x.get_device(), x2.data_ptr(), w.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, D or 1, eps, code)
     return q, scale_
@@ -1298,8 +1298,8 @@ def add_rms_norm_q8(r: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: floa
         raise ValueError(f"add_rms_norm_q8: r {tuple(r.shape)} {r.dtype} on {r.device} and x {tuple(shape)} {x.dtype} on {x.device} do not fit")
     x2, M, ldx = _flat_rows(x, shape)
     r2, _, ldr = _flat_rows(r, shape)
-    total = torch.empty(shape, dtype=x.dtype, device=x.device)
-    q, scale_ = torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    total = x.new_empty(shape)
+    q, scale_ = x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     D = shape[-1]
     _launch("tpamd_add_rms_norm_q8", lib().tpamd_add_rms_norm_q8, x.get_device(), x2.data_ptr(), r2.data_ptr(), w.data_ptr(), total.data_ptr(), q.data_ptr(), scale_.data_ptr(),
             M, D, ldx, ldr, D or 1, D or 1, eps, code)
@@ -1320,11 +1320,12 @@ def dequantize_rows(q: torch.Tensor, scale_: torch.Tensor, dtype: torch.dtype) -
     if not q.is_cuda:
         require_device(q, "dequantize_rows")
     shape = _check_codes(q, scale_, "dequantize_rows")
-    y = torch.empty(shape, dtype=dtype, device=q.device)
+    y = q.new_empty(shape, dtype=dtype)
+    scale_ = scale_ if scale_.is_contiguous() else scale_.contiguous()
     q2, M, ldq = _flat_rows(q, shape)
     D = shape[-1]
-    _launch("tpamd_dequantize_rows", lib().tpamd_dequantize_rows, q.get_device(), q2.data_ptr(), (scale_ if scale_.is_contiguous() else scale_.contiguous()).data_ptr(), y.data_ptr(),
-            M, D, ldq, D or 1, dtype_code(dtype))
+    _launch("tpamd_dequantize_rows", lib().tpamd_dequantize_rows, q.get_device(), q2.data_ptr(), scale_.data_ptr(), y.data_ptr(), M, D, ldq, D or 1,
+            dtype_code(dtype))
     return y
 
 
@@ -1362,7 +1363,7 @@ def linear_a8(q: torch.Tensor, scale_: torch.Tensor, wq: torch.Tensor, wscale: t
         raise ValueError("linear_a8: addend must have the shape, dtype and device of the result")
     if copy is not None and (addend is None or copy.dtype is not dtype or copy.get_device() != index or copy.shape != out_shape or not copy.is_contiguous()):
         raise ValueError("linear_a8: copy goes with an addend and must be a contiguous tensor of the result's shape, dtype and device")
-    y = torch.empty(out_shape, dtype=dtype, device=q.device)
+    y = q.new_empty(out_shape, dtype=dtype)
     if addend is None:
         _launch("tpamd_linear_a8", lib().tpamd_linear_a8, index, q2.data_ptr(), s2.data_ptr(), w2.data_ptr(), ws.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
                 M, N, K, ldx, ldw, N, code, act)
@@ -1384,7 +1385,7 @@ def swiglu_up_a8(q: torch.Tensor, scale_: torch.Tensor, gate: torch.Tensor, gsca
         raise ValueError(f"swiglu_up_a8: {N} gate columns and {Nu} up columns")
     if ldg != ldu:
         g2, u2, ldg = g2.contiguous(), u2.contiguous(), K or 1
-    h = torch.empty((*shape[:-1], N), dtype=dtype, device=q.device)
+    h = q.new_empty((*shape[:-1], N), dtype=dtype)
     _launch("tpamd_swiglu_up_a8", lib().tpamd_swiglu_up_a8, index, q2.data_ptr(), s2.data_ptr(), g2.data_ptr(), gs.data_ptr(), u2.data_ptr(), us.data_ptr(), h.data_ptr(),
             M, N, K, ldx, ldg, N, code)
     return h
