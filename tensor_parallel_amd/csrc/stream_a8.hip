@@ -54,6 +54,9 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
     const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + static_cast<int64_t>(n0) * ldw, w_extent);
     const __amdgpu_buffer_rsrc_t w2_rsrc = PAIR ? make_rsrc(p.w2 + static_cast<int64_t>(n0) * ldw, w_extent) : w_rsrc;
     const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(p.x, static_cast<uint32_t>(p.M - 1) * ldx + static_cast<uint32_t>(p.K));
+    // Weights pass the caches by, unless rows begin inside 128-byte lines: the next unit then asks for the rest of a line (the pair of 8 x 5504 x 4112 15.4 -> 13.6 us, 16 x 16384 x 8208
+    // 40.7 -> 34.4; whole lines kept in the caches cost 16 x 16384 x 8192 26.4 -> 28.9)
+    const bool whole_lines = ((reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.w2) | static_cast<uintptr_t>(p.ldw)) & 127) == 0;
     char *ring = smem + wave * RING;
     auto load = [&](int stage_off, int i) __attribute__((always_inline)) {  // unit number i of this wavefront; behind the last one the same count of loads from outside the descriptors
         const int t = i < units ? skew + i : 0;  // (the wavefront-uniform offset stays inside the extents)
@@ -61,7 +64,11 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
         const uint32_t none = i < units ? 0u : 0x80000000u;
         unrolled<NB>([&](auto jc) {
             constexpr int j = decltype(jc)::value;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(PAIR && j >= NB / 2 ? w2_rsrc : w_rsrc, (lds_void *)(ring + stage_off + j * 1024), 16, static_cast<int>(w_off[j] | none), u * PITCH, 0, 2);
+            const __amdgpu_buffer_rsrc_t rsrc = PAIR && j >= NB / 2 ? w2_rsrc : w_rsrc;
+            lds_void *to = (lds_void *)(ring + stage_off + j * 1024);
+            const int at = static_cast<int>(w_off[j] | none);
+            if (whole_lines) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 16, at, u * PITCH, 0, 2);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 16, at, u * PITCH, 0, 0);
         });
         unrolled<XB>([&](auto jc) {
             constexpr int j = decltype(jc)::value;
