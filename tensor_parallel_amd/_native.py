@@ -1262,14 +1262,24 @@ def _half_code(x: torch.Tensor, what: str) -> int:
     return code
 
 
+def _new_codes(x: torch.Tensor, shape: torch.Size, M: int, D: int) -> tuple:
+    """Codes of M rows of x's shape, their scales, and the elements between rows: those of tiled products (more than 64 rows) begin on 128-byte boundaries (2048 x 4096 x 2752 31.7 us, in lines 28.9;
+    fewer rows stay in the L2, where it makes a difference of 0.5)."""
+    scale_ = x.new_empty(shape[:-1], dtype=torch.float32)
+    if M <= 64 or D % 128 == 0 or D % 16 != 0:
+        return x.new_empty(shape, dtype=torch.int8), scale_, D or 1
+    ld = (D + 127) // 128 * 128
+    return x.new_empty((*shape[:-1], ld), dtype=torch.int8).narrow(-1, 0, D), scale_, ld
+
+
 def quantize_rows(x: torch.Tensor) -> tuple:
     """(codes int8, scale fp32 [...]) of the rows of x: code = the integer nearest to 127 x / max |x| of the row (ties to even), scale = max |x| / 127; 1 for a row of
     zeros, NaN (and codes of 0) for one with an infinity or NaN."""
     code, shape = _half_code(x, "quantize_rows"), x.shape
     x2, M, ldx = _flat_rows(x, shape)
-    q, scale_ = x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     D = shape[-1]
-    _launch("tpamd_quantize_rows", lib().tpamd_quantize_rows, x.get_device(), x2.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, D or 1, code)
+    q, scale_, ldq = _new_codes(x, shape, M, D)
+    _launch("tpamd_quantize_rows", lib().tpamd_quantize_rows, x.get_device(), x2.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, ldq, code)
     return q, scale_
 
 
@@ -1284,9 +1294,9 @@ def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float) -> tuple:
     code, shape = _half_code(x, "rms_norm_q8"), x.shape
     w = _check_norm_weight(x, w, "rms_norm_q8")
     x2, M, ldx = _flat_rows(x, shape)
-    q, scale_ = x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     D = shape[-1]
-    _launch("tpamd_rms_norm_q8", lib().tpamd_rms_norm_q8, x.get_device(), x2.data_ptr(), w.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, D or 1, eps, code)
+    q, scale_, ldq = _new_codes(x, shape, M, D)
+    _launch("tpamd_rms_norm_q8", lib().tpamd_rms_norm_q8, x.get_device(), x2.data_ptr(), w.data_ptr(), q.data_ptr(), scale_.data_ptr(), M, D, ldx, ldq, eps, code)
     return q, scale_
 
 
@@ -1299,10 +1309,10 @@ def add_rms_norm_q8(r: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: floa
     x2, M, ldx = _flat_rows(x, shape)
     r2, _, ldr = _flat_rows(r, shape)
     total = x.new_empty(shape)
-    q, scale_ = x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32)
     D = shape[-1]
+    q, scale_, ldq = _new_codes(x, shape, M, D)
     _launch("tpamd_add_rms_norm_q8", lib().tpamd_add_rms_norm_q8, x.get_device(), x2.data_ptr(), r2.data_ptr(), w.data_ptr(), total.data_ptr(), q.data_ptr(), scale_.data_ptr(),
-            M, D, ldx, ldr, D or 1, D or 1, eps, code)
+            M, D, ldx, ldr, D or 1, ldq, eps, code)
     return total, q, scale_
 
 

@@ -1,5 +1,8 @@
 """Linears of 8-bit rows as modules: `ShardLinearA8` and a run of the operators against their definition in 64 bits, a tensor-parallel Llama and a Falcon whose Linears were replaced by
 `quantize_linears_(..., activations=True)`, and which of their forwards take rows from the norms' launches."""
+import copy
+import pickle
+
 import pytest
 import torch
 from torch import nn
@@ -46,6 +49,27 @@ def test_module_matches_the_definition(dtype, M, N, K, bias):
         mod(x.float())
     with pytest.raises(NotImplementedError):
         mod(x.clone().requires_grad_()).sum().backward()
+
+
+def test_rows_in_lines():
+    """Rows of a multiple of 16 codes that is none of 128 begin on 128-byte boundaries, in modules and in the codes of many rows; what stands between them is nowhere in results or saved weights."""
+    torch.manual_seed(3)
+    weight, x = torch.randn(130, 1376, device=DEV).bfloat16(), torch.randn(3, 50, 1376, device=DEV).bfloat16()
+    mod = ShardLinearA8.from_weight(weight)
+    assert mod.wq.shape == (130, 1376) and mod.wq.stride() == (1408, 1) and mod.wq.data_ptr() % 128 == 0
+    rows, few = int8.quantize_activations(x), int8.quantize_activations(x[0])
+    assert rows.codes.shape == x.shape and rows.codes.stride() == (50 * 1408, 1408, 1) and few.codes.is_contiguous()
+    want = mod(x)
+    wq, scale, *_ = quantize_rows(weight)
+    assert torch.equal(want, int8.linear(QuantizedRows(rows.codes.contiguous(), rows.scale, x.dtype), wq, scale))
+    assert torch.equal(want[0], mod(few)) and torch.equal(rows.dequantize()[0], few.dequantize())
+    saved = mod.state_dict()
+    assert torch.equal(saved["wq"], wq) and all(t.is_contiguous() for t in saved.values())
+    for other in (copy.deepcopy(mod), pickle.loads(pickle.dumps(mod))):
+        assert other.wq.stride() == (1408, 1) and torch.equal(other(x), want)
+    other = ShardLinearA8.from_weight(torch.randn_like(weight))
+    other.load_state_dict(saved)
+    assert other.wq.stride() == (1408, 1) and torch.equal(other(x), want)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
