@@ -544,7 +544,9 @@ def is_gated_silu_a8_mlp(module: nn.Module) -> bool:
 
 
 def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
-    """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch."""
+    """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch; its own forward where gate or up was replaced or is watched since."""
+    if not _has_a8(self, ("gate_proj", "up_proj")):
+        return type(self).forward(self, x if isinstance(x, torch.Tensor) else x.dequantize())
     gate, up, down = self.gate_proj, self.up_proj, self.down_proj
     return down(int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))
 

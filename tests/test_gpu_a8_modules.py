@@ -257,3 +257,33 @@ def test_layers_that_stay():
         ShardLinearA8.from_weight(torch.zeros(4, 131072, dtype=torch.float16, device=DEV))
     rows = QuantizedRows(torch.zeros(2, 3, 8, dtype=torch.int8, device=DEV), torch.ones(2, 3, device=DEV), torch.float16)
     assert rows.shape == (2, 3, 8) and rows.dim() == 3 and rows.device == DEV
+
+
+def test_a_fused_block_whose_parts_change():
+    """Once gate and up are one launch: a hook on one of them is told again, a Linear put in its place is called, and the launch comes back when both are as they were."""
+    class Mlp(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate_proj, self.up_proj, self.down_proj, self.act_fn = nn.Linear(64, 96, bias=False), nn.Linear(64, 96, bias=False), nn.Linear(96, 64, bias=False), nn.SiLU()
+
+        def forward(self, x):
+            return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+    torch.manual_seed(0)
+    mlp = Mlp().to(DEV, torch.bfloat16)
+    x = torch.randn(5, 64, device=DEV).bfloat16()
+    with torch.no_grad():
+        quantize_linears_(mlp, activations=True)
+        mlp(x)
+        assert mlp.forward.__func__ is shard_modules._gated_mlp_a8_forward
+        want, told = mlp(x), []
+        handle = mlp.up_proj.register_forward_hook(lambda mod, args, out: told.append(out.shape))
+        near(mlp(x), want)
+        assert told == [(5, 96)]
+        near(mlp(int8.quantize_activations(x)), want)
+        handle.remove()
+        kept, mlp.gate_proj = mlp.gate_proj, nn.Linear(64, 96, bias=False).to(DEV, torch.bfloat16)
+        nn.init.zeros_(mlp.gate_proj.weight)
+        assert bool((mlp(x) == 0).all())
+        mlp.gate_proj = kept
+        assert torch.equal(mlp(x), want)
