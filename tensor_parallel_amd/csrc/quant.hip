@@ -147,7 +147,8 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
             if (i < n) s[i] = v[c];
         }
     }
-    float f[CH][8], sum = 0.f;
+    float f[CH][8], sum = 0.f, zero = -0.f;
+    asm("" : "+v"(zero));  // products by fused operations that take their factors from 16 bits (fp16), instead of two conversions and a multiplication
     uint32_t most = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -158,8 +159,8 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
             float a = lo_half_to_f32<DT>(u[j]), b = hi_half_to_f32<DT>(u[j]);
             if constexpr (NORM) {
                 sum = fmaf(a, a, fmaf(b, b, sum));
-                a *= lo_half_to_f32<DT>(g[j]);
-                b *= hi_half_to_f32<DT>(g[j]);
+                a = fmaf(a, lo_half_to_f32<DT>(g[j]), zero);
+                b = fmaf(b, hi_half_to_f32<DT>(g[j]), zero);
             }
             f[c][2 * j] = a;
             f[c][2 * j + 1] = b;
