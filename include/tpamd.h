@@ -15,8 +15,8 @@
  *   - every entry point may be called concurrently from several host threads. Besides the thread-local error
  *     message the library keeps one piece of state: tpamd_linear / tpamd_linear_add / tpamd_swiglu_up split K for
  *     shapes with few output tiles (M from 17 to a few thousand, decided by a cost model), tpamd_linear_w8 does so
- *     from 2 rows on large matrices, tpamd_attention splits long key ranges, and they keep fp32 scratch buffers for
- *     the partial results: one per (device, stream), 68 MiB on a 256-CU part, allocated with hipMalloc at the
+ *     from 2 rows on large matrices, products of 8-bit rows from a few dozen, tpamd_attention splits long key ranges, and they keep
+ *     scratch buffers for the partial results: one per (device, stream), 68 MiB on a 256-CU part, allocated with hipMalloc at the
  *     stream's first such call and kept until the process ends (at most 32 streams per device get one; calls on
  *     further streams run unsplit). Streams never share a buffer, so such calls on different streams of a device
  *     need no ordering among themselves. Nothing can be allocated while a stream is being captured: the first
@@ -443,7 +443,8 @@ int tpamd_add_rms_norm_q8(const void *x_dev, const void *r_dev, const void *w_de
 
 /* Shard Linears of 8-bit rows: y[m,n] = act(xscale[m] * wscale[n] * sum_k x[m,k] * w[n,k] + bias[n]), x int8 [M,K], w int8 [N,K], scales fp32, y and bias in `dtype` (BF16 or
  * F16). The sum is exact in int32 (K up to 131071, TPAMD_ERR_UNSUPPORTED beyond), so results do not depend on how it is taken; everything behind it in fp32, rounded
- * once. Any shape, pitch and alignment is accepted. */
+ * once. Any pitch and alignment, and shapes of fewer than 2^24 tiles (of 64 x 64 outputs at the smallest); K a multiple of 16 and rows of x and w on 16-byte boundaries run on the matrix pipe,
+ * rows on 128-byte boundaries fastest. A call may split K, its partial sums in the stream's scratch buffer. */
 int tpamd_linear_a8(const void *x_dev, const void *xscale_dev, const void *w_dev, const void *wscale_dev, const void *bias_dev, void *y_dev, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t ldy, int dtype, int act, void *stream);
 /* Followed by one step of the partial-sum reduction, y = round_dtype(round_dtype(...) + addend), as tpamd_linear_add; with copy_dev (may be NULL) every result is stored there

@@ -97,6 +97,10 @@ __device__ __forceinline__ void lds_write_acc(uint32_t addr, i32x4 v) {
 // barrier: tile g + 1 has landed, tile g is read out; the loads of tile g + NS go into its stage in the rest of that step and the first of the next tile.
 // K ends in a multiple of 16: in the last stage the pieces of x behind it are asked for outside the descriptor's range, which gives zeros, and what stands in those of w
 // (the next row, or the bytes between rows) counts for nothing.
+// Bound: by the power that the matrix pipe takes on real codes: a K tile of a 256 x 256 tile takes 1.6 us with every CU at it (2.7 POP/s), 1.06 on zeros. 4096 x 4096 x 5504 in 82 us (2.25 POP/s; 93
+// with an addend that comes from memory, whose 34 MB and the outputs' are moved when all blocks end at once), 4096 x 16384 x 8192 in 445 (2.47), the pair of 4096 x 5504 x 4096 in 165 (2.24).
+// Smaller tiles by what LDS and the L2 deliver: 645 x 6144 x 4096 on 128 x 192 tiles, one to a CU, 24 us, 28 on weights from memory; a fourth or fifth stage changes nothing. Rows that begin
+// inside 128-byte lines cost a fifth more (each of their lines is asked for in two K tiles).
 // SPLIT: a block has one of t.splits ranges of K; its sums go to t.ws as they lie in the registers and are added by finish_a8_kernel.
 constexpr int a8_slab_rows(int tm, int tn) { return tm == 3 && tn == 4 ? 1 : tm == 4 ? 2 : tm; }  // MFMA tiles of rows
 constexpr int a8_lds(int tm, int tn, int ns) {
@@ -270,7 +274,8 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
 
     const int m_wave = m0 + wm * TM * 32, n_wave = n0 + wn * TN * CB;
     const bool with_addend = MODE == MODE_LINEAR && p.addend != nullptr;
-    // ---- epilogue from the registers, 32 rows at a time: two lanes exchange halves of groups of 8 columns, and a store has 32 bytes of 32 rows, which the L2 puts together
+    // ---- epilogue from the registers, 32 rows at a time: two lanes exchange halves of groups of 8 columns, and a store has 32 bytes of 32 rows, which the L2 puts together.
+    // A 256 x 256 tile takes 11000 cycles with it, 25000 with the loop over LDS below
     if (t.direct) {
         constexpr int CHUNKS = CB / 16;  // groups of 8 outputs that a lane has of an MFMA tile
         float4 sw[TN][4];

@@ -9,7 +9,9 @@
 // compared with the half exactly; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
 // A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
 //
-// Bound: at a few rows by the latency of a launch, else by HBM (x, r read once; sum and codes written once).
+// Bound: at a few rows by the latency of a launch (2.4-2.8 us in a graph, 1 x 4096), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
+// once, by the instructions between their loads and their stores: 2103 x 4096 quantised in 9.0 us (2.9 TB/s), normed 9.5, 4096 x 8192 19.1 (5.3 TB/s) and 20.7, with the addition 37.5 (6.3 TB/s);
+// the way back of 4096 x 8192 to fp32 27.7 (6.0 TB/s).
 #include "common.h"
 
 namespace tpamd {

@@ -1,4 +1,4 @@
-"""int8 weight-only shard Linears with outlier columns kept in 16 bits, from the Python layer.
+"""int8 shard Linears from the Python layer: weight-only with outlier columns kept in 16 bits, or of rows in 8 bits.
 
 The reference has no int8 code of its own: its users quantise the wrapped model with a third-party library before or
 after `tp.tensor_parallel` (README of the reference, LLM.int8 notebooks). This module is that step for the shards of this
