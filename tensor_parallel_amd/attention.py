@@ -173,6 +173,49 @@ def _share_qkv_storage(module: torch.nn.Module) -> bool:
     return True
 
 
+def share_qkv_a8(module: torch.nn.Module) -> bool:
+    """The same of Linears of 8-bit rows, where a module has them as q_proj, k_proj and v_proj: each one's codes and scales (and biases) become views of one matrix's rows."""
+    from .shard_modules import _has_a8
+
+    if not _has_a8(module, ("q_proj", "k_proj", "v_proj")):
+        return False
+    parts = [module._modules[name] for name in ("q_proj", "k_proj", "v_proj")]
+    first = parts[0]
+    if any(p.in_features != first.in_features or p.dtype != first.dtype or p.wq.device != first.wq.device or (p.bias is None) != (first.bias is None) for p in parts):
+        return False
+    rows = sum(p.out_features for p in parts)
+    whole = (first.wq.new_zeros((rows, first.wq.stride(0)))[:, :first.in_features], torch.cat([p.scale for p in parts]),
+             None if first.bias is None else torch.cat([p.bias for p in parts]))
+    row = 0
+    for p in parts:
+        end = row + p.out_features
+        whole[0][row:end] = p.wq
+        p.wq, p.scale = whole[0][row:end], whole[1][row:end]
+        if p.bias is not None:
+            p.bias = whole[2][row:end]
+        row = end
+    module.__dict__["_tp_qkv8"] = whole
+    return True
+
+
+def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
+    """The three Linears of `share_qkv_a8` in one launch; None (and never again) where one of them no longer is a view of the matrix."""
+    from .shard_modules import _guard
+
+    wq, scale, bias = self.__dict__["_tp_qkv8"]
+    row = 0
+    for name in ("q_proj", "k_proj", "v_proj"):
+        part = self._modules[name]
+        if (part.wq.data_ptr() != wq.data_ptr() + row * wq.stride(0) or part.wq.stride() != wq.stride() or part.scale.data_ptr() != scale.data_ptr() + row * 4
+                or (None if part.bias is None else part.bias.data_ptr()) != (None if bias is None else bias.data_ptr() + row * bias.element_size())):
+            break
+        row += part.out_features
+    if row != wq.shape[0]:
+        del self.__dict__["_tp_qkv8"]
+        return None
+    return _guard(_native.linear_a8(rows.codes, rows.scale, wq, scale, bias, rows.dtype), rows.scale)
+
+
 def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     """q, k, v as [B, S, heads, D]: one call on the shared weight matrix when the three Linears still are views of it; Linears of 8-bit rows on rows that are
     quantised once."""
@@ -181,6 +224,10 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     B, S, _ = hidden_states.shape
     if _has_a8(self, ("q_proj", "k_proj", "v_proj")) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
         hidden_states = self.q_proj.rows_of(hidden_states)
+        if "_tp_qkv8" in self.__dict__:
+            qkv = _project_shared_a8(self, hidden_states)
+            if qkv is not None:
+                return [part.view(B, S, -1, D) for part in qkv.split([self._modules[name].out_features for name in ("q_proj", "k_proj", "v_proj")], -1)]
     shared = self.__dict__.get("_tp_qkv")
     if shared is not None:
         w, b = shared

@@ -33,6 +33,7 @@ from torch import nn
 
 from . import _native, together
 from . import shard_modules
+from .attention import share_qkv_a8
 from .shard_modules import _guard, is_conv1d, product_in_context
 
 OutlierChoice = Union[None, Mapping[str, Sequence[int]], Callable[[str, nn.Module], Optional[Sequence[int]]]]
@@ -259,7 +260,7 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
     Linear)` keeps a Linear as it is (an output head, say). Returns how many were replaced.
 
     `activations=True`: both operands in 8 bits (`ShardLinearA8`; no outlier columns). A SiLU-gated MLP block then quantises its input once for gate and up, which are one launch
-    (`swiglu_up`), a fused attention of the Llama pattern its input once for q, k and v, and a Llama decoder layer takes their inputs from the launches of its norms (`rms_norm`,
+    (`swiglu_up`), a fused attention of the Llama pattern its input once for q, k and v, which are one launch too, and a Llama decoder layer takes their inputs from the launches of its norms (`rms_norm`,
     `add_rms_norm`) where nothing watches the norms."""
     if activations and outlier_cols is not None:
         raise ValueError("quantize_linears_: with 8-bit activations there are no outlier columns")
@@ -284,6 +285,8 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
             fused = parent.__dict__.get("forward")
             if getattr(fused, "__func__", None) in (shard_modules._gated_mlp_forward, shard_modules._gated_mlp_first_forward):
                 del parent.forward
+        if activations:
+            share_qkv_a8(parent)
         if activations and shard_modules.is_gated_silu_a8_mlp(parent):
             parent.forward = types.MethodType(shard_modules._gated_mlp_a8_first_forward, parent)
     return replaced

@@ -287,3 +287,64 @@ def test_a_fused_block_whose_parts_change():
         assert bool((mlp(x) == 0).all())
         mlp.gate_proj = kept
         assert torch.equal(mlp(x), want)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_one_launch_for_q_k_and_v(bias, monkeypatch):
+    """Their codes and scales are views of one matrix, which a fused attention multiplies at once; where one of them is something else since, they are three launches again."""
+    from transformers import DynamicCache, LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    config = LlamaConfig(vocab_size=300, hidden_size=528, intermediate_size=768, num_hidden_layers=1, num_attention_heads=6, num_key_value_heads=2, head_dim=64, max_position_embeddings=256,
+                         attention_bias=bias)
+    model = LlamaForCausalLM(config).to(DEV, torch.bfloat16).eval()
+    model.config._attn_implementation = tp.attention.register()
+    shard_modules.install_shard_kernels(model)
+    tp.attention.fuse_rotary_(model)
+    attn = model.model.layers[0].self_attn
+    if bias:
+        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+            nn.init.normal_(attn._modules[name].bias)
+    weights = {name: attn._modules[name].weight.detach().clone() for name in ("q_proj", "k_proj", "v_proj")}
+    quantize_linears_(model, skip=not_the_head, activations=True)
+    whole = attn.__dict__["_tp_qkv8"]
+    assert whole[0].shape == (6 * 64 + 4 * 64, 528) and whole[0].stride() == (640, 1)
+    for name, w in weights.items():
+        wq, scale, *_ = quantize_rows(w)
+        part = attn._modules[name]
+        assert torch.equal(part.wq, wq) and torch.equal(part.scale, scale) and part.wq.untyped_storage().data_ptr() == whole[0].untyped_storage().data_ptr()
+        assert all(t.is_contiguous() for t in part.state_dict().values())
+    ids = torch.randint(2, 300, (2, 40), device=DEV)
+    launches = []
+    inner = _native.linear_a8
+    monkeypatch.setattr(_native, "linear_a8", lambda *a, **k: launches.append(a[2].shape[0]) or inner(*a, **k))  # q, k, v (q_proj has 384 rows, the others 128), o_proj, down_proj
+
+    def forward():
+        cache, outs = DynamicCache(), []
+        for part in (ids[:, :39], ids[:, 39:]):
+            launches.clear()
+            outs.append(model(input_ids=part, past_key_values=cache, use_cache=True).logits)
+        return outs
+
+    with torch.no_grad():
+        forward()
+        want = forward()
+        assert launches == [640, 528, 528]
+        told = []
+        handle = attn.k_proj.register_forward_hook(lambda mod, args, out: told.append(out.shape[-1]))
+        watched = forward()
+        assert launches.count(128) == 2 and told == [128, 128]
+        handle.remove()
+        forward()
+        assert launches == [640, 528, 528]
+        copied = copy.deepcopy(model)
+        attn.v_proj.scale = attn.v_proj.scale.clone()
+        apart = forward()
+        assert launches == [384, 128, 128, 528, 528] and "_tp_qkv8" not in attn.__dict__
+        launches.clear()
+        cache = DynamicCache()
+        again = [copied(input_ids=part, past_key_values=cache, use_cache=True).logits for part in (ids[:, :39], ids[:, 39:])]
+    # the same codes, scales and sums; the head and the attention are the same launches
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, apart, again))
+    for a, b in zip(want, watched):
+        near(b, a)
