@@ -456,6 +456,21 @@ int tpamd_linear_a8_add(const void *x_dev, const void *xscale_dev, const void *w
 int tpamd_swiglu_up_a8(const void *x_dev, const void *xscale_dev, const void *wg_dev, const void *gscale_dev, const void *wu_dev, const void *uscale_dev, void *h_dev, int64_t M,
                        int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int dtype, void *stream);
 
+/* Calls of several ranks' shards on one device, of one form (sizes, leading dimensions, dtype; all or none with a bias in a launch), two ranks in a launch where that is the faster way: products
+ * of up to 64 rows, rows of whole 16-byte pieces. w2, w2scale: the up projection of a gated pair, ignored by tpamd_linear_a8_ranks. */
+typedef struct {
+    const void *x, *xscale, *w, *wscale, *w2, *w2scale, *bias;
+    void *y;
+} tpamd_a8_rank;
+int tpamd_linear_a8_ranks(int n, const tpamd_a8_rank *ranks, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldy, int dtype, int act, void *stream);
+int tpamd_swiglu_up_a8_ranks(int n, const tpamd_a8_rank *ranks, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int dtype, void *stream);
+/* tpamd_quantize_rows (w NULL in every rank: ldr, ldsum and eps are ignored), tpamd_rms_norm_q8 (r NULL) or tpamd_add_rms_norm_q8. */
+typedef struct {
+    const void *x, *r, *w;
+    void *sum, *q, *scale;
+} tpamd_q8_rank;
+int tpamd_rows_q8_ranks(int n, const tpamd_q8_rank *ranks, int64_t rows, int64_t D, int64_t ldx, int64_t ldr, int64_t ldsum, int64_t ldq, float eps, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,6 +74,9 @@ EXPORTS = (
     "tpamd_linear_a8",
     "tpamd_linear_a8_add",
     "tpamd_swiglu_up_a8",
+    "tpamd_linear_a8_ranks",
+    "tpamd_swiglu_up_a8_ranks",
+    "tpamd_rows_q8_ranks",
 )
 
 ABI_VERSION = 6
@@ -121,6 +124,14 @@ class DecodeRank(ctypes.Structure):
 
 class W8Rank(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in ("x", "wq", "scale", "outlier_idx", "w_out", "bias", "y")]
+
+
+class A8Rank(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "xscale", "w", "wscale", "w2", "w2scale", "bias", "y")]
+
+
+class Q8Rank(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "r", "w", "sum", "q", "scale")]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -237,6 +248,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.tpamd_linear_a8_add.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, ci, ci, vp]
     lib.tpamd_swiglu_up_a8.restype = ci
     lib.tpamd_swiglu_up_a8.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, ci, vp]
+    lib.tpamd_linear_a8_ranks.restype = ci
+    lib.tpamd_linear_a8_ranks.argtypes = [ci, c.POINTER(A8Rank), i64, i64, i64, i64, i64, i64, ci, ci, vp]
+    lib.tpamd_swiglu_up_a8_ranks.restype = ci
+    lib.tpamd_swiglu_up_a8_ranks.argtypes = [ci, c.POINTER(A8Rank), i64, i64, i64, i64, i64, i64, ci, vp]
+    lib.tpamd_rows_q8_ranks.restype = ci
+    lib.tpamd_rows_q8_ranks.argtypes = [ci, c.POINTER(Q8Rank), i64, i64, i64, i64, i64, i64, c.c_float, ci, vp]
 
 
 def _load() -> None:
@@ -1399,3 +1416,94 @@ def swiglu_up_a8(q: torch.Tensor, scale_: torch.Tensor, gate: torch.Tensor, gsca
     _launch("tpamd_swiglu_up_a8", lib().tpamd_swiglu_up_a8, index, q2.data_ptr(), s2.data_ptr(), g2.data_ptr(), gs.data_ptr(), u2.data_ptr(), us.data_ptr(), h.data_ptr(),
             M, N, K, ldx, ldg, N, code)
     return h
+
+
+def _same_form(what: str, forms: list) -> None:
+    if any(form != forms[0] for form in forms):
+        raise ValueError(f"{what}: the ranks' calls are of different forms")
+
+
+def _q8_ranks(what: str, calls: list, eps: float) -> list:
+    """(total or None, codes, scale) of each rank's (x, r or None, w or None)."""
+    ranks, outs, keep, forms = (Q8Rank * len(calls))(), [], [], []
+    for rank, (x, r, w) in zip(ranks, calls):
+        code, shape = _half_code(x, what), x.shape
+        x2, M, ldx = _flat_rows(x, shape)
+        D, ldr, total = shape[-1], 0, None
+        if w is not None:
+            w = _check_norm_weight(x, w, what)
+            rank.w = w.data_ptr()
+        if r is not None:
+            if r.shape != shape or r.dtype is not x.dtype or r.get_device() != x.get_device():
+                raise ValueError(f"{what}: r {tuple(r.shape)} {r.dtype} on {r.device} and x {tuple(shape)} {x.dtype} on {x.device} do not fit")
+            r, _, ldr = _flat_rows(r, shape)
+            total = x.new_empty(shape)
+            rank.r, rank.sum = r.data_ptr(), total.data_ptr()
+        q, scale_, ldq = _new_codes(x, shape, M, D)
+        rank.x, rank.q, rank.scale = x2.data_ptr(), q.data_ptr(), scale_.data_ptr()
+        outs.append((total, q, scale_))
+        keep.append((x2, w, r))
+        forms.append((x.get_device(), M, D, ldx, ldr, D or 1, ldq, code, w is None, r is None))
+    _same_form(what, forms)
+    index, M, D, ldx, ldr, ldsum, ldq, code, *_ = forms[0]
+    _launch("tpamd_rows_q8_ranks", lib().tpamd_rows_q8_ranks, index, len(calls), ranks, M, D, ldx, ldr, ldsum, ldq, eps, code)
+    return outs
+
+
+def quantize_rows_ranks(calls: Sequence[tuple]) -> list:
+    """`quantize_rows(x)` for the operands of several ranks."""
+    return [out[1:] for out in _q8_ranks("quantize_rows", [(x, None, None) for x, in calls], 0.0)]
+
+
+def rms_norm_q8_ranks(calls: Sequence[tuple]) -> list:
+    """`rms_norm_q8(x, w, eps)` for the operands of several ranks (with one eps)."""
+    return [out[1:] for out in _q8_ranks("rms_norm_q8", [(x, None, w) for x, w, _ in calls], calls[0][2])]
+
+
+def add_rms_norm_q8_ranks(calls: Sequence[tuple]) -> list:
+    """`add_rms_norm_q8(r, x, w, eps)` for the operands of several ranks (with one eps)."""
+    return _q8_ranks("add_rms_norm_q8", [(x, r, w) for r, x, w, _ in calls], calls[0][3])
+
+
+def linear_a8_ranks(calls: Sequence[tuple]) -> list:
+    """`linear_a8(q, scale, wq, wscale, bias, dtype, act)` for the operands of several ranks."""
+    ranks, outs, keep, forms = (A8Rank * len(calls))(), [], [], []
+    for rank, (q, scale_, wq, wscale, bias, dtype, act) in zip(ranks, calls):
+        code, shape, s2, q2, M, ldx = _a8_rows("linear_a8", q, scale_, dtype)
+        K, index = shape[-1], q.get_device()
+        w2, ws, N, ldw = _a8_weight("linear_a8", wq, wscale, K, index)
+        if bias is not None:
+            if bias.shape != (N,) or bias.dtype is not dtype or bias.get_device() != index:
+                raise ValueError(f"linear_a8: bias must have shape [{N}] and {dtype} and live on {q.device}")
+            bias = bias.contiguous()
+            rank.bias = bias.data_ptr()
+        y = q.new_empty((*shape[:-1], N), dtype=dtype)
+        rank.x, rank.xscale, rank.w, rank.wscale, rank.y = q2.data_ptr(), s2.data_ptr(), w2.data_ptr(), ws.data_ptr(), y.data_ptr()
+        outs.append(y)
+        keep.append((q2, s2, w2, ws, bias))
+        forms.append((index, M, N, K, ldx, ldw, N, code, act))
+    _same_form("linear_a8", forms)
+    _launch("tpamd_linear_a8_ranks", lib().tpamd_linear_a8_ranks, forms[0][0], len(calls), ranks, *forms[0][1:])
+    return outs
+
+
+def swiglu_up_a8_ranks(calls: Sequence[tuple]) -> list:
+    """`swiglu_up_a8(q, scale, gate, gscale, up, uscale, dtype)` for the operands of several ranks."""
+    ranks, outs, keep, forms = (A8Rank * len(calls))(), [], [], []
+    for rank, (q, scale_, gate, gscale, up, uscale, dtype) in zip(ranks, calls):
+        code, shape, s2, q2, M, ldx = _a8_rows("swiglu_up_a8", q, scale_, dtype)
+        K, index = shape[-1], q.get_device()
+        g2, gs, N, ldg = _a8_weight("swiglu_up_a8", gate, gscale, K, index)
+        u2, us, Nu, ldu = _a8_weight("swiglu_up_a8", up, uscale, K, index)
+        if N != Nu:
+            raise ValueError(f"swiglu_up_a8: {N} gate columns and {Nu} up columns")
+        if ldg != ldu:
+            g2, u2, ldg = g2.contiguous(), u2.contiguous(), K or 1
+        h = q.new_empty((*shape[:-1], N), dtype=dtype)
+        rank.x, rank.xscale, rank.w, rank.wscale, rank.w2, rank.w2scale, rank.y = (t.data_ptr() for t in (q2, s2, g2, gs, u2, us, h))
+        outs.append(h)
+        keep.append((q2, s2, g2, gs, u2, us))
+        forms.append((index, M, N, K, ldx, ldg, N, code))
+    _same_form("swiglu_up_a8", forms)
+    _launch("tpamd_swiglu_up_a8_ranks", lib().tpamd_swiglu_up_a8_ranks, forms[0][0], len(calls), ranks, *forms[0][1:])
+    return outs

@@ -213,7 +213,7 @@ def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
     if row != wq.shape[0]:
         del self.__dict__["_tp_qkv8"]
         return None
-    return _guard(_native.linear_a8(rows.codes, rows.scale, wq, scale, bias, rows.dtype), rows.scale)
+    return _guard(together.linear_a8(rows.codes, rows.scale, wq, scale, bias, rows.dtype), rows.scale)
 
 
 def _project_qkv(self, hidden_states: torch.Tensor, D: int):

@@ -14,6 +14,7 @@ struct A8Params {
     int M, N, K;
     int64_t ldx, ldw, ldadd, ldy;      // elements
     int act;
+    struct { int64_t x, w, w2, sx, sw, sw2, bias, y; } to;  // byte distances to a second rank's operands
 };
 
 constexpr int64_t A8_MAX_K = 131071;   // 128 * 128 * K < 2^31
@@ -44,8 +45,8 @@ static inline bool a8_fast(const A8Params &p) {
 }
 // gemm_a8.hip: tiles of 64 * tm x-rows by 64 * tn w-rows (a pair: 32 * tn columns), K in at most `splits` ranges. stream_a8.hip: up to 64 rows on one block per CU. Operands of a8_fast.
 int gemm_a8(const A8Params &p, bool pair, int dtype, int tm, int tn, int splits, hipStream_t s);
-bool stream_a8_takes(const A8Params &p, bool pair, int cus);
+bool stream_a8_takes(const A8Params &p, bool pair, int ranks, int cus);
 float stream_a8_us(const A8Params &p, bool pair, int cus);  // predicted
-int stream_a8(const A8Params &p, bool pair, int dtype, int cus, hipStream_t s);
+int stream_a8(const A8Params &p, bool pair, int dtype, int ranks, int cus, hipStream_t s);  // ranks: 1, or 2 (no addend)
 
 }  // namespace tpamd

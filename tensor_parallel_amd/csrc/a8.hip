@@ -73,18 +73,25 @@ int launch_any(const A8Params &p, int dtype, hipStream_t s) {
     return TPAMD_OK;
 }
 
+// Whether operands of a8_fast go to the streaming kernel; else `tile` is the choice among tiles.
+bool a8_streams(const A8Params &p, bool pair, int cus, A8Choice *tile) {
+    const Tuning &t = tuning();
+    const bool stream = t.stream != 0 && t.a8_tile == TUNE_UNSET && stream_a8_takes(p, pair, 1, cus);
+    if (stream && t.stream == 1) return true;
+    *tile = a8_choose(pair, p.M, p.N, p.K, cus, static_cast<int64_t>(scratch_reserve(cus)));
+    // Tiles have to be predicted a sixth faster (the two models' errors at few rows): with that the choice is 1.2 % off the best of both in the geometric mean over 300 shapes of 1-64 rows, 1.0 % on
+    // 150 others (worst 38 %), streaming always 1.9 and 2.6 (16384 x 1376 at 45 rows 13.8 us streamed, 9.2 on tiles; 5504 x 8192 the other way round at 62 rows)
+    return stream && stream_a8_us(p, pair, cus) <= 1.2f * tile->us;
+}
+
 int a8_dispatch(const A8Params &p, bool pair, int dtype, hipStream_t s) {
     int dev = 0, cus = 256;
     TPAMD_HIP(hipGetDevice(&dev));
     if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
     if (a8_fast(p)) {
+        A8Choice tile{};
+        if (a8_streams(p, pair, cus, &tile)) return stream_a8(p, pair, dtype, 1, cus, s);
         const Tuning &t = tuning();
-        const bool stream = t.stream != 0 && t.a8_tile == TUNE_UNSET && stream_a8_takes(p, pair, cus);
-        if (stream && t.stream == 1) return stream_a8(p, pair, dtype, cus, s);
-        A8Choice tile = a8_choose(pair, p.M, p.N, p.K, cus, static_cast<int64_t>(scratch_reserve(cus)));
-        // Tiles have to be predicted a sixth faster (the two models' errors at few rows): with that the choice is 1.2 % off the best of both in the geometric mean over 300 shapes of 1-64 rows, 1.0 % on
-        // 150 others (worst 38 %), streaming always 1.9 and 2.6 (16384 x 1376 at 45 rows 13.8 us streamed, 9.2 on tiles; 5504 x 8192 the other way round at 62 rows)
-        if (stream && stream_a8_us(p, pair, cus) <= 1.2f * tile.us) return stream_a8(p, pair, dtype, cus, s);
         if (t.a8_tile != TUNE_UNSET) tile = {t.a8_tile / 1000 / 64, t.a8_tile % 1000 / 64, 1, 0.f};
         if (t.a8_splits != TUNE_UNSET) tile.ranges = t.a8_splits < 1 ? 1 : t.a8_splits;
         return gemm_a8(p, pair, dtype, tile.tm, tile.tn, tile.ranges, s);
@@ -125,6 +132,41 @@ int linear_a8(const char *who, const void *x, const void *sx, const void *w, con
     return a8_dispatch(p, false, dtype, static_cast<hipStream_t>(stream));
 }
 
+// Several ranks' products of one form, two in a launch where each by itself would stream and half the CUs hold a rank's columns; else one after another. 216 random shapes of 1-64 rows, time of one
+// launch for both in that of two: Linears 0.61, pairs 0.70, none above 1.01.
+int a8_ranks(const char *who, int n, const tpamd_a8_rank *ranks, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldy, bool pair, int dtype, int act, hipStream_t s) {
+    TPAMD_REQUIRE(n >= 0 && (n == 0 || ranks != nullptr), "%s: null pointer", who);
+    TPAMD_REQUIRE(act == TPAMD_ACT_NONE || act == TPAMD_ACT_GELU, "%s: unknown activation %d", who, act);
+    auto params = [&](const tpamd_a8_rank &r) {
+        A8Params p{};
+        p.x = static_cast<const char *>(r.x); p.w = static_cast<const char *>(r.w); p.w2 = pair ? static_cast<const char *>(r.w2) : nullptr;
+        p.sx = static_cast<const float *>(r.xscale); p.sw = static_cast<const float *>(r.wscale); p.sw2 = pair ? static_cast<const float *>(r.w2scale) : nullptr;
+        p.bias = pair ? nullptr : static_cast<const char *>(r.bias); p.y = static_cast<char *>(r.y);
+        p.ldx = ldx; p.ldw = ldw; p.ldy = ldy; p.act = act;
+        return p;
+    };
+    for (int i = 0; i < n; ++i)
+        if (int rc = a8_check(who, params(ranks[i]), M, N, K, pair, dtype); rc != TPAMD_OK) return rc;
+    if (M == 0 || N == 0) return TPAMD_OK;
+    int dev = 0, cus = 256;
+    TPAMD_HIP(hipGetDevice(&dev));
+    if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
+    for (int i = 0; i < n; ++i) {
+        A8Params p = params(ranks[i]), q = params(ranks[i + 1 < n ? i + 1 : i]);
+        p.M = q.M = static_cast<int>(M); p.N = q.N = static_cast<int>(N); p.K = q.K = static_cast<int>(K);
+        A8Choice tile{};
+        if (i + 1 < n && a8_fast(p) && a8_fast(q) && (p.bias == nullptr) == (q.bias == nullptr) && stream_a8_takes(p, pair, 2, cus) && a8_streams(p, pair, cus, &tile)) {
+            p.to = {bytes_from(p.x, q.x), bytes_from(p.w, q.w), bytes_from(p.w2, q.w2), bytes_from(p.sx, q.sx), bytes_from(p.sw, q.sw), bytes_from(p.sw2, q.sw2),
+                    bytes_from(p.bias, q.bias), bytes_from(p.y, q.y)};
+            if (int rc = stream_a8(p, pair, dtype, 2, cus, s); rc != TPAMD_OK) return rc;
+            ++i;
+        } else if (int rc = a8_dispatch(p, pair, dtype, s); rc != TPAMD_OK) {
+            return rc;
+        }
+    }
+    return TPAMD_OK;
+}
+
 }  // namespace
 }  // namespace tpamd
 
@@ -154,4 +196,12 @@ extern "C" int tpamd_swiglu_up_a8(const void *x_dev, const void *xscale_dev, con
     if (M == 0 || N == 0) return TPAMD_OK;
     p.M = static_cast<int>(M); p.N = static_cast<int>(N); p.K = static_cast<int>(K);
     return a8_dispatch(p, true, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int tpamd_linear_a8_ranks(int n, const tpamd_a8_rank *ranks, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldy, int dtype, int act, void *stream) {
+    return a8_ranks("tpamd_linear_a8_ranks", n, ranks, M, N, K, ldx, ldw, ldy, false, dtype, act, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int tpamd_swiglu_up_a8_ranks(int n, const tpamd_a8_rank *ranks, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int dtype, void *stream) {
+    return a8_ranks("tpamd_swiglu_up_a8_ranks", n, ranks, M, N, K, ldx, ldw, ldh, true, dtype, TPAMD_ACT_NONE, static_cast<hipStream_t>(stream));
 }

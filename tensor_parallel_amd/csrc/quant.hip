@@ -24,6 +24,7 @@ struct QuantParams {
     int64_t ldx, ldr, lds, ldq;  // elements between rows
     int D;
     float eps;
+    struct { int64_t x, w, r, s, q, scale; } to;  // blockIdx.y = 1: byte distances to a second rank's operands
 };
 
 // What a row has in common: its scale, 127 / a, and a (0: codes of 0).
@@ -116,6 +117,10 @@ template <int DT, int WAVES, int CH, bool NORM, bool ADD>
 __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
     constexpr int T = 64 * WAVES;
     __shared__ uint2 part[WAVES];
+    if (blockIdx.y != 0) {
+        p.x += p.to.x; p.w += p.to.w; p.r += p.to.r; p.s += p.to.s; p.q += p.to.q;
+        p.scale = reinterpret_cast<float *>(reinterpret_cast<char *>(p.scale) + p.to.scale);
+    }
     const int64_t row = blockIdx.x;
     const uint4 *x = reinterpret_cast<const uint4 *>(p.x + row * p.ldx * 2);
     const uint4 *w = reinterpret_cast<const uint4 *>(p.w);
@@ -216,8 +221,8 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
 constexpr int64_t MANY_VALUES = 1 << 23;
 
 template <int DT, bool NORM, bool ADD>
-void launch_rows(const QuantParams &p, int64_t rows, bool vec, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(rows));
+void launch_rows(const QuantParams &p, int64_t rows, int ranks, bool vec, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(ranks));
     const int n = p.D / 8;  // 16-byte chunks per row
     if constexpr (!ADD) {
         if (vec && n > 64 && rows * p.D > MANY_VALUES) {
@@ -240,9 +245,9 @@ void launch_rows(const QuantParams &p, int64_t rows, bool vec, hipStream_t s) {
 constexpr int64_t ROWS_PER_LAUNCH = 1ll << 20;
 
 template <int DT, bool NORM, bool ADD>
-int launch(QuantParams p, int64_t rows, bool vec, hipStream_t s) {
+int launch(QuantParams p, int64_t rows, int ranks, bool vec, hipStream_t s) {
     for (; rows > 0; rows -= ROWS_PER_LAUNCH) {
-        launch_rows<DT, NORM, ADD>(p, rows < ROWS_PER_LAUNCH ? rows : ROWS_PER_LAUNCH, vec, s);
+        launch_rows<DT, NORM, ADD>(p, rows < ROWS_PER_LAUNCH ? rows : ROWS_PER_LAUNCH, ranks, vec, s);
         TPAMD_HIP(hipGetLastError());
         p.x += ROWS_PER_LAUNCH * p.ldx * 2;
         p.q += ROWS_PER_LAUNCH * p.ldq;
@@ -256,7 +261,7 @@ int launch(QuantParams p, int64_t rows, bool vec, hipStream_t s) {
 }
 
 template <bool NORM, bool ADD>
-int quantize_entry(const char *who, const QuantParams &p, int64_t rows, int64_t D, int dtype, void *stream) {
+int quantize_check(const char *who, const QuantParams &p, int64_t rows, int64_t D, int dtype) {
     TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 31), "%s: dimension negative or over 2^31 (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
     TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16, "%s: rows of bfloat16 or float16 are quantised, not dtype %d", who, dtype);
     if (rows == 0) return TPAMD_OK;
@@ -265,10 +270,49 @@ int quantize_entry(const char *who, const QuantParams &p, int64_t rows, int64_t 
     TPAMD_REQUIRE(p.ldx >= D && p.ldq >= D && (!ADD || (p.ldr >= D && p.lds >= D)), "%s: leading dimension smaller than the row (ldx=%lld ldr=%lld lds=%lld ldq=%lld)", who,
                   (long long)p.ldx, (long long)p.ldr, (long long)p.lds, (long long)p.ldq);
     TPAMD_REQUIRE(aligned(p.x, 2) && aligned(p.w, 2) && aligned(p.r, 2) && aligned(p.s, 2) && aligned(p.scale, 4), "%s: a pointer is not aligned to its type", who);
-    const bool vec = D > 0 && D % 8 == 0 && D <= 16384 && aligned(p.x, 16) && p.ldx % 8 == 0 && aligned(p.q, 8) && p.ldq % 8 == 0 && (!NORM || aligned(p.w, 16)) &&
+    return TPAMD_OK;
+}
+
+// Rows for quantize_kernel.
+template <bool NORM, bool ADD>
+bool quantize_vec(const QuantParams &p, int64_t D) {
+    return D > 0 && D % 8 == 0 && D <= 16384 && aligned(p.x, 16) && p.ldx % 8 == 0 && aligned(p.q, 8) && p.ldq % 8 == 0 && (!NORM || aligned(p.w, 16)) &&
                      (!ADD || (aligned(p.r, 16) && p.ldr % 8 == 0 && aligned(p.s, 16) && p.lds % 8 == 0));
+}
+
+template <bool NORM, bool ADD>
+int quantize_entry(const char *who, const QuantParams &p, int64_t rows, int64_t D, int dtype, void *stream, int ranks = 1) {
+    if (int rc = quantize_check<NORM, ADD>(who, p, rows, D, dtype); rc != TPAMD_OK || rows == 0) return rc;
+    const bool vec = quantize_vec<NORM, ADD>(p, D);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return dtype == TPAMD_BF16 ? launch<TPAMD_BF16, NORM, ADD>(p, rows, vec, s) : launch<TPAMD_F16, NORM, ADD>(p, rows, vec, s);
+    return dtype == TPAMD_BF16 ? launch<TPAMD_BF16, NORM, ADD>(p, rows, ranks, vec, s) : launch<TPAMD_F16, NORM, ADD>(p, rows, ranks, vec, s);
+}
+
+// Several ranks' rows, two in a launch where quantize_kernel takes both.
+template <bool NORM, bool ADD>
+int quantize_ranks(const char *who, int n, const tpamd_q8_rank *ranks, const QuantParams &form, int64_t rows, int64_t D, int dtype, void *stream) {
+    auto params = [&](const tpamd_q8_rank &r) {
+        QuantParams p = form;
+        p.x = static_cast<const char *>(r.x); p.w = static_cast<const char *>(r.w); p.r = static_cast<const char *>(r.r);
+        p.s = static_cast<char *>(r.sum); p.q = static_cast<char *>(r.q); p.scale = static_cast<float *>(r.scale);
+        return p;
+    };
+    for (int i = 0; i < n; ++i)
+        if (int rc = quantize_check<NORM, ADD>(who, params(ranks[i]), rows, D, dtype); rc != TPAMD_OK) return rc;
+    for (int i = 0; i < n; ++i) {
+        QuantParams p = params(ranks[i]);
+        int together = 1;
+        if (i + 1 < n) {
+            const QuantParams q = params(ranks[i + 1]);
+            if (quantize_vec<NORM, ADD>(p, D) && quantize_vec<NORM, ADD>(q, D)) {
+                p.to = {bytes_from(p.x, q.x), bytes_from(p.w, q.w), bytes_from(p.r, q.r), bytes_from(p.s, q.s), bytes_from(p.q, q.q), bytes_from(p.scale, q.scale)};
+                together = 2;
+                ++i;
+            }
+        }
+        if (int rc = quantize_entry<NORM, ADD>(who, p, rows, D, dtype, stream, together); rc != TPAMD_OK) return rc;
+    }
+    return TPAMD_OK;
 }
 
 // A product as an fp32 value of its own: the compiler would otherwise make one instruction of it and its conversion to fp16, which rounds once where the packed conversion behind
@@ -359,6 +403,20 @@ extern "C" int tpamd_add_rms_norm_q8(const void *x_dev, const void *r_dev, const
     p.s = static_cast<char *>(sum_dev); p.q = static_cast<char *>(q_dev); p.scale = static_cast<float *>(scale_dev);
     p.ldx = ldx; p.ldr = ldr; p.lds = ldsum; p.ldq = ldq; p.D = static_cast<int>(D); p.eps = eps;
     return quantize_entry<true, true>("tpamd_add_rms_norm_q8", p, rows, D, dtype, stream);
+}
+
+extern "C" int tpamd_rows_q8_ranks(int n, const tpamd_q8_rank *ranks, int64_t rows, int64_t D, int64_t ldx, int64_t ldr, int64_t ldsum, int64_t ldq, float eps, int dtype, void *stream) {
+    const char *who = "tpamd_rows_q8_ranks";
+    TPAMD_REQUIRE(n >= 0 && (n == 0 || ranks != nullptr), "%s: null pointer", who);
+    if (n == 0) return TPAMD_OK;
+    for (int i = 1; i < n; ++i)
+        TPAMD_REQUIRE((ranks[i].w == nullptr) == (ranks[0].w == nullptr) && (ranks[i].r == nullptr) == (ranks[0].r == nullptr), "%s: ranks of different forms", who);
+    TPAMD_REQUIRE(ranks[0].w != nullptr || ranks[0].r == nullptr, "%s: an addition goes with a norm", who);
+    QuantParams p{};
+    p.ldx = ldx; p.ldr = ldr; p.lds = ldsum; p.ldq = ldq; p.D = static_cast<int>(D); p.eps = eps;
+    if (ranks[0].w == nullptr) return quantize_ranks<false, false>(who, n, ranks, p, rows, D, dtype, stream);
+    if (ranks[0].r == nullptr) return quantize_ranks<true, false>(who, n, ranks, p, rows, D, dtype, stream);
+    return quantize_ranks<true, true>(who, n, ranks, p, rows, D, dtype, stream);
 }
 
 extern "C" int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, void *y_dev, int64_t rows, int64_t D, int64_t ldq, int64_t ldy, int dtype, void *stream) {

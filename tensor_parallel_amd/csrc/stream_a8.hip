@@ -18,8 +18,11 @@ constexpr int SA_DEPTH = 4;     // most stages
 // The matrix pipe idles (a stage's MFMAs take 2-6 % of its time), so the half-rate 16 x 16 form serves, whose rows of 16 fit few columns a CU.
 // Bound: memory, N K bytes of weights: 16 x 16384 x 8192 in 26.0 us, 5.2 TB/s where a large copy has 6.0; at smaller matrices its latency: a launch and the first loads are 3.4 us of 6.1 for
 // 1 x 4096 x 5504 (22.5 MB), of 10.5 for the pair of 8 x 5504 x 4096 (45 MB). From 33 rows on x, which every CU reads whole from the L2: 64 x 4096 x 5504 12.8.
+// Two ranks' products are one launch with half the CUs each (blockIdx.y).
 // Slower, tried: weights straight into registers in the order of the matrix instructions (16 rows x 64 bytes a load: 37 us for the first), two blocks of half the LDS to a CU (26.4, all others
 // slower), eight stages, eight wavefronts.
+__device__ __forceinline__ const float *by_bytes(const float *p, int64_t bytes) { return reinterpret_cast<const float *>(reinterpret_cast<const char *>(p) + bytes); }
+
 template <int DT, bool PAIR, int NR, int XR, int D>
 __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
     constexpr int NT = (NR + 15) / 16, MT = (XR + 15) / 16, KK = 2;
@@ -32,6 +35,10 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
     constexpr int XLAST = XR - (MT - 1) * 16;  // staged rows of the last 16 of x: the lanes of the others read these again
     static_assert(NT * 16 * PITCH <= STAGE && NB * 1024 + ((MT - 1) * 16 + XLAST) * PITCH <= STAGE && (XLAST & (XLAST - 1)) == 0, "fragments are read inside their stage");
     extern __shared__ __align__(16) char smem[];
+    if (blockIdx.y != 0) {
+        p.x += p.to.x; p.w += p.to.w; p.w2 += p.to.w2; p.bias += p.to.bias; p.y += p.to.y;
+        p.sx = by_bytes(p.sx, p.to.sx); p.sw = by_bytes(p.sw, p.to.sw); p.sw2 = by_bytes(p.sw2, p.to.sw2);
+    }
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lq = lane >> 4, rb = lane >> 3;
@@ -153,7 +160,7 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
 }
 
 template <int DT, bool PAIR, int NR, int XR>
-int launch_nr(const A8Params &p, int blocks, hipStream_t s) {
+int launch_nr(const A8Params &p, int blocks, int ranks, hipStream_t s) {
     constexpr int L = (NR + XR) / 8, DM = SA_LDS_KB / SA_NW / L, D = DM < SA_DEPTH ? DM : SA_DEPTH;
     static_assert(D >= 2, "LDS");
     constexpr int LDS = SA_NW * D * L * 1024;
@@ -165,14 +172,14 @@ int launch_nr(const A8Params &p, int blocks, hipStream_t s) {
         TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
         configured_dev = dev;
     }
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(SA_NW * 64), LDS, s, p);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(ranks)), dim3(SA_NW * 64), LDS, s, p);
     TPAMD_HIP(hipGetLastError());
     return TPAMD_OK;
 }
 
 template <int DT, bool PAIR, int XR>
-int launch_xr(const A8Params &p, int nr, int blocks, hipStream_t s) {
-#define SA_ROWS(n) case n: return launch_nr<DT, PAIR, n, XR>(p, blocks, s)
+int launch_xr(const A8Params &p, int nr, int blocks, int ranks, hipStream_t s) {
+#define SA_ROWS(n) case n: return launch_nr<DT, PAIR, n, XR>(p, blocks, ranks, s)
     switch (nr) {
         SA_ROWS(32);
         SA_ROWS(48);
@@ -192,18 +199,18 @@ int launch_xr(const A8Params &p, int nr, int blocks, hipStream_t s) {
 }
 
 template <int DT, bool PAIR>
-int launch_m(const A8Params &p, int nr, int blocks, hipStream_t s) {
-    if (p.M <= 8) return launch_xr<DT, PAIR, 8>(p, nr, blocks, s);
-    if (p.M <= 16) return launch_xr<DT, PAIR, 16>(p, nr, blocks, s);
-    if (p.M <= 24) return launch_xr<DT, PAIR, 24>(p, nr, blocks, s);
-    if (p.M <= 32) return launch_xr<DT, PAIR, 32>(p, nr, blocks, s);
-    if (p.M <= 48) return launch_xr<DT, PAIR, 48>(p, nr, blocks, s);
-    return launch_xr<DT, PAIR, 64>(p, nr, blocks, s);
+int launch_m(const A8Params &p, int nr, int blocks, int ranks, hipStream_t s) {
+    if (p.M <= 8) return launch_xr<DT, PAIR, 8>(p, nr, blocks, ranks, s);
+    if (p.M <= 16) return launch_xr<DT, PAIR, 16>(p, nr, blocks, ranks, s);
+    if (p.M <= 24) return launch_xr<DT, PAIR, 24>(p, nr, blocks, ranks, s);
+    if (p.M <= 32) return launch_xr<DT, PAIR, 32>(p, nr, blocks, ranks, s);
+    if (p.M <= 48) return launch_xr<DT, PAIR, 48>(p, nr, blocks, ranks, s);
+    return launch_xr<DT, PAIR, 64>(p, nr, blocks, ranks, s);
 }
 
 }  // namespace
 
-bool stream_a8_takes(const A8Params &p, bool pair, int cus) { return p.M <= 64 && stream_cut(p.N, 1, pair, false, cus).groups > 0; }
+bool stream_a8_takes(const A8Params &p, bool pair, int ranks, int cus) { return p.M <= 64 && stream_cut(p.N, ranks, pair, false, cus).groups > 0; }
 
 // Fitted to 300 shapes of 1-64 rows (within 8 % of them in the mean, and of 150 others): each turn of the blocks costs 3.4 us, what it stages of weight rows (padded ones too) 0.010 us per KB,
 // of x 0.012, what it reads of memory 0.028 with every CU at it, and a thousand outputs 1.6.
@@ -216,11 +223,11 @@ float stream_a8_us(const A8Params &p, bool pair, int cus) {
            (3.37f + k * (0.0101f * static_cast<float>(cut.rows) + 0.0118f * static_cast<float>(xr) + 0.028f * columns * busy) + 1.62e-3f * columns * static_cast<float>(p.M));
 }
 
-int stream_a8(const A8Params &p, bool pair, int dtype, int cus, hipStream_t s) {
-    const StreamCut cut = stream_cut(p.N, 1, pair, false, cus);
+int stream_a8(const A8Params &p, bool pair, int dtype, int ranks, int cus, hipStream_t s) {
+    const StreamCut cut = stream_cut(p.N, ranks, pair, false, cus);
     TPAMD_REQUIRE(cut.groups > 0, "a8: no cut of %d columns", p.N);
-    if (dtype == TPAMD_BF16) return pair ? launch_m<TPAMD_BF16, true>(p, cut.rows, cut.blocks, s) : launch_m<TPAMD_BF16, false>(p, cut.rows, cut.blocks, s);
-    return pair ? launch_m<TPAMD_F16, true>(p, cut.rows, cut.blocks, s) : launch_m<TPAMD_F16, false>(p, cut.rows, cut.blocks, s);
+    if (dtype == TPAMD_BF16) return pair ? launch_m<TPAMD_BF16, true>(p, cut.rows, cut.blocks, ranks, s) : launch_m<TPAMD_BF16, false>(p, cut.rows, cut.blocks, ranks, s);
+    return pair ? launch_m<TPAMD_F16, true>(p, cut.rows, cut.blocks, ranks, s) : launch_m<TPAMD_F16, false>(p, cut.rows, cut.blocks, ranks, s);
 }
 
 }  // namespace tpamd

@@ -362,6 +362,53 @@ def linear_w8_sum(x: torch.Tensor, wq: torch.Tensor, scale: torch.Tensor, outlie
     return _call(_not_together, _linear_w8_sum, (x, wq, scale, outlier_idx, w_out, bias), (op,), (rank,))
 
 
+# Rows in 8 bits and their products meet up to as many rows: more go to tiles, which take a rank at a time. A recorded step of four 7B-shaped layers on two ranks, 1 / 8 / 32 rows: 448 -> 385,
+# 505 -> 424, 646 -> 543 us (sums as one launch of both and one that adds included: the last one 562 with the second rank's product adding the first's).
+A8_TOGETHER_ROWS = 64
+
+
+def linear_a8(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor, bias: Optional[torch.Tensor], dtype: torch.dtype, act: int = _native.ACT_NONE) -> torch.Tensor:
+    if q.numel() > A8_TOGETHER_ROWS * q.shape[-1]:
+        return _native.linear_a8(q, scale, wq, wscale, bias, dtype, act)
+    return _call(_native.linear_a8, _native.linear_a8_ranks, (q, scale, wq, wscale, bias), (dtype, act))
+
+
+def _linear_a8_sum(calls: List[tuple]) -> Sequence[torch.Tensor]:
+    parts = _native.linear_a8_ranks([call[:7] for call in sorted(calls, key=lambda call: call[-1])])
+    copy = torch.empty_like(parts[0])
+    return [copy, _native.reduce_partials(parts, copy=copy)]
+
+
+def linear_a8_sum(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor, bias: Optional[torch.Tensor], dtype: torch.dtype, act: int, rank: int,
+                  op: Any = None) -> Optional[torch.Tensor]:
+    """The sum of two ranks' products, for each a tensor of its own: a launch of both and one that adds; None where this rank is on its own. `op` as above."""
+    return _call(_not_together, _linear_a8_sum, (q, scale, wq, wscale, bias), (dtype, act, op), (rank,))
+
+
+def swiglu_up_a8(q: torch.Tensor, scale: torch.Tensor, gate: torch.Tensor, gscale: torch.Tensor, up: torch.Tensor, uscale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    if q.numel() > A8_TOGETHER_ROWS * q.shape[-1]:
+        return _native.swiglu_up_a8(q, scale, gate, gscale, up, uscale, dtype)
+    return _call(_native.swiglu_up_a8, _native.swiglu_up_a8_ranks, (q, scale, gate, gscale, up, uscale), (dtype,))
+
+
+def quantize_rows(x: torch.Tensor) -> tuple:
+    if x.dim() == 0 or x.numel() > A8_TOGETHER_ROWS * x.shape[-1]:
+        return _native.quantize_rows(x)
+    return _call(_native.quantize_rows, _native.quantize_rows_ranks, (x,))
+
+
+def rms_norm_q8(x: torch.Tensor, w: torch.Tensor, eps: float) -> tuple:
+    if x.numel() > A8_TOGETHER_ROWS * w.numel():
+        return _native.rms_norm_q8(x, w, eps)
+    return _call(_native.rms_norm_q8, _native.rms_norm_q8_ranks, (x, w), (eps,))
+
+
+def add_rms_norm_q8(r: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float) -> tuple:
+    if x.numel() > A8_TOGETHER_ROWS * w.numel():
+        return _native.add_rms_norm_q8(r, x, w, eps)
+    return _call(_native.add_rms_norm_q8, _native.add_rms_norm_q8_ranks, (r, x, w), (eps,))
+
+
 def _gather(calls: List[tuple]) -> Sequence[torch.Tensor]:
     return _native.linear_gather_ranks([call[:3] for call in sorted(calls, key=lambda call: call[-1])])  # (every rank's result is the same)
 

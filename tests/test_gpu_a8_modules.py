@@ -166,6 +166,9 @@ def test_norms_hand_rows_to_attention_and_mlp(ranks, static, monkeypatch):
     for name in ("rms_norm_q8", "add_rms_norm_q8", "quantize_rows", "rms_norm", "rms_norm_ranks", "add_rms_norm", "add_rms_norm_ranks", "swiglu_up_a8"):
         inner = getattr(_native, name)
         monkeypatch.setattr(_native, name, lambda *a, _f=inner, _n=name, **k: counts.update({_n: counts.get(_n, 0) + 1}) or _f(*a, **k))
+    for name in ("rms_norm_q8", "add_rms_norm_q8", "quantize_rows", "swiglu_up_a8"):  # two ranks' calls in one
+        inner = getattr(_native, name + "_ranks")
+        monkeypatch.setattr(_native, name + "_ranks", lambda calls, _f=inner, _n=name: counts.update({_n: counts.get(_n, 0) + len(calls), "met": counts.get("met", 0) + 1}) or _f(calls))
     with torch.no_grad():
         forward()
         counts.clear()
@@ -173,6 +176,7 @@ def test_norms_hand_rows_to_attention_and_mlp(ranks, static, monkeypatch):
         layers = 2 * ranks * 2  # over both calls
         assert counts["rms_norm_q8"] == counts["add_rms_norm_q8"] == counts["swiglu_up_a8"] == layers
         assert counts["quantize_rows"] == 2 * layers  # the attention's output and the hidden rows
+        assert counts.get("met", 0) == (5 * 2 if ranks == 2 else 0)  # all of them in the step of one position, of each of the two layers
         seen = []
         handles = []
         for m in split.modules():
