@@ -9,10 +9,10 @@
 // compared with the half exactly; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
 // A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
 //
-// Bound: at a few rows by the latency of a launch (2.4-2.8 us in a graph, 1 x 4096), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
-// once, by the instructions between their loads and their stores: 2103 x 4096 quantised in 9.0 us (2.9 TB/s), normed 9.5, 4096 x 8192 19.1 (5.3 TB/s) and 20.7, with the addition 37.5 (6.3 TB/s);
+// Bound: at a few rows by the latency of a launch (2.2-2.5 us in a graph, 1 x 4096; an empty kernel 1.7), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
+// once, by the instructions between their loads and their stores: 2103 x 4096 quantised in 8.8 us (2.9 TB/s), normed 9.2, 4096 x 8192 18.8 (5.3 TB/s) and 20.5, with the addition 37.3 (6.3 TB/s);
 // the way back of 4096 x 8192 to fp32 27.7 (6.0 TB/s).
-#include "common.h"
+#include "gemm_tile.h"
 
 namespace tpamd {
 namespace {
@@ -89,15 +89,34 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const RowCode &c) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// Step S of a butterfly over the wavefront whose earlier steps are done: one of a pair of lanes' values and, in `other`, the other one. Within rows of 16 lanes by the operand's lane permutation, between
+// rows by swaps: no trip through LDS.
+template <int S>
+__device__ __forceinline__ uint32_t partner(uint32_t v, uint32_t &other) {
+    if constexpr (S < 4) {
+        constexpr int CTRL = S == 0 ? 0xB1 : S == 1 ? 0x4E : S == 2 ? 0x141 : 0x140;  // quads 1 0 3 2, 2 3 0 1; halves of a row and rows mirrored
+        other = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+        return v;
+    } else {
+        const auto both = S == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        other = both[1];
+        return both[0];
+    }
+}
+
 // Sum (SUM) and maximum over the block, the same in every thread. `part`: two words for each wavefront.
 template <int WAVES, bool SUM>
 __device__ __forceinline__ void block_sum_max(float &sum, uint32_t &most, uint2 *part) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        if constexpr (SUM) sum += __shfl_xor(sum, d);
-        const uint32_t other = __shfl_xor(most, d);
+    unrolled<6>([&](auto stage) {
+        uint32_t other;
+        if constexpr (SUM) {
+            const uint32_t mine = __float_as_uint(sum);
+            sum = __uint_as_float(partner<decltype(stage)::value>(mine, other));
+            sum += __uint_as_float(other);
+        }
+        most = partner<decltype(stage)::value>(most, other);
         most = most > other ? most : other;
-    }
+    });
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_uint2(__float_as_uint(sum), most);
         __syncthreads();
@@ -216,8 +235,8 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
 }
 
 // Without the addition, rows of a large launch are held by fewer wavefronts with four chunks a lane: more rows are under way on a CU, and a row's meeting costs less. Quantised / normed, us:
-// 2103 x 4096 9.6 -> 9.0 / 10.9 -> 9.5, 4096 x 5504 16.4 -> 15.0 / 19.0 -> 16.3, 4096 x 16384 36.1 -> 34.1 / 42.4 -> 37.1, 1024 x 11008 10.9 -> 9.9 / 12.3 -> 11.0; smaller ones lose, 1024 x 4096
-// 6.1 -> 6.9, 2048 x 2048 6.0 -> 6.7, and with the addition 4096 x 8192 37.6 -> 38.7.
+// 2103 x 4096 9.2 -> 8.8 / 10.1 -> 9.2, 4096 x 5504 15.2 -> 14.6 / 17.9 -> 15.6, 4096 x 16384 35.5 -> 33.5 / 40.9 -> 36.3, 1024 x 11008 10.0 -> 9.6 / 11.6 -> 10.7; smaller ones lose, 1024 x 4096
+// 6.0 -> 6.7, 2048 x 2048 6.0 -> 6.5, and with the addition 4096 x 8192 37.8 -> 38.3, 2103 x 4096 13.3 -> 13.9.
 constexpr int64_t MANY_VALUES = 1 << 23;
 
 template <int DT, bool NORM, bool ADD>
