@@ -9,7 +9,9 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int SA_NW = 4;        // wavefronts per block
 constexpr int SA_LDS_KB = 160;  // one block per CU
-constexpr int SA_DEPTH = 4;     // most stages
+// Most stages, by the loads of one. Three are enough but where a stage is small: 16 x 16384 x 8192 26.4 us with four, 25.9 with three, 32 x 4096 x 5504 10.4 and 10.2, the pair of 8 x 5504 x 4096
+// 10.7 and 10.5, but 1 x 4096 x 5504 6.0 and 6.1, 1 x 2048 x 4096 4.6 and 4.75; six or eight cost 1-6 % on small matrices and change nothing on large ones.
+constexpr int sa_depth(int loads) { return loads <= 4 ? 4 : 3; }
 
 // stream_a8_kernel: products of up to 64 rows of 8-bit codes on one block per CU, cut and staged as stream_kernel cuts and stages 16-bit ones (stream.hip): a block owns an even share of the
 // columns and all of K, its wavefronts contiguous quarters of K, 128 elements (bytes) of NR weight rows (a pair: gate rows, then up rows) and XR rows of x at a time through rings of their own in
@@ -20,7 +22,7 @@ constexpr int SA_DEPTH = 4;     // most stages
 // 1 x 4096 x 5504 (22.5 MB), of 10.5 for the pair of 8 x 5504 x 4096 (45 MB). From 33 rows on x, which every CU reads whole from the L2: 64 x 4096 x 5504 12.8.
 // Two ranks' products are one launch with half the CUs each (blockIdx.y).
 // Slower, tried: weights straight into registers in the order of the matrix instructions (16 rows x 64 bytes a load: 37 us for the first), two blocks of half the LDS to a CU (26.4, all others
-// slower), eight stages, eight wavefronts.
+// slower), eight wavefronts.
 __device__ __forceinline__ const float *by_bytes(const float *p, int64_t bytes) { return reinterpret_cast<const float *>(reinterpret_cast<const char *>(p) + bytes); }
 
 template <int DT, bool PAIR, int NR, int XR, int D>
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
 
 template <int DT, bool PAIR, int NR, int XR>
 int launch_nr(const A8Params &p, int blocks, int ranks, hipStream_t s) {
-    constexpr int L = (NR + XR) / 8, DM = SA_LDS_KB / SA_NW / L, D = DM < SA_DEPTH ? DM : SA_DEPTH;
+    constexpr int L = (NR + XR) / 8, DM = SA_LDS_KB / SA_NW / L, D = DM < sa_depth(L) ? DM : sa_depth(L);
     static_assert(D >= 2, "LDS");
     constexpr int LDS = SA_NW * D * L * 1024;
     auto kern = stream_a8_kernel<DT, PAIR, NR, XR, D>;
