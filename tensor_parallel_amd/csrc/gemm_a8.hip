@@ -18,7 +18,7 @@ struct A8Tiles {
     int tiles_m, tiles_n;
     int kt_per_split, splits;  // K tiles of a range, ranges
     int *ws;                   // partial tiles
-    bool direct;               // the epilogue from the registers: no activation, rows of outputs and addend and the scales on 16-byte boundaries (bias: 8), N a multiple of 8
+    bool direct;               // the epilogue from the registers: no activation, rows of outputs and addend and the scales on 16-byte boundaries (bias: 8), N a multiple of 8, rows of the addend within reach of 32-bit offsets
     int store;                 // values of a row that outputs and addend are accessed by: 8 (N a multiple of 8), 2 (N even) or 1, as their rows allow
 };
 
@@ -97,8 +97,8 @@ __device__ __forceinline__ void lds_write_acc(uint32_t addr, i32x4 v) {
 // barrier: tile g + 1 has landed, tile g is read out; the loads of tile g + NS go into its stage in the rest of that step and the first of the next tile.
 // K ends in a multiple of 16: in the last stage the pieces of x behind it are asked for outside the descriptor's range, which gives zeros, and what stands in those of w
 // (the next row, or the bytes between rows) counts for nothing.
-// Bound: by the power that the matrix pipe takes on real codes: a K tile of a 256 x 256 tile takes 1.6 us with every CU at it (2.7 POP/s), 1.06 on zeros. 4096 x 4096 x 5504 in 82 us (2.25 POP/s; 93
-// with an addend that comes from memory, whose 34 MB and the outputs' are moved when all blocks end at once), 4096 x 16384 x 8192 in 445 (2.47), the pair of 4096 x 5504 x 4096 in 165 (2.24).
+// Bound: by the power that the matrix pipe takes on real codes: a K tile of a 256 x 256 tile takes 1.6 us with every CU at it (2.7 POP/s), 1.06 on zeros. 4096 x 4096 x 5504 in 82-86 us (2.15-2.25 POP/s; 90
+// with an addend that comes from memory, most of it under the last K tiles), 4096 x 16384 x 8192 in 445 (2.47), the pair of 4096 x 5504 x 4096 in 165 (2.24).
 // Smaller tiles by what LDS and the L2 deliver: 645 x 6144 x 4096 on 128 x 192 tiles, one to a CU, 24 us, 28 on weights from memory; a fourth or fifth stage changes nothing. Rows that begin
 // inside 128-byte lines cost a fifth more (each of their lines is asked for in two K tiles).
 // SPLIT: a block has one of t.splits ranges of K; its sums go to t.ws as they lie in the registers and are added by finish_a8_kernel.
@@ -107,7 +107,7 @@ constexpr int a8_lds(int tm, int tn, int ns) {
     const int stages = ns * 64 * (tm + tn) * 128, slabs = 4 * (a8_slab_rows(tm, tn) * 32 * (tn * 128 + 16) + tm * 128);
     return stages > slabs ? stages : slabs;
 }
-template <int DT, int MODE, int TM, int TN, int NS, bool SPLIT>
+template <int DT, int MODE, int TM, int TN, int NS, bool SPLIT, bool ADD>
 __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
     constexpr int BM = 64 * TM, BN = 64 * TN, BN_OUT = MODE == MODE_SWIGLU ? BN / 2 : BN;
     constexpr int XREG = BM * 128, STAGE = (BM + BN) * 128;
@@ -156,16 +156,34 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
         make_rsrc(p.x + static_cast<int64_t>(m0) * p.ldx, static_cast<uint32_t>(x_rows - 1) * static_cast<uint32_t>(p.ldx) + static_cast<uint32_t>(p.K));
     const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + static_cast<int64_t>(n0) * p.ldw, w_extent);
     const __amdgpu_buffer_rsrc_t w2_rsrc = MODE == MODE_SWIGLU ? make_rsrc(p.w2 + static_cast<int64_t>(n0) * p.ldw, w_extent) : w_rsrc;
-    // load number ic of K tile kt of this range; behind the last one the same count of loads from outside the descriptors (with the uniform offset inside their extents)
-    auto load = [&](auto ic, int kt, int stage_off) __attribute__((always_inline)) {
+    // the addend's rows of this wavefront (ADD), for the epilogue from the registers: EARLY slabs of 32 rows take the place of K tiles behind the last one. 4096 x 8192 x 4096 150 -> 140 us, 4096 x
+    // 4096 x 5504 94 -> 90 against requests in the epilogue
+    const int m_wave = m0 + wm * TM * 32, n_wave = n0 + wn * TN * CB;
+    constexpr int SLAB_LOADS = 2 * TN, AHEAD = (NS - 1) * LPT + HALF, EARLY = AHEAD / SLAB_LOADS < TM ? AHEAD / SLAB_LOADS : TM;
+    static_assert(TM - EARLY <= 1, "the rest of the addend is held in registers");
+    const uint32_t add_pitch = static_cast<uint32_t>(p.ldadd) * 2;
+    uint32_t add_extent = 0;
+    if (ADD && t.direct && m_wave < p.M && n_wave < p.N)
+        add_extent = static_cast<uint32_t>((p.M - m_wave < TM * 32 ? p.M - m_wave : TM * 32) - 1) * add_pitch + static_cast<uint32_t>(p.N - n_wave < TN * CB ? p.N - n_wave : TN * CB) * 2;
+    const __amdgpu_buffer_rsrc_t add_rsrc = add_extent != 0 ? make_rsrc(p.addend + (static_cast<int64_t>(m_wave) * p.ldadd + n_wave) * 2, add_extent) : x_rsrc;
+    auto slot = [&](int i) { return i < XL ? (wave * XL + i) * 1024 : XREG + (wave * WL + i - XL) * 1024; };  // of load i in its stage
+    // load number ic of K tile kt of this range; behind the last one (which `inside` rules out) the same count of loads, of the addend or from outside the descriptors (with the uniform offset inside
+    // their extents)
+    auto load = [&](auto ic, int kt, int stage_off, auto inside) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
-        const uint32_t none = kt < KT ? 0u : 0x80000000u;
-        const int at = (first + (kt < KT ? kt : 0)) * A8_BK;
-        if constexpr (i < XL) {
-            const uint32_t end = kt == last_kt ? behind[i & 1] : none;  // (XL is even)
-            buffer_load16_to_lds(x_rsrc, x_off[i] | end, at, smem + stage_off + (wave * XL + i) * 1024);
+        char *to = smem + stage_off + slot(i);
+        const bool here = decltype(inside)::value || kt < KT;
+        const uint32_t from = i < XL ? x_off[i < XL ? i : 0] | (kt == last_kt ? behind[i & 1] : 0u) : w_off[i < XL ? 0 : i - XL];  // (XL is even)
+        const __amdgpu_buffer_rsrc_t rsrc = i < XL ? x_rsrc : is_up(i - XL) ? w2_rsrc : w_rsrc;
+        if constexpr (decltype(inside)::value) {
+            buffer_load16_to_lds(rsrc, from, (first + kt) * A8_BK, to);
+        } else if constexpr (!ADD) {
+            buffer_load16_to_lds(rsrc, here ? from : 0x80000000u, here ? (first + kt) * A8_BK : 0, to);
         } else {
-            buffer_load16_to_lds(is_up(i - XL) ? w2_rsrc : w_rsrc, w_off[i - XL] | none, at, smem + stage_off + XREG + (wave * WL + i - XL) * 1024);
+            const uint32_t j = static_cast<uint32_t>(kt - KT) * LPT + i, a = j / SLAB_LOADS, at = a * 32 * add_pitch + j % SLAB_LOADS * 32;
+            const bool there = a < EARLY && at < add_extent;
+            const uint32_t lane_at = there ? static_cast<uint32_t>(l32) * add_pitch + static_cast<uint32_t>(lh) * 16 : 0x80000000u;
+            buffer_load16_to_lds(here ? rsrc : add_rsrc, here ? from : lane_at, here ? (first + kt) * A8_BK : there ? static_cast<int>(at) : 0, to);
         }
     };
 
@@ -208,7 +226,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
     // ---- first stages: the second half of the last one is loaded in the first step
     unrolled<NS>([&](auto sc) {
         constexpr int s = decltype(sc)::value;
-        unrolled<(s < NS - 1 ? LPT : HALF)>([&](auto ic) { load(ic, s, s * STAGE); });
+        unrolled<(s < NS - 1 ? LPT : HALF)>([&](auto ic) { load(ic, s, s * STAGE, std::false_type{}); });
     });
     if constexpr (!SPLIT) {
 #pragma unroll
@@ -219,7 +237,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
     fence();
 
     int cur = 0, nxt = STAGE, old = (NS - 1) * STAGE;  // offsets of the stages of K tiles g, g + 1 and g + NS - 1
-    for (int g = 0; g < KT; ++g) {
+    auto k_tile = [&](int g, auto inside) __attribute__((always_inline)) {
         const int k_old = g + NS - 1, k_cur = g + NS;
         unrolled<4>([&](auto sc) {
             constexpr int s = decltype(sc)::value, bar = s == 3 ? BAR : 0, slots = MF - bar, per = (READS + slots - 1) / slots;
@@ -240,8 +258,8 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
                     constexpr int r0 = (m - bar) * per, r1 = r0 + per < READS ? r0 + per : READS;
                     unrolled<(r1 > r0 ? r1 - r0 : 0)>([&](auto rc) { read(then, std::integral_constant<int, r0 + decltype(rc)::value>{}, xa, wa); });
                     constexpr int l0 = (m - bar) * HALF / slots, l1 = (m + 1 - bar) * HALF / slots;
-                    if constexpr (s == 3) unrolled<l1 - l0>([&](auto lc) { load(std::integral_constant<int, l0 + decltype(lc)::value>{}, k_cur, cur); });
-                    if constexpr (s == 0) unrolled<l1 - l0>([&](auto lc) { load(std::integral_constant<int, HALF + l0 + decltype(lc)::value>{}, k_old, old); });
+                    if constexpr (s == 3) unrolled<l1 - l0>([&](auto lc) { load(std::integral_constant<int, l0 + decltype(lc)::value>{}, k_cur, cur, inside); });
+                    if constexpr (s == 0) unrolled<l1 - l0>([&](auto lc) { load(std::integral_constant<int, HALF + l0 + decltype(lc)::value>{}, k_old, old, inside); });
                 }
                 fence();
             });
@@ -249,7 +267,11 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
         old = cur;
         cur = nxt;
         nxt = nxt + STAGE == NS * STAGE ? 0 : nxt + STAGE;
-    }
+    };
+    // two loops: asked in every load, whether it lies behind the last K tile costs 8 % of a 256 x 256 tile's time
+    int g = 0;
+    for (; g < KT - NS; ++g) k_tile(g, std::true_type{});
+    for (; g < KT; ++g) k_tile(g, std::false_type{});
     // every load and fragment read of this wavefront is done before another use of the stages and registers
     landed(set0);
     (void)set1;
@@ -272,15 +294,13 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
         return;
     }
 
-    const int m_wave = m0 + wm * TM * 32, n_wave = n0 + wn * TN * CB;
-    const bool with_addend = MODE == MODE_LINEAR && p.addend != nullptr;
     // ---- epilogue from the registers, 32 rows at a time: two lanes exchange halves of groups of 8 columns, and a store has 32 bytes of 32 rows, which the L2 puts together.
     // A 256 x 256 tile takes 11000 cycles with it, 25000 with the loop over LDS below
     if (t.direct) {
         constexpr int CHUNKS = CB / 16;  // groups of 8 outputs that a lane has of an MFMA tile
         float4 sw[TN][4];
         uint2 braw[TN][4];
-        uint4 addend[TN][CHUNKS];
+        uint4 rest[TN][CHUNKS];  // of the addend
         unrolled<TN>([&](auto bc) {
             constexpr int b = decltype(bc)::value;
 #pragma unroll
@@ -290,15 +310,13 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
                 braw[b][q] = MODE == MODE_LINEAR && p.bias != nullptr ? *reinterpret_cast<const uint2 *>(p.bias + static_cast<int64_t>(n) * 2) : make_uint2(0, 0);
             }
         });
-        auto request = [&](auto ac, auto bc) __attribute__((always_inline)) {  // the addend of an MFMA tile, when the one above it has been added
-            constexpr int a = decltype(ac)::value, b = decltype(bc)::value;
+        if constexpr (ADD && EARLY < TM) {
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                const int m = m_wave + a * 32 + l32, n = n_wave + b * CB + c * 16 + lh * 8;
-                addend[b][c] = a < TM && m < p.M && n < p.N ? *reinterpret_cast<const uint4 *>(p.addend + (static_cast<int64_t>(m) * p.ldadd + n) * 2) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < TN * CHUNKS; ++i) {
+                const int m = m_wave + EARLY * 32 + l32, n = n_wave + i * 16 + lh * 8;
+                rest[i / CHUNKS][i % CHUNKS] = m < p.M && n < p.N ? *reinterpret_cast<const uint4 *>(p.addend + (static_cast<int64_t>(m) * p.ldadd + n) * 2) : make_uint4(0, 0, 0, 0);
             }
-        };
-        if (with_addend) unrolled<TN>([&](auto bc) { request(std::integral_constant<int, 0>{}, bc); });
+        }
         unrolled<TM>([&](auto ac) {
             constexpr int a = decltype(ac)::value;
             const int m = m_wave + a * 32 + l32;
@@ -331,13 +349,20 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
                     const auto x = __builtin_amdgcn_permlane32_swap(w[2 * c].x, w[2 * c + 1].x, false, false);
                     const auto y = __builtin_amdgcn_permlane32_swap(w[2 * c].y, w[2 * c + 1].y, false, false);
                     uint4 u = make_uint4(x[0], y[0], x[1], y[1]);
-                    if (with_addend) u = add8<DT>(u, addend[b][c]);
+                    if constexpr (ADD) {
+                        if constexpr (a < EARLY) {
+                            constexpr int j = a * SLAB_LOADS + b * 2, behind_last = j / LPT;
+                            const int stage_off = behind_last == 0 ? cur : behind_last == 1 ? nxt : old;  // (two stages: nxt is old)
+                            u = add8<DT>(u, *reinterpret_cast<const uint4 *>(smem + stage_off + slot(j % LPT + c) + lane * 16));
+                        } else {
+                            u = add8<DT>(u, rest[b][c]);
+                        }
+                    }
                     if (m < p.M && n_wave + b * CB + c * 16 + lh * 8 < p.N) {
                         *reinterpret_cast<uint4 *>(row + b * CB * 2 + c * 32) = u;
                         if (MODE == MODE_LINEAR && p.copy != 0) *reinterpret_cast<uint4 *>(row + b * CB * 2 + c * 32 + p.copy) = u;
                     }
                 }
-                if (a + 1 < TM && with_addend) request(std::integral_constant<int, a + 1>{}, bc);
             });
         });
         return;
@@ -361,7 +386,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
     constexpr int U = MODE == MODE_SWIGLU ? 2 : 4, STEP = U * RPP;  // rows of a lane at a time, of the wavefront
     uint4 ahead[U];
     auto request = [&](int r0) __attribute__((always_inline)) {  // the addend of the wavefront's rows from r0 on
-        if (!with_addend) return;
+        if constexpr (!ADD) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int r = r0 + u * RPP + my_row, m = m_wave + r;
@@ -395,7 +420,7 @@ __global__ __launch_bounds__(256) void gemm_a8_kernel(A8Params p, A8Tiles t) {
                 const int g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w}, up[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
                 o[u] = a8_finish8<DT, MODE>(g, up, scales[a0 * 32 + r], sw, sw2, bias, p.act);
             }
-            if (with_addend) {
+            if constexpr (ADD) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) o[u] = add8<DT>(o[u], ahead[u]);
                 request(a0 * 32 + r0 + STEP < a0 * 32 + ROWS ? a0 * 32 + r0 + STEP : (a0 + AH) * 32);
@@ -469,10 +494,10 @@ int values_by(const void *a, int64_t copy, int64_t ld, int N) {
     return N % 2 == 0 && ld % 2 == 0 && at % 4 == 0 ? 2 : 1;
 }
 
-template <int DT, int MODE, int TM, int TN, int NS, bool SPLIT>
+template <int DT, int MODE, int TM, int TN, int NS, bool SPLIT, bool ADD>
 int launch_tiles(const A8Params &p, const A8Tiles &t, hipStream_t s) {
     constexpr int LDS = SPLIT ? NS * 64 * (TM + TN) * 128 : a8_lds(TM, TN, NS);
-    auto kern = gemm_a8_kernel<DT, MODE, TM, TN, NS, SPLIT>;
+    auto kern = gemm_a8_kernel<DT, MODE, TM, TN, NS, SPLIT, ADD>;
     static thread_local int configured_dev = -1;  // per instantiation and host thread
     int dev = 0;
     TPAMD_HIP(hipGetDevice(&dev));
@@ -495,7 +520,8 @@ int launch_a8(const A8Params &p, int splits, hipStream_t s) {
     t.tiles_n = (p.N + BN_OUT - 1) / BN_OUT;
     const int out = values_by(p.y, p.copy, p.ldy, p.N), in = p.addend == nullptr ? 8 : values_by(p.addend, 0, p.ldadd, p.N);
     t.store = out < in ? out : in;
-    t.direct = t.store == 8 && (MODE == MODE_SWIGLU || p.act == TPAMD_ACT_NONE) && aligned(p.sw, 16) && aligned(p.sw2, 16) && aligned(p.bias, 8);
+    t.direct = t.store == 8 && (MODE == MODE_SWIGLU || p.act == TPAMD_ACT_NONE) && aligned(p.sw, 16) && aligned(p.sw2, 16) && aligned(p.bias, 8) &&
+               (p.addend == nullptr || p.ldadd < (1ll << 21));
     const int kt = (p.K + A8_BK - 1) / A8_BK;
     t.kt_per_split = (kt + splits - 1) / splits;
     t.splits = (kt + t.kt_per_split - 1) / t.kt_per_split;
@@ -509,7 +535,7 @@ int launch_a8(const A8Params &p, int splits, hipStream_t s) {
         if (int rc = splitk_scratch(dev, s, need, scratch_reserve(cus), &ws); rc != TPAMD_OK) return rc;
         if (ws != nullptr) {
             t.ws = static_cast<int *>(ws);
-            if (int rc = launch_tiles<DT, MODE, TM, TN, NS, true>(p, t, s); rc != TPAMD_OK) return rc;
+            if (int rc = launch_tiles<DT, MODE, TM, TN, NS, true, false>(p, t, s); rc != TPAMD_OK) return rc;
             const int64_t units = static_cast<int64_t>(t.tiles_m) * t.tiles_n * 4 * TM * TN;
             hipLaunchKernelGGL((finish_a8_kernel<DT, MODE, TM, TN>), dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, s, p, t);
             TPAMD_HIP(hipGetLastError());
@@ -518,7 +544,9 @@ int launch_a8(const A8Params &p, int splits, hipStream_t s) {
         t.splits = 1;  // no scratch memory for the stream: all of K in a block
         t.kt_per_split = kt;
     }
-    return launch_tiles<DT, MODE, TM, TN, NS, false>(p, t, s);
+    if constexpr (MODE == MODE_LINEAR)
+        if (p.addend != nullptr) return launch_tiles<DT, MODE, TM, TN, NS, false, true>(p, t, s);
+    return launch_tiles<DT, MODE, TM, TN, NS, false, false>(p, t, s);
 }
 
 template <int DT, int MODE>
