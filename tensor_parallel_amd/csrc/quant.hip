@@ -9,7 +9,7 @@
 // compared with the half exactly; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
 // A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
 //
-// Bound: at a few rows by the latency of a launch (2.2-2.5 us in a graph, 1 x 4096; an empty kernel 1.7), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
+// Bound: at a few rows by the latency of a launch (2.2-2.5 us in a graph, 1 x 4096; the shortest launches here take 1.7), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
 // once, by the instructions between their loads and their stores: 2103 x 4096 quantised in 8.8 us (2.9 TB/s), normed 9.2, 4096 x 8192 18.8 (5.3 TB/s) and 20.5, with the addition 37.3 (6.3 TB/s);
 // the way back of 4096 x 8192 to fp32 27.7 (6.0 TB/s).
 #include "gemm_tile.h"

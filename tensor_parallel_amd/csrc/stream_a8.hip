@@ -16,9 +16,9 @@ constexpr int sa_depth(int loads) { return loads <= 4 ? 4 : 3; }
 // stream_a8_kernel: products of up to 64 rows of 8-bit codes on one block per CU, cut and staged as stream_kernel cuts and stages 16-bit ones (stream.hip): a block owns an even share of the
 // columns and all of K, its wavefronts contiguous quarters of K, 128 elements (bytes) of NR weight rows (a pair: gate rows, then up rows) and XR rows of x at a time through rings of their own in
 // LDS, filled by loads that go straight there; the wavefronts' sums meet in LDS. K ends in a multiple of 16: the pieces of x behind it are asked for outside the descriptor's range, which
-// gives zeros, and so are rows that there are none of, which cost no memory traffic (they read the last row again before: 16 x 16384 x 8192 28.0 us, now 26.0).
+// gives zeros, and so are rows that there are none of, which cost no memory traffic (they read the last row again before: 16 x 16384 x 8192 28.0 us, then 26.0).
 // The matrix pipe idles (a stage's MFMAs take 2-6 % of its time), so the half-rate 16 x 16 form serves, whose rows of 16 fit few columns a CU.
-// Bound: memory, N K bytes of weights: 16 x 16384 x 8192 in 26.0 us, 5.2 TB/s where a large copy has 6.0; at smaller matrices its latency: a launch and the first loads are 3.4 us of 6.1 for
+// Bound: memory, N K bytes of weights: 16 x 16384 x 8192 in 25.9 us, 5.2 TB/s where a large copy has 6.0; at smaller matrices its latency: a launch and the first loads are 3.4 us of 6.0 for
 // 1 x 4096 x 5504 (22.5 MB), of 10.5 for the pair of 8 x 5504 x 4096 (45 MB). From 33 rows on x, which every CU reads whole from the L2: 64 x 4096 x 5504 12.8.
 // Two ranks' products are one launch with half the CUs each (blockIdx.y).
 // Slower, tried: weights straight into registers in the order of the matrix instructions (16 rows x 64 bytes a load: 37 us for the first), two blocks of half the LDS to a CU (26.4, all others

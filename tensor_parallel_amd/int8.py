@@ -96,22 +96,27 @@ class QuantizedRows(NamedTuple):
         return _guard(_native.dequantize_rows(self.codes, self.scale, self.dtype if dtype is None else dtype), self.scale)
 
 
+def _calls():
+    """The library's calls: made together with the other ranks where ranks take turns."""
+    return _native if together.current_turn() is None else together
+
+
 def quantize_activations(x: torch.Tensor) -> QuantizedRows:
     """The rows of x (bfloat16 or float16, on a HIP device) in 8 bits, by the definition in the module docstring. Inference only, as everything here: a
     backward pass through the rows' scales, or what Linears make of them, raises."""
-    codes, scale = together.quantize_rows(x)
+    codes, scale = _calls().quantize_rows(x)
     return QuantizedRows(codes, _guard(scale, x), x.dtype)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> QuantizedRows:
     """The RMS norm of x's rows in 8 bits, in one launch: weight * x * rsqrt(mean(x^2) + eps), not rounded in between."""
-    codes, scale = together.rms_norm_q8(x, weight, eps)
+    codes, scale = _calls().rms_norm_q8(x, weight, eps)
     return QuantizedRows(codes, _guard(scale, x, weight), x.dtype)
 
 
 def add_rms_norm(r: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float) -> Tuple[torch.Tensor, QuantizedRows]:
     """(r + x, the RMS norm of that sum in 8 bits), in one launch: a residual stream and the input of the Linears behind its norm."""
-    total, codes, scale = together.add_rms_norm_q8(r, x, weight, eps)
+    total, codes, scale = _calls().add_rms_norm_q8(r, x, weight, eps)
     return _guard(total, r, x), QuantizedRows(codes, _guard(scale, r, x, weight), x.dtype)
 
 
@@ -126,7 +131,7 @@ def linear(rows: QuantizedRows, wq: torch.Tensor, wscale: torch.Tensor, bias: Op
 def swiglu_up(rows: QuantizedRows, gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor) -> torch.Tensor:
     """silu(g) * u of the Linears g and u of 8-bit rows (as in `linear`, no bias), in one launch and rounded once."""
     codes, scale, dtype = rows
-    return _guard(together.swiglu_up_a8(codes, scale, gate, gate_scale, up, up_scale, dtype), scale, gate_scale, up_scale)
+    return _guard(_calls().swiglu_up_a8(codes, scale, gate, gate_scale, up, up_scale, dtype), scale, gate_scale, up_scale)
 
 
 # From 65 to this many rows a Linear neither meets its peer nor hands a sum over: the host sets the pace of an eager prompt there, and the reduction kernel's launch costs it
