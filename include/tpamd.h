@@ -429,8 +429,8 @@ int tpamd_linear_w8_add(const void *x_dev, const void *wq_dev, const void *scale
  *
  * Rows in 8 bits with a scale each: a = max over the row of |x|, q = round_half_even(127 x / a) of the exact quotient, scale = a / 127 (fp32); scale = 1 and codes of
  * 0 where no value of the row is 2^-100 or more; scale = NaN and codes of 0 where the row holds an infinity or NaN. x [rows, D] in `dtype` (BF16 or F16), q int8 [rows, D],
- * scale fp32 [rows]; elements between rows in ldx, ldq, the bytes between D and ldq are left alone. Any length and alignment; rows of up to 16384 elements, a multiple
- * of 8, on 16-byte boundaries (q: 8) are read once. Outputs overlap no input. */
+ * scale fp32 [rows]; elements between rows in ldx, ldq, the bytes between D and ldq are left alone. Any length below 2^30 and any alignment; rows of up to 16384
+ * elements, a multiple of 8, on 16-byte boundaries (q: 8) are read once. Outputs overlap no input. */
 int tpamd_quantize_rows(const void *x_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldq, int dtype, void *stream);
 /* y = scale * q, rounded to `dtype` (BF16, F16 or F32). */
 int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, void *y_dev, int64_t rows, int64_t D, int64_t ldq, int64_t ldy, int dtype, void *stream);

@@ -101,7 +101,7 @@ int a8_dispatch(const A8Params &p, bool pair, int dtype, hipStream_t s) {
 
 int a8_check(const char *who, const A8Params &p, int64_t M, int64_t N, int64_t K, bool pair, int dtype) {
     TPAMD_REQUIRE(M >= 0 && N >= 0 && K >= 0, "%s: negative dimension (M=%lld N=%lld K=%lld)", who, (long long)M, (long long)N, (long long)K);
-    TPAMD_REQUIRE(M < (1ll << 31) && N < (1ll << 31), "%s: dimension over 2^31", who);
+    TPAMD_REQUIRE(M < (1ll << 30) && N < (1ll << 30), "%s: dimension of 2^30 or more (M=%lld N=%lld)", who, (long long)M, (long long)N);  // (indices of a tile behind the ends fit 32 bits)
     TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16, "%s: outputs are bfloat16 or float16, not dtype %d", who, dtype);
     if (K > A8_MAX_K) {
         set_error("%s: K=%lld products of 8-bit codes may not fit 32 bits (at most %lld do)", who, (long long)K, (long long)A8_MAX_K);

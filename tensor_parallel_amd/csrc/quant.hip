@@ -281,7 +281,7 @@ int launch(QuantParams p, int64_t rows, int ranks, bool vec, hipStream_t s) {
 
 template <bool NORM, bool ADD>
 int quantize_check(const char *who, const QuantParams &p, int64_t rows, int64_t D, int dtype) {
-    TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 31), "%s: dimension negative or over 2^31 (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
+    TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 30), "%s: dimension negative or too large (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
     TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16, "%s: rows of bfloat16 or float16 are quantised, not dtype %d", who, dtype);
     if (rows == 0) return TPAMD_OK;
     TPAMD_REQUIRE(p.scale != nullptr && (D == 0 || (p.x != nullptr && p.q != nullptr && (!NORM || p.w != nullptr) && (!ADD || (p.r != nullptr && p.s != nullptr)))),
@@ -440,7 +440,7 @@ extern "C" int tpamd_rows_q8_ranks(int n, const tpamd_q8_rank *ranks, int64_t ro
 
 extern "C" int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, void *y_dev, int64_t rows, int64_t D, int64_t ldq, int64_t ldy, int dtype, void *stream) {
     const char *who = "tpamd_dequantize_rows";
-    TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 31), "%s: dimension negative or over 2^31 (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
+    TPAMD_REQUIRE(rows >= 0 && D >= 0 && rows < (1ll << 31) && D < (1ll << 30), "%s: dimension negative or too large (rows=%lld D=%lld)", who, (long long)rows, (long long)D);
     TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16 || dtype == TPAMD_F32, "%s: unknown dtype %d", who, dtype);
     if (rows == 0 || D == 0) return TPAMD_OK;
     TPAMD_REQUIRE(q_dev != nullptr && scale_dev != nullptr && y_dev != nullptr, "%s: null pointer", who);

@@ -92,3 +92,15 @@ def test_entry_points_check_what_they_are_given():
     assert add(a=NULL) == add(lda=3) == add(a=at(1)) == add(c=P) == add(c=at(1)) == INVALID
     pair = lambda u=P, su=P, ldw=16, k=16: lib.tpamd_swiglu_up_a8(P, P, P, P, u, su, P, 2, 4, k, 16, ldw, 4, 1, NULL)  # noqa: E731
     assert pair(u=NULL) == pair(su=NULL) == pair(ldw=15) == INVALID and pair(k=1 << 20) == UNSUPPORTED
+
+
+def test_sizes_that_indices_do_not_reach():
+    lib, most = _native.lib(), 1 << 30
+    for d in (most, (1 << 31) - 1, 1 << 31):
+        assert lib.tpamd_quantize_rows(P, P, P, 2, d, d, d, 0, NULL) == INVALID
+        assert lib.tpamd_rms_norm_q8(P, P, P, P, 2, d, d, d, 1e-5, 0, NULL) == INVALID
+        assert lib.tpamd_add_rms_norm_q8(P, P, P, P, P, P, 2, d, d, d, d, d, 1e-5, 0, NULL) == INVALID
+        assert lib.tpamd_dequantize_rows(P, P, P, 2, d, d, d, 0, NULL) == INVALID
+        for m, n in ((d, 16), (16, d)):
+            assert lib.tpamd_linear_a8(P, P, P, P, NULL, P, m, n, 16, 16, 16, n, 0, 0, NULL) == INVALID
+            assert lib.tpamd_swiglu_up_a8(P, P, P, P, P, P, P, m, n, 16, 16, 16, n, 0, NULL) == INVALID

@@ -242,3 +242,32 @@ def test_ranges_of_k_under_capture_and_without_scratch_memory(tile, splits, tune
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     for *_, stream in graphs:
         _native.release_scratch(DEV, stream.cuda_stream)
+
+
+def test_threads_on_streams_of_their_own(tune):
+    """Four host threads, each with a stream, K in ranges and several tiles: each one's results are those of calls in turn."""
+    import threading
+
+    sizes = [(300, 512, 4096), (40, 1000, 2064), (130, 256, 8192), (700, 688, 1024)]
+    work = [operands(m, n, k, torch.bfloat16, i) for i, (m, n, k) in enumerate(sizes)]
+    tune("TPAMD_A8_SPLITS", 4)
+    want = [(_native.linear_a8(x, sx, g, sg, bias, torch.bfloat16), _native.swiglu_up_a8(x, sx, g, sg, u, su, torch.bfloat16)) for x, sx, g, sg, u, su, bias, _ in work]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        x, sx, g, sg, u, su, bias, _ = work[i]
+        stream = torch.cuda.Stream(DEV)
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                one, pair = _native.linear_a8(x, sx, g, sg, bias, torch.bfloat16), _native.swiglu_up_a8(x, sx, g, sg, u, su, torch.bfloat16)
+                if not (torch.equal(one, want[i][0]) and torch.equal(pair, want[i][1])):
+                    wrong.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
