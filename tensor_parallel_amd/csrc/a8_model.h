@@ -2,6 +2,8 @@
 #pragma once
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace tpamd {
 
 // A launch on tiles of 64 tm x 64 tn (a pair: 32 tn columns): fixed + whole rounds of the CUs * (round + full * K tiles) + a last round that costs part + K tiles at a rate between
@@ -31,10 +33,12 @@ constexpr A8Tile A8_TILES[2][6] = {
         {4, 4, 1, 3.4, 7.3, 1.64, 1.03, 6.0, 0, 0, 0.8, 0.21, 0.00},
     },
 };
-inline float a8_tile_us(const A8Tile &t, bool pair, int64_t M, int64_t N, int64_t K, int ranges, int cus, float *mb) {
-    const int64_t columns = (pair ? 32 : 64) * t.tn, tiles = (M + 64 * t.tm - 1) / (64 * t.tm) * ((N + columns - 1) / columns);
-    const int64_t all = (K + 127) / 128, kt = (all + ranges - 1) / ranges, splits = (all + kt - 1) / kt, blocks = tiles * splits;
-    const int64_t round = static_cast<int64_t>(t.blocks_per_cu) * cus, rounds = blocks / round, rest = blocks % round;
+inline float a8_tile_us(const A8Tile &t, bool pair, uint32_t M, uint32_t N, uint32_t K, uint32_t ranges, int cus, float *mb) {
+    // (divisions in 32 bits, sizes are below 2^30: a choice takes the host 0.5 us, 0.8 with 64)
+    const uint32_t rows = static_cast<uint32_t>(64 * t.tm), columns = static_cast<uint32_t>((pair ? 32 : 64) * t.tn);
+    const uint32_t all = (K + 127) / 128, kt = (all + ranges - 1) / ranges, splits = (all + kt - 1) / kt;
+    const int64_t blocks = static_cast<int64_t>((M + rows - 1) / rows) * ((N + columns - 1) / columns) * splits;
+    const int64_t round = static_cast<int64_t>(t.blocks_per_cu) * cus, rounds = blocks < round ? 0 : blocks / round, rest = blocks - rounds * round;
     const float k = static_cast<float>(kt), part = static_cast<float>(rest) / static_cast<float>(cus);
     float us = static_cast<float>(rounds) * (t.round + t.full * k);
     if (rest > 0) {
@@ -52,15 +56,15 @@ struct A8Choice {
     float us;
 };
 // The fastest by the model; partial sums of at most `scratch` bytes.
-inline A8Choice a8_choose(bool pair, int64_t M, int64_t N, int64_t K, int cus, int64_t scratch) {
+inline A8Choice a8_choose(bool pair, uint32_t M, uint32_t N, uint32_t K, int cus, int64_t scratch) {
     A8Choice best{4, 4, 1, 1e30f};
     for (const A8Tile &t : A8_TILES[pair])
-        for (int ranges : {1, 2, 3, 4, 6, 8, 12}) {
+        for (uint32_t ranges : {1, 2, 3, 4, 6, 8, 12}) {
             if (ranges > 1 && (K + 127) / 128 < 2 * ranges) break;
             float mb = 0.f;
             const float us = a8_tile_us(t, pair, M, N, K, ranges, cus, &mb);
             if (ranges > 1 && mb * 1e6f > static_cast<float>(scratch)) break;
-            if (us < best.us) best = {t.tm, t.tn, ranges, us};
+            if (us < best.us) best = {t.tm, t.tn, static_cast<int>(ranges), us};
         }
     return best;
 }
