@@ -264,6 +264,7 @@ def test_threads_on_streams_of_their_own(tune):
                 if not (torch.equal(one, want[i][0]) and torch.equal(pair, want[i][1])):
                     wrong.append(i)
         stream.synchronize()
+        _native.release_scratch(DEV, stream.cuda_stream)
 
     threads = [threading.Thread(target=run, args=(i,)) for i in range(len(work))]
     for t in threads:
