@@ -304,7 +304,7 @@ def takes_rows(module, hidden_states=None, kwargs=None) -> bool:
     block = module._modules.get("tp_wrapped_module", module)
     own = getattr(block.__dict__.get("forward"), "__func__", None)
     if hidden_states is None:
-        if own is not _gated_mlp_a8_forward or not _has_a8(block, ("gate_proj", "up_proj", "down_proj")):
+        if own is not _gated_mlp_a8_forward or not _is_gated_a8(block, ("gate_proj", "up_proj", "down_proj")):
             return False
     else:
         if own is None or not _has_a8(block, ("q_proj", "k_proj", "v_proj")):
@@ -534,18 +534,37 @@ def _gated_mlp_first_forward(self, x: torch.Tensor) -> torch.Tensor:
     return own
 
 
-def is_gated_silu_a8_mlp(module: nn.Module) -> bool:
-    """As is_gated_silu_mlp, of Linears with 8-bit rows."""
-    if "forward" in module.__dict__ or not _has_a8(module, ("gate_proj", "up_proj", "down_proj")):
+_own_silu, _functional_silu = nn.SiLU.forward, nn.functional.silu
+
+
+def _is_plain_silu(act) -> bool:
+    """Whether this is the SiLU, torch's function, its module or transformers', and nothing else, and nobody watches it."""
+    if nn.functional.silu is not _functional_silu:
+        return False
+    if act is _functional_silu:
+        return True
+    if not isinstance(act, nn.Module) or "forward" in act.__dict__ or _has_hooks(act):
+        return False
+    return type(act) is nn.SiLU and nn.SiLU.forward is _own_silu or \
+        type(act).__name__ == "SiLUActivation" and _native.stock_function(type(act).forward, "transformers.activations", "SiLUActivation.forward", ("nn", "functional", "silu"), ("self", "input"))
+
+
+def _is_gated_a8(module: nn.Module, names: tuple = ("gate_proj", "up_proj")) -> bool:
+    """Whether gate and up can be one launch as they are now: Linears of 8-bit rows of one form, without a bias, and the SiLU, none of which anybody watches."""
+    if not _has_a8(module, names):
         return False
     gate, up = module._modules["gate_proj"], module._modules["up_proj"]
-    return gate.bias is None and up.bias is None and gate.wq.shape == up.wq.shape and gate.dtype == up.dtype and \
-        _is_silu(module._modules.get("act_fn", module.__dict__.get("act_fn")))
+    return gate.bias is None and up.bias is None and gate.wq.shape == up.wq.shape and gate.dtype == up.dtype and _is_plain_silu(module._modules.get("act_fn", module.__dict__.get("act_fn")))
+
+
+def is_gated_silu_a8_mlp(module: nn.Module) -> bool:
+    """As is_gated_silu_mlp, of Linears with 8-bit rows."""
+    return "forward" not in module.__dict__ and _is_gated_a8(module, ("gate_proj", "up_proj", "down_proj"))
 
 
 def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
-    """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch; its own forward where gate or up was replaced or is watched since."""
-    if not _has_a8(self, ("gate_proj", "up_proj")):
+    """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch; its own forward where that is no longer what its parts are."""
+    if not _is_gated_a8(self):
         return type(self).forward(self, x if isinstance(x, torch.Tensor) else x.dequantize())
     gate, up, down = self.gate_proj, self.up_proj, self.down_proj
     return down(int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))

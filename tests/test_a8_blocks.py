@@ -1,0 +1,104 @@
+"""Gated MLPs and projections of 8-bit rows as modules: which calls their fused forwards make for the block's own and which they leave to it. The library's calls are stood in for by their definitions on
+host tensors, so no GPU is needed."""
+import pytest
+import torch
+from torch import nn
+
+from tensor_parallel_amd import _native, int8, shard_modules
+from tensor_parallel_amd.int8 import ShardLinearA8, quantize_linears_
+
+
+def rows64(p):
+    """(codes, scale) of the rows of p, by the definition."""
+    p = p.double()
+    a = p.abs().amax(-1)
+    empty = a < 2.0**-100
+    codes = torch.where(empty[..., None], 0.0, (127 * p / torch.where(empty, 1.0, a)[..., None]).round())
+    return codes.to(torch.int8), torch.where(empty, 1.0, a / 127).float()
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The names of the library's calls that are made, which the definitions answer."""
+    made = []
+
+    def product(q, scale, wq, wscale):
+        return (q.double() @ wq.double().t()) * scale.double()[..., None] * wscale.double()
+
+    def quantize(x):
+        made.append("quantize_rows")
+        return rows64(x)
+
+    def linear(q, scale, wq, wscale, bias=None, dtype=torch.bfloat16, act=0, addend=None, copy=None):
+        made.append("linear_a8")
+        y = product(q, scale, wq, wscale)
+        return (y if bias is None else y + bias.double()).to(dtype)
+
+    def pair(q, scale, gate, gscale, up, uscale, dtype=torch.bfloat16):
+        made.append("swiglu_up_a8")
+        return (nn.functional.silu(product(q, scale, gate, gscale)) * product(q, scale, up, uscale)).to(dtype)
+
+    for name, call in (("quantize_rows", quantize), ("linear_a8", linear), ("swiglu_up_a8", pair), ("dequantize_rows", lambda q, s, dtype: (q.double() * s.double()[..., None]).to(dtype))):
+        monkeypatch.setattr(_native, name, call)
+    return made
+
+
+class Mlp(nn.Module):
+    def __init__(self, act=None):
+        super().__init__()
+        torch.manual_seed(0)
+        for name, shape in (("gate_proj", (96, 64)), ("up_proj", (96, 64)), ("down_proj", (64, 96))):
+            setattr(self, name, a8(*shape))
+        self.act_fn = nn.SiLU() if act is None else act
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+def a8(n, k, bias=False):
+    return ShardLinearA8(*rows64(torch.randn(n, k).bfloat16() * k**-0.5), torch.randn(n).bfloat16() if bias else None, torch.bfloat16)
+
+
+def fused(block, x):
+    """The block as its users have it: armed by quantize_linears_, and called."""
+    quantize_linears_(block, activations=True)
+    with torch.no_grad():
+        block(x)
+    assert block.forward.__func__ is shard_modules._gated_mlp_a8_forward
+    return block
+
+
+def inputs(rows=5):
+    return torch.randn(rows, 64, generator=torch.Generator().manual_seed(1)).bfloat16()
+
+
+@pytest.mark.parametrize("change", [
+    lambda m: setattr(m, "gate_proj", a8(96, 64, bias=True)),
+    lambda m: setattr(m, "up_proj", a8(96, 64, bias=True)),
+    lambda m: setattr(m.gate_proj, "bias", torch.randn(96).bfloat16()),
+    lambda m: setattr(m, "act_fn", nn.ReLU()),
+    lambda m: setattr(m, "act_fn", nn.GELU()),
+    lambda m: setattr(m.act_fn, "forward", torch.tanh),
+    lambda m: m.act_fn.register_forward_hook(lambda mod, args, out: 2 * out),
+], ids=["gate with a bias", "up with a bias", "a bias assigned", "ReLU", "GELU", "a forward of the SiLU's own", "a hook on the SiLU"])
+def test_a_part_that_is_something_else_since(calls, change):
+    """What stands in gate's, up's or the activation's place is what the block computes with, whether a Linear or the layer around hands the input over."""
+    x, block = inputs(), fused(Mlp(), inputs())
+    change(block)
+    assert not shard_modules.takes_rows(block)
+    calls.clear()
+    with torch.no_grad():
+        got, want = block(x), type(block).forward(block, x)
+    assert "swiglu_up_a8" not in calls and torch.equal(got, want)
+
+
+def test_the_launch_comes_back(calls):
+    x, block = inputs(), fused(Mlp(), inputs())
+    with torch.no_grad():
+        want = block(x)
+        block.act_fn = nn.ReLU()
+        assert not torch.equal(block(x), want)
+        block.act_fn = nn.SiLU()
+        calls.clear()
+        assert torch.equal(block(x), want) and calls == ["quantize_rows", "swiglu_up_a8", "quantize_rows", "linear_a8"] and shard_modules.takes_rows(block)
+        assert torch.equal(block(int8.quantize_activations(x)), want)
