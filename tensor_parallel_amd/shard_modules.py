@@ -126,7 +126,7 @@ def hands_through(ctx, module: nn.Module) -> bool:
         return True
     own, cls = wrapped.__dict__.get("forward"), type(wrapped)
     if own is not None:
-        return getattr(own, "__func__", None) in (_gated_mlp_forward, _gated_mlp_a8_forward) and wrapped._modules.get("down_proj") is module
+        return getattr(own, "__func__", None) is _gated_mlp_forward and wrapped._modules.get("down_proj") is module
     last = "o_proj" if cls.forward is _llama_attention_forward else "dense_4h_to_h" if cls.forward is _falcon_mlp_forward else None
     return last is not None and cls._tp_base.forward is cls._tp_replaced and wrapped._modules.get(last) is module
 
@@ -566,8 +566,8 @@ def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
     """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch; its own forward where that is no longer what its parts are."""
     if not _is_gated_a8(self):
         return type(self).forward(self, x if isinstance(x, torch.Tensor) else x.dequantize())
-    gate, up, down = self.gate_proj, self.up_proj, self.down_proj
-    return down(int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))
+    gate, up = self.gate_proj, self.up_proj
+    return returned(self, _gated_mlp_a8_forward, self.down_proj, int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))
 
 
 def _gated_mlp_a8_first_forward(self, x: torch.Tensor) -> torch.Tensor:

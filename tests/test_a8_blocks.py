@@ -4,7 +4,8 @@ import pytest
 import torch
 from torch import nn
 
-from tensor_parallel_amd import _native, int8, shard_modules
+from tensor_parallel_amd import _native, int8, shard_modules, together
+from tensor_parallel_amd.collectives import SumContext
 from tensor_parallel_amd.int8 import ShardLinearA8, quantize_linears_
 
 
@@ -102,3 +103,20 @@ def test_the_launch_comes_back(calls):
         calls.clear()
         assert torch.equal(block(x), want) and calls == ["quantize_rows", "swiglu_up_a8", "quantize_rows", "linear_a8"] and shard_modules.takes_rows(block)
         assert torch.equal(block(int8.quantize_activations(x)), want)
+
+
+def test_who_is_said_to_return_the_down_projections_output(calls):
+    """A Linear may hold other ranks' parts of a sum where the wrapped block is known to return its output as it is: the fused forward does, of the block's own forward nobody knows."""
+    x, block = inputs(), fused(Mlp(), inputs())
+    known = []
+    for act in (nn.SiLU(), nn.Tanh()):
+        block.act_fn = act
+        ctx = SumContext(None, 0, nn.Module(), block)
+        together.push_sum_context(ctx)
+        try:
+            with torch.inference_mode():
+                block(x)
+        finally:
+            together.pop_sum_context()
+        known.append(shard_modules.hands_through(ctx, block.down_proj))
+    assert known == [True, False]
