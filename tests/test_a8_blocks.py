@@ -120,3 +120,13 @@ def test_who_is_said_to_return_the_down_projections_output(calls):
             together.pop_sum_context()
         known.append(shard_modules.hands_through(ctx, block.down_proj))
     assert known == [True, False]
+
+
+def test_every_call_gives_the_same(calls):
+    """A block's first call as well, whose gate and up would be rounded to 16 bits by its own forward."""
+    block, x = Mlp(), inputs(40)
+    with torch.no_grad():
+        own = block(x)
+        quantize_linears_(block, activations=True)
+        first, second = block(x), block(x)
+    assert torch.equal(first, second) and not torch.equal(first, own)
