@@ -294,5 +294,5 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
         if activations:
             share_qkv_a8(parent)
         if activations and shard_modules.is_gated_silu_a8_mlp(parent):
-            parent.forward = types.MethodType(shard_modules._gated_mlp_a8_first_forward, parent)
+            parent.forward = types.MethodType(shard_modules._gated_mlp_a8_forward, parent)
     return replaced

@@ -17,6 +17,7 @@ input must already have the weight's dtype (a mismatch raises TypeError where `n
 """
 from __future__ import annotations
 
+import functools
 import types
 
 import torch
@@ -549,17 +550,47 @@ def _is_plain_silu(act) -> bool:
         type(act).__name__ == "SiLUActivation" and _native.stock_function(type(act).forward, "transformers.activations", "SiLUActivation.forward", ("nn", "functional", "silu"), ("self", "input"))
 
 
+class _Term:
+    """Stands in for a tensor of a forward that is read rather than run: what it was made of, by the block's children and products."""
+
+    __slots__ = ("of",)
+
+    def __init__(self, *of):
+        self.of = of
+
+    def __mul__(self, other):
+        return _Term(self.of, other.of) if type(other) is _Term else NotImplemented
+
+
+_GATED_PARTS = ("gate_proj", "up_proj", "act_fn", "down_proj")
+
+
+@functools.lru_cache(maxsize=256)
+def _computes_gated(forward) -> bool:
+    """Whether a function is forward(self, x) = down(act(gate(x)) * up(x)) of these children, whatever x: it looks up nothing else (so calling it changes nothing), and gives that for terms. An example
+    could not tell: the block's own roundings move hidden codes by a step here and there, a percent of the result, as much as another formula might, and a row of zeros is zero by any."""
+    code = getattr(forward, "__code__", None)
+    if type(forward) is not types.FunctionType or code.co_argcount != 2 or code.co_kwonlyargcount or code.co_freevars or not set(code.co_names) <= set(_GATED_PARTS):
+        return False
+    children = {name: lambda term, name=name: _Term(name, term.of) for name in _GATED_PARTS}
+    try:
+        (down, (first, second)) = forward(types.SimpleNamespace(**children), _Term("x")).of
+    except Exception:  # a term takes part in nothing else
+        return False
+    return down == "down_proj" and {first, second} == {("act_fn", ("gate_proj", ("x",))), ("up_proj", ("x",))}
+
+
 def _is_gated_a8(module: nn.Module, names: tuple = ("gate_proj", "up_proj")) -> bool:
-    """Whether gate and up can be one launch as they are now: Linears of 8-bit rows of one form, without a bias, and the SiLU, none of which anybody watches."""
-    if not _has_a8(module, names):
+    """Whether gate and up can be one launch as they are now: a block of that formula, Linears of 8-bit rows of one form, without a bias, and the SiLU, none of which anybody watches."""
+    if not _computes_gated(type(module).forward) or not _has_a8(module, names):
         return False
     gate, up = module._modules["gate_proj"], module._modules["up_proj"]
     return gate.bias is None and up.bias is None and gate.wq.shape == up.wq.shape and gate.dtype == up.dtype and _is_plain_silu(module._modules.get("act_fn", module.__dict__.get("act_fn")))
 
 
 def is_gated_silu_a8_mlp(module: nn.Module) -> bool:
-    """As is_gated_silu_mlp, of Linears with 8-bit rows."""
-    return "forward" not in module.__dict__ and _is_gated_a8(module, ("gate_proj", "up_proj", "down_proj"))
+    """As is_gated_silu_mlp, of Linears with 8-bit rows, by the block's own formula."""
+    return "forward" not in module.__dict__ and not any(hasattr(type(module), name) for name in _GATED_PARTS) and _is_gated_a8(module, ("gate_proj", "up_proj", "down_proj"))
 
 
 def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
@@ -568,23 +599,6 @@ def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
         return type(self).forward(self, x if isinstance(x, torch.Tensor) else x.dequantize())
     gate, up = self.gate_proj, self.up_proj
     return returned(self, _gated_mlp_a8_forward, self.down_proj, int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))
-
-
-def _gated_mlp_a8_first_forward(self, x: torch.Tensor) -> torch.Tensor:
-    """First call, as of _gated_mlp_first_forward, and the fused result, as every later call gives it. The block's own forward rounds gate, up and their product to 16 bits, which moves hidden codes by a step of 127 here and there: the two are
-    a percent of the result's spread apart in the mean (single values up to 8), where another function would be as far off as the result is large."""
-    del self.forward  # the class's forward is visible again
-    own = type(self).forward(self, x)
-    try:
-        fused = _gated_mlp_a8_forward(self, x)
-        same = isinstance(own, torch.Tensor) and own.shape == fused.shape and bool(
-            (own.detach().float() - fused.detach().float()).square().sum() <= 0.05**2 * own.detach().float().square().sum())
-    except (TypeError, ValueError, RuntimeError):
-        same = False
-    if not same:
-        return own
-    self.forward = types.MethodType(_gated_mlp_a8_forward, self)
-    return fused
 
 
 def install_shard_kernels(shard: nn.Module) -> None:

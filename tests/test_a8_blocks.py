@@ -130,3 +130,101 @@ def test_every_call_gives_the_same(calls):
         quantize_linears_(block, activations=True)
         first, second = block(x), block(x)
     assert torch.equal(first, second) and not torch.equal(first, own)
+
+
+class Exchanged(Mlp):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.up_proj(x)) * self.gate_proj(x))
+
+
+class Scaled(Mlp):
+    def forward(self, x):
+        return 1.02 * self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+class Shifted(Mlp):
+    def forward(self, x):
+        out = self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+        out += 0.01
+        return out
+
+
+class Residual(Mlp):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x)) + 0.01 * x
+
+
+class OneOfTwo(Mlp):
+    def forward(self, x):
+        if x.shape[0] > 7:
+            return self.up_proj(x)[:, :64]
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+class Squared(Mlp):
+    def forward(self, x):
+        g = self.act_fn(self.gate_proj(x))
+        return self.down_proj(g * g)
+
+
+class WithASetting(Mlp):
+    def forward(self, x, scale=None):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+@pytest.mark.parametrize("cls", [Exchanged, Scaled, Shifted, Residual, OneOfTwo, Squared, WithASetting])
+@pytest.mark.parametrize("first", ["zeros", "values"])
+def test_blocks_of_another_formula(calls, cls, first):
+    """They keep their own forward, whatever they are called with first."""
+    block = cls()
+    quantize_linears_(block, activations=True)
+    with torch.no_grad():
+        block(torch.zeros(5, 64).bfloat16() if first == "zeros" else inputs())
+        calls.clear()
+        for x in (inputs(), inputs(9)):
+            assert torch.equal(block(x), cls.forward(block, x))
+    assert "swiglu_up_a8" not in calls and not shard_modules.takes_rows(block)
+
+
+class InSteps(Mlp):
+    def forward(self, hidden):
+        """The same formula."""
+        up = self.up_proj(hidden)
+        up *= self.act_fn(self.gate_proj(hidden))
+        down = self.down_proj(up)
+        return down
+
+
+@pytest.mark.parametrize("cls", [Mlp, InSteps])
+def test_blocks_of_this_formula(calls, cls):
+    block = cls()
+    quantize_linears_(block, activations=True)
+    with torch.no_grad():
+        assert not block(torch.zeros(5, 64).bfloat16()).any()
+        assert calls == ["quantize_rows", "swiglu_up_a8", "quantize_rows", "linear_a8"]
+
+
+def test_a_class_that_is_given_another_forward(calls):
+    class Own(Mlp):
+        forward = Mlp.forward
+
+    block, x = fused(Own(), inputs()), inputs()
+    Own.forward = Scaled.forward
+    with torch.no_grad():
+        assert torch.equal(block(x), Scaled.forward(block, x)) and not shard_modules.takes_rows(block)
+
+
+def test_a_forward_that_keeps_something_is_not_called_ahead(calls):
+    """quantize_linears_ calls no forward of a program's that could tell."""
+    seen = []
+
+    class Counting(Mlp):
+        def forward(self, x):
+            seen.append(type(x))
+            return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+    block = Counting()
+    quantize_linears_(block, activations=True)
+    with torch.no_grad():
+        block(inputs())
+    assert seen == [torch.Tensor]
