@@ -173,13 +173,16 @@ def _share_qkv_storage(module: torch.nn.Module) -> bool:
     return True
 
 
+QKV = ("q_proj", "k_proj", "v_proj")
+
+
 def share_qkv_a8(module: torch.nn.Module) -> bool:
     """The same of Linears of 8-bit rows, where a module has them as q_proj, k_proj and v_proj: each one's codes and scales (and biases) become views of one matrix's rows."""
     from .shard_modules import _has_a8
 
-    if not _has_a8(module, ("q_proj", "k_proj", "v_proj")):
+    if not _has_a8(module, QKV):
         return False
-    parts = [module._modules[name] for name in ("q_proj", "k_proj", "v_proj")]
+    parts = [module._modules[name] for name in QKV]
     first = parts[0]
     if any(p.in_features != first.in_features or p.dtype != first.dtype or p.wq.device != first.wq.device or (p.bias is None) != (first.bias is None) for p in parts):
         return False
@@ -204,7 +207,7 @@ def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
 
     wq, scale, bias = self.__dict__["_tp_qkv8"]
     row = 0
-    for name in ("q_proj", "k_proj", "v_proj"):
+    for name in QKV:
         part = self._modules[name]
         if (part.wq.data_ptr() != wq.data_ptr() + row * wq.stride(0) or part.wq.stride() != wq.stride() or part.scale.data_ptr() != scale.data_ptr() + row * 4
                 or (None if part.bias is None else part.bias.data_ptr()) != (None if bias is None else bias.data_ptr() + row * bias.element_size())):
@@ -222,12 +225,13 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     from .shard_modules import ShardLinear, _guard, _has_a8
 
     B, S, _ = hidden_states.shape
-    if _has_a8(self, ("q_proj", "k_proj", "v_proj")) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
+    if _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
+        self.__dict__.pop("_tp_qkv", None)  # (of Linears that were replaced one by one)
         hidden_states = self.q_proj.rows_of(hidden_states)
         if "_tp_qkv8" in self.__dict__:
             qkv = _project_shared_a8(self, hidden_states)
             if qkv is not None:
-                return [part.view(B, S, -1, D) for part in qkv.split([self._modules[name].out_features for name in ("q_proj", "k_proj", "v_proj")], -1)]
+                return [part.view(B, S, -1, D) for part in qkv.split([self._modules[name].out_features for name in QKV], -1)]
     shared = self.__dict__.get("_tp_qkv")
     if shared is not None:
         w, b = shared
@@ -313,7 +317,7 @@ def _caches_for(self, hidden_states, position_embeddings, attention_mask, past_k
 
 def takes_rows(module: torch.nn.Module, forward, hidden_states: torch.Tensor, kwargs: dict) -> bool:
     """Whether a fused attention module would take this call, and only project the hidden states, by Linears of 8-bit rows."""
-    if forward is not _fused_rotary_forward or any(module._modules[name].dtype != hidden_states.dtype for name in ("q_proj", "k_proj", "v_proj")):
+    if forward is not _fused_rotary_forward or any(module._modules[name].dtype != hidden_states.dtype for name in QKV):
         return False
     more = dict(kwargs)
     return _caches_for(module, hidden_states, more.pop("position_embeddings", None), more.pop("attention_mask", None), more.pop("past_key_values", None), more) != (None, None)

@@ -33,7 +33,7 @@ from torch import nn
 
 from . import _native, together
 from . import shard_modules
-from .attention import share_qkv_a8
+from .attention import QKV, share_qkv_a8
 from .shard_modules import _guard, is_conv1d, product_in_context
 
 OutlierChoice = Union[None, Mapping[str, Sequence[int]], Callable[[str, nn.Module], Optional[Sequence[int]]]]
@@ -287,6 +287,8 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
                 new = ShardLinearW8.from_weight(weight, getattr(child, "bias", None), _outliers_of(outlier_cols, name, child))
             setattr(parent, child_name, new)
             replaced += 1
+            if child_name in QKV:  # their 16-bit weights laid out as one matrix (fuse_rotary_) have no reader any more
+                parent.__dict__.pop("_tp_qkv", None)
             # a SiLU-gated MLP block whose fused forward reads gate_proj.weight / up_proj.weight goes back to its own forward
             fused = parent.__dict__.get("forward")
             if getattr(fused, "__func__", None) in (shard_modules._gated_mlp_forward, shard_modules._gated_mlp_first_forward):

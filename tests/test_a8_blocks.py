@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch import nn
 
-from tensor_parallel_amd import _native, int8, shard_modules, together
+from tensor_parallel_amd import _native, attention, int8, shard_modules, together
 from tensor_parallel_amd.collectives import SumContext
 from tensor_parallel_amd.int8 import ShardLinearA8, quantize_linears_
 
@@ -228,3 +228,18 @@ def test_a_forward_that_keeps_something_is_not_called_ahead(calls):
     with torch.no_grad():
         block(inputs())
     assert seen == [torch.Tensor]
+
+
+def test_linears_of_8_bits_put_in_one_by_one_end_the_16_bit_sharing(calls):
+    """The matrix of 16-bit weights that fuse_rotary_ has laid out is given back once all three projections are of 8-bit rows."""
+    attn = nn.Module()
+    whole = torch.randn(3 * 64, 64).bfloat16()
+    attn.__dict__["_tp_qkv"] = (whole, None)
+    for i, name in enumerate(("q_proj", "k_proj", "v_proj")):
+        setattr(attn, name, ShardLinearA8(*rows64(whole[64 * i:64 * i + 64]), None, torch.bfloat16))
+    assert attention.share_qkv_a8(attn)
+    x = inputs()[None]
+    with torch.no_grad():
+        got = attention._project_qkv(attn, x, 32)
+    assert all(torch.equal(part.flatten(2), attn._modules[name](x)) for part, name in zip(got, ("q_proj", "k_proj", "v_proj")))
+    assert "_tp_qkv" not in attn.__dict__

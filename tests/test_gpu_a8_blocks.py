@@ -1,0 +1,36 @@
+"""Models of 8-bit rows on the device: what they leave of their 16-bit weights, and what moving and reloading them leaves of the layout that their products are fastest on."""
+import weakref
+
+import pytest
+import torch
+
+import tensor_parallel_amd as tp
+from tensor_parallel_amd import shard_modules
+from tensor_parallel_amd.int8 import quantize_linears_
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def llama(hidden=528):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    config = LlamaConfig(vocab_size=300, hidden_size=hidden, intermediate_size=720, num_hidden_layers=1, num_attention_heads=6, num_key_value_heads=2, head_dim=64, max_position_embeddings=256)
+    model = LlamaForCausalLM(config).to(DEV, torch.bfloat16).eval()
+    model.config._attn_implementation = tp.attention.register()
+    shard_modules.install_shard_kernels(model)
+    tp.attention.fuse_rotary_(model)
+    return model
+
+
+@pytest.mark.parametrize("activations", [True, False])
+def test_16_bit_weights_of_q_k_and_v_are_given_back(activations):
+    model = llama()
+    attn = model.model.layers[0].self_attn
+    whole = weakref.ref(attn.__dict__["_tp_qkv"][0])
+    before = torch.cuda.memory_allocated(DEV)
+    bits16 = whole().numel() * 2
+    n = quantize_linears_(model.model.layers, activations=activations)
+    assert n == 7 and whole() is None and "_tp_qkv" not in attn.__dict__
+    assert before - torch.cuda.memory_allocated(DEV) > bits16 // 3  # (the codes take half, and their rows begin on 128-byte boundaries)
