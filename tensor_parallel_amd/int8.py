@@ -272,6 +272,7 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
         raise ValueError("quantize_linears_: with 8-bit activations there are no outlier columns")
     replaced = 0
     for parent_name, parent in list(module.named_modules()):
+        projections = False  # whether one of q, k and v is replaced here
         for child_name, child in list(parent.named_children()):
             name = f"{parent_name}.{child_name}" if parent_name else child_name
             conv1d = is_conv1d(child)
@@ -289,11 +290,12 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
             replaced += 1
             if child_name in QKV:  # their 16-bit weights laid out as one matrix (fuse_rotary_) have no reader any more
                 parent.__dict__.pop("_tp_qkv", None)
+                projections = True
             # a SiLU-gated MLP block whose fused forward reads gate_proj.weight / up_proj.weight goes back to its own forward
             fused = parent.__dict__.get("forward")
             if getattr(fused, "__func__", None) in (shard_modules._gated_mlp_forward, shard_modules._gated_mlp_first_forward):
                 del parent.forward
-        if activations:
+        if activations and projections:  # (others' codes stay where they are: a recorded graph may read them)
             share_qkv_a8(parent)
         if activations and shard_modules.is_gated_silu_a8_mlp(parent):
             parent.forward = types.MethodType(shard_modules._gated_mlp_a8_forward, parent)

@@ -230,16 +230,30 @@ def test_a_forward_that_keeps_something_is_not_called_ahead(calls):
     assert seen == [torch.Tensor]
 
 
+def projections(whole, bias=False):
+    attn = nn.Module()
+    for i, name in enumerate(attention.QKV):
+        setattr(attn, name, ShardLinearA8(*rows64(whole[64 * i:64 * i + 64]), torch.randn(64).bfloat16() if bias else None, torch.bfloat16))
+    return attn
+
+
 def test_linears_of_8_bits_put_in_one_by_one_end_the_16_bit_sharing(calls):
     """The matrix of 16-bit weights that fuse_rotary_ has laid out is given back once all three projections are of 8-bit rows."""
-    attn = nn.Module()
     whole = torch.randn(3 * 64, 64).bfloat16()
+    attn = projections(whole)
     attn.__dict__["_tp_qkv"] = (whole, None)
-    for i, name in enumerate(("q_proj", "k_proj", "v_proj")):
-        setattr(attn, name, ShardLinearA8(*rows64(whole[64 * i:64 * i + 64]), None, torch.bfloat16))
     assert attention.share_qkv_a8(attn)
     x = inputs()[None]
     with torch.no_grad():
         got = attention._project_qkv(attn, x, 32)
-    assert all(torch.equal(part.flatten(2), attn._modules[name](x)) for part, name in zip(got, ("q_proj", "k_proj", "v_proj")))
+    assert all(torch.equal(part.flatten(2), attn._modules[name](x)) for part, name in zip(got, attention.QKV))
     assert "_tp_qkv" not in attn.__dict__
+
+
+def test_codes_stay_where_they_are_when_other_linears_are_quantised(calls):
+    """A graph that was recorded before may read them."""
+    model = nn.ModuleList([projections(torch.randn(3 * 64, 64).bfloat16())])
+    assert attention.share_qkv_a8(model[0])
+    at = [model[0]._modules[name].wq.data_ptr() for name in attention.QKV]
+    quantize_linears_(model, activations=True)
+    assert at == [model[0]._modules[name].wq.data_ptr() for name in attention.QKV]
