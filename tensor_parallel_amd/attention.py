@@ -222,10 +222,10 @@ def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
 def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     """q, k, v as [B, S, heads, D]: one call on the shared weight matrix when the three Linears still are views of it; Linears of 8-bit rows on rows that are
     quantised once."""
-    from .shard_modules import ShardLinear, _guard, _has_a8
+    from .shard_modules import ShardLinear, _guard, _has_a8, all_watched
 
     B, S, _ = hidden_states.shape
-    if _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
+    if not all_watched() and _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
         self.__dict__.pop("_tp_qkv", None)  # (of Linears that were replaced one by one)
         hidden_states = self.q_proj.rows_of(hidden_states)
         if "_tp_qkv8" in self.__dict__:

@@ -300,7 +300,7 @@ def int8_rows():
 def takes_rows(module, hidden_states=None, kwargs=None) -> bool:
     """Whether a block (wrapped by a rank's rules or not) of Linears with 8-bit rows may be handed `QuantizedRows` in the place of its input: a gated MLP, or, with the call's hidden
     states and arguments, a fused attention that will project them and do nothing else with them. Not where rules or hooks are told of the input."""
-    if module is None:
+    if module is None or all_watched():
         return False
     block = module._modules.get("tp_wrapped_module", module)
     own = getattr(block.__dict__.get("forward"), "__func__", None)
@@ -318,6 +318,12 @@ def takes_rows(module, hidden_states=None, kwargs=None) -> bool:
             "forward" in module.__dict__ or _has_hooks(block) or any(isinstance(target, int) or target in ("hidden_states", "x") for target in module.input_actions or ())):
         return False
     return True
+
+
+def all_watched() -> bool:
+    """Whether somebody is told of every module's calls (torch's hooks on all modules), which a launch for several of them would leave out."""
+    hooks = torch.nn.modules.module
+    return bool(hooks._global_forward_hooks or hooks._global_forward_pre_hooks)
 
 
 def _has_a8(module: nn.Module, names: tuple) -> bool:
@@ -595,7 +601,7 @@ def is_gated_silu_a8_mlp(module: nn.Module) -> bool:
 
 def _gated_mlp_a8_forward(self, x) -> torch.Tensor:
     """A SiLU-gated MLP of 8-bit rows, its input quantised once (or handed in as `QuantizedRows`), gate and up in one launch; its own forward where that is no longer what its parts are."""
-    if not _is_gated_a8(self):
+    if all_watched() or not _is_gated_a8(self):
         return type(self).forward(self, x if isinstance(x, torch.Tensor) else x.dequantize())
     gate, up = self.gate_proj, self.up_proj
     return returned(self, _gated_mlp_a8_forward, self.down_proj, int8_rows().swiglu_up(gate.rows_of(x), gate.wq, gate.scale, up.wq, up.scale))

@@ -257,3 +257,25 @@ def test_codes_stay_where_they_are_when_other_linears_are_quantised(calls):
     at = [model[0]._modules[name].wq.data_ptr() for name in attention.QKV]
     quantize_linears_(model, activations=True)
     assert at == [model[0]._modules[name].wq.data_ptr() for name in attention.QKV]
+
+
+def test_hooks_on_all_modules_are_told_of_every_linear(calls):
+    x, block, attn = inputs(), fused(Mlp(), inputs()), projections(torch.randn(3 * 64, 64).bfloat16())
+    attention.share_qkv_a8(attn)
+    told = []
+    for register in (nn.modules.module.register_module_forward_hook, nn.modules.module.register_module_forward_pre_hook):
+        told.clear()
+        handle = register(lambda mod, *rest: told.append(mod))
+        try:
+            with torch.no_grad():
+                block(x)
+                attention._project_qkv(attn, x[None], 32)
+            assert not shard_modules.takes_rows(block)
+        finally:
+            handle.remove()
+        assert {m for m in told if type(m) is ShardLinearA8} == {block.gate_proj, block.up_proj, block.down_proj, attn.q_proj, attn.k_proj, attn.v_proj}
+    calls.clear()
+    with torch.no_grad():
+        block(x)
+        attention._project_qkv(attn, x[None], 32)
+    assert calls == ["quantize_rows", "swiglu_up_a8", "quantize_rows", "linear_a8", "quantize_rows", "linear_a8"]
