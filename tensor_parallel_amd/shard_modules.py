@@ -127,7 +127,7 @@ def hands_through(ctx, module: nn.Module) -> bool:
         return True
     own, cls = wrapped.__dict__.get("forward"), type(wrapped)
     if own is not None:
-        return getattr(own, "__func__", None) is _gated_mlp_forward and wrapped._modules.get("down_proj") is module
+        return False
     last = "o_proj" if cls.forward is _llama_attention_forward else "dense_4h_to_h" if cls.forward is _falcon_mlp_forward else None
     return last is not None and cls._tp_base.forward is cls._tp_replaced and wrapped._modules.get(last) is module
 
@@ -494,11 +494,24 @@ def _is_silu(fn) -> bool:
     return name in ("silu", "siluactivation", "swish") or fn is torch.nn.functional.silu
 
 
-def _gated_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
-    gate, up, down = self.gate_proj, self.up_proj, self.down_proj
+def _gate_up(self, x: torch.Tensor) -> torch.Tensor:
+    gate, up = self.gate_proj, self.up_proj
     h = together.swiglu_up(x.detach(), gate.weight.detach(), up.weight.detach())
-    h = _guard(h, x, gate.weight, up.weight)
-    return down(h)
+    return _guard(h, x, gate.weight, up.weight)
+
+
+def _gated_parts(module: nn.Module) -> tuple:
+    return module._modules.get("gate_proj"), module._modules.get("up_proj"), module._modules.get("act_fn", module.__dict__.get("act_fn"))
+
+
+def _gated_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
+    """A SiLU-gated MLP with gate and up in one launch; its own forward where these and the activation no longer are the ones that it was found the same with, have a bias since, or are watched."""
+    gate, up, act = _gated_parts(self)
+    known = self.__dict__.get("_tp_gated", (gate, up, act))  # (a block that was pickled before there was this)
+    if (gate is not known[0] or up is not known[1] or act is not known[2] or all_watched() or gate.bias is not None or up.bias is not None
+            or any(isinstance(part, nn.Module) and ("forward" in part.__dict__ or _has_hooks(part)) for part in known)):
+        return type(self).forward(self, x)
+    return returned(self, _gated_mlp_forward, self.down_proj, _gate_up(self, x))
 
 
 def _has_hooks(module: nn.Module) -> bool:
@@ -531,12 +544,13 @@ def _gated_mlp_first_forward(self, x: torch.Tensor) -> torch.Tensor:
     del self.forward  # the class's forward is visible again
     own = type(self).forward(self, x)
     try:
-        fused = _gated_mlp_forward(self, x)
+        fused = self.down_proj(_gate_up(self, x))
         same = isinstance(own, torch.Tensor) and own.shape == fused.shape and torch.allclose(
             own.detach().float(), fused.detach().float(), rtol=2e-2, atol=2e-2 * float(own.detach().float().std()) + 1e-6)
     except (TypeError, ValueError, RuntimeError):
         same = False
     if same:
+        self.__dict__["_tp_gated"] = _gated_parts(self)
         self.forward = types.MethodType(_gated_mlp_forward, self)
     return own
 

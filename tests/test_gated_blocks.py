@@ -1,0 +1,105 @@
+"""Gated MLPs of 16-bit Linears whose parts change once gate and up are one launch. The launch is stood in for by torch on host tensors, so no GPU is needed."""
+import copy
+
+import pytest
+import torch
+from torch import nn
+
+from tensor_parallel_amd import _native, shard_modules, together
+from tensor_parallel_amd.collectives import SumContext
+
+
+class Mlp(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.gate_proj, self.up_proj, self.down_proj, self.act_fn = nn.Linear(64, 96, bias=False), nn.Linear(64, 96, bias=False), nn.Linear(96, 64, bias=False), nn.SiLU()
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+
+    def pair(x, wg, wu):
+        made.append("swiglu_up")
+        return nn.functional.silu(x @ wg.t()) * (x @ wu.t())
+
+    monkeypatch.setattr(_native, "swiglu_up", pair)
+    monkeypatch.setattr(_native, "linear", lambda x, w, b=None, **more: nn.functional.linear(x, w, b))
+    return made
+
+
+def fused():
+    torch.manual_seed(0)
+    block = Mlp().bfloat16()
+    shard_modules.install_shard_kernels(block)
+    with torch.no_grad():
+        block(inputs())
+    assert block.forward.__func__ is shard_modules._gated_mlp_forward
+    return block
+
+
+def inputs():
+    return torch.randn(5, 64, generator=torch.Generator().manual_seed(1)).bfloat16()
+
+
+def with_bias():
+    return nn.Linear(64, 96).bfloat16()
+
+
+@pytest.mark.parametrize("change", [
+    lambda m: setattr(m, "gate_proj", with_bias()),
+    lambda m: setattr(m, "up_proj", with_bias()),
+    lambda m: setattr(m.gate_proj, "bias", nn.Parameter(torch.randn(96).bfloat16())),
+    lambda m: setattr(m, "act_fn", nn.ReLU()),
+    lambda m: setattr(m.act_fn, "forward", torch.tanh),
+    lambda m: m.act_fn.register_forward_hook(lambda mod, args, out: 2 * out),
+    lambda m: m.up_proj.register_forward_hook(lambda mod, args, out: 2 * out),
+], ids=["gate with a bias", "up with a bias", "a bias assigned", "ReLU", "a forward of the SiLU's own", "a hook on the SiLU", "a hook on up"])
+def test_a_part_that_is_something_else_since(calls, change):
+    x, block = inputs(), fused()
+    with torch.no_grad():
+        before = block(x)
+        change(block)
+        calls.clear()
+        got, want = block(x), Mlp.forward(block, x)
+    assert not calls and torch.equal(got, want) and not torch.equal(got, before)
+
+
+def test_hooks_on_all_modules(calls):
+    block, told = fused(), []
+    handle = nn.modules.module.register_module_forward_hook(lambda mod, *rest: told.append(mod))
+    try:
+        with torch.no_grad():
+            block(inputs())
+    finally:
+        handle.remove()
+    assert block.gate_proj in told and block.up_proj in told and block.act_fn in told
+
+
+def test_the_launch_comes_back_and_goes_with_a_copy(calls):
+    x, block = inputs(), fused()
+    with torch.no_grad():
+        want, kept = block(x), block.act_fn
+        block.act_fn = nn.ReLU()
+        block(x)
+        block.act_fn = kept
+        calls.clear()
+        assert torch.equal(block(x), want) and torch.equal(copy.deepcopy(block)(x), want) and calls == ["swiglu_up"] * 2
+
+
+def test_who_is_said_to_return_the_down_projections_output(calls):
+    block, known = fused(), []
+    for act in (block.act_fn, nn.Tanh()):
+        block.act_fn = act
+        ctx = SumContext(None, 0, nn.Module(), block)
+        together.push_sum_context(ctx)
+        try:
+            with torch.inference_mode():
+                block(inputs())
+        finally:
+            together.pop_sum_context()
+        known.append(shard_modules.hands_through(ctx, block.down_proj))
+    assert known == [True, False]
