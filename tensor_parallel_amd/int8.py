@@ -214,6 +214,16 @@ class ShardLinearA8(nn.Module):
         self.register_buffer("scale", scale.contiguous())
         self.register_buffer("bias", None if bias is None else bias.detach().to(dtype).contiguous())
 
+    def _apply(self, fn, recurse=True):
+        """Moves with its module, and stays what it was quantised for: a model that is told its dtype once more (`.to(torch.bfloat16)`) would otherwise have 16-bit scales, which no product takes."""
+        scale, bias = self.scale, self.bias
+        super()._apply(fn, recurse)
+        if self.scale.dtype is not torch.float32:
+            self.scale = scale.to(self.scale.device)
+        if bias is not None and self.bias.dtype is not self.dtype:
+            self.bias = bias.to(self.bias.device)
+        return self
+
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)
         destination[prefix + "wq"] = destination[prefix + "wq"].contiguous()  # without the bytes between its rows

@@ -279,3 +279,17 @@ def test_hooks_on_all_modules_are_told_of_every_linear(calls):
         block(x)
         attention._project_qkv(attn, x[None], 32)
     assert calls == ["quantize_rows", "swiglu_up_a8", "quantize_rows", "linear_a8", "quantize_rows", "linear_a8"]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_model_that_is_told_its_dtype(calls, dtype):
+    """Scales stay in 32 bits and the bias in what the Linear was quantised for: the other dtype is refused with the input, as before."""
+    model = nn.ModuleList([a8(96, 64, bias=True), nn.Linear(4, 4)])
+    with torch.no_grad():
+        want = model[0](inputs())
+        model.to(dtype)
+        assert model[1].weight.dtype is dtype and model[0].scale.dtype is torch.float32 and model[0].bias.dtype is torch.bfloat16
+        assert torch.equal(model[0](inputs()), want)
+        if dtype is not torch.bfloat16:
+            with pytest.raises(TypeError, match="quantised for"):
+                model[0](inputs().to(dtype))
