@@ -193,6 +193,8 @@ def _in_lines(wq: torch.Tensor) -> torch.Tensor:
     K = wq.shape[1]
     if K % 128 == 0 or K % 16 != 0:
         return wq.contiguous()
+    if wq.stride(1) == 1 and wq.stride(0) % 128 == 0 and wq.stride(0) >= K and wq.storage_offset() % 128 == 0:
+        return wq  # they are
     lines = wq.new_zeros((wq.shape[0], (K + 127) // 128 * 128))
     lines[:, :K] = wq
     return lines[:, :K]
@@ -215,14 +217,21 @@ class ShardLinearA8(nn.Module):
         self.register_buffer("bias", None if bias is None else bias.detach().to(dtype).contiguous())
 
     def _apply(self, fn, recurse=True):
-        """Moves with its module, and stays what it was quantised for: a model that is told its dtype once more (`.to(torch.bfloat16)`) would otherwise have 16-bit scales, which no product takes."""
-        scale, bias = self.scale, self.bias
+        """Moves with its module, and stays what it was quantised for: a model that is told its dtype once more (`.to(torch.bfloat16)`) would otherwise have 16-bit scales, which no product takes.
+        Codes that have moved begin their rows on 128-byte boundaries again."""
+        scale, bias, codes = self.scale, self.bias, self.wq
         super()._apply(fn, recurse)
+        if self.wq is not codes:
+            self.wq = _in_lines(self.wq)
         if self.scale.dtype is not torch.float32:
             self.scale = scale.to(self.scale.device)
         if bias is not None and self.bias.dtype is not self.dtype:
             self.bias = bias.to(self.bias.device)
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self.wq = _in_lines(self.wq)  # (assign=True puts the saved tensor in)
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)

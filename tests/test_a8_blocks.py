@@ -293,3 +293,19 @@ def test_a_model_that_is_told_its_dtype(calls, dtype):
         if dtype is not torch.bfloat16:
             with pytest.raises(TypeError, match="quantised for"):
                 model[0](inputs().to(dtype))
+
+
+def moved(module):
+    """The module after a move to another device and back: as torch copies a view, without the bytes between its rows."""
+    return module._apply(lambda t: t.clone(memory_format=torch.contiguous_format))
+
+
+@pytest.mark.parametrize("change", [moved, lambda m: m.load_state_dict(m.state_dict(), assign=True)], ids=["moved", "assigned"])
+def test_rows_in_lines_again(calls, change):
+    mod, whole = a8(96, 80), a8(96, 256)
+    x = torch.randn(5, 80, generator=torch.Generator().manual_seed(1)).bfloat16()
+    with torch.no_grad():
+        want = mod(x)
+        for m in (mod, whole):
+            change(m)
+        assert mod.wq.stride() == (128, 1) and whole.wq.stride() == (256, 1) and torch.equal(mod(x), want)
