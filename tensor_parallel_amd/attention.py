@@ -187,8 +187,8 @@ def share_qkv_a8(module: torch.nn.Module) -> bool:
     if any(p.in_features != first.in_features or p.dtype != first.dtype or p.wq.device != first.wq.device or (p.bias is None) != (first.bias is None) for p in parts):
         return False
     rows = sum(p.out_features for p in parts)
-    whole = (first.wq.new_zeros((rows, first.wq.stride(0)))[:, :first.in_features], torch.cat([p.scale for p in parts]),
-             None if first.bias is None else torch.cat([p.bias for p in parts]))
+    whole = [first.wq.new_zeros((rows, first.wq.stride(0)))[:, :first.in_features], torch.cat([p.scale for p in parts]),
+             None if first.bias is None else torch.cat([p.bias for p in parts])]
     row = 0
     for p in parts:
         end = row + p.out_features
@@ -196,6 +196,7 @@ def share_qkv_a8(module: torch.nn.Module) -> bool:
         p.wq, p.scale = whole[0][row:end], whole[1][row:end]
         if p.bias is not None:
             p.bias = whole[2][row:end]
+        p.__dict__["_tp_rows_of"] = whole  # whichever of them moves empties it: the module does not keep what none of them reads
         row = end
     module.__dict__["_tp_qkv8"] = whole
     return True
@@ -228,7 +229,7 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     if not all_watched() and _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
         self.__dict__.pop("_tp_qkv", None)  # (of Linears that were replaced one by one)
         hidden_states = self.q_proj.rows_of(hidden_states)
-        if "_tp_qkv8" in self.__dict__:
+        if self.__dict__.get("_tp_qkv8"):
             qkv = _project_shared_a8(self, hidden_states)
             if qkv is not None:
                 return [part.view(B, S, -1, D) for part in qkv.split([self._modules[name].out_features for name in QKV], -1)]

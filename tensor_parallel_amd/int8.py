@@ -218,11 +218,12 @@ class ShardLinearA8(nn.Module):
 
     def _apply(self, fn, recurse=True):
         """Moves with its module, and stays what it was quantised for: a model that is told its dtype once more (`.to(torch.bfloat16)`) would otherwise have 16-bit scales, which no product takes.
-        Codes that have moved begin their rows on 128-byte boundaries again."""
+        Codes that have moved begin their rows on 128-byte boundaries again, and let go of the matrix that they were laid out in with others (attention.share_qkv_a8)."""
         scale, bias, codes = self.scale, self.bias, self.wq
         super()._apply(fn, recurse)
         if self.wq is not codes:
             self.wq = _in_lines(self.wq)
+            self.__dict__.pop("_tp_rows_of", []).clear()
         if self.scale.dtype is not torch.float32:
             self.scale = scale.to(self.scale.device)
         if bias is not None and self.bias.dtype is not self.dtype:
@@ -314,7 +315,7 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
             fused = parent.__dict__.get("forward")
             if getattr(fused, "__func__", None) in (shard_modules._gated_mlp_forward, shard_modules._gated_mlp_first_forward):
                 del parent.forward
-        if activations and projections:  # (others' codes stay where they are: a recorded graph may read them)
+        if activations and (projections or not parent.__dict__.get("_tp_qkv8")):  # (codes that are laid out already stay where they are: a recorded graph may read them)
             share_qkv_a8(parent)
         if activations and shard_modules.is_gated_silu_a8_mlp(parent):
             parent.forward = types.MethodType(shard_modules._gated_mlp_a8_forward, parent)

@@ -1,5 +1,8 @@
 """Gated MLPs and projections of 8-bit rows as modules: which calls their fused forwards make for the block's own and which they leave to it. The library's calls are stood in for by their definitions on
 host tensors, so no GPU is needed."""
+import copy
+import weakref
+
 import pytest
 import torch
 from torch import nn
@@ -309,3 +312,26 @@ def test_rows_in_lines_again(calls, change):
         for m in (mod, whole):
             change(m)
         assert mod.wq.stride() == (128, 1) and whole.wq.stride() == (256, 1) and torch.equal(mod(x), want)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_projections_that_move(calls, bias):
+    """They are three launches again, nothing keeps the matrix that they were laid out in, and quantize_linears_ lays them out anew."""
+    attn = projections(torch.randn(3 * 64, 64).bfloat16(), bias)
+    assert attention.share_qkv_a8(attn)
+    kept = [weakref.ref(t) for t in attn.__dict__["_tp_qkv8"] if t is not None]
+    with torch.no_grad():
+        want = attention._project_qkv(attn, inputs()[None], 32)
+        moved(attn)
+        assert not any(ref() is not None for ref in kept)
+        calls.clear()
+        got = attention._project_qkv(attn, inputs()[None], 32)
+        assert calls == ["quantize_rows"] + ["linear_a8"] * 3 and all(map(torch.equal, got, want))
+        quantize_linears_(nn.ModuleList([attn]), activations=True)
+        calls.clear()
+        got = attention._project_qkv(attn, inputs()[None], 32)
+        assert calls == ["quantize_rows", "linear_a8"] and all(map(torch.equal, got, want))
+        copied = copy.deepcopy(attn)
+        moved(attn)
+        calls.clear()
+        assert all(map(torch.equal, attention._project_qkv(copied, inputs()[None], 32), want)) and calls == ["quantize_rows", "linear_a8"]

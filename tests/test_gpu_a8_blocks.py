@@ -34,3 +34,28 @@ def test_16_bit_weights_of_q_k_and_v_are_given_back(activations):
     n = quantize_linears_(model.model.layers, activations=activations)
     assert n == 7 and whole() is None and "_tp_qkv" not in attn.__dict__
     assert before - torch.cuda.memory_allocated(DEV) > bits16 // 3  # (the codes take half, and their rows begin on 128-byte boundaries)
+
+
+def test_a_model_that_moves_to_the_host_and_back():
+    """Nothing of it stays on the device meanwhile; its rows begin on 128-byte boundaries again, and its logits are the same."""
+    from transformers import DynamicCache
+
+    before = torch.cuda.memory_allocated(DEV)
+    model = llama()
+    attn = model.model.layers[0].self_attn
+    quantize_linears_(model.model.layers, activations=True)
+    ids = torch.randint(2, 300, (2, 17), device=DEV)
+
+    def forward():
+        with torch.no_grad():
+            return model(input_ids=ids, past_key_values=DynamicCache(), use_cache=True).logits
+
+    want = forward()
+    model.to("cpu")
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated(DEV) - before <= want.numel() * 2 + ids.numel() * 8 + 4096
+    model.to(DEV)
+    assert attn.q_proj.wq.stride() == (640, 1) and model.model.layers[0].mlp.down_proj.wq.stride() == (768, 1)
+    assert torch.equal(forward(), want)
+    quantize_linears_(model.model.layers, activations=True)
+    assert attn.q_proj.wq.untyped_storage().data_ptr() == attn.v_proj.wq.untyped_storage().data_ptr() and torch.equal(forward(), want)
