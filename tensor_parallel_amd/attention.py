@@ -432,7 +432,8 @@ def fuse_rotary_(model: torch.nn.Module, class_names=FUSABLE_ATTENTION_CLASSES, 
     `share_qkv=True` (Llama pattern, rank shards already on the device): the weights of q_proj / k_proj / v_proj move into
     one matrix that each of them keeps a view of (names, shapes and values in `state_dict` stay what they were), and the
     fused forward multiplies by it once instead of three times: two launches and two host calls fewer per module and
-    decode step. A projection that is replaced later (quantised, say) ends the sharing for its module."""
+    decode step. A projection that is replaced later (quantised, say) ends the sharing for its module. Linears of 8-bit rows share by themselves
+    (`int8.quantize_linears_`), until they move to another device; a second call lays them out anew."""
     count = 0
     for module in model.modules():
         if "forward" in module.__dict__:
@@ -443,6 +444,8 @@ def fuse_rotary_(model: torch.nn.Module, class_names=FUSABLE_ATTENTION_CLASSES, 
                     module.__dict__["_tp_no_padding"] = True
                 if share_qkv and "_tp_qkv" not in module.__dict__:
                     _share_qkv_storage(module)
+                if share_qkv and not module.__dict__.get("_tp_qkv8"):  # (Linears of 8-bit rows, laid out when they were made, that have moved since)
+                    share_qkv_a8(module)
             continue
         if _is_llama_pattern(module, class_names):
             module.forward = types.MethodType(_fused_rotary_forward, module)

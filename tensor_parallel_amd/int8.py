@@ -315,7 +315,7 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
             fused = parent.__dict__.get("forward")
             if getattr(fused, "__func__", None) in (shard_modules._gated_mlp_forward, shard_modules._gated_mlp_first_forward):
                 del parent.forward
-        if activations and (projections or not parent.__dict__.get("_tp_qkv8")):  # (codes that are laid out already stay where they are: a recorded graph may read them)
+        if activations and projections:  # (others' codes stay where they are: a recorded graph may read them)
             share_qkv_a8(parent)
         if activations and shard_modules.is_gated_silu_a8_mlp(parent):
             parent.forward = types.MethodType(shard_modules._gated_mlp_a8_forward, parent)

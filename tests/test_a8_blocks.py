@@ -1,6 +1,7 @@
 """Gated MLPs and projections of 8-bit rows as modules: which calls their fused forwards make for the block's own and which they leave to it. The library's calls are stood in for by their definitions on
 host tensors, so no GPU is needed."""
 import copy
+import types
 import weakref
 
 import pytest
@@ -316,7 +317,7 @@ def test_rows_in_lines_again(calls, change):
 
 @pytest.mark.parametrize("bias", [False, True])
 def test_projections_that_move(calls, bias):
-    """They are three launches again, nothing keeps the matrix that they were laid out in, and quantize_linears_ lays them out anew."""
+    """They are three launches again, nothing keeps the matrix that they were laid out in, and fuse_rotary_ lays them out anew, where quantize_linears_ leaves what it does not replace."""
     attn = projections(torch.randn(3 * 64, 64).bfloat16(), bias)
     assert attention.share_qkv_a8(attn)
     kept = [weakref.ref(t) for t in attn.__dict__["_tp_qkv8"] if t is not None]
@@ -327,7 +328,11 @@ def test_projections_that_move(calls, bias):
         calls.clear()
         got = attention._project_qkv(attn, inputs()[None], 32)
         assert calls == ["quantize_rows"] + ["linear_a8"] * 3 and all(map(torch.equal, got, want))
+        at = [attn._modules[name].wq.data_ptr() for name in attention.QKV]
         quantize_linears_(nn.ModuleList([attn]), activations=True)
+        assert at == [attn._modules[name].wq.data_ptr() for name in attention.QKV]
+        attn.forward = types.MethodType(attention._fused_rotary_forward, attn)
+        attention.fuse_rotary_(nn.ModuleList([attn]))
         calls.clear()
         got = attention._project_qkv(attn, inputs()[None], 32)
         assert calls == ["quantize_rows", "linear_a8"] and all(map(torch.equal, got, want))

@@ -57,5 +57,5 @@ def test_a_model_that_moves_to_the_host_and_back():
     model.to(DEV)
     assert attn.q_proj.wq.stride() == (640, 1) and model.model.layers[0].mlp.down_proj.wq.stride() == (768, 1)
     assert torch.equal(forward(), want)
-    quantize_linears_(model.model.layers, activations=True)
+    tp.attention.fuse_rotary_(model)
     assert attn.q_proj.wq.untyped_storage().data_ptr() == attn.v_proj.wq.untyped_storage().data_ptr() and torch.equal(forward(), want)
