@@ -523,13 +523,18 @@ int launch_a8(const A8Params &p, int splits, hipStream_t s) {
     t.direct = t.store == 8 && (MODE == MODE_SWIGLU || p.act == TPAMD_ACT_NONE) && aligned(p.sw, 16) && aligned(p.sw2, 16) && aligned(p.bias, 8) &&
                (p.addend == nullptr || p.ldadd < (1ll << 21));
     const int kt = (p.K + A8_BK - 1) / A8_BK;
+    int dev = 0, cus = 256;
+    const size_t plane = static_cast<size_t>(t.tiles_m) * t.tiles_n * (BM * 64 * TN) * sizeof(int);  // a range's partial tiles
+    if (splits > 1) {  // no more ranges than every stream's buffer has room for, whichever call allocated it
+        TPAMD_HIP(hipGetDevice(&dev));
+        if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
+        const size_t most = scratch_reserve(cus) / plane;
+        splits = most < 1 ? 1 : most < static_cast<size_t>(splits) ? static_cast<int>(most) : splits;
+    }
     t.kt_per_split = (kt + splits - 1) / splits;
     t.splits = (kt + t.kt_per_split - 1) / t.kt_per_split;
     if (t.splits > 1) {
-        int dev = 0, cus = 256;
-        TPAMD_HIP(hipGetDevice(&dev));
-        if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
-        const size_t need = static_cast<size_t>(t.splits) * t.tiles_m * t.tiles_n * (BM * 64 * TN) * sizeof(int);
+        const size_t need = t.splits * plane;
         std::lock_guard<std::mutex> hold(splitk_mutex(dev));
         void *ws = nullptr;
         if (int rc = splitk_scratch(dev, s, need, scratch_reserve(cus), &ws); rc != TPAMD_OK) return rc;
