@@ -89,53 +89,74 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const RowCode &c) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// Step S of a butterfly over the wavefront whose earlier steps are done: one of a pair of lanes' values and, in `other`, the other one. Within rows of 16 lanes by the operand's lane permutation, between
-// rows by swaps: no trip through LDS.
+// Steps of a butterfly over the wavefront, between halves, rows of 16 lanes and inside rows: no trip through LDS. Swapping halves (or odd rows with even ones) of two registers and adding them up
+// also makes one of two values, each in the lanes of its half (of its rows), for the price of one.
+__device__ __forceinline__ float add_halves(float a, float b) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+__device__ __forceinline__ float add_rows(float a, float b) {
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
 template <int S>
-__device__ __forceinline__ uint32_t partner(uint32_t v, uint32_t &other) {
-    if constexpr (S < 4) {
-        constexpr int CTRL = S == 0 ? 0xB1 : S == 1 ? 0x4E : S == 2 ? 0x141 : 0x140;  // quads 1 0 3 2, 2 3 0 1; halves of a row and rows mirrored
-        other = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
-        return v;
-    } else {
-        const auto both = S == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        other = both[1];
-        return both[0];
-    }
+__device__ __forceinline__ uint32_t partner_in_row(uint32_t v) {
+    constexpr int CTRL = S == 0 ? 0xB1 : S == 1 ? 0x4E : S == 2 ? 0x141 : 0x140;  // quads 1 0 3 2, 2 3 0 1; halves of a row and rows mirrored
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float add_in_rows(float v) {
+    unrolled<4>([&](auto stage) { v += __uint_as_float(partner_in_row<decltype(stage)::value>(__float_as_uint(v))); });
+    return v;
+}
+__device__ __forceinline__ uint32_t most_of_wave(uint32_t v) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(halves[0], halves[1]);
+    const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(rows[0], rows[1]);
+    unrolled<4>([&](auto stage) { v = max(v, partner_in_row<decltype(stage)::value>(v)); });
+    return v;
 }
 
-// Sum (SUM) and maximum over the block, the same in every thread. `part`: two words for each wavefront.
-template <int WAVES, bool SUM>
-__device__ __forceinline__ void block_sum_max(float &sum, uint32_t &most, uint2 *part) {
-    unrolled<6>([&](auto stage) {
-        uint32_t other;
-        if constexpr (SUM) {
-            const uint32_t mine = __float_as_uint(sum);
-            sum = __uint_as_float(partner<decltype(stage)::value>(mine, other));
-            sum += __uint_as_float(other);
-        }
-        most = partner<decltype(stage)::value>(most, other);
-        most = most > other ? most : other;
-    });
+// Sum (SUM) and maximum over the block, the same in every thread. A thread has CH sums, of chunks that lie 64 * WAVES apart: each is added up over the wavefront, and the results, one for every 64
+// chunks of the row, as a tree: the row's two halves first, then halves of halves, its neighbours last. So a row's sum does not depend on how many wavefronts hold it, which a launch's number of
+// rows decides, and the tree's first steps are those inside a wavefront in every form.
+template <int WAVES, bool SUM, int CH>
+__device__ __forceinline__ float block_sum_max(const float (&sum)[CH], uint32_t &most) {
+    static_assert(CH == 1 || CH == 2 || CH == 4, "halves and rows of a wavefront");
+    __shared__ uint2 part[WAVES];
+    most = most_of_wave(most);
+    float s = 0.f;
+    if constexpr (SUM) {
+        if constexpr (CH == 1) s = add_halves(sum[0], sum[0]), s = add_in_rows(add_rows(s, s));
+        if constexpr (CH == 2) s = add_halves(sum[0], sum[1]), s = add_in_rows(add_rows(s, s)), s = add_halves(s, s);  // sums 0 and 1 in the halves
+        if constexpr (CH == 4) s = add_in_rows(add_rows(add_halves(sum[0], sum[1]), add_halves(sum[2], sum[3]))), s = add_rows(s, s), s = add_halves(s, s);  // sums 0, 2, 1, 3 in the rows
+    }
     if constexpr (WAVES > 1) {
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_uint2(__float_as_uint(sum), most);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_uint2(__float_as_uint(s), most);
         __syncthreads();
-        sum = 0.f;
+        float t[WAVES];
         most = 0;
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) {
             const uint2 v = part[i];
-            if constexpr (SUM) sum += __uint_as_float(v.x);
-            most = most > v.y ? most : v.y;
+            t[i] = __uint_as_float(v.x);
+            most = max(most, v.y);
+        }
+        if constexpr (SUM) {
+#pragma unroll
+            for (int n = WAVES / 2; n > 0; n /= 2)
+#pragma unroll
+                for (int i = 0; i < n; ++i) t[i] += t[i + n];
+            s = t[0];
         }
     }
+    return s;
 }
 
 // Rows of D elements, D a multiple of 8 and at most 64 * WAVES * CH * 8, every row of x, r, s on a 16-byte boundary and of q on an 8-byte one. A block holds its row in registers.
 template <int DT, int WAVES, int CH, bool NORM, bool ADD>
 __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
     constexpr int T = 64 * WAVES;
-    __shared__ uint2 part[WAVES];
     if (blockIdx.y != 0) {
         p.x += p.to.x; p.w += p.to.w; p.r += p.to.r; p.s += p.to.s; p.q += p.to.q;
         p.scale = reinterpret_cast<float *>(reinterpret_cast<char *>(p.scale) + p.to.scale);
@@ -173,18 +194,19 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
             if (i < n) s[i] = v[c];
         }
     }
-    float f[CH][8], sum = 0.f, zero = -0.f;
+    float f[CH][8], sum[CH], zero = -0.f;
     asm("" : "+v"(zero));  // products by fused operations that take their factors from 16 bits (fp16), instead of two conversions and a multiplication
     uint32_t most = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const uint32_t u[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
         const uint32_t g[4] = {wv[NORM ? c : 0].x, wv[NORM ? c : 0].y, wv[NORM ? c : 0].z, wv[NORM ? c : 0].w};
+        sum[c] = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float a = lo_half_to_f32<DT>(u[j]), b = hi_half_to_f32<DT>(u[j]);
             if constexpr (NORM) {
-                sum = fmaf(a, a, fmaf(b, b, sum));
+                sum[c] = fmaf(a, a, fmaf(b, b, sum[c]));
                 a = fmaf(a, lo_half_to_f32<DT>(g[j]), zero);
                 b = fmaf(b, hi_half_to_f32<DT>(g[j]), zero);
             }
@@ -193,8 +215,8 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
             most = max(most, max(abs_bits(a), abs_bits(b)));
         }
     }
-    block_sum_max<WAVES, NORM>(sum, most, part);
-    const RowCode code = row_code(most, NORM ? rsqrtf(sum / static_cast<float>(p.D) + p.eps) : 1.f);
+    const float squares = block_sum_max<WAVES, NORM>(sum, most);
+    const RowCode code = row_code(most, NORM ? rsqrtf(squares / static_cast<float>(p.D) + p.eps) : 1.f);
     if (threadIdx.x == 0) p.scale[row] = code.scale;
     uint2 *q = reinterpret_cast<uint2 *>(p.q + row * p.ldq);
 #pragma unroll
@@ -208,12 +230,11 @@ __global__ __launch_bounds__(64 * WAVES) void quantize_kernel(QuantParams p) {
 // Any length and alignment: element loads, x (ADD: the stored sum, by the thread that stored it) read twice.
 template <int DT, bool NORM, bool ADD>
 __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
-    __shared__ uint2 part[4];
     const int64_t row = blockIdx.x;
     const uint16_t *x = reinterpret_cast<const uint16_t *>(p.x) + row * p.ldx, *w = reinterpret_cast<const uint16_t *>(p.w);
     const uint16_t *r = reinterpret_cast<const uint16_t *>(p.r) + row * p.ldr;
     uint16_t *s = reinterpret_cast<uint16_t *>(p.s) + row * p.lds;
-    float sum = 0.f;
+    float sum[1] = {0.f};
     uint32_t most = 0;
     for (int i = threadIdx.x; i < p.D; i += 256) {
         float a = half_to_f32<DT>(x[i]);
@@ -221,12 +242,12 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
             s[i] = f32_to_half<DT>(half_to_f32<DT>(r[i]) + a);
             a = half_to_f32<DT>(s[i]);
         }
-        sum = fmaf(a, a, sum);
+        sum[0] = fmaf(a, a, sum[0]);
         if constexpr (NORM) a *= half_to_f32<DT>(w[i]);
         most = max(most, abs_bits(a));
     }
-    block_sum_max<4, NORM>(sum, most, part);
-    const RowCode code = row_code(most, NORM ? rsqrtf(sum / static_cast<float>(p.D) + p.eps) : 1.f);
+    const float squares = block_sum_max<4, NORM>(sum, most);
+    const RowCode code = row_code(most, NORM ? rsqrtf(squares / static_cast<float>(p.D) + p.eps) : 1.f);
     if (threadIdx.x == 0) p.scale[row] = code.scale;
     for (int i = threadIdx.x; i < p.D; i += 256) {
         const float a = half_to_f32<DT>(ADD ? s[i] : x[i]);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import tensor_parallel_amd as tp
-from tensor_parallel_amd import shard_modules
+from tensor_parallel_amd import int8, shard_modules
 from tensor_parallel_amd.int8 import quantize_linears_
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +59,19 @@ def test_a_model_that_moves_to_the_host_and_back():
     assert torch.equal(forward(), want)
     tp.attention.fuse_rotary_(model)
     assert attn.q_proj.wq.untyped_storage().data_ptr() == attn.v_proj.wq.untyped_storage().data_ptr() and torch.equal(forward(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [512, 1000, 2048, 2056, 4096, 5504, 8192, 11008, 16384])
+def test_a_row_has_the_same_scale_in_every_batch(d, dtype):
+    """Few rows are held by more wavefronts than the many of a large launch (2^23 values): codes and scales are the same bits, and with the addition in the same launch too."""
+    rows = (1 << 23) // d + 1
+    g = torch.Generator(device=DEV).manual_seed(d)
+    x = (torch.randn(rows, d, device=DEV, generator=g) * (torch.rand(rows, 1, device=DEV, generator=g) + 0.01)).to(dtype)
+    w = (1 + 0.3 * torch.randn(d, device=DEV, generator=g)).to(dtype)
+    whole = int8.rms_norm(x, w, 1e-5)
+    for n in (1, 7, rows - 1):
+        part = int8.rms_norm(x[:n], w, 1e-5)
+        assert torch.equal(part.codes, whole.codes[:n]) and torch.equal(part.scale, whole.scale[:n])
+    total, rows_ = int8.add_rms_norm(torch.zeros_like(x), x, w, 1e-5)
+    assert torch.equal(total, x) and torch.equal(rows_.codes, whole.codes) and torch.equal(rows_.scale, whole.scale)
