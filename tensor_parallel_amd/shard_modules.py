@@ -508,8 +508,8 @@ def _gated_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
     """A SiLU-gated MLP with gate and up in one launch; its own forward where these and the activation no longer are the ones that it was found the same with, have a bias since, or are watched."""
     gate, up, act = _gated_parts(self)
     known = self.__dict__.get("_tp_gated", (gate, up, act))  # (a block that was pickled before there was this)
-    if (gate is not known[0] or up is not known[1] or act is not known[2] or all_watched() or gate.bias is not None or up.bias is not None
-            or any(isinstance(part, nn.Module) and ("forward" in part.__dict__ or _has_hooks(part)) for part in known)):
+    if (gate is not known[0] or up is not known[1] or act is not known[2] or gate._parameters.get("bias", 0) is not None or up._parameters.get("bias", 0) is not None or all_watched()
+            or "forward" in gate.__dict__ or "forward" in up.__dict__ or _has_hooks(gate) or _has_hooks(up) or isinstance(act, nn.Module) and ("forward" in act.__dict__ or _has_hooks(act))):
         return type(self).forward(self, x)
     return returned(self, _gated_mlp_forward, self.down_proj, _gate_up(self, x))
 
@@ -566,8 +566,12 @@ def _is_plain_silu(act) -> bool:
         return True
     if not isinstance(act, nn.Module) or "forward" in act.__dict__ or _has_hooks(act):
         return False
-    return type(act) is nn.SiLU and nn.SiLU.forward is _own_silu or \
-        type(act).__name__ == "SiLUActivation" and _native.stock_function(type(act).forward, "transformers.activations", "SiLUActivation.forward", ("nn", "functional", "silu"), ("self", "input"))
+    return nn.SiLU.forward is _own_silu if type(act) is nn.SiLU else type(act).__name__ == "SiLUActivation" and _is_transformers_silu(type(act).forward)
+
+
+@functools.lru_cache(maxsize=16)
+def _is_transformers_silu(forward) -> bool:
+    return _native.stock_function(forward, "transformers.activations", "SiLUActivation.forward", ("nn", "functional", "silu"), ("self", "input"))
 
 
 class _Term:
@@ -605,7 +609,8 @@ def _is_gated_a8(module: nn.Module, names: tuple = ("gate_proj", "up_proj")) -> 
     if not _computes_gated(type(module).forward) or not _has_a8(module, names):
         return False
     gate, up = module._modules["gate_proj"], module._modules["up_proj"]
-    return gate.bias is None and up.bias is None and gate.wq.shape == up.wq.shape and gate.dtype == up.dtype and _is_plain_silu(module._modules.get("act_fn", module.__dict__.get("act_fn")))
+    return gate._buffers.get("bias", 0) is None and up._buffers.get("bias", 0) is None and gate.out_features == up.out_features and gate.in_features == up.in_features and gate.dtype is up.dtype and \
+        _is_plain_silu(module._modules.get("act_fn", module.__dict__.get("act_fn")))
 
 
 def is_gated_silu_a8_mlp(module: nn.Module) -> bool:

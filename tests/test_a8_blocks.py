@@ -81,11 +81,12 @@ def inputs(rows=5):
     lambda m: setattr(m, "gate_proj", a8(96, 64, bias=True)),
     lambda m: setattr(m, "up_proj", a8(96, 64, bias=True)),
     lambda m: setattr(m.gate_proj, "bias", torch.randn(96).bfloat16()),
+    lambda m: setattr(m.gate_proj, "bias", nn.Parameter(torch.randn(96).bfloat16())),
     lambda m: setattr(m, "act_fn", nn.ReLU()),
     lambda m: setattr(m, "act_fn", nn.GELU()),
     lambda m: setattr(m.act_fn, "forward", torch.tanh),
     lambda m: m.act_fn.register_forward_hook(lambda mod, args, out: 2 * out),
-], ids=["gate with a bias", "up with a bias", "a bias assigned", "ReLU", "GELU", "a forward of the SiLU's own", "a hook on the SiLU"])
+], ids=["gate with a bias", "up with a bias", "a bias assigned", "a bias to be learned", "ReLU", "GELU", "a forward of the SiLU's own", "a hook on the SiLU"])
 def test_a_part_that_is_something_else_since(calls, change):
     """What stands in gate's, up's or the activation's place is what the block computes with, whether a Linear or the layer around hands the input over."""
     x, block = inputs(), fused(Mlp(), inputs())
