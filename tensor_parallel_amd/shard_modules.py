@@ -505,10 +505,11 @@ def _gated_parts(module: nn.Module) -> tuple:
 
 
 def _gated_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
-    """A SiLU-gated MLP with gate and up in one launch; its own forward where these and the activation no longer are the ones that it was found the same with, have a bias since, or are watched."""
+    """A SiLU-gated MLP with gate and up in one launch; its own forward where these no longer are of the classes, or the activation the one, that it was found the same with, have a bias since, or are
+    watched."""
     gate, up, act = _gated_parts(self)
-    known = self.__dict__.get("_tp_gated", (gate, up, act))  # (a block that was pickled before there was this)
-    if (gate is not known[0] or up is not known[1] or act is not known[2] or gate._parameters.get("bias", 0) is not None or up._parameters.get("bias", 0) is not None or all_watched()
+    known = self.__dict__.get("_tp_gated", (type(gate), type(up), act))  # (a block that was pickled before there was this)
+    if (type(gate) is not known[0] or type(up) is not known[1] or act is not known[2] or gate._parameters.get("bias", 0) is not None or up._parameters.get("bias", 0) is not None or all_watched()
             or "forward" in gate.__dict__ or "forward" in up.__dict__ or _has_hooks(gate) or _has_hooks(up) or isinstance(act, nn.Module) and ("forward" in act.__dict__ or _has_hooks(act))):
         return type(self).forward(self, x)
     return returned(self, _gated_mlp_forward, self.down_proj, _gate_up(self, x))
@@ -550,7 +551,8 @@ def _gated_mlp_first_forward(self, x: torch.Tensor) -> torch.Tensor:
     except (TypeError, ValueError, RuntimeError):
         same = False
     if same:
-        self.__dict__["_tp_gated"] = _gated_parts(self)
+        gate, up, act = _gated_parts(self)
+        self.__dict__["_tp_gated"] = (type(gate), type(up), act)
         self.forward = types.MethodType(_gated_mlp_forward, self)
     return own
 

@@ -1,5 +1,7 @@
 """Gated MLPs of 16-bit Linears whose parts change once gate and up are one launch. The launch is stood in for by torch on host tensors, so no GPU is needed."""
 import copy
+import gc
+import weakref
 
 import pytest
 import torch
@@ -88,6 +90,21 @@ def test_the_launch_comes_back_and_goes_with_a_copy(calls):
         block.act_fn = kept
         calls.clear()
         assert torch.equal(block(x), want) and torch.equal(copy.deepcopy(block)(x), want) and calls == ["swiglu_up"] * 2
+
+
+def test_a_linear_of_the_same_kind_in_gates_place(calls):
+    """It is what the launch multiplies by, and nothing keeps the one before."""
+    x, block = inputs(), fused()
+    before = weakref.ref(block.gate_proj)
+    new = nn.Linear(64, 96, bias=False).bfloat16()
+    new.__class__ = shard_modules.ShardLinear
+    block.gate_proj = new
+    calls.clear()
+    with torch.no_grad():
+        assert torch.equal(block(x), Mlp.forward(block, x)) and calls == ["swiglu_up"]
+    del new
+    gc.collect()
+    assert before() is None
 
 
 def test_who_is_said_to_return_the_down_projections_output(calls):
