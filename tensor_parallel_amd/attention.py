@@ -223,10 +223,11 @@ def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
 def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     """q, k, v as [B, S, heads, D]: one call on the shared weight matrix when the three Linears still are views of it; Linears of 8-bit rows on rows that are
     quantised once."""
-    from .shard_modules import ShardLinear, _guard, _has_a8, all_watched
+    from .shard_modules import ShardLinear, _guard, _has_a8, _has_hooks, all_watched
 
     B, S, _ = hidden_states.shape
-    if not all_watched() and _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
+    watched = all_watched()
+    if not watched and _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
         self.__dict__.pop("_tp_qkv", None)  # (of Linears that were replaced one by one)
         hidden_states = self.q_proj.rows_of(hidden_states)
         if self.__dict__.get("_tp_qkv8"):
@@ -245,7 +246,7 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
             intact = (q_proj.weight.data_ptr() == w.data_ptr() and q_proj.weight.shape[0] == nq and v_proj.weight.shape[0] == nk
                       and k_proj.weight.data_ptr() == w.data_ptr() + nq * row_bytes
                       and v_proj.weight.data_ptr() == w.data_ptr() + (nq + nk) * row_bytes)
-        if intact and hidden_states.dtype == w.dtype:
+        if intact and hidden_states.dtype == w.dtype and not watched and not any("forward" in p.__dict__ or _has_hooks(p) for p in (q_proj, k_proj, v_proj)):
             qkv = _guard(together.linear(hidden_states.detach(), w, b), hidden_states, q_proj.weight)
             return (qkv[..., :nq].view(B, S, -1, D), qkv[..., nq:nq + nk].view(B, S, -1, D), qkv[..., nq + nk:].view(B, S, -1, D))
         if not intact:  # a projection was replaced (quantised, re-assigned): three calls from now on

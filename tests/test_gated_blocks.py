@@ -1,4 +1,5 @@
-"""Gated MLPs of 16-bit Linears whose parts change once gate and up are one launch. The launch is stood in for by torch on host tensors, so no GPU is needed."""
+"""Gated MLPs and projections of 16-bit Linears whose parts change, or are watched, once gate and up, or q, k and v, are one launch. The launch is stood in for by torch on host tensors, so no GPU is
+needed."""
 import copy
 import gc
 import weakref
@@ -7,7 +8,7 @@ import pytest
 import torch
 from torch import nn
 
-from tensor_parallel_amd import _native, shard_modules, together
+from tensor_parallel_amd import _native, attention, shard_modules, together
 from tensor_parallel_amd.collectives import SumContext
 
 
@@ -120,3 +121,36 @@ def test_who_is_said_to_return_the_down_projections_output(calls):
             together.pop_sum_context()
         known.append(shard_modules.hands_through(ctx, block.down_proj))
     assert known == [True, False]
+
+
+def test_projections_that_are_watched(calls, monkeypatch):
+    """A hook on one of q, k and v or on all modules is told of their calls; without one they are one launch again."""
+    inner, launches = _native.linear, []
+    monkeypatch.setattr(_native, "linear", lambda x, w, b=None, **more: launches.append(w.shape[0]) or inner(x, w, b))
+    torch.manual_seed(0)
+    attn, whole = nn.Module(), torch.randn(96, 64).bfloat16()
+    for name, rows in (("q_proj", (0, 64)), ("k_proj", (64, 80)), ("v_proj", (80, 96))):
+        part = nn.Linear(64, rows[1] - rows[0], bias=False)
+        part.__class__, part.weight = shard_modules.ShardLinear, nn.Parameter(whole[slice(*rows)])
+        setattr(attn, name, part)
+    attn.__dict__["_tp_qkv"] = (whole, None)
+    x, told = inputs()[None], []
+
+    def project():
+        launches.clear()
+        with torch.no_grad():
+            return [part.flatten(2) for part in attention._project_qkv(attn, x, 16)]
+
+    want = project()
+    assert launches == [96]
+    for register in (attn.k_proj.register_forward_hook, nn.modules.module.register_module_forward_hook):
+        handle = register(lambda mod, args, out: told.append(mod))
+        try:
+            got = project()
+        finally:
+            handle.remove()
+        assert launches == [64, 16, 16] and attn.k_proj in told
+        for a, b in zip(got, want):
+            torch.testing.assert_close(a.float(), b.float(), rtol=2.0**-7, atol=64 * 2.0**-24 * 64)  # (torch may add these up in another order: a step of bf16 each)
+        told.clear()
+    assert all(map(torch.equal, project(), want)) and launches == [96]
