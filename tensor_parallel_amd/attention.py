@@ -246,6 +246,8 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
             intact = (q_proj.weight.data_ptr() == w.data_ptr() and q_proj.weight.shape[0] == nq and v_proj.weight.shape[0] == nk
                       and k_proj.weight.data_ptr() == w.data_ptr() + nq * row_bytes
                       and v_proj.weight.data_ptr() == w.data_ptr() + (nq + nk) * row_bytes)
+            for p, row in ((q_proj, 0), (k_proj, nq), (v_proj, nq + nk)):
+                intact = intact and (p.bias is None if b is None else p.bias is not None and p.bias.data_ptr() == b.data_ptr() + row * b.element_size())
         if intact and hidden_states.dtype == w.dtype and not watched and not any("forward" in p.__dict__ or _has_hooks(p) for p in (q_proj, k_proj, v_proj)):
             qkv = _guard(together.linear(hidden_states.detach(), w, b), hidden_states, q_proj.weight)
             return (qkv[..., :nq].view(B, S, -1, D), qkv[..., nq:nq + nk].view(B, S, -1, D), qkv[..., nq + nk:].view(B, S, -1, D))

@@ -123,17 +123,25 @@ def test_who_is_said_to_return_the_down_projections_output(calls):
     assert known == [True, False]
 
 
+def projections(bias):
+    """q, k and v as fuse_rotary_ lays them out."""
+    torch.manual_seed(0)
+    attn, whole, shift = nn.Module(), torch.randn(96, 64).bfloat16(), torch.randn(96).bfloat16()
+    for name, rows in (("q_proj", (0, 64)), ("k_proj", (64, 80)), ("v_proj", (80, 96))):
+        part = nn.Linear(64, rows[1] - rows[0], bias=bias)
+        part.__class__, part.weight = shard_modules.ShardLinear, nn.Parameter(whole[slice(*rows)])
+        if bias:
+            part.bias = nn.Parameter(shift[slice(*rows)])
+        setattr(attn, name, part)
+    attn.__dict__["_tp_qkv"] = (whole, shift if bias else None)
+    return attn
+
+
 def test_projections_that_are_watched(calls, monkeypatch):
     """A hook on one of q, k and v or on all modules is told of their calls; without one they are one launch again."""
     inner, launches = _native.linear, []
     monkeypatch.setattr(_native, "linear", lambda x, w, b=None, **more: launches.append(w.shape[0]) or inner(x, w, b))
-    torch.manual_seed(0)
-    attn, whole = nn.Module(), torch.randn(96, 64).bfloat16()
-    for name, rows in (("q_proj", (0, 64)), ("k_proj", (64, 80)), ("v_proj", (80, 96))):
-        part = nn.Linear(64, rows[1] - rows[0], bias=False)
-        part.__class__, part.weight = shard_modules.ShardLinear, nn.Parameter(whole[slice(*rows)])
-        setattr(attn, name, part)
-    attn.__dict__["_tp_qkv"] = (whole, None)
+    attn = projections(False)
     x, told = inputs()[None], []
 
     def project():
@@ -154,3 +162,13 @@ def test_projections_that_are_watched(calls, monkeypatch):
             torch.testing.assert_close(a.float(), b.float(), rtol=2.0**-7, atol=64 * 2.0**-24 * 64)  # (torch may add these up in another order: a step of bf16 each)
         told.clear()
     assert all(map(torch.equal, project(), want)) and launches == [96]
+
+
+@pytest.mark.parametrize("change", ["another", "none", "one where there was none"])
+def test_a_projection_with_another_bias(calls, change):
+    attn, x = projections(change != "one where there was none"), inputs()[None]
+    with torch.no_grad():
+        attention._project_qkv(attn, x, 16)
+        attn.k_proj.bias = None if change == "none" else nn.Parameter(torch.randn(16).bfloat16())
+        got = attention._project_qkv(attn, x, 16)
+        assert all(torch.equal(part.flatten(2), attn._modules[name](x)) for part, name in zip(got, attention.QKV))
