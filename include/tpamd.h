@@ -430,7 +430,8 @@ int tpamd_linear_w8_add(const void *x_dev, const void *wq_dev, const void *scale
  * Rows in 8 bits with a scale each: a = max over the row of |x|, q = round_half_even(127 x / a) of the exact quotient, scale = a / 127 (fp32); scale = 1 and codes of
  * 0 where no value of the row is 2^-100 or more; scale = NaN and codes of 0 where the row holds an infinity or NaN. x [rows, D] in `dtype` (BF16 or F16), q int8 [rows, D],
  * scale fp32 [rows]; elements between rows in ldx, ldq, the bytes between D and ldq are left alone. Any length below 2^30 and any alignment; rows of up to 16384
- * elements, a multiple of 8, on 16-byte boundaries (q: 8) are read once. Outputs overlap no input. */
+ * elements, a multiple of 8, on 16-byte boundaries (q: 8) are read once. Outputs overlap no input. A row's codes and scale do not depend on the other rows of a call, nor on their number; the scale of a
+ * norm's row off these boundaries may differ by rounding from that of the same row on them. */
 int tpamd_quantize_rows(const void *x_dev, void *q_dev, void *scale_dev, int64_t rows, int64_t D, int64_t ldx, int64_t ldq, int dtype, void *stream);
 /* y = scale * q, rounded to `dtype` (BF16, F16 or F32). */
 int tpamd_dequantize_rows(const void *q_dev, const void *scale_dev, void *y_dev, int64_t rows, int64_t D, int64_t ldq, int64_t ldy, int dtype, void *stream);
@@ -444,7 +445,7 @@ int tpamd_add_rms_norm_q8(const void *x_dev, const void *r_dev, const void *w_de
 /* Shard Linears of 8-bit rows: y[m,n] = act(xscale[m] * wscale[n] * sum_k x[m,k] * w[n,k] + bias[n]), x int8 [M,K], w int8 [N,K], scales fp32, y and bias in `dtype` (BF16 or
  * F16). The sum is exact in int32 (K up to 131071, TPAMD_ERR_UNSUPPORTED beyond), so results do not depend on how it is taken; everything behind it in fp32, rounded
  * once. Any pitch and alignment, and shapes of fewer than 2^24 tiles (of 64 x 64 outputs at the smallest); K a multiple of 16 and rows of x and w on 16-byte boundaries run on the matrix pipe,
- * rows on 128-byte boundaries fastest. A call may split K, its partial sums in the stream's scratch buffer. */
+ * rows on 128-byte boundaries fastest; any others take 20 to 75 times as long (append zeros to rows of another K). A call may split K, its partial sums in the stream's scratch buffer. */
 int tpamd_linear_a8(const void *x_dev, const void *xscale_dev, const void *w_dev, const void *wscale_dev, const void *bias_dev, void *y_dev, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t ldy, int dtype, int act, void *stream);
 /* Followed by one step of the partial-sum reduction, y = round_dtype(round_dtype(...) + addend), as tpamd_linear_add; with copy_dev (may be NULL) every result is stored there

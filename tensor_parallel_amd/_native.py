@@ -1280,8 +1280,8 @@ def _half_code(x: torch.Tensor, what: str) -> int:
 
 
 def _new_codes(x: torch.Tensor, shape: torch.Size, M: int, D: int) -> tuple:
-    """Codes of M rows of x's shape, their scales, and the elements between rows: those of tiled products (more than 64 rows) begin on 128-byte boundaries (2048 x 4096 x 2752 31.7 us, in lines 28.9;
-    fewer rows stay in the L2, where it makes a difference of 0.5)."""
+    """Codes of M rows of x's shape, their scales, and the elements between rows: those of tiled products (more than 64 rows) begin on 128-byte boundaries (2048 x 4096 x 2752 30.2 us, weights' and
+    input's rows in lines 27.9; fewer rows stay in the L2, where it makes a difference of 0.5)."""
     scale_ = x.new_empty(shape[:-1], dtype=torch.float32)
     if M <= 64 or D % 128 == 0 or D % 16 != 0:
         return x.new_empty(shape, dtype=torch.int8), scale_, D or 1
@@ -1290,8 +1290,8 @@ def _new_codes(x: torch.Tensor, shape: torch.Size, M: int, D: int) -> tuple:
 
 
 def quantize_rows(x: torch.Tensor) -> tuple:
-    """(codes int8, scale fp32 [...]) of the rows of x: code = the integer nearest to 127 x / max |x| of the row (ties to even), scale = max |x| / 127; 1 for a row of
-    zeros, NaN (and codes of 0) for one with an infinity or NaN."""
+    """(codes int8, scale fp32 [...]) of the rows of x: code = the integer nearest to 127 x / max |x| of the row (ties to even), scale = max |x| / 127; 1 (and codes of 0)
+    for a row without a value of 2^-100 or more, NaN (and codes of 0) for one with an infinity or NaN."""
     code, shape = _half_code(x, "quantize_rows"), x.shape
     x2, M, ldx = _flat_rows(x, shape)
     D = shape[-1]

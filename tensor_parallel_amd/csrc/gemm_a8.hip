@@ -97,10 +97,10 @@ __device__ __forceinline__ void lds_write_acc(uint32_t addr, i32x4 v) {
 // barrier: tile g + 1 has landed, tile g is read out; the loads of tile g + NS go into its stage in the rest of that step and the first of the next tile.
 // K ends in a multiple of 16: in the last stage the pieces of x behind it are asked for outside the descriptor's range, which gives zeros, and what stands in those of w
 // (the next row, or the bytes between rows) counts for nothing.
-// Bound: by the power that the matrix pipe takes on real codes: a K tile of a 256 x 256 tile takes 1.6 us with every CU at it (2.7 POP/s), 1.06 on zeros. 4096 x 4096 x 5504 in 82-86 us (2.15-2.25 POP/s; 90
-// with an addend that comes from memory, most of it under the last K tiles), 4096 x 16384 x 8192 in 445 (2.47), the pair of 4096 x 5504 x 4096 in 165 (2.24).
-// Smaller tiles by what LDS and the L2 deliver: 645 x 6144 x 4096 on 128 x 192 tiles, one to a CU, 24 us, 28 on weights from memory; a fourth or fifth stage changes nothing. Rows that begin
-// inside 128-byte lines cost a fifth more (each of their lines is asked for in two K tiles).
+// Bound: by the power that the matrix pipe takes on real codes: a K tile of a 256 x 256 tile takes 1.6 us with every CU at it (2.7 POP/s), 1.06 on zeros. 4096 x 4096 x 5504 in 78-86 us (2.15-2.35 POP/s; 86-91
+// with an addend, most of it loaded under the last K tiles; 95 with the GELU, whose epilogue goes through LDS), 4096 x 16384 x 8192 in 439 (2.5; with the GELU 489), the pair of 4096 x 5504 x 4096 in 162 (2.28).
+// Smaller tiles by what LDS and the L2 deliver: 645 x 6144 x 4096 on 128 x 192 tiles, one to a CU, 23 us, 25-28 on weights from memory; a fourth or fifth stage changes nothing. Rows that begin
+// inside 128-byte lines cost 8-20 % more (each of their lines is asked for in two K tiles): the pair of 4096 x 5504 x 4112 198 us, in lines 170, 2048 x 4096 x 2752 30.2 and 27.9.
 // SPLIT: a block has one of t.splits ranges of K; its sums go to t.ws as they lie in the registers and are added by finish_a8_kernel.
 constexpr int a8_slab_rows(int tm, int tn) { return tm == 3 && tn == 4 ? 1 : tm == 4 ? 2 : tm; }  // MFMA tiles of rows
 constexpr int a8_lds(int tm, int tn, int ns) {

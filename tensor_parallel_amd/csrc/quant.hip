@@ -3,15 +3,17 @@
 //   p = x, or t w of the norm's input t (round(r + x) with a residual);  a = max |p| over the row
 //   codes  round_half_even(127 p / a)     scale  a f / 127, f = 1 or rsqrt(mean t^2 + eps)
 // The norm's factor is the same for a whole row, so it is in the scale alone: a row's codes do not depend on how its squares are summed, the maximum is found in
-// the pass that sums them, and one meeting of the block serves both.
+// the pass that sums them, and one meeting of the block serves both. The scale does not depend on the launch's number of rows either (block_sum_max); rows off the boundaries of quantize_kernel
+// sum in an order of their own, and theirs may differ by rounding.
 // A code is the integer nearest to the exact quotient: in rows of 16-bit values many quotients lie on a half (a value of half the largest is 63.5), which a product with a
 // rounded 127 / a would put on either side. What the product leaves within 2^-15 of a half (its error is below 127 * 2 * 2^-24: one rounding each of 127 / a and of the product) is
 // compared with the half exactly; p is exact in fp32 (two 16-bit significands). Eight codes ask once whether one is that near.
 // A row that holds an infinity or NaN has no scale: it gets NaN, and codes of 0, so that products with it are NaN. One without a value of 2^-100 or more gets 1 and codes of 0.
 //
-// Bound: at a few rows by the latency of a launch (2.2-2.5 us in a graph, 1 x 4096; the shortest launches here take 1.7), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
-// once, by the instructions between their loads and their stores: 2103 x 4096 quantised in 8.8 us (2.9 TB/s), normed 9.2, 4096 x 8192 18.8 (5.3 TB/s) and 20.5, with the addition 37.3 (6.3 TB/s);
-// the way back of 4096 x 8192 to fp32 27.7 (6.0 TB/s).
+// Bound: at a few rows by the latency of a launch (2.1-2.3 us in a graph, 1 x 4096; the shortest launches here take 1.7), else by HBM (x, r read once; sum and codes written once) and, as all rows of up to some 2000 are under way at
+// once, by the instructions between their loads and their stores. In a graph, operands and results rotated through more memory than the caches hold, bf16: 2103 x 4096 quantised in 9.3 us (2.8 TB/s), normed 8.7,
+// with the addition 14.5 (4.1); 4096 x 8192 21.2 (4.8), 21.3 and 42 (5.6); 4096 x 16384 37.7 (5.3), 37.9 and 83 (5.7), the way back of those to fp32 56.6 (5.9). Rows off the boundaries, single values at a time:
+// 2103 x 4098 24, 25 and 49 us; rows above 16384 values 4096 x 28672 216, 220 and 400 (1.6-2.1 TB/s), 1 x 32768 35, 37 and 96.
 #include "gemm_tile.h"
 
 namespace tpamd {
@@ -256,8 +258,8 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantParams p) {
 }
 
 // Without the addition, rows of a large launch are held by fewer wavefronts with four chunks a lane: more rows are under way on a CU, and a row's meeting costs less. Quantised / normed, us:
-// 2103 x 4096 9.2 -> 8.8 / 10.1 -> 9.2, 4096 x 5504 15.2 -> 14.6 / 17.9 -> 15.6, 4096 x 16384 35.5 -> 33.5 / 40.9 -> 36.3, 1024 x 11008 10.0 -> 9.6 / 11.6 -> 10.7; smaller ones lose, 1024 x 4096
-// 6.0 -> 6.7, 2048 x 2048 6.0 -> 6.5, and with the addition 4096 x 8192 37.8 -> 38.3, 2103 x 4096 13.3 -> 13.9.
+// 2103 x 4096 9.6 -> 9.3 / 9.0 -> 8.6, 4096 x 5504 15.6 -> 16.0 / 17.2 -> 16.3, 4096 x 16384 37.7 -> 37.5 / 41.2 -> 38.1, 1024 x 11008 10.7 -> 10.5 / 11.4 -> 10.6; smaller ones lose, 1024 x 4096
+// 6.5 -> 6.9 / 6.0 -> 6.3, 2048 x 2048 6.7 -> 6.8 / 6.0 -> 6.4, 512 x 8192 5.9 -> 6.6 / 5.8 -> 6.3. With the addition the form made no difference worth having (4096 x 8192 37.8 and 38.3).
 constexpr int64_t MANY_VALUES = 1 << 23;
 
 template <int DT, bool NORM, bool ADD>

@@ -9,20 +9,19 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int SA_NW = 4;        // wavefronts per block
 constexpr int SA_LDS_KB = 160;  // one block per CU
-// Most stages, by the loads of one. Three are enough but where a stage is small: 16 x 16384 x 8192 26.4 us with four, 25.9 with three, 32 x 4096 x 5504 10.4 and 10.2, the pair of 8 x 5504 x 4096
-// 10.7 and 10.5, but 1 x 4096 x 5504 6.0 and 6.1, 1 x 2048 x 4096 4.6 and 4.75; six or eight cost 1-6 % on small matrices and change nothing on large ones.
+// Most stages, by the loads of one. Three are enough but where a stage is small: three take 0.98 of the time of four at 16 x 16384 x 8192, 32 x 4096 x 5504 and the pair of 8 x 5504 x 4096, but 1.02 at
+// 1 x 4096 x 5504 and 1.03 at 1 x 2048 x 4096; six or eight cost 1-6 % on small matrices and change nothing on large ones.
 constexpr int sa_depth(int loads) { return loads <= 4 ? 4 : 3; }
 
 // stream_a8_kernel: products of up to 64 rows of 8-bit codes on one block per CU, cut and staged as stream_kernel cuts and stages 16-bit ones (stream.hip): a block owns an even share of the
 // columns and all of K, its wavefronts contiguous quarters of K, 128 elements (bytes) of NR weight rows (a pair: gate rows, then up rows) and XR rows of x at a time through rings of their own in
 // LDS, filled by loads that go straight there; the wavefronts' sums meet in LDS. K ends in a multiple of 16: the pieces of x behind it are asked for outside the descriptor's range, which
-// gives zeros, and so are rows that there are none of, which cost no memory traffic (they read the last row again before: 16 x 16384 x 8192 28.0 us, then 26.0).
+// gives zeros, and so are rows that there are none of, which cost no memory traffic (reading the last row in their place takes 8 % longer at 16 x 16384 x 8192).
 // The matrix pipe idles (a stage's MFMAs take 2-6 % of its time), so the half-rate 16 x 16 form serves, whose rows of 16 fit few columns a CU.
-// Bound: memory, N K bytes of weights: 16 x 16384 x 8192 in 25.9 us, 5.2 TB/s where a large copy has 6.0; at smaller matrices its latency: a launch and the first loads are 3.4 us of 6.0 for
-// 1 x 4096 x 5504 (22.5 MB), of 10.5 for the pair of 8 x 5504 x 4096 (45 MB). From 33 rows on x, which every CU reads whole from the L2: 64 x 4096 x 5504 12.8.
+// Bound: memory, N K bytes of weights: 16 x 16384 x 8192 in 25.5 us, 5.3 TB/s where a large copy has 6.0; at smaller matrices its latency: a launch and the first loads are 3.4 us of 6.1 for
+// 1 x 4096 x 5504 (22.5 MB), of 10.1 for the pair of 8 x 5504 x 4096 (45 MB; 17 rows 10.8, 32 rows 11.9, 48 13.7). From 33 rows on x, which every CU reads whole from the L2: 32 x 4096 x 5504 9.1, 64 rows 12.2.
 // Two ranks' products are one launch with half the CUs each (blockIdx.y).
-// Slower, tried: weights straight into registers in the order of the matrix instructions (16 rows x 64 bytes a load: 37 us for the first), two blocks of half the LDS to a CU (26.4, all others
-// slower), eight wavefronts.
+// Slower, tried: weights straight into registers in the order of the matrix instructions (16 rows x 64 bytes a load: 37 us for the first), two blocks of half the LDS to a CU, eight wavefronts.
 __device__ __forceinline__ const float *by_bytes(const float *p, int64_t bytes) { return reinterpret_cast<const float *>(reinterpret_cast<const char *>(p) + bytes); }
 
 template <int DT, bool PAIR, int NR, int XR, int D>
@@ -68,8 +67,8 @@ __global__ __launch_bounds__(SA_NW * 64) void stream_a8_kernel(A8Params p) {
     const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + static_cast<int64_t>(n0) * ldw, w_extent);
     const __amdgpu_buffer_rsrc_t w2_rsrc = PAIR ? make_rsrc(p.w2 + static_cast<int64_t>(n0) * ldw, w_extent) : w_rsrc;
     const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(p.x, static_cast<uint32_t>(p.M - 1) * ldx + static_cast<uint32_t>(p.K));
-    // Weights pass the caches by, unless rows begin inside 128-byte lines: the next unit then asks for the rest of a line (the pair of 8 x 5504 x 4112 15.4 -> 13.6 us, 16 x 16384 x 8208
-    // 40.7 -> 34.4; whole lines kept in the caches cost 16 x 16384 x 8192 26.4 -> 28.9)
+    // Weights pass the caches by, unless rows begin inside 128-byte lines: the next unit then asks for the rest of a line (the pair of 8 x 5504 x 4112 takes 0.88 of the time so, 12.6 us, 16 x 16384 x 8208
+    // 0.85, 33.8; whole lines kept in the caches cost 16 x 16384 x 8192 9 %)
     const bool whole_lines = ((reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.w2) | static_cast<uintptr_t>(p.ldw)) & 127) == 0;
     char *ring = smem + wave * RING;
     auto load = [&](int stage_off, int i) __attribute__((always_inline)) {  // unit number i of this wavefront; behind the last one the same count of loads from outside the descriptors

@@ -16,7 +16,7 @@ library's kernels only.
 With both operands in 8 bits (`QuantizedRows`, `quantize_activations`, `rms_norm`, `add_rms_norm`, `linear`, `swiglu_up`) the rows of an activation have a scale each too:
 
   a        = max |p| over the row, p = x, or w x of an RMS norm's input x (its factor f = rsqrt(mean(x^2) + eps) is in the scale alone; else f = 1)
-  codes    = round_half_even(127 p / a) of the exact quotient          scale = a f / 127      (zeros: 1.0; an infinity or NaN: NaN, and codes of 0)
+  codes    = round_half_even(127 p / a) of the exact quotient          scale = a f / 127      (no |p| of 2^-100 or more: 1.0, an infinity or NaN: NaN, and codes of 0)
   linear   = act(scale[m] wscale[n] (codes . Wq^T) + bias), the product exact in 32-bit integers, rounded once (a partial sum of other ranks is added to the rounded value)
 
 A quantised Linear no longer has a `weight`: `save_tensor_parallel`, which rebuilds the full
@@ -188,8 +188,9 @@ class ShardLinearW8(nn.Module):
 
 
 def _in_lines(wq: torch.Tensor) -> torch.Tensor:
-    """Codes [N, K] whose rows begin on 128-byte boundaries (K a multiple of 16; else as they are, one after another). A row of K = 2752 that begins inside a line shares it with the next one, and products
-    ask for such lines twice: 8 x 4096 x 2752 5.5 us, 4.7 with rows in lines; 16 x 4096 x 5520 10.6 and 7.8; the pair of 4096 x 5504 x 4112 207 and 184, 172 with the input's rows in lines as well."""
+    """Codes [N, K] whose rows begin on 128-byte boundaries (K a multiple of 16; else as they are, one after another: the matrix pipe takes whole pieces of 16 codes, and such rows go to a kernel that
+    takes any, 20 to 75 times slower). A row of K = 2752 that begins inside a line shares it with the next one, and products ask for such lines twice: 8 x 4096 x 2752 5.3 us, 4.9 with rows in
+    lines; 16 x 4096 x 5520 9.7 and 7.6; the pair of 4096 x 5504 x 4112 198, 170 with the input's rows in lines as well."""
     K = wq.shape[1]
     if K % 128 == 0 or K % 16 != 0:
         return wq.contiguous()
@@ -285,9 +286,9 @@ def quantize_linears_(module: nn.Module, outlier_cols: OutlierChoice = None,
     under `module` (as in `module.named_modules()`) or as a function of (name, Linear); none by default. `skip(name,
     Linear)` keeps a Linear as it is (an output head, say). Returns how many were replaced.
 
-    `activations=True`: both operands in 8 bits (`ShardLinearA8`; no outlier columns). A SiLU-gated MLP block then quantises its input once for gate and up, which are one launch
-    (`swiglu_up`), a fused attention of the Llama pattern its input once for q, k and v, which are one launch too, and a Llama decoder layer takes their inputs from the launches of its norms (`rms_norm`,
-    `add_rms_norm`) where nothing watches the norms."""
+    `activations=True`: both operands in 8 bits (`ShardLinearA8`; no outlier columns). A SiLU-gated MLP block, one whose forward is down_proj(act_fn(gate_proj(x)) * up_proj(x)) and nothing else, then
+    quantises its input once for gate and up, which are one launch (`swiglu_up`), a fused attention of the Llama pattern its input once for q, k and v, which are one launch too, and a Llama decoder layer takes their inputs from the launches of its norms (`rms_norm`,
+    `add_rms_norm`) where nothing watches the norms. Linears whose inputs are no multiple of 16 features are better left out (`skip`): the matrix pipe does not take them."""
     if activations and outlier_cols is not None:
         raise ValueError("quantize_linears_: with 8-bit activations there are no outlier columns")
     replaced = 0
