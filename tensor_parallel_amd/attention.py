@@ -202,11 +202,11 @@ def share_qkv_a8(module: torch.nn.Module) -> bool:
     return True
 
 
-def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
+def _project_shared_a8(self, rows, whole) -> Optional[torch.Tensor]:
     """The three Linears of `share_qkv_a8` in one launch; None (and never again) where one of them no longer is a view of the matrix."""
     from .shard_modules import _guard
 
-    wq, scale, bias = self.__dict__["_tp_qkv8"]
+    wq, scale, bias = whole
     row = 0
     for name in QKV:
         part = self._modules[name]
@@ -215,7 +215,7 @@ def _project_shared_a8(self, rows) -> Optional[torch.Tensor]:
             break
         row += part.out_features
     if row != wq.shape[0]:
-        del self.__dict__["_tp_qkv8"]
+        self.__dict__.pop("_tp_qkv8", None)  # (another thread's call may have)
         return None
     return _guard(together.linear_a8(rows.codes, rows.scale, wq, scale, bias, rows.dtype), rows.scale)
 
@@ -230,8 +230,9 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     if not watched and _has_a8(self, QKV) and self.q_proj.dtype == self.k_proj.dtype == self.v_proj.dtype:
         self.__dict__.pop("_tp_qkv", None)  # (of Linears that were replaced one by one)
         hidden_states = self.q_proj.rows_of(hidden_states)
-        if self.__dict__.get("_tp_qkv8"):
-            qkv = _project_shared_a8(self, hidden_states)
+        whole = self.__dict__.get("_tp_qkv8")
+        if whole:
+            qkv = _project_shared_a8(self, hidden_states, whole)
             if qkv is not None:
                 return [part.view(B, S, -1, D) for part in qkv.split([self._modules[name].out_features for name in QKV], -1)]
     shared = self.__dict__.get("_tp_qkv")
@@ -252,7 +253,7 @@ def _project_qkv(self, hidden_states: torch.Tensor, D: int):
             qkv = _guard(together.linear(hidden_states.detach(), w, b), hidden_states, q_proj.weight)
             return (qkv[..., :nq].view(B, S, -1, D), qkv[..., nq:nq + nk].view(B, S, -1, D), qkv[..., nq + nk:].view(B, S, -1, D))
         if not intact:  # a projection was replaced (quantised, re-assigned): three calls from now on
-            del self.__dict__["_tp_qkv"]
+            self.__dict__.pop("_tp_qkv", None)
     return (self.q_proj(hidden_states).view(B, S, -1, D), self.k_proj(hidden_states).view(B, S, -1, D),
             self.v_proj(hidden_states).view(B, S, -1, D))
 

@@ -255,6 +255,24 @@ def test_linears_of_8_bits_put_in_one_by_one_end_the_16_bit_sharing(calls):
     assert "_tp_qkv" not in attn.__dict__
 
 
+def test_two_calls_that_find_the_sharing_ended(calls):
+    """The second of two threads finds that the first has ended it already."""
+    attn = projections(torch.randn(3 * 64, 64).bfloat16())
+    attention.share_qkv_a8(attn)
+
+    class Ended(list):
+        def __iter__(self):
+            attn.__dict__.pop("_tp_qkv8", None)
+            return super().__iter__()
+
+    attn.__dict__["_tp_qkv8"] = Ended(attn.__dict__["_tp_qkv8"])
+    attn.v_proj.scale = attn.v_proj.scale.clone()
+    x = inputs()[None]
+    with torch.no_grad():
+        got = attention._project_qkv(attn, x, 32)
+        assert all(torch.equal(part.flatten(2), attn._modules[name](x)) for part, name in zip(got, attention.QKV))
+
+
 def test_codes_stay_where_they_are_when_other_linears_are_quantised(calls):
     """A graph that was recorded before may read them."""
     model = nn.ModuleList([projections(torch.randn(3 * 64, 64).bfloat16())])
