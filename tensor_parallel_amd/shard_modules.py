@@ -509,7 +509,7 @@ def _gated_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
     watched."""
     gate, up, act = _gated_parts(self)
     known = self.__dict__.get("_tp_gated", (type(gate), type(up), act))  # (a block that was pickled before there was this)
-    if (type(gate) is not known[0] or type(up) is not known[1] or act is not known[2] or gate._parameters.get("bias", 0) is not None or up._parameters.get("bias", 0) is not None or all_watched()
+    if (not _computes_gated(type(self).forward) or type(gate) is not known[0] or type(up) is not known[1] or act is not known[2] or gate._parameters.get("bias", 0) is not None or up._parameters.get("bias", 0) is not None or all_watched()
             or "forward" in gate.__dict__ or "forward" in up.__dict__ or _has_hooks(gate) or _has_hooks(up) or isinstance(act, nn.Module) and ("forward" in act.__dict__ or _has_hooks(act))):
         return type(self).forward(self, x)
     return returned(self, _gated_mlp_forward, self.down_proj, _gate_up(self, x))
@@ -540,10 +540,12 @@ def is_gated_silu_mlp(module: nn.Module) -> bool:
 
 def _gated_mlp_first_forward(self, x: torch.Tensor) -> torch.Tensor:
     """First call of a block that looks like a SiLU-gated MLP: its own forward and the fused one both run on this input.
-    If they agree the fused forward takes over, otherwise the block keeps its own (a forward that slices its weights
+    If they agree, and the block's own is this formula of a plain SiLU (rows of zeros agree by any), the fused forward takes over, otherwise the block keeps its own (a forward that slices its weights
     for pretraining_tp, adds projections or orders the operations differently is not this pattern)."""
-    del self.forward  # the class's forward is visible again
+    self.__dict__.pop("forward", None)  # the class's forward is visible again (also to a second thread's first call)
     own = type(self).forward(self, x)
+    if not _computes_gated(type(self).forward) or not _is_plain_silu(_gated_parts(self)[2]):
+        return own
     try:
         fused = self.down_proj(_gate_up(self, x))
         same = isinstance(own, torch.Tensor) and own.shape == fused.shape and torch.allclose(

@@ -172,3 +172,49 @@ def test_a_projection_with_another_bias(calls, change):
         attn.k_proj.bias = None if change == "none" else nn.Parameter(torch.randn(16).bfloat16())
         got = attention._project_qkv(attn, x, 16)
         assert all(torch.equal(part.flatten(2), attn._modules[name](x)) for part, name in zip(got, attention.QKV))
+
+
+class Exchanged(Mlp):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.up_proj(x)) * self.gate_proj(x))
+
+
+class Scaled(Mlp):
+    def forward(self, x):
+        return 1.01 * self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+class Steep(Mlp):
+    class Swish(nn.Module):
+        def forward(self, x):
+            return x * torch.sigmoid(1.7 * x)
+
+    def __init__(self):
+        super().__init__()
+        self.act_fn = self.Swish()
+
+
+@pytest.mark.parametrize("cls", [Exchanged, Scaled, Steep])
+@pytest.mark.parametrize("first", ["zeros", "values"])
+def test_blocks_of_another_formula(calls, cls, first):
+    """They keep their own forward, whatever they are called with first."""
+    torch.manual_seed(0)
+    block, x = cls().bfloat16(), inputs()
+    shard_modules.install_shard_kernels(block)
+    with torch.no_grad():
+        block(torch.zeros_like(x) if first == "zeros" else x)
+        assert torch.equal(block(x), cls.forward(block, x))
+
+
+def test_a_class_that_is_given_another_forward(calls):
+    class Own(Mlp):
+        forward = Mlp.forward
+
+    torch.manual_seed(0)
+    block, x = Own().bfloat16(), inputs()
+    shard_modules.install_shard_kernels(block)
+    with torch.no_grad():
+        block(x)
+        assert block.forward.__func__ is shard_modules._gated_mlp_forward
+        Own.forward = Scaled.forward
+        assert torch.equal(block(x), Scaled.forward(block, x))
