@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define TPAMD_ABI_VERSION 6
+#define TPAMD_ABI_VERSION 7
 
 typedef enum tpamd_status {
     TPAMD_OK = 0,
@@ -471,6 +471,62 @@ typedef struct {
     void *sum, *q, *scale;
 } tpamd_q8_rank;
 int tpamd_rows_q8_ranks(int n, const tpamd_q8_rank *ranks, int64_t rows, int64_t D, int64_t ldx, int64_t ldr, int64_t ldsum, int64_t ldq, float eps, int dtype, void *stream);
+
+/* ---- heads and paged caches -----------------------------------------------------------------------------------------------------------
+ * What a serving program needs between the projection of q, k and v and the output projection where its sequences differ in length: the wrapped attention modules (run by
+ * src/tensor_parallel/wrapper.py:69-72) do this with torch ops on caches of one length, and the reference only routes those (src/tensor_parallel/aux_actions.py:7-15). Defined here in
+ * closed form.
+ *
+ * Heads: rows of q [rows, Hq, D] and k [rows, Hkv, D], views of a projection's output (strides in elements, D contiguous; query head i at (i / g) * q_group + (i % g) * q_head,
+ * g = Hq / Hkv). Of each head x
+ *   x' = x * rsqrt(mean(x^2) + eps) * norm                                           where q_norm / k_norm ([D], in dtype) is not NULL,
+ *   (a, b) -> (a c - b s, b c + a s)                                                  for the pairs of its first `part` elements: neighbours (2 i, 2 i + 1) where `interleaved`, else (i, i + part / 2),
+ * c and s = scaling times cos and sin of position * inv_freq[i] (fp32 [part / 2]; the angle in 64 bits), or scaling times the tables cos / sin [rows, part / 2] (table_dtype; table_row
+ * elements between rows, 0 where all rows share one). Everything in fp32, rounded once. part = 0: nothing is turned. positions: int64 [rows].
+ * Any even D up to 512, any alignment; fewer than 2^24 rows. Rows, sizes and strides of whole 16-byte pieces (part too: a multiple of 16 elements) are fastest, of 8-byte ones next; any others
+ * are read by single elements. Outputs overlap no input. */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_row, q_group, q_head, k_row, k_head, v_row, v_head;
+    const void *q_norm, *k_norm;
+    float eps, scaling;
+    const float *inv_freq;
+    const void *cos, *sin;
+    int64_t table_row;
+    int table_dtype, interleaved;
+    int64_t part;
+    const int64_t *positions;
+    void *q_out, *k_out;
+    int64_t qo_row, qo_head, ko_row, ko_head;
+} tpamd_heads;
+/* q_out [rows, Hq, D], k_out [rows, Hkv, D] (v is ignored). */
+int tpamd_rotate_heads(const tpamd_heads *heads, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int dtype, void *stream);
+
+/* A cache whose positions lie in pages: k_pages, v_pages [pages, Hkv, page, D] by strides (elements; D contiguous), `page` a power of two from 16 on. Position j of sequence b is in slot
+ * j % page of page table[b][j / page] (int32 [seqs, columns], table_row elements between rows). lengths (int32 [seqs]) count a sequence's positions WITH its new rows, which are the last ones.
+ * The new rows of all sequences follow one another: those of b are rows starts[b] .. starts[b + 1] - 1 (int32 [seqs + 1], not decreasing), or, with starts NULL, the first counts[b] (int32; NULL: all) of the
+ * rows / seqs rows from b * rows / seqs on. Rows of no sequence are neither read nor written.
+ * All of this is read on the device when the kernels run (a captured call serves every step) and held to the rows there are and the room of the table; a page that the pool does not have (-1,
+ * say) holds zeros and takes nothing. */
+typedef struct {
+    void *k_pages, *v_pages;
+    int64_t pages, page, k_page, k_head, k_pos, v_page, v_head, v_pos;
+    const int32_t *table;
+    int64_t table_row, columns;
+    const int32_t *lengths, *starts, *counts;
+    int64_t seqs;
+} tpamd_pages;
+/* Heads of the new rows: q turned into q_out, k turned and v as it is into their positions' pages (k_out is ignored). positions NULL: each row's place in its sequence. */
+int tpamd_append_paged(const tpamd_heads *heads, const tpamd_pages *pages, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int dtype, void *stream);
+
+/* out [rows, Hq, D] = softmax(scale q k^T) v of the new rows on the pages, a row on the positions up to its own; zeros for a row before position 0 (a sequence with fewer positions than new
+ * rows). What stands at positions a row does not see, infinities and NaN too, does not reach it. Scores, softmax and sums in fp32, probabilities rounded to dtype in front of the
+ * second product, the result once. D 64, 96, 128 or 256, BF16 or F16; rows of q and of the pools on 16-byte boundaries, of out on 8.
+ * max_new: no sequence has more new rows (rows of one that does may be left out); max_length: none has more positions (a hint: only the time depends on it). Bounds that hold for every
+ * replay, where the call is captured. workspace_dev: tpamd_attention_paged_workspace() bytes, 16-byte aligned, for the call alone until it has run; out overlaps nothing else. */
+int tpamd_attention_paged(const void *q_dev, int64_t q_row, int64_t q_head, const tpamd_pages *pages, void *out_dev, int64_t o_row, int64_t o_head, int64_t rows, int64_t Hq, int64_t Hkv,
+                          int64_t D, int64_t max_new, int64_t max_length, float scale, int dtype, void *workspace_dev, uint64_t workspace_bytes, void *stream);
+int tpamd_attention_paged_workspace(const tpamd_pages *pages, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_length, uint64_t *bytes_out);
 
 #ifdef __cplusplus
 }

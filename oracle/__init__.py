@@ -17,6 +17,8 @@ Modules and the reference code each one follows:
   rope.py           rotary embedding of the new query / key rows and their hand-over to the rank-local cache, in the
                     arithmetic of the wrapped transformers module (the reference only routes the cache tensors:
                     src/tensor_parallel/aux_actions.py:7-15)
+  paged.py          heads normed and turned to their positions, paged key/value caches and attention on them, float64;
+                    NOT in the reference (it routes the wrapped model's cache tensors): defined in closed form
   sharding.py       flat per-rank shards of the replicated parameters and their recombination
                     (src/tensor_parallel/sharding.py:96-180)
   quant.py          int8 weight-only quantisation with outlier columns - NOT in the reference: parity
@@ -34,6 +36,8 @@ How each function is pinned (tests/test_oracle_*.py):
                grouped heads and Sq < Skv causal, rows of probabilities sum to one, a single visible key returns its value
   rope         transformers' apply_rotary_pos_emb bit for bit (bf16, fp16, fp32), the complex-rotation closed form in
                fp64, norm preservation, identity at position 0
+  paged        transformers' rotation of halves, complex multiplication for neighbours, oracle/attention.py on contiguous
+               caches, unit mean square behind a norm, rows that see nothing are zero
   sharding     combine(make(x)) == x on ragged sizes, equal flat lengths, the parameter counts asserted by the
                reference's own test (tests/test_basic.py:110-135)
   quant        dequantised weights within scale/2 of the originals; fp64 matmul of the definition

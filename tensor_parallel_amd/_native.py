@@ -10,6 +10,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 from array import array
 from pathlib import Path
 from typing import Optional, Sequence
@@ -77,9 +78,13 @@ EXPORTS = (
     "tpamd_linear_a8_ranks",
     "tpamd_swiglu_up_a8_ranks",
     "tpamd_rows_q8_ranks",
+    "tpamd_rotate_heads",
+    "tpamd_append_paged",
+    "tpamd_attention_paged",
+    "tpamd_attention_paged_workspace",
 )
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 BF16, F16, F32 = 0, 1, 2
 ACCUM_STEPWISE, ACCUM_F32 = 0, 1
@@ -254,6 +259,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.tpamd_swiglu_up_a8_ranks.argtypes = [ci, c.POINTER(A8Rank), i64, i64, i64, i64, i64, i64, ci, vp]
     lib.tpamd_rows_q8_ranks.restype = ci
     lib.tpamd_rows_q8_ranks.argtypes = [ci, c.POINTER(Q8Rank), i64, i64, i64, i64, i64, i64, c.c_float, ci, vp]
+    lib.tpamd_rotate_heads.restype = ci
+    lib.tpamd_rotate_heads.argtypes = [vp, i64, i64, i64, i64, ci, vp]
+    lib.tpamd_append_paged.restype = ci
+    lib.tpamd_append_paged.argtypes = [vp, vp, i64, i64, i64, i64, ci, vp]
+    lib.tpamd_attention_paged.restype = ci
+    lib.tpamd_attention_paged.argtypes = [vp, i64, i64, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, c.c_float, ci, vp, u64, vp]
+    lib.tpamd_attention_paged_workspace.restype = ci
+    lib.tpamd_attention_paged_workspace.argtypes = [vp, i64, i64, i64, i64, i64, i64, c.POINTER(u64)]
 
 
 def _load() -> None:
@@ -1507,3 +1520,187 @@ def swiglu_up_a8_ranks(calls: Sequence[tuple]) -> list:
     _same_form("swiglu_up_a8", forms)
     _launch("tpamd_swiglu_up_a8_ranks", lib().tpamd_swiglu_up_a8_ranks, forms[0][0], len(calls), ranks, *forms[0][1:])
     return outs
+
+
+# ---- heads and paged caches ----------------------------------------------------------------------------------------------
+_HEADS = struct.Struct("@3P7q2P2f3Pq2iqP2P4q")  # tpamd_heads
+_PAGES = struct.Struct("@2P8qP2q3Pq")           # tpamd_pages
+
+
+def _one_axis(t: torch.Tensor, axes: int) -> torch.Tensor:
+    """t with its first `axes` axes as one (a view where its strides allow)."""
+    return t if axes == 1 else t.flatten(0, axes - 1) if axes > 1 else t.unsqueeze(0)
+
+
+def _heads_operands(what: str, q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
+    """q [rows, Hq, D] or [rows, Hkv, per, D], k, v [rows, Hkv, D], and the axes that the rows had; what they have in common is checked."""
+    if not q.is_cuda:
+        require_device(q, what)
+    code = _HALF_CODES.get(q.dtype)
+    if code is None or k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+        raise TypeError(f"{what}: q, k and v must share bfloat16 or float16")
+    axes = k.dim() - 2
+    if axes < 0 or q.dim() not in (k.dim(), k.dim() + 1) or q.shape[:axes] != k.shape[:axes] or q.shape[-1] != k.shape[-1] or (v is not None and v.shape != k.shape) or (
+            q.dim() > k.dim() and q.shape[axes] != k.shape[axes]):
+        raise ValueError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}{'' if v is None else f', v {tuple(v.shape)}'} do not fit")
+    if k.device != q.device or (v is not None and v.device != q.device):
+        raise ValueError(f"{what}: q, k and v lie on different devices")
+    shape = k.shape[:axes]
+    q, k, v = (None if t is None else _one_axis(t, axes) for t in (q, k, v))
+    if k.shape[-1] > 1 and (q.stride(-1) != 1 or k.stride(-1) != 1 or (v is not None and v.stride(-1) != 1)):
+        raise ValueError(f"{what}: heads must be contiguous")
+    return code, shape, q, k, v
+
+
+def _pack_heads(what: str, q, k, v, q_out, k_out, shape, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps) -> tuple:
+    """tpamd_heads of these operands, and the tensors that it points to."""
+    rows, Hkv, D = k.shape
+    device = q.device
+    q_head, q_group = (q.stride(1), q.stride(1) * (q.shape[1] // Hkv if Hkv else 1)) if q.dim() == 3 else (q.stride(2), q.stride(1))
+    part, table_row, table_code = 0, 0, 0
+    if inv_freq is not None:
+        if cos is not None or sin is not None:
+            raise ValueError(f"{what}: frequencies or tables of cos and sin, not both")
+        if inv_freq.dim() != 1 or inv_freq.device != device:
+            raise ValueError(f"{what}: inv_freq must have one axis and lie on {device}, got {tuple(inv_freq.shape)} on {inv_freq.device}")
+        if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+            inv_freq = inv_freq.float().contiguous()
+        part = 2 * inv_freq.shape[0]
+    elif cos is not None or sin is not None:
+        if cos is None or sin is None or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.device != device or sin.device != device or cos.dim() < 1:
+            raise ValueError(f"{what}: cos and sin must be tables of one shape and dtype on {device}")
+        table_code = dtype_code(cos.dtype)
+        half = cos.shape[-1]
+        if cos.numel() == half:
+            cos, sin = cos.reshape(1, half).contiguous(), sin.reshape(1, half).contiguous()
+        else:
+            cos, sin = (t.expand(*shape, half).reshape(rows, half) for t in (cos, sin))
+            if half > 1 and cos.stride(1) != 1 or cos.stride() != sin.stride():
+                cos, sin = cos.contiguous(), sin.contiguous()
+            table_row = cos.stride(0)
+        part = 2 * half
+    if positions is not None:
+        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != shape or positions.device != device:
+            raise ValueError(f"{what}: positions must be int64 or int32 {tuple(shape)} on {device}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
+        positions = positions.to(torch.int64).reshape(rows).contiguous()
+    norms = []
+    for norm in (q_norm, k_norm):
+        if norm is not None and (norm.shape != (D,) or norm.dtype != q.dtype or norm.device != device):
+            raise ValueError(f"{what}: a norm's weight must be [{D}] {q.dtype} on {device}, got {tuple(norm.shape)} {norm.dtype} on {norm.device}")
+        norms.append(None if norm is None else norm.contiguous())
+    q_norm, k_norm = norms
+
+    def at(t):
+        return 0 if t is None else t.data_ptr()
+
+    packed = _HEADS.pack(q.data_ptr(), k.data_ptr(), at(v), q.stride(0), q_group, q_head, k.stride(0), k.stride(1), 0 if v is None else v.stride(0), 0 if v is None else v.stride(1),
+                         at(q_norm), at(k_norm), eps, scaling, at(inv_freq), at(cos), at(sin), table_row, table_code, 1 if interleaved else 0, part, at(positions),
+                         q_out.data_ptr(), at(k_out), q_out.stride(0), q_out.stride(1), 0 if k_out is None else k_out.stride(0), 0 if k_out is None else k_out.stride(1))
+    return packed, (inv_freq, cos, sin, positions, q_norm, k_norm)
+
+
+def _pack_pages(what: str, q: torch.Tensor, rows: int, Hkv: int, D: int, k_pages, v_pages, table, lengths, starts, counts) -> tuple:
+    """tpamd_pages of these operands, and the tensors that it points to."""
+    device = q.device
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
+        raise ValueError(f"{what}: pools must be [pages, {Hkv}, positions of a page, {D}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    if k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        raise TypeError(f"{what}: the pools must be {q.dtype}, got {k_pages.dtype} and {v_pages.dtype}")
+    if table.dim() != 2 or lengths.shape != table.shape[:1]:
+        raise ValueError(f"{what}: the table must be [sequences, pages of one] and the lengths one for each sequence, got {tuple(table.shape)} and {tuple(lengths.shape)}")
+    seqs = table.shape[0]
+    if starts is not None and starts.shape != (seqs + 1,) or counts is not None and counts.shape != (seqs,):
+        raise ValueError(f"{what}: starts must be [{seqs + 1}] and counts [{seqs}]")
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("table", table), ("lengths", lengths), ("starts", starts), ("counts", counts)):
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{what}: q is on {device}, {name} on {t.device}")
+        if name[1:] == "_pages":
+            if t.stride(3) != 1 and D > 1:
+                raise ValueError(f"{what}: {name} must have contiguous rows")
+        elif t.dtype != torch.int32:
+            raise TypeError(f"{what}: {name} must be int32, got {t.dtype}")
+    if table.shape[1] > 1 and table.stride(1) != 1:
+        table = table.contiguous()
+    lengths, starts, counts = (None if t is None else t.contiguous() for t in (lengths, starts, counts))
+    pages, _, page, _ = k_pages.shape
+    packed = _PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *k_pages.stride()[:3], *v_pages.stride()[:3], table.data_ptr(), table.stride(0), table.shape[1],
+                         lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if counts is None else counts.data_ptr(), seqs)
+    return packed, (table, lengths, starts, counts)
+
+
+def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                 sin: Optional[torch.Tensor] = None, scaling: float = 1.0, interleaved: bool = False, q_norm: Optional[torch.Tensor] = None,
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> tuple:
+    """(q, k) with their heads normed and turned (`attention.rotate` says how), as [..., Hq, D] and [..., Hkv, D]."""
+    code, shape, q, k, _ = _heads_operands("rotate", q, k, None)
+    rows, Hkv, D = k.shape
+    if inv_freq is not None and positions is None:
+        raise ValueError("rotate: frequencies need positions")
+    Hq = q.shape[1] if q.dim() == 3 else q.shape[1] * q.shape[2]
+    q_out, k_out = q.new_empty((rows, Hq, D)), q.new_empty((rows, Hkv, D))
+    packed, keep = _pack_heads("rotate", q, k, None, q_out, k_out, shape, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
+    _launch("tpamd_rotate_heads", lib().tpamd_rotate_heads, q.get_device(), packed, rows, Hq, Hkv, D, code)
+    return q_out.view(*shape, Hq, D), k_out.view(*shape, Hkv, D)
+
+
+def append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                 starts: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                 cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, scaling: float = 1.0, interleaved: bool = False, q_norm: Optional[torch.Tensor] = None,
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """k and v of the new rows into their pages, k (and q, which is returned) normed and turned (`paged.append` says how)."""
+    code, shape, q, k, v = _heads_operands("append", q, k, v)
+    rows, Hkv, D = k.shape
+    Hq = q.shape[1] if q.dim() == 3 else q.shape[1] * q.shape[2]
+    pages, keep_pages = _pack_pages("append", q, rows, Hkv, D, k_pages, v_pages, table, lengths, starts, counts)
+    q_out = q.new_empty((rows, Hq, D))
+    packed, keep = _pack_heads("append", q, k, v, q_out, None, shape, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
+    _launch("tpamd_append_paged", lib().tpamd_append_paged, q.get_device(), packed, pages, rows, Hq, Hkv, D, code)
+    return q_out.view(*shape, Hq, D)
+
+
+def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
+                    counts: Optional[torch.Tensor] = None, scale: Optional[float] = None, max_new: Optional[int] = None, max_length: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of the new rows q [..., Hq, D] on their sequences' pages (`paged.attend` says how)."""
+    if not q.is_cuda:
+        require_device(q, "attend")
+    code = _HALF_CODES.get(q.dtype)
+    if code is None:
+        raise TypeError(f"attend: q must be bfloat16 or float16, got {q.dtype}")
+    if q.dim() < 2 or k_pages.dim() != 4:
+        raise ValueError(f"attend: q must be [..., heads, head_dim] and the pools [pages, heads, positions, head_dim], got {tuple(q.shape)} and {tuple(k_pages.shape)}")
+    shape = q.shape
+    q = _one_axis(q, q.dim() - 2)
+    rows, Hq, D = q.shape
+    Hkv = k_pages.shape[1]
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if out is None:
+        rows_out = q.new_empty((rows, Hq, D))
+        out = rows_out.view(shape)
+    else:
+        if out.shape != shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1:
+            raise ValueError(f"attend: out must be a {tuple(shape)} {q.dtype} tensor on {q.device} with contiguous heads")
+        rows_out = _one_axis(out, out.dim() - 2)
+        if rows_out.numel() and rows_out.data_ptr() != out.data_ptr():
+            raise ValueError("attend: the rows of out must follow one another")
+    pages, keep = _pack_pages("attend", q, rows, Hkv, D, k_pages, v_pages, table, lengths, starts, counts)
+    if max_new is None:
+        max_new = rows
+    if max_length is None:
+        max_length = table.shape[1] * k_pages.shape[2]
+    index, need = q.get_device(), ctypes.c_uint64()
+    prev = _device_of_thread()
+    if prev != index:
+        torch.cuda.set_device(index)
+    try:
+        _check(lib().tpamd_attention_paged_workspace(pages, rows, Hq, Hkv, D, max_new, max_length, ctypes.byref(need)), "tpamd_attention_paged_workspace")
+    finally:
+        if prev != index:
+            torch.cuda.set_device(prev)
+    work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    _launch("tpamd_attention_paged", lib().tpamd_attention_paged, index, q.data_ptr(), q.stride(0), q.stride(1), pages, rows_out.data_ptr(), rows_out.stride(0), rows_out.stride(1),
+            rows, Hq, Hkv, D, max_new, max_length, float(scale if scale is not None else D ** -0.5), code, 0 if work is None else work.data_ptr(), need.value)
+    return out

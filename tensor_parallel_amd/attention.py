@@ -25,7 +25,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native, together
-from .shard_modules import returned
+from .shard_modules import _guard, returned
 
 IMPLEMENTATION_NAME = "tpamd"
 
@@ -48,6 +48,21 @@ def attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.T
     # one new position on a cache sees every key: the aligned-to-the-end causal rule says the same
     out = _native.attention(query, key, value, scale=scaling, causal=bool(causal))
     return out, None
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor] = None, *, inv_freq: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+           sin: Optional[torch.Tensor] = None, scaling: float = 1.0, interleaved: bool = False, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+           eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The heads of q [..., Hq, D] (or [..., Hkv, Hq / Hkv, D]) and k [..., Hkv, D] (bfloat16 or float16, views of projection outputs) turned to their rows' positions in one launch; returns
+    both, contiguous, as [..., H, D]. Any even D up to 512.
+
+    Pairs (a, b) become (a c - b s, b c + a s), c and s `scaling` times cos and sin of position * inv_freq[i], angles in 64 bits: positions [...] (int64 or int32) and inv_freq [part / 2]; or
+    `scaling` times the tables cos and sin [..., part / 2] (16 or 32 bits, one value a pair). Of a head's first `part` elements the pairs are (i, i + part / 2), or with `interleaved`
+    neighbours (2 i, 2 i + 1); the others stay as they are. Frequencies and scaling are those that a model's rotary embedding has for long contexts, too.
+
+    q_norm, k_norm [D]: each head is x * rsqrt(mean(x^2) + eps) * weight first, in the same pass. All of it in fp32, rounded once. Inference only: a backward pass raises."""
+    q_out, k_out = _native.rotate_heads(q, k, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
+    return _guard(q_out, q, q_norm), _guard(k_out, k, k_norm)
 
 
 # What the mask kernel stands in for: the names that `sdpa_mask` and the causal rule look up, their arguments and locals.
@@ -204,8 +219,6 @@ def share_qkv_a8(module: torch.nn.Module) -> bool:
 
 def _project_shared_a8(self, rows, whole) -> Optional[torch.Tensor]:
     """The three Linears of `share_qkv_a8` in one launch; None (and never again) where one of them no longer is a view of the matrix."""
-    from .shard_modules import _guard
-
     wq, scale, bias = whole
     row = 0
     for name in QKV:
@@ -223,7 +236,7 @@ def _project_shared_a8(self, rows, whole) -> Optional[torch.Tensor]:
 def _project_qkv(self, hidden_states: torch.Tensor, D: int):
     """q, k, v as [B, S, heads, D]: one call on the shared weight matrix when the three Linears still are views of it; Linears of 8-bit rows on rows that are
     quantised once."""
-    from .shard_modules import ShardLinear, _guard, _has_a8, _has_hooks, all_watched
+    from .shard_modules import ShardLinear, _has_a8, _has_hooks, all_watched
 
     B, S, _ = hidden_states.shape
     watched = all_watched()

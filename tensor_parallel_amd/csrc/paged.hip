@@ -1,0 +1,963 @@
+// Attention of new rows on keys and values that lie in pages: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the positions j <= length - count + i of the row's
+// sequence. Sequences of one call differ in length and in how many new rows they have, and none of that is known to the host: lengths, starts and the page table are
+// read by the kernels.
+//
+// A sequence whose rows (new rows times query heads of a key/value head) fill at most one MFMA tile of 16 goes to paged_few_kernel, which is bound by reading keys and
+// values once; any other to paged_many_kernel, bound by its matrix products and exponentials. A call that may have both kinds launches both; each leaves the
+// other's sequences alone.
+//
+// Both load K and V straight into LDS, 16 positions by 16 positions: those lie in one page (pages have 16 positions or more, a power of two), so that a page is looked
+// up once for them and the loads have one descriptor and fixed offsets. A piece (16 bytes) c of a staged row r is in slot c ^ turned(r): rows are read as MFMA operands
+// (16 or 32 rows, one piece each) and through the transposing read (4 consecutive rows, 2 or 4 neighbouring pieces) without bank conflicts.
+#include "attention_model.h"
+#include "gemm_tile.h"
+#include "paged.h"
+
+#include <math.h>
+
+namespace tpamd {
+namespace {
+
+constexpr int FEW = 16;    // rows of a paged_few_kernel item
+constexpr int GROUP = 16;  // positions that lie in one page
+constexpr int UNIT = 64;   // positions of a piece of paged_few_kernel's work: a group for each of its wavefronts
+
+struct PagedParams {
+    const char *q;
+    char *o;
+    int64_t q_row, q_head, o_row, o_head;  // elements
+    float *part;
+    float scale_log2;  // scale * log2(e)
+    int Hkv, G, D;
+    int few, many;     // which of the kernels run
+    int splits;        // paged_many_kernel: key ranges
+    int least;         // paged_few_kernel: units a block takes at least; 0: a block takes one item, whole
+    PagesView pages;
+};
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+template <int D>
+__device__ __forceinline__ constexpr int turned(int r) {
+    if constexpr (D == 64) return ((r >> 1) & 1) << 2 | ((r >> 3) & 1) << 1 | ((r >> 2) & 1);  // two rows share 256 bytes
+    else if constexpr (D == 96) return (r >> 2) & 3;
+    else return (r & 3) << 2 | ((r >> 2) & 3);
+}
+
+__device__ __forceinline__ u32x2 lds_transpose_read(uint32_t at) {  // ds_read_b64_tr_b16, unseen by the compiler (as lds_read16)
+    u32x2 v;
+    asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(v) : "v"(at));
+    return v;
+}
+__device__ __forceinline__ void half_landed(u32x2 &r) { asm volatile("" : "+v"(r)); }
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16_k16(u32x2 a, u32x2 b, f32x4 c) {
+    if constexpr (DT == TPAMD_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c, 0, 0, 0);
+    } else {
+        typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+    }
+}
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (DT == TPAMD_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Values that some rows of a tile do not see may be infinite or NaN, and zero times those would reach the rows through the matrix product. They go in as zeros, and where there are any, two
+// more products with ones in the place of +inf and NaN, and of -inf and NaN, say which sums they belong to.
+template <int DT>
+struct Beyond {
+    static constexpr uint32_t E = DT == TPAMD_BF16 ? 0x7f80u : 0x7c00u, ONE = DT == TPAMD_BF16 ? 0x3f80u : 0x3c00u;
+    static __device__ __forceinline__ bool any(uint32_t two) { return (two & E) == E || (two & (E << 16)) == (E << 16); }
+    static __device__ __forceinline__ uint32_t finite(uint32_t two) {
+        return two & (((two & E) == E ? 0u : 0xffffu) | ((two & (E << 16)) == (E << 16) ? 0u : 0xffff0000u));
+    }
+    static __device__ __forceinline__ uint32_t one(uint32_t h, uint32_t sign) {  // of the low half: ONE for NaN and for the infinity of this sign
+        return (h & E) == E && ((h & 0x7fffu) != E || (h & 0x8000u) == sign) ? ONE : 0u;
+    }
+    static __device__ __forceinline__ uint32_t ones(uint32_t two, uint32_t sign) { return one(two & 0xffffu, sign) | one(two >> 16, sign) << 16; }
+};
+
+// The descriptor of 16 rows that begin at `base`: nothing (loads give zeros) where there is no page.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t group_rsrc(const char *pool, int page, int64_t page_step, int64_t head, int slot, int64_t pos_step, int D) {
+    const char *base = pool + (static_cast<int64_t>(page < 0 ? 0 : page) * page_step + head + static_cast<int64_t>(slot) * pos_step) * 2;
+    const uint32_t extent = page < 0 ? 0u : (15u * static_cast<uint32_t>(pos_step) + static_cast<uint32_t>(D)) * 2u;
+    return make_rsrc(base, extent);
+}
+
+// rows_of, of a sequence that the whole wavefront asks for.
+__device__ __forceinline__ SeqRows same_rows_of(const PagesView &p, int b) {
+    SeqRows s = rows_of(p, b);
+    s.first = __builtin_amdgcn_readfirstlane(s.first);
+    s.count = __builtin_amdgcn_readfirstlane(s.count);
+    s.length = __builtin_amdgcn_readfirstlane(s.length);
+    return s;
+}
+// A value that was loaded is here from now on: the compiler would otherwise wait for it inside the loop that uses it, and with it for loads that the loop has requested.
+__device__ __forceinline__ void arrived(int &v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void arrived(u32x4 &v) { asm volatile("" : "+v"(v)); }
+
+// ---- which rows go where ---------------------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ bool is_few(const PagedParams &p, int count) { return p.few && count > 0 && count * p.G <= FEW; }
+__device__ __forceinline__ int units_of(const PagedParams &p, const SeqRows &s) {
+    return is_few(p, s.count) ? max((s.length + UNIT - 1) / UNIT, 1) : 0;  // one for a sequence without positions too: its rows are zeros
+}
+// Row tiles of ROWS rows, 0 for the other kernel's sequences.
+template <int ROWS>
+__device__ __forceinline__ int tiles_of(const PagedParams &p, const SeqRows &s) {
+    return s.count > 0 && !is_few(p, s.count) ? (s.count * p.G + ROWS - 1) / ROWS : 0;
+}
+// The sum over all sequences of what `of` gives, and (where `at` is one of the units) the sequence it falls into with the sum before it. By all lanes of a wavefront.
+template <class F>
+__device__ __forceinline__ int sum_over(const PagedParams &p, F &&of) {
+    const int lane = threadIdx.x & 63;
+    int mine = 0;
+    for (int b0 = 0; b0 < p.pages.seqs; b0 += 64)
+        if (b0 + lane < p.pages.seqs) mine += of(rows_of(p.pages, b0 + lane));
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d);
+    return __builtin_amdgcn_readfirstlane(mine);
+}
+template <class F>
+__device__ __forceinline__ int find_in(const PagedParams &p, int at, int &before, F &&of) {
+    const int lane = threadIdx.x & 63;
+    int done = 0;
+    for (int b0 = 0; b0 < p.pages.seqs; b0 += 64) {
+        const int mine = b0 + lane < p.pages.seqs ? of(rows_of(p.pages, b0 + lane)) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int other = __shfl_up(sum, d);
+            if (lane >= d) sum += other;
+        }
+        const uint64_t hit = __ballot(done + sum > at);
+        if (hit != 0) {
+            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            before = __builtin_amdgcn_readfirstlane(done + __shfl(sum - mine, l));
+            return __builtin_amdgcn_readfirstlane(b0 + l);
+        }
+        done += __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+    }
+    return -1;
+}
+// Units of work of one block of paged_few_kernel: alike for all, but `least` at least.
+__device__ __forceinline__ int share_of(const PagedParams &p, int units, int blocks) { return max(p.least, (units + blocks - 1) / blocks); }
+
+// ---- few rows --------------------------------------------------------------------------------------------------------------------------------------------------------
+// An item is one key/value head of one sequence, its work the sequence's positions in units of 64. The units of all items, one after another, are cut into equal shares,
+// one for a block, so that a batch of sequences of very different lengths keeps all blocks busy to the end; where a cut falls inside an item, both sides leave
+// (m, l, O) as partials, and paged_few_merge_kernel joins them. A block has at most two such pieces (its first and its last), so the partials' memory does not
+// grow with the batch. `least` == 0: a block takes an item whole and nothing is merged.
+//
+// Inside a block the four wavefronts take every fourth 16 positions through LDS stages of their own and meet at the end of an item.
+template <int DT, int D, int NST>
+__global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
+    constexpr int PITCH = D * 2, LK = D / 32, LPS = 2 * LK, VAT = GROUP * PITCH, STAGE = 2 * VAT, RING = NST * STAGE;
+    constexpr int DK = D / 32, DT16 = D / 16, PW = D + 4, PIECES = D / 8;
+    static_assert(NST >= 2 && (NST - 1) * LPS < 64, "the count in s_waitcnt");
+    static_assert(FEW * PW * 4 <= RING, "the partials take the place of the stages");
+    extern __shared__ __align__(1024) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, lq = lane >> 4;
+    char *ring = smem + wave * RING;
+
+    // ---- this block's share
+    int b, hkv, unit, left;  // where it begins, and how many units it has
+    const int share_index = blockIdx.x;
+    auto units = [&](const SeqRows &s) { return units_of(p, s); };
+    if (p.least == 0) {
+        b = share_index / p.Hkv;
+        hkv = share_index - b * p.Hkv;
+        unit = 0;
+        left = units_of(p, same_rows_of(p.pages, b));
+        if (left == 0) return;
+    } else {
+        const int all = sum_over(p, units) * p.Hkv, share = share_of(p, all, gridDim.x);
+        const int64_t from = static_cast<int64_t>(share_index) * share;
+        if (from >= all) return;
+        left = min(share, all - static_cast<int>(from));
+        // units of a sequence before all heads': the scan counts a sequence's units once
+        int before;
+        b = find_in(p, static_cast<int>(from) / p.Hkv, before, units);
+        // (the sequence whose Hkv * units hold `from`)
+        const int u = units_of(p, same_rows_of(p.pages, b)), inside = static_cast<int>(from) - before * p.Hkv;
+        hkv = inside / u;
+        unit = inside - hkv * u;
+    }
+    // pieces of 1024 bytes of a group: which row and piece this lane loads
+    uint32_t k_off[LK], v_off[LK];
+#pragma unroll
+    for (int j = 0; j < LK; ++j) {
+        const int at = j * 64 + lane, r = at / PIECES, piece = (at % PIECES) ^ turned<D>(r);
+        k_off[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.pages.k_pos) * 2 + piece * 16;
+        v_off[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.pages.v_pos) * 2 + piece * 16;
+    }
+    const int vkey = 4 * lq + (l16 >> 2);  // the row and 8-byte piece that this lane points the transposing read at
+    const uint32_t k_rd = lds_addr_of(ring) + l16 * PITCH + (lq ^ turned<D>(l16)) * 16;
+    const uint32_t v_rd = lds_addr_of(ring) + VAT + vkey * PITCH + (((l16 & 3) >> 1) ^ turned<D>(vkey)) * 16 + (l16 & 1) * 8;
+
+    while (left > 0 && b < p.pages.seqs) {
+        const SeqRows s = same_rows_of(p.pages, b);
+        const int n_units = units_of(p, s);
+        if (n_units == 0) {  // the other kernel's, or empty
+            ++b;
+            continue;
+        }
+        const int take = min(left, n_units - unit);
+        const int k_begin = unit * UNIT, k_end = min((unit + take) * UNIT, s.length);
+        const bool from_start = unit == 0, to_end = unit + take == n_units;
+        const int rows = s.count * p.G;
+        const int groups = k_end > k_begin ? (k_end - k_begin + GROUP - 1) / GROUP : 0;
+        const int n = (groups - wave + 3) / 4;  // of this wavefront: wave, wave + 4, ...
+
+        // ---- this lane's row (those past the last: row 0, never stored)
+        const int row = l16 < rows ? l16 : 0, place = row / p.G;
+        const int last = s.length - s.count + place;  // position that the row sees last
+        const int seen_by_all = s.length - s.count;
+        const char *qrow = p.q + (static_cast<int64_t>(s.first + place) * p.q_row + static_cast<int64_t>(hkv * p.G + row - place * p.G) * p.q_head) * 2;
+        u32x4 qf[DK];
+#pragma unroll
+        for (int kk = 0; kk < DK; ++kk) qf[kk] = *reinterpret_cast<const u32x4 *>(qrow + (32 * kk + 8 * lq) * 2);
+
+        f32x4 acc[DT16];
+        float m_run = -INFINITY, l_run = 0.f;  // l_run: of the positions that this lane saw
+#pragma unroll
+        for (int dt = 0; dt < DT16; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (n > 0) {
+            const int group0 = k_begin / GROUP + wave;  // of the sequence
+            const int64_t k_at = hkv * p.pages.k_head, v_at = hkv * p.pages.v_head;
+            // the pages of this wavefront's next 64 groups, one in a lane
+            auto pages_from = [&](int i) {
+                const int g = group0 + 4 * (i + lane);
+                return g * GROUP < s.length ? page_of(p.pages, b, g * GROUP) : -1;
+            };
+            int my_page = pages_from(0), base = 0;
+            arrived(my_page);
+            unrolled<DK>([&](auto kc) { arrived(qf[decltype(kc)::value]); });
+            auto load = [&](int stage_off, int i) __attribute__((always_inline)) {
+                if (i < n) {
+                    if (i - base == 64) {
+                        base = i;
+                        my_page = pages_from(i);
+                        arrived(my_page);
+                    }
+                    const int page = __builtin_amdgcn_readlane(my_page, i - base);
+                    const int slot = ((group0 + 4 * i) * GROUP) & ((1 << p.pages.shift) - 1);
+                    const __amdgpu_buffer_rsrc_t kr = group_rsrc(p.pages.k, page, p.pages.k_page, k_at, slot, p.pages.k_pos, D);
+                    const __amdgpu_buffer_rsrc_t vr = group_rsrc(p.pages.v, page, p.pages.v_page, v_at, slot, p.pages.v_pos, D);
+#pragma unroll
+                    for (int j = 0; j < LK; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void *)(ring + stage_off + j * 1024), 16, static_cast<int>(k_off[j]), 0, 0, 2);
+#pragma unroll
+                    for (int j = 0; j < LK; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *)(ring + stage_off + VAT + j * 1024), 16, static_cast<int>(v_off[j]), 0, 0, 2);
+                } else {  // as many loads, so that the waits can count: of nothing
+                    const __amdgpu_buffer_rsrc_t none = make_rsrc(p.pages.k, 0);
+#pragma unroll
+                    for (int j = 0; j < LPS; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(none, (lds_void *)(ring + stage_off + j * 1024), 16, 0, 0, 0, 0);
+                }
+            };
+            unrolled<NST>([&](auto sc) { load(decltype(sc)::value * STAGE, decltype(sc)::value); });
+            int stage_off = 0;
+            for (int i = 0; i < n; ++i) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * LPS) : "memory");
+                u32x4 kf[DK];
+                u32x2 vf[DT16];
+                unrolled<DK>([&](auto kc) {
+                    constexpr int kk = decltype(kc)::value;
+                    kf[kk] = lds_read16<0>(D == 96 ? k_rd + stage_off + kk * 64 : (k_rd + stage_off) ^ (kk * 64));
+                });
+                unrolled<DT16>([&](auto dc) {
+                    constexpr int dt = decltype(dc)::value;
+                    vf[dt] = lds_transpose_read(D == 96 ? ((v_rd + stage_off) ^ ((dt & 1) * 32)) + (dt >> 1) * 64 : (v_rd + stage_off) ^ (dt * 32));
+                });
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                unrolled<DK>([&](auto kc) { already_landed(kf[decltype(kc)::value]); });
+                unrolled<DT16>([&](auto dc) { half_landed(vf[decltype(dc)::value]); });
+                load(stage_off, i + NST);
+                stage_off = stage_off + STAGE == RING ? 0 : stage_off + STAGE;
+
+                // S^T = K Q^T: sc[j] = score of position 4 lq + j of the group against this lane's row
+                f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < DK; ++kk) sc = mfma16<DT>(kf[kk], qf[kk], sc);
+                const int k0 = (group0 + 4 * i) * GROUP;
+                const bool partly = k0 + GROUP - 1 > seen_by_all;  // some row does not see all of them
+                if (partly) {
+                    // the values behind the sequence's end are whatever the page held
+                    const int have = s.length - k0 - 4 * lq;
+                    const uint32_t m0 = have >= 2 ? 0xffffffffu : have == 1 ? 0xffffu : 0u, m1 = have >= 4 ? 0xffffffffu : have == 3 ? 0xffffu : 0u;
+#pragma unroll
+                    for (int dt = 0; dt < DT16; ++dt) vf[dt] &= u32x2{m0, m1};
+                }
+                // online softmax: probabilities are taken against a maximum that is raised only when a score outgrows it by 2^LAZY
+                constexpr float LAZY = 6.0f;
+                const float neg_ref = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[j] = fmaf(sc[j], p.scale_log2, neg_ref);
+                if (partly) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[j] = k0 + 4 * lq + j <= last ? sc[j] : -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+                if (__any(mx > LAZY || m_run == -INFINITY)) {
+                    mx = fmaxf(mx, __shfl_xor(mx, 16));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32));
+                    const float m_abs = mx - neg_ref;
+                    const bool up = m_abs > m_run + LAZY;  // false for -inf on either side
+                    const float m_new = up ? m_abs : m_run;
+                    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+                    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+                    const float move = -neg_ref - m_use;
+                    m_run = m_new;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < DT16; ++dt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[dt][j] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[j] += move;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[j] = __builtin_amdgcn_exp2f(sc[j]);
+                l_run += (sc[0] + sc[1]) + (sc[2] + sc[3]);
+                // probabilities are rounded to the dtype (half a step of it each, as errors of either sign that the sum averages)
+                const u32x2 pf = {pack2_half<DT>(sc[0], sc[1]), pack2_half<DT>(sc[2], sc[3])};
+                u32x2 all[DT16];
+                bool apart = false;
+                if (partly && s.count > 1) {
+#pragma unroll
+                    for (int dt = 0; dt < DT16; ++dt) {
+                        apart = apart || Beyond<DT>::any(vf[dt].x) || Beyond<DT>::any(vf[dt].y);
+                        all[dt] = vf[dt];
+                        vf[dt] = u32x2{Beyond<DT>::finite(vf[dt].x), Beyond<DT>::finite(vf[dt].y)};
+                    }
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT16; ++dt) acc[dt] = mfma16_k16<DT>(vf[dt], pf, acc[dt]);
+                if (__any(apart)) {
+#pragma unroll
+                    for (int dt = 0; dt < DT16; ++dt) {
+                        const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+                        const f32x4 plus = mfma16_k16<DT>(u32x2{Beyond<DT>::ones(all[dt].x, 0), Beyond<DT>::ones(all[dt].y, 0)}, pf, zero);
+                        const f32x4 minus = mfma16_k16<DT>(u32x2{Beyond<DT>::ones(all[dt].x, 0x8000u), Beyond<DT>::ones(all[dt].y, 0x8000u)}, pf, zero);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[dt][j] += (plus[j] > 0.f ? INFINITY : 0.f) - (minus[j] > 0.f ? INFINITY : 0.f);
+                    }
+                }
+            }
+        }
+        l_run += __shfl_xor(l_run, 16);
+        l_run += __shfl_xor(l_run, 32);
+        // ---- the four wavefronts' results meet in the place of the stages, once every load into them has landed
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        float *mine = reinterpret_cast<float *>(smem) + (wave * FEW + l16) * PW;
+        if (l16 < rows) {
+#pragma unroll
+            for (int dt = 0; dt < DT16; ++dt) *reinterpret_cast<f32x4 *>(mine + 16 * dt + 4 * lq) = acc[dt];
+            if (lq == 0) *reinterpret_cast<float2 *>(mine + D) = make_float2(m_run, l_run);
+        }
+        __syncthreads();
+        constexpr int per_row = D / 4;
+        const float *parts = reinterpret_cast<const float *>(smem);
+        const bool whole = from_start && to_end;
+        // the block's first piece, where it continues an item, has its even slot, one that goes on behind the block its odd slot
+        float *out_part = p.part + (static_cast<int64_t>(2 * share_index) + (from_start ? 1 : 0)) * FEW * PW;
+        for (int e = tid; e < rows * per_row; e += 256) {
+            const int r = e / per_row, d4 = (e % per_row) * 4;
+            float M = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) M = fmaxf(M, parts[(v * FEW + r) * PW + D]);
+            const float m_use = M == -INFINITY ? 0.f : M;
+            float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float weight = exp2f(parts[(v * FEW + r) * PW + D] - m_use);
+                const f32x4 ov = *reinterpret_cast<const f32x4 *>(parts + (v * FEW + r) * PW + d4);
+                l += weight * parts[(v * FEW + r) * PW + D + 1];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] += weight * ov[j];
+            }
+            if (whole) {
+                const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // a sum of NaN stays one
+                const int at = r / p.G;
+                *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + at) * p.o_row + static_cast<int64_t>(hkv * p.G + r - at * p.G) * p.o_head + d4) * 2) =
+                    make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
+            } else {
+                *reinterpret_cast<f32x4 *>(out_part + r * PW + d4) = f32x4{o[0], o[1], o[2], o[3]};
+                if (d4 == 0) *reinterpret_cast<float2 *>(out_part + r * PW + D) = make_float2(M, l);
+            }
+        }
+        __syncthreads();  // read before the next item's loads
+        left -= take;
+        unit = 0;
+        if (++hkv == p.Hkv) {
+            hkv = 0;
+            ++b;
+        }
+    }
+}
+
+// Joins the pieces of the items that paged_few_kernel's shares cut: a block an item.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int blocks) {
+    constexpr int PW = D + 4, per_row = D / 4;
+    const int b = blockIdx.x / p.Hkv, hkv = blockIdx.x - b * p.Hkv, lane = threadIdx.x & 63;
+    const SeqRows s = rows_of(p.pages, b);
+    const int n = units_of(p, s);
+    if (n == 0) return;
+    int all = 0, before = 0;
+    for (int b0 = 0; b0 < p.pages.seqs; b0 += 64) {
+        const int u = b0 + lane < p.pages.seqs ? units_of(p, rows_of(p.pages, b0 + lane)) : 0;
+        all += u;
+        before += b0 + lane < b ? u : 0;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        all += __shfl_xor(all, d);
+        before += __shfl_xor(before, d);
+    }
+    const int share = share_of(p, all * p.Hkv, blocks);
+    const int from = before * p.Hkv + hkv * n, first = from / share, last = (from + n - 1) / share;
+    if (first == last) return;  // whole in one block, which has stored it
+    const int rows = s.count * p.G;
+    const int64_t pitch = 2 * FEW * PW;
+    for (int e = threadIdx.x; e < rows * per_row; e += 256) {
+        const int r = e / per_row, d4 = (e % per_row) * 4;
+        // the piece of block i: its odd slot where the item begins in it
+        const float *base = p.part + r * PW;
+        auto piece = [&](int i) { return base + i * pitch + (i == first ? FEW * PW : 0); };
+        float M = -INFINITY;
+        for (int i0 = first; i0 <= last; i0 += 8) {
+            float ms[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ms[j] = piece(min(i0 + j, last))[D];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) M = fmaxf(M, ms[j]);
+        }
+        const float m_use = M == -INFINITY ? 0.f : M;
+        float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+        for (int i0 = first; i0 <= last; i0 += 8) {
+            float2 ml[8];
+            f32x4 ov[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float *from_piece = piece(min(i0 + j, last));
+                ml[j] = *reinterpret_cast<const float2 *>(from_piece + D);
+                ov[j] = *reinterpret_cast<const f32x4 *>(from_piece + d4);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (i0 + j > last) continue;
+                const float weight = exp2f(ml[j].x - m_use);
+                l += weight * ml[j].y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] += weight * ov[j][i];
+            }
+        }
+        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+        const int at = r / p.G;
+        *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + at) * p.o_row + static_cast<int64_t>(hkv * p.G + r - at * p.G) * p.o_head + d4) * 2) =
+            make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
+    }
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------------------------------------------------------------------
+// A block has 32 rows of one key/value head of one sequence for each of its 8 wavefronts (4 where heads have 256 elements); row = new row * G + query head, so that the heads of a group meet the
+// same keys. It walks the positions in tiles of KT through NST stages in LDS, each wavefront loading 16 rows of K or V; one barrier a tile says that the tile is there
+// and that the stage before it is free.
+//   S^T = K Q^T   v_mfma_f32_32x32x16 with K rows as the first operand: a lane has, of ONE query row, 16 of 32 positions, and one exchange with lane ^ 32 finishes a row's maximum
+//   O^T += V^T P^T  the lane's probabilities are the second operand as they are (8 positions of each 16, in an order that the transposing read of V follows)
+// Blocks are given out with the longest key ranges first; of few blocks the positions are cut into `splits` ranges, joined by paged_many_merge_kernel.
+template <int DT, int D, int WAVES, int KT, int NST>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void paged_many_kernel(PagedParams p) {
+    constexpr int MANY = WAVES * 32, PITCH = D * 2, PIECES = D / 8, KTILE = KT * PITCH, STAGE = 2 * KTILE, PW = D + 4;
+    constexpr int NL = D / 32, KK = D / 16, DT32 = D / 32, T32 = KT / 32;
+    static_assert(WAVES / 2 == KT / GROUP, "a wavefront loads 16 rows of K or V");
+    static_assert(NST >= 3 && (NST - 2) * NL < 64, "the count in s_waitcnt");
+    extern __shared__ __align__(1024) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, h = lane >> 5;
+
+    // ---- which rows: the last sequence's last tile first
+    auto tiles_in = [&](const SeqRows &s) { return tiles_of<MANY>(p, s); };
+    const int hkv = blockIdx.x % p.Hkv, nth = blockIdx.x / p.Hkv;
+    const int all = sum_over(p, tiles_in);
+    if (nth >= all) return;
+    int before;
+    const int b = find_in(p, all - 1 - nth, before, tiles_in);
+    const int row0 = (all - 1 - nth - before) * MANY;
+    const SeqRows s = same_rows_of(p.pages, b);
+    const int rows = s.count * p.G, seen_before = s.length - s.count;
+    // a wavefront's number fixes its SIMD: rows that end early share one with rows that end late
+    const int wave_row0 = row0 + (wave < 4 ? wave : 11 - wave) * 32;
+    const int row = wave_row0 + l32, safe = row < rows ? row : wave_row0 < rows ? wave_row0 : 0, place = safe / p.G;
+    const int last = seen_before + place;
+    const int wave_first = seen_before + (wave_row0 < rows ? wave_row0 : 0) / p.G;              // what every row of the wavefront sees ends here
+    const int wave_last = wave_row0 < rows ? seen_before + min(wave_row0 + 31, rows - 1) / p.G : -1;  // and what some row sees here
+    const int seen = max(seen_before + min(row0 + MANY - 1, rows - 1) / p.G + 1, 0);
+    const int range = ((seen + KT - 1) / KT + p.splits - 1) / p.splits * KT;
+    const int k_begin = min(static_cast<int>(blockIdx.y) * range, seen), k_end = min(k_begin + range, seen);
+    const int tiles = (k_end - k_begin + KT - 1) / KT;
+
+    const char *qrow = p.q + (static_cast<int64_t>(s.first + place) * p.q_row + static_cast<int64_t>(hkv * p.G + safe - place * p.G) * p.q_head) * 2;
+    u32x4 qf[KK];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const u32x4 *>(qrow + (16 * kk + 8 * h) * 2);
+
+    // ---- this wavefront's loads: 16 rows of K or V
+    const bool loads_v = wave >= WAVES / 2;
+    const char *pool = loads_v ? p.pages.v : p.pages.k;
+    const int64_t page_step = loads_v ? p.pages.v_page : p.pages.k_page, pos_step = loads_v ? p.pages.v_pos : p.pages.k_pos, head_at = hkv * (loads_v ? p.pages.v_head : p.pages.k_head);
+    const int group = wave % (WAVES / 2);
+    uint32_t off[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        const int at = j * 64 + lane, r = at / PIECES;
+        off[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(pos_step) * 2 + ((at % PIECES) ^ turned<D>(r)) * 16;
+    }
+    char *to = smem + (loads_v ? KTILE : 0) + group * GROUP * PITCH;
+    auto pages_from = [&](int i) {
+        const int at = k_begin + (i + lane) * KT + group * GROUP;
+        return at < s.length ? page_of(p.pages, b, at) : -1;
+    };
+    int my_page = pages_from(0), base = 0;
+    arrived(my_page);
+    unrolled<KK>([&](auto kc) { arrived(qf[decltype(kc)::value]); });
+    auto load = [&](int stage_off, int i) __attribute__((always_inline)) {
+        if (i < tiles && i - base == 64) {
+            base = i;
+            my_page = pages_from(i);
+            arrived(my_page);
+        }
+        const int page = i < tiles ? __builtin_amdgcn_readlane(my_page, i - base) : -1;  // behind the last tile: as many loads, of nothing
+        const int slot = (k_begin + i * KT + group * GROUP) & ((1 << p.pages.shift) - 1);
+        const __amdgpu_buffer_rsrc_t rsrc = group_rsrc(pool, page, page_step, head_at, slot, pos_step, D);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(to + stage_off + j * 1024), 16, static_cast<int>(off[j]), 0, 0, 0);
+    };
+
+    f32x16 acc[DT32];
+    float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[dt][j] = 0.f;
+
+    // fragment addresses: row l32 of 32, piece 2 kk + h of K; rows 4 h + (l16 / 4) of 16 (and 8 further), elements 16 (l32 / 16) + 4 (l16 % 4) of 32 of V
+    const uint32_t lds0 = lds_addr_of(smem);
+    const uint32_t k_rd = lds0 + l32 * PITCH + (h ^ turned<D>(l32 & 15)) * 16;
+    const int vkey = 4 * h + ((lane & 15) >> 2), vpiece = 2 * (l32 >> 4) + ((lane & 3) >> 1);
+    const uint32_t v_rd0 = lds0 + KTILE + vkey * PITCH + (vpiece ^ turned<D>(vkey)) * 16 + (lane & 1) * 8;
+    const uint32_t v_rd1 = lds0 + KTILE + (vkey + 8) * PITCH + (vpiece ^ turned<D>(vkey + 8)) * 16 + (lane & 1) * 8;
+
+    unrolled<NST - 1>([&](auto sc) { load(decltype(sc)::value * STAGE, decltype(sc)::value); });
+    int stage_off = 0, next_off = (NST - 1) * STAGE;
+    for (int i = 0; i < tiles; ++i) {
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NST - 2) * NL) : "memory");
+        load(next_off, i + NST - 1);
+        next_off = stage_off;
+        const int k0 = k_begin + i * KT;
+        const uint32_t at = stage_off;
+        stage_off = stage_off + STAGE == NST * STAGE ? 0 : stage_off + STAGE;
+        if (k0 > wave_last) continue;
+
+        // ---- scores: sc[t][i] = position k0 + 32 t + 8 (i / 4) + 4 h + i % 4 against this lane's row
+        f32x16 sc[T32];
+        constexpr int AHEAD = KK < 4 ? KK : 4;  // fragments of K that are on their way
+        u32x4 kf[T32][AHEAD];
+        auto k_read = [&](auto kc) {
+            constexpr int kk = decltype(kc)::value;
+            unrolled<T32>([&](auto tc) {
+                constexpr int t = decltype(tc)::value;
+                // (piece 2 kk + h: of 12 pieces a row only the low two bits are turned)
+                kf[t][kk % AHEAD] = lds_read16<t * 32 * PITCH>(D == 96 ? ((k_rd + at) ^ ((kk & 1) * 32)) + (kk >> 1) * 64 : (k_rd + at) ^ (kk * 32));
+            });
+        };
+        unrolled<AHEAD>(k_read);
+#pragma unroll
+        for (int t = 0; t < T32; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sc[t][j] = 0.f;
+        unrolled<KK>([&](auto kc) {
+            constexpr int kk = decltype(kc)::value;
+            constexpr int younger = (AHEAD - 1 < KK - 1 - kk ? AHEAD - 1 : KK - 1 - kk) * T32;
+            unrolled<T32>([&](auto tc) {
+                constexpr int t = decltype(tc)::value;
+                reads_landed<younger + T32 - 1 - t>(kf[t][kk % AHEAD]);
+                sc[t] = mfma32<DT>(kf[t][kk % AHEAD], qf[kk], sc[t]);
+            });
+            if constexpr (kk + AHEAD < KK) k_read(std::integral_constant<int, kk + AHEAD>{});
+        });
+
+        // ---- online softmax, as in paged_few_kernel
+        constexpr float LAZY = 6.0f;
+        const bool partly = k0 + KT - 1 > wave_first;
+        const float neg_ref = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+        for (int t = 0; t < T32; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sc[t][j] = fmaf(sc[t][j], p.scale_log2, neg_ref);
+        if (partly) {
+            const int vis = last - k0 - 4 * h;
+#pragma unroll
+            for (int t = 0; t < T32; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sc[t][j] = 32 * t + 8 * (j >> 2) + (j & 3) <= vis ? sc[t][j] : -INFINITY;
+        }
+        float mx = fmaxf(sc[0][0], sc[0][1]);
+#pragma unroll
+        for (int t = 0; t < T32; ++t)
+#pragma unroll
+            for (int j = (t == 0 ? 2 : 0); j < 16; j += 2) mx = fmaxf(fmaxf(mx, sc[t][j]), sc[t][j + 1]);
+        if (__any(mx > LAZY || m_run == -INFINITY)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float m_abs = mx - neg_ref;
+            const bool up = m_abs > m_run + LAZY;  // false for -inf on either side
+            const float m_new = up ? m_abs : m_run;
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+            const float move = -neg_ref - m_use;
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[dt][j] *= alpha;
+#pragma unroll
+            for (int t = 0; t < T32; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sc[t][j] += move;
+        }
+        u32x4 pf[2 * T32];
+#pragma unroll
+        for (int t = 0; t < T32; ++t) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sc[t][j] = __builtin_amdgcn_exp2f(sc[t][j]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                pf[2 * t + u] = u32x4{pack2_half<DT>(sc[t][8 * u], sc[t][8 * u + 1]), pack2_half<DT>(sc[t][8 * u + 2], sc[t][8 * u + 3]), pack2_half<DT>(sc[t][8 * u + 4], sc[t][8 * u + 5]),
+                                      pack2_half<DT>(sc[t][8 * u + 6], sc[t][8 * u + 7])};
+            }
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) l_run += (sc[t][j] + sc[t][j + 1]) + (sc[t][j + 2] + sc[t][j + 3]);
+        }
+
+        // ---- O^T += V^T P^T, 16 positions at a time
+        auto v_reads = [&](auto uc, u32x2 (&lo)[DT32], u32x2 (&hi)[DT32]) {
+            constexpr int u = decltype(uc)::value;
+            unrolled<DT32>([&](auto dc) {
+                constexpr int dt = decltype(dc)::value;
+                const uint32_t a0 = D == 96 ? v_rd0 + at + dt * 64 : (v_rd0 + at) ^ (dt * 64), a1 = D == 96 ? v_rd1 + at + dt * 64 : (v_rd1 + at) ^ (dt * 64);
+                lo[dt] = lds_transpose_read(a0 + u * GROUP * PITCH);
+                hi[dt] = lds_transpose_read(a1 + u * GROUP * PITCH);
+            });
+        };
+        unrolled<2 * T32>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            u32x2 lo[DT32], hi[DT32];
+            v_reads(uc, lo, hi);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            unrolled<DT32>([&](auto dc) {
+                half_landed(lo[decltype(dc)::value]);
+                half_landed(hi[decltype(dc)::value]);
+            });
+            if (!partly) {
+                unrolled<DT32>([&](auto dc) {
+                    constexpr int dt = decltype(dc)::value;
+                    acc[dt] = mfma32<DT>(u32x4{lo[dt].x, lo[dt].y, hi[dt].x, hi[dt].y}, pf[u], acc[dt]);
+                });
+                return;
+            }
+            // the values behind the sequence's end are whatever the page held
+            const int have = s.length - (k0 + 16 * u + 4 * h), more = have - 8;
+            const u32x2 m_lo = {have >= 2 ? 0xffffffffu : have == 1 ? 0xffffu : 0u, have >= 4 ? 0xffffffffu : have == 3 ? 0xffffu : 0u};
+            const u32x2 m_hi = {more >= 2 ? 0xffffffffu : more == 1 ? 0xffffu : 0u, more >= 4 ? 0xffffffffu : more == 3 ? 0xffffu : 0u};
+            unrolled<DT32>([&](auto dc) {
+                constexpr int dt = decltype(dc)::value;
+                const u32x4 v = u32x4{lo[dt].x, lo[dt].y, hi[dt].x, hi[dt].y} & u32x4{m_lo.x, m_lo.y, m_hi.x, m_hi.y};
+                acc[dt] = mfma32<DT>(u32x4{Beyond<DT>::finite(v.x), Beyond<DT>::finite(v.y), Beyond<DT>::finite(v.z), Beyond<DT>::finite(v.w)}, pf[u], acc[dt]);
+                if (!__any(Beyond<DT>::any(v.x) || Beyond<DT>::any(v.y) || Beyond<DT>::any(v.z) || Beyond<DT>::any(v.w))) return;
+#pragma unroll
+                for (uint32_t sign : {0u, 0x8000u}) {
+                    f32x16 found;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) found[j] = 0.f;
+                    found = mfma32<DT>(u32x4{Beyond<DT>::ones(v.x, sign), Beyond<DT>::ones(v.y, sign), Beyond<DT>::ones(v.z, sign), Beyond<DT>::ones(v.w, sign)}, pf[u], found);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[dt][j] += found[j] > 0.f ? (sign != 0 ? -INFINITY : INFINITY) : 0.f;
+                }
+            });
+        });
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads into LDS end before the block does
+    l_run += __shfl_xor(l_run, 32);
+
+    // ---- acc[dt][i] = O[this lane's row][32 dt + 8 (i / 4) + 4 h + i % 4]
+    if (row >= rows) return;
+    const int64_t token = s.first + place;
+    const int head = hkv * p.G + row - place * p.G;
+    if (p.splits == 1) {
+        const float inv = l_run > 0.f ? 1.0f / l_run : l_run == 0.f ? 0.f : l_run;  // a sum of NaN stays one
+        char *orow = p.o + (token * p.o_row + head * p.o_head) * 2;
+#pragma unroll
+        for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+                *reinterpret_cast<uint2 *>(orow + (32 * dt + 2 * j + 4 * h) * 2) =
+                    make_uint2(pack2_half<DT>(acc[dt][j] * inv, acc[dt][j + 1] * inv), pack2_half<DT>(acc[dt][j + 2] * inv, acc[dt][j + 3] * inv));
+        return;
+    }
+    float *pr = p.part + ((static_cast<int64_t>(blockIdx.y) * p.pages.rows + token) * (p.Hkv * p.G) + head) * PW;
+#pragma unroll
+    for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) *reinterpret_cast<f32x4 *>(pr + 32 * dt + 2 * j + 4 * h) = f32x4{acc[dt][j], acc[dt][j + 1], acc[dt][j + 2], acc[dt][j + 3]};
+    if (h == 0) *reinterpret_cast<float2 *>(pr + D) = make_float2(m_run, l_run);
+}
+
+// Joins the key ranges of paged_many_kernel's rows: a block a new row, all its query heads.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_many_merge_kernel(PagedParams p) {
+    constexpr int PW = D + 4, per_row = D / 4;
+    const int token = blockIdx.x, Hq = p.Hkv * p.G;
+    int place;
+    const int b = seq_of_row(p.pages, token, place);
+    if (b < 0) return;
+    const SeqRows s = rows_of(p.pages, b);
+    if (place >= s.count || is_few(p, s.count)) return;
+    const int64_t pitch = static_cast<int64_t>(p.pages.rows) * Hq * PW;
+    for (int e = blockIdx.y * 256 + threadIdx.x; e < Hq * per_row; e += gridDim.y * 256) {
+        const int head = e / per_row, d4 = (e % per_row) * 4;
+        const float *pr = p.part + (static_cast<int64_t>(token) * Hq + head) * PW;
+        float M = -INFINITY;
+        for (int i0 = 0; i0 < p.splits; i0 += 8) {
+            float ms[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ms[j] = pr[min(i0 + j, p.splits - 1) * pitch + D];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) M = fmaxf(M, ms[j]);
+        }
+        const float m_use = M == -INFINITY ? 0.f : M;
+        float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+        for (int i0 = 0; i0 < p.splits; i0 += 8) {
+            float2 ml[8];
+            f32x4 ov[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float *from = pr + min(i0 + j, p.splits - 1) * pitch;
+                ml[j] = *reinterpret_cast<const float2 *>(from + D);
+                ov[j] = *reinterpret_cast<const f32x4 *>(from + d4);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (i0 + j >= p.splits) continue;
+                const float weight = exp2f(ml[j].x - m_use);
+                l += weight * ml[j].y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] += weight * ov[j][i];
+            }
+        }
+        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+        *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(token) * p.o_row + static_cast<int64_t>(head) * p.o_head + d4) * 2) =
+            make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------------------------------------
+// How a call is laid out, from what the host knows: the number of rows and sequences, and bounds of their new rows and lengths.
+struct Plan {
+    bool few, many;
+    int few_blocks, least;  // paged_few_kernel: blocks, and units a block takes at least (0: a block an item)
+    int64_t tiles;          // paged_many_kernel: row tiles of a key/value head, at most
+    int splits;
+    uint64_t bytes;         // of partials
+};
+
+// Heads of 256 elements need the registers of two wavefronts each.
+constexpr int waves_of(int64_t D) { return D == 256 ? 4 : 8; }
+
+Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, bool packed, bool counted, int64_t max_new, int64_t max_length, int64_t room, int cus) {
+    const int64_t G = Hq / Hkv, each = packed ? 0 : rows / seqs;
+    const int64_t most = packed ? (max_new < rows ? max_new : rows) : (max_new < each ? max_new : each);  // new rows of a sequence
+    Plan p{};
+    p.few = G <= FEW && (packed || counted || most * G <= FEW);
+    p.many = most * G > FEW;
+    if (p.few) {
+        const int64_t items = seqs * Hkv;
+        const int per_cu = D <= 64 ? 5 : D <= 96 ? 3 : D <= 128 ? 2 : 1;
+        const bool cut = decode_splits(items, max_length > 0 ? max_length : 1, D <= 64 ? 64 : 128, cus) > 1 || (items < 4ll * per_cu * cus && max_length > 512);
+        if (cut && items * (room / UNIT + 1) < (1ll << 31)) {  // units are counted in 32 bits
+            p.few_blocks = per_cu * cus;
+            p.least = 4;
+            p.bytes = static_cast<uint64_t>(2) * p.few_blocks * FEW * (D + 4) * sizeof(float);
+        } else {
+            p.few_blocks = static_cast<int>(items);
+        }
+    }
+    if (p.many) {
+        const int64_t MANY = waves_of(D) * 32;
+        p.tiles = packed ? rows * G / MANY + seqs : seqs * ((each * G + MANY - 1) / MANY);
+        p.splits = 1;
+        const int64_t blocks = (rows * G + MANY - 1) / MANY * Hkv, keys = max_length > 0 ? max_length : 1;
+        if (blocks < cus) {
+            int64_t splits = cus / blocks;
+            if (splits > keys / 256) splits = keys / 256;  // a range has 256 positions or more
+            if (splits > 32) splits = 32;
+            if (splits < 1) splits = 1;
+            p.splits = static_cast<int>(splits);
+        }
+        if (p.splits > 1) {
+            const uint64_t more = static_cast<uint64_t>(p.splits) * rows * Hq * (D + 4) * sizeof(float);
+            if (more > p.bytes) p.bytes = more;
+        }
+    }
+    return p;
+}
+
+template <int DT, int D>
+int launch(const PagedParams &base, const Plan &plan, hipStream_t s) {
+    PagedParams p = base;
+    int dev = 0;
+    TPAMD_HIP(hipGetDevice(&dev));
+    if (plan.many) {
+        constexpr int WAVES = waves_of(D), KT = WAVES * 8, NST = D >= 128 ? 4 : 3, LDS = NST * 2 * KT * D * 2;
+        static thread_local int configured = -1;
+        if (configured != dev) {
+            TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DT, D, WAVES, KT, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+            configured = dev;
+        }
+        p.splits = plan.splits;
+        const int64_t blocks = plan.tiles * p.Hkv;
+        TPAMD_REQUIRE(blocks * plan.splits < (1ll << 23), "tpamd_attention_paged: too many rows for one launch");
+        hipLaunchKernelGGL((paged_many_kernel<DT, D, WAVES, KT, NST>), dim3(static_cast<unsigned>(blocks), plan.splits), dim3(WAVES * 64), LDS, s, p);
+        TPAMD_HIP(hipGetLastError());
+        if (plan.splits > 1) {
+            const unsigned y = static_cast<unsigned>((static_cast<int64_t>(p.Hkv) * p.G * (D / 4) + 255) / 256);
+            hipLaunchKernelGGL((paged_many_merge_kernel<DT, D>), dim3(static_cast<unsigned>(p.pages.rows), y < 4 ? y : 4), dim3(256), 0, s, p);
+            TPAMD_HIP(hipGetLastError());
+        }
+    }
+    if (plan.few) {  // behind the other: their partials share the memory
+        constexpr int NST = 2, LDS = 4 * NST * 2 * GROUP * D * 2;
+        static thread_local int configured = -1;
+        if (configured != dev) {
+            TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_few_kernel<DT, D, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+            configured = dev;
+        }
+        p.least = plan.least;
+        hipLaunchKernelGGL((paged_few_kernel<DT, D, NST>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(256), LDS, s, p);
+        TPAMD_HIP(hipGetLastError());
+        if (plan.least > 0) {
+            hipLaunchKernelGGL((paged_few_merge_kernel<DT, D>), dim3(static_cast<unsigned>(p.pages.seqs * p.Hkv)), dim3(256), 0, s, p, plan.few_blocks);
+            TPAMD_HIP(hipGetLastError());
+        }
+    }
+    return TPAMD_OK;
+}
+
+}  // namespace
+
+int take_pages(const char *who, const tpamd_pages *g, int64_t rows, int64_t Hkv, int64_t D, PagesView *out) {
+    TPAMD_REQUIRE(g->seqs >= 0 && g->seqs < (1ll << 24) && g->columns >= 0 && g->pages >= 0 && g->pages < (1ll << 31), "%s: bad dimension", who);
+    TPAMD_REQUIRE(g->page >= GROUP && g->page < (1ll << 30) && (g->page & (g->page - 1)) == 0, "%s: a page has %lld positions: a power of two from %d on is needed", who, (long long)g->page, GROUP);
+    TPAMD_REQUIRE(g->columns * g->page < (1ll << 31), "%s: %lld pages of %lld positions a sequence are too many", who, (long long)g->columns, (long long)g->page);
+    TPAMD_REQUIRE(g->starts == nullptr || g->counts == nullptr, "%s: starts (packed rows) or counts (padded rows), not both", who);
+    TPAMD_REQUIRE(g->seqs == 0 || g->starts != nullptr || rows % g->seqs == 0, "%s: %lld rows are not the same number for each of %lld sequences", who, (long long)rows, (long long)g->seqs);
+    for (int64_t s : {g->k_page, g->k_head, g->k_pos, g->v_page, g->v_head, g->v_pos, g->table_row}) TPAMD_REQUIRE(s >= 0, "%s: a negative stride", who);
+    PagesView v{};
+    v.seqs = static_cast<int>(g->seqs);
+    if (g->seqs > 0) {
+        TPAMD_REQUIRE(g->lengths != nullptr && (g->columns == 0 || g->table != nullptr) && (g->pages == 0 || (g->k_pages && g->v_pages)), "%s: null pointer", who);
+        v.each = g->starts != nullptr ? 0 : static_cast<int>(rows / g->seqs);
+    }
+    v.k = static_cast<char *>(g->k_pages); v.v = static_cast<char *>(g->v_pages);
+    v.k_page = g->k_page; v.k_head = g->k_head; v.k_pos = g->k_pos; v.v_page = g->v_page; v.v_head = g->v_head; v.v_pos = g->v_pos;
+    v.table = g->table; v.lengths = g->lengths; v.starts = g->starts; v.counts = g->counts; v.table_row = g->table_row;
+    v.pages = static_cast<int>(g->pages);
+    v.shift = __builtin_ctzll(static_cast<unsigned long long>(g->page));
+    v.rows = static_cast<int>(rows);
+    v.room = static_cast<int>(g->columns * g->page);
+    *out = v;
+    return TPAMD_OK;
+}
+
+namespace {
+int check_sizes(const char *who, const tpamd_pages *g, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D) {
+    TPAMD_REQUIRE(g != nullptr, "%s: null pointer", who);
+    TPAMD_REQUIRE(rows >= 0 && rows < (1ll << 24) && Hq > 0 && Hkv > 0 && Hq < (1ll << 16), "%s: bad dimension", who);
+    TPAMD_REQUIRE(Hq % Hkv == 0, "%s: %lld query heads are not a multiple of %lld key/value heads", who, (long long)Hq, (long long)Hkv);
+    TPAMD_REQUIRE(rows * Hq < (1ll << 31) && g->seqs * Hkv < (1ll << 24), "%s: too many rows or sequences for one call", who);
+    if (D != 64 && D != 96 && D != 128 && D != 256) {
+        set_error("%s: head_dim must be 64, 96, 128 or 256", who);
+        return TPAMD_ERR_UNSUPPORTED;
+    }
+    return TPAMD_OK;
+}
+}  // namespace
+
+}  // namespace tpamd
+
+using namespace tpamd;
+
+extern "C" int tpamd_attention_paged_workspace(const tpamd_pages *pages, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_length, uint64_t *bytes_out) {
+    const char *who = "tpamd_attention_paged_workspace";
+    if (int rc = check_sizes(who, pages, rows, Hq, Hkv, D); rc != TPAMD_OK) return rc;
+    TPAMD_REQUIRE(bytes_out != nullptr && max_new >= 0 && max_length >= 0, "%s: bad argument", who);
+    *bytes_out = 0;
+    PagesView view;
+    if (int rc = take_pages(who, pages, rows, Hkv, D, &view); rc != TPAMD_OK) return rc;
+    if (rows == 0 || view.seqs == 0) return TPAMD_OK;
+    int dev = 0, cus = 256;
+    TPAMD_HIP(hipGetDevice(&dev));
+    if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
+    *bytes_out = plan_of(rows, view.seqs, Hq, Hkv, D, view.starts != nullptr, view.counts != nullptr, max_new, max_length < view.room ? max_length : view.room, view.room, cus).bytes;
+    return TPAMD_OK;
+}
+
+extern "C" int tpamd_attention_paged(const void *q_dev, int64_t q_row, int64_t q_head, const tpamd_pages *pages, void *out_dev, int64_t o_row, int64_t o_head, int64_t rows, int64_t Hq,
+                                     int64_t Hkv, int64_t D, int64_t max_new, int64_t max_length, float scale, int dtype, void *workspace_dev, uint64_t workspace_bytes, void *stream) {
+    const char *who = "tpamd_attention_paged";
+    TPAMD_REQUIRE(dtype == TPAMD_BF16 || dtype == TPAMD_F16, "%s: dtype must be BF16 or F16", who);
+    if (int rc = check_sizes(who, pages, rows, Hq, Hkv, D); rc != TPAMD_OK) return rc;
+    TPAMD_REQUIRE(max_new >= 0 && max_length >= 0 && q_row >= 0 && q_head >= 0 && o_row >= 0 && o_head >= 0, "%s: bad argument", who);
+    PagedParams p{};
+    if (int rc = take_pages(who, pages, rows, Hkv, D, &p.pages); rc != TPAMD_OK) return rc;
+    if (rows == 0 || p.pages.seqs == 0) return TPAMD_OK;
+    TPAMD_REQUIRE(q_dev != nullptr && out_dev != nullptr, "%s: null pointer", who);
+    bool ok = aligned(q_dev, 16) && q_row % 8 == 0 && q_head % 8 == 0 && aligned(out_dev, 8) && o_row % 4 == 0 && o_head % 4 == 0 && aligned(p.pages.k, 16) && aligned(p.pages.v, 16);
+    for (int64_t s : {p.pages.k_page, p.pages.k_head, p.pages.k_pos, p.pages.v_page, p.pages.v_head, p.pages.v_pos}) ok = ok && s % 8 == 0;
+    ok = ok && p.pages.k_pos < (1ll << 26) && p.pages.v_pos < (1ll << 26);  // 16 positions by 32-bit byte offsets
+    if (!ok) {
+        set_error("%s: rows of q, keys and values must lie on 16-byte boundaries (out: 8), positions of a page within 2^26 elements", who);
+        return TPAMD_ERR_UNSUPPORTED;
+    }
+    int dev = 0, cus = 256;
+    TPAMD_HIP(hipGetDevice(&dev));
+    if (int rc = device_cus(dev, &cus); rc != TPAMD_OK) return rc;
+    const Plan plan = plan_of(rows, p.pages.seqs, Hq, Hkv, D, p.pages.starts != nullptr, p.pages.counts != nullptr, max_new, max_length < p.pages.room ? max_length : p.pages.room, p.pages.room, cus);
+    TPAMD_REQUIRE(workspace_bytes >= plan.bytes && (plan.bytes == 0 || (workspace_dev != nullptr && aligned(workspace_dev, 16))), "%s: %llu bytes of workspace on a 16-byte boundary are needed", who,
+                  (unsigned long long)plan.bytes);
+    p.q = static_cast<const char *>(q_dev);
+    p.o = static_cast<char *>(out_dev);
+    p.q_row = q_row; p.q_head = q_head; p.o_row = o_row; p.o_head = o_head;
+    p.part = static_cast<float *>(workspace_dev);
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv); p.D = static_cast<int>(D);
+    p.few = plan.few; p.many = plan.many;
+    p.splits = 1;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool bf = dtype == TPAMD_BF16;
+    switch (D) {
+        case 64: return bf ? launch<TPAMD_BF16, 64>(p, plan, s) : launch<TPAMD_F16, 64>(p, plan, s);
+        case 96: return bf ? launch<TPAMD_BF16, 96>(p, plan, s) : launch<TPAMD_F16, 96>(p, plan, s);
+        case 128: return bf ? launch<TPAMD_BF16, 128>(p, plan, s) : launch<TPAMD_F16, 128>(p, plan, s);
+        default: return bf ? launch<TPAMD_BF16, 256>(p, plan, s) : launch<TPAMD_F16, 256>(p, plan, s);
+    }
+}
