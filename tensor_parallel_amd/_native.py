@@ -1532,101 +1532,127 @@ def _one_axis(t: torch.Tensor, axes: int) -> torch.Tensor:
     return t if axes == 1 else t.flatten(0, axes - 1) if axes > 1 else t.unsqueeze(0)
 
 
-def _heads_operands(what: str, q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor]) -> tuple:
-    """q [rows, Hq, D] or [rows, Hkv, per, D], k, v [rows, Hkv, D], and the axes that the rows had; what they have in common is checked."""
+def _elsewhere(what: str, q: torch.Tensor, name: str, t: torch.Tensor) -> None:
+    raise ValueError(f"{what}: q is on {q.device}, {name} on {t.device}")
+
+
+def _heads(what: str, q, k, v, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps) -> tuple:
+    """Checks the operands of `rotate_heads` and (with v) `append_paged`; (tpamd_heads, what it points to, outputs, sizes, the rows' axes)."""
     if not q.is_cuda:
         require_device(q, what)
-    code = _HALF_CODES.get(q.dtype)
-    if code is None or k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+    dtype, index = q.dtype, q.get_device()
+    code = _HALF_CODES.get(dtype)
+    if code is None or k.dtype != dtype or (v is not None and v.dtype != dtype):
         raise TypeError(f"{what}: q, k and v must share bfloat16 or float16")
-    axes = k.dim() - 2
-    if axes < 0 or q.dim() not in (k.dim(), k.dim() + 1) or q.shape[:axes] != k.shape[:axes] or q.shape[-1] != k.shape[-1] or (v is not None and v.shape != k.shape) or (
-            q.dim() > k.dim() and q.shape[axes] != k.shape[axes]):
-        raise ValueError(f"{what}: shapes q {tuple(q.shape)}, k {tuple(k.shape)}{'' if v is None else f', v {tuple(v.shape)}'} do not fit")
-    if k.device != q.device or (v is not None and v.device != q.device):
+    qs, ks = q.shape, k.shape
+    axes = len(ks) - 2
+    if axes < 0 or len(qs) - len(ks) not in (0, 1) or qs[:axes] != ks[:axes] or qs[-1] != ks[-1] or (v is not None and v.shape != ks) or (len(qs) > len(ks) and qs[axes] != ks[axes]):
+        raise ValueError(f"{what}: shapes q {tuple(qs)}, k {tuple(ks)}{'' if v is None else f', v {tuple(v.shape)}'} do not fit")
+    if k.get_device() != index or (v is not None and v.get_device() != index):
         raise ValueError(f"{what}: q, k and v lie on different devices")
-    shape = k.shape[:axes]
-    q, k, v = (None if t is None else _one_axis(t, axes) for t in (q, k, v))
-    if k.shape[-1] > 1 and (q.stride(-1) != 1 or k.stride(-1) != 1 or (v is not None and v.stride(-1) != 1)):
+    axis = ks[:axes]
+    if axes != 1:
+        q, k, v = (None if t is None else _one_axis(t, axes) for t in (q, k, v))
+        qs, ks = q.shape, k.shape
+    rows, Hkv, D = ks
+    q_step, k_step = q.stride(), k.stride()
+    v_step = k_step if v is None else v.stride()
+    if D > 1 and (q_step[-1] != 1 or k_step[2] != 1 or v_step[2] != 1):
         raise ValueError(f"{what}: heads must be contiguous")
-    return code, shape, q, k, v
-
-
-def _pack_heads(what: str, q, k, v, q_out, k_out, shape, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps) -> tuple:
-    """tpamd_heads of these operands, and the tensors that it points to."""
-    rows, Hkv, D = k.shape
-    device = q.device
-    q_head, q_group = (q.stride(1), q.stride(1) * (q.shape[1] // Hkv if Hkv else 1)) if q.dim() == 3 else (q.stride(2), q.stride(1))
-    part, table_row, table_code = 0, 0, 0
+    if len(qs) == 3:
+        Hq, q_head, q_group = qs[1], q_step[1], q_step[1] * (qs[1] // Hkv if Hkv else 1)
+    else:
+        Hq, q_head, q_group = qs[1] * qs[2], q_step[2], q_step[1]
+    part = table_row = table_code = freq_at = cos_at = sin_at = pos_at = q_norm_at = k_norm_at = 0
     if inv_freq is not None:
         if cos is not None or sin is not None:
             raise ValueError(f"{what}: frequencies or tables of cos and sin, not both")
-        if inv_freq.dim() != 1 or inv_freq.device != device:
-            raise ValueError(f"{what}: inv_freq must have one axis and lie on {device}, got {tuple(inv_freq.shape)} on {inv_freq.device}")
+        if inv_freq.dim() != 1 or inv_freq.get_device() != index:
+            raise ValueError(f"{what}: inv_freq must have one axis and lie on {q.device}, got {tuple(inv_freq.shape)} on {inv_freq.device}")
+        if positions is None and v is None:
+            raise ValueError(f"{what}: frequencies need positions")
         if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
             inv_freq = inv_freq.float().contiguous()
-        part = 2 * inv_freq.shape[0]
+        part, freq_at = 2 * inv_freq.shape[0], inv_freq.data_ptr()
     elif cos is not None or sin is not None:
-        if cos is None or sin is None or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.device != device or sin.device != device or cos.dim() < 1:
-            raise ValueError(f"{what}: cos and sin must be tables of one shape and dtype on {device}")
+        if cos is None or sin is None or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.get_device() != index or sin.get_device() != index or cos.dim() < 1:
+            raise ValueError(f"{what}: cos and sin must be tables of one shape and dtype on {q.device}")
         table_code = dtype_code(cos.dtype)
         half = cos.shape[-1]
-        if cos.numel() == half:
+        if cos.numel() == half:  # one row for all
             cos, sin = cos.reshape(1, half).contiguous(), sin.reshape(1, half).contiguous()
         else:
-            cos, sin = (t.expand(*shape, half).reshape(rows, half) for t in (cos, sin))
+            cos, sin = (t.expand(*axis, half).reshape(rows, half) for t in (cos, sin))
             if half > 1 and cos.stride(1) != 1 or cos.stride() != sin.stride():
                 cos, sin = cos.contiguous(), sin.contiguous()
             table_row = cos.stride(0)
-        part = 2 * half
+        part, cos_at, sin_at = 2 * half, cos.data_ptr(), sin.data_ptr()
     if positions is not None:
-        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != shape or positions.device != device:
-            raise ValueError(f"{what}: positions must be int64 or int32 {tuple(shape)} on {device}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
-        positions = positions.to(torch.int64).reshape(rows).contiguous()
-    norms = []
+        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != axis or positions.get_device() != index:
+            raise ValueError(f"{what}: positions must be int64 or int32 {tuple(axis)} on {q.device}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
+        if positions.dtype != torch.int64 or not positions.is_contiguous():
+            positions = positions.to(torch.int64).contiguous()
+        pos_at = positions.data_ptr()
     for norm in (q_norm, k_norm):
-        if norm is not None and (norm.shape != (D,) or norm.dtype != q.dtype or norm.device != device):
-            raise ValueError(f"{what}: a norm's weight must be [{D}] {q.dtype} on {device}, got {tuple(norm.shape)} {norm.dtype} on {norm.device}")
-        norms.append(None if norm is None else norm.contiguous())
-    q_norm, k_norm = norms
+        if norm is not None and (norm.shape != (D,) or norm.dtype != dtype or norm.get_device() != index):
+            raise ValueError(f"{what}: a norm's weight must be [{D}] {dtype} on {q.device}, got {tuple(norm.shape)} {norm.dtype} on {norm.device}")
+    if q_norm is not None:
+        q_norm = q_norm.contiguous()
+        q_norm_at = q_norm.data_ptr()
+    if k_norm is not None:
+        k_norm = k_norm.contiguous()
+        k_norm_at = k_norm.data_ptr()
+    q_out = q.new_empty((rows, Hq, D))
+    k_out = q.new_empty(ks) if v is None else None
+    packed = _HEADS.pack(q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), q_step[0], q_group, q_head, k_step[0], k_step[1], v_step[0], v_step[1],
+                         q_norm_at, k_norm_at, eps, scaling, freq_at, cos_at, sin_at, table_row, table_code, 1 if interleaved else 0, part, pos_at,
+                         q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), Hq * D, D, Hkv * D, D)
+    if axes != 1:
+        q_out, k_out = q_out.view(*axis, Hq, D), None if k_out is None else k_out.view(*axis, Hkv, D)
+    return packed, (q, k, v, inv_freq, cos, sin, positions, q_norm, k_norm), q_out, k_out, (rows, Hq, Hkv, D, code), index
 
-    def at(t):
-        return 0 if t is None else t.data_ptr()
 
-    packed = _HEADS.pack(q.data_ptr(), k.data_ptr(), at(v), q.stride(0), q_group, q_head, k.stride(0), k.stride(1), 0 if v is None else v.stride(0), 0 if v is None else v.stride(1),
-                         at(q_norm), at(k_norm), eps, scaling, at(inv_freq), at(cos), at(sin), table_row, table_code, 1 if interleaved else 0, part, at(positions),
-                         q_out.data_ptr(), at(k_out), q_out.stride(0), q_out.stride(1), 0 if k_out is None else k_out.stride(0), 0 if k_out is None else k_out.stride(1))
-    return packed, (inv_freq, cos, sin, positions, q_norm, k_norm)
-
-
-def _pack_pages(what: str, q: torch.Tensor, rows: int, Hkv: int, D: int, k_pages, v_pages, table, lengths, starts, counts) -> tuple:
-    """tpamd_pages of these operands, and the tensors that it points to."""
-    device = q.device
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
-        raise ValueError(f"{what}: pools must be [pages, {Hkv}, positions of a page, {D}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+def _pages(what: str, q: torch.Tensor, index: int, Hkv: int, D: int, k_pages, v_pages, table, lengths, starts, counts) -> tuple:
+    """tpamd_pages of these operands, and what it points to."""
+    pool, step = k_pages.shape, k_pages.stride()
+    if len(pool) != 4 or v_pages.shape != pool or pool[1] != Hkv or pool[3] != D:
+        raise ValueError(f"{what}: pools must be [pages, {Hkv}, positions of a page, {D}], got {tuple(pool)} and {tuple(v_pages.shape)}")
     if k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
         raise TypeError(f"{what}: the pools must be {q.dtype}, got {k_pages.dtype} and {v_pages.dtype}")
+    v_step = v_pages.stride()
+    if D > 1 and (step[3] != 1 or v_step[3] != 1):
+        raise ValueError(f"{what}: the pools' rows must be contiguous")
     if table.dim() != 2 or lengths.shape != table.shape[:1]:
         raise ValueError(f"{what}: the table must be [sequences, pages of one] and the lengths one for each sequence, got {tuple(table.shape)} and {tuple(lengths.shape)}")
-    seqs = table.shape[0]
+    seqs, columns = table.shape
     if starts is not None and starts.shape != (seqs + 1,) or counts is not None and counts.shape != (seqs,):
         raise ValueError(f"{what}: starts must be [{seqs + 1}] and counts [{seqs}]")
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("table", table), ("lengths", lengths), ("starts", starts), ("counts", counts)):
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{what}: q is on {device}, {name} on {t.device}")
-        if name[1:] == "_pages":
-            if t.stride(3) != 1 and D > 1:
-                raise ValueError(f"{what}: {name} must have contiguous rows")
-        elif t.dtype != torch.int32:
-            raise TypeError(f"{what}: {name} must be int32, got {t.dtype}")
-    if table.shape[1] > 1 and table.stride(1) != 1:
+    if k_pages.get_device() != index or v_pages.get_device() != index:
+        _elsewhere(what, q, "a pool", k_pages if k_pages.get_device() != index else v_pages)
+    if table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise TypeError(f"{what}: table and lengths must be int32, got {table.dtype} and {lengths.dtype}")
+    if table.get_device() != index or lengths.get_device() != index:
+        _elsewhere(what, q, "the table or the lengths", table if table.get_device() != index else lengths)
+    if not table.is_contiguous() and columns > 1 and table.stride(1) != 1:
         table = table.contiguous()
-    lengths, starts, counts = (None if t is None else t.contiguous() for t in (lengths, starts, counts))
-    pages, _, page, _ = k_pages.shape
-    packed = _PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), pages, page, *k_pages.stride()[:3], *v_pages.stride()[:3], table.data_ptr(), table.stride(0), table.shape[1],
-                         lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if counts is None else counts.data_ptr(), seqs)
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    starts_at = counts_at = 0
+    for rows in (starts, counts):
+        if rows is None:
+            continue
+        if rows.dtype != torch.int32:
+            raise TypeError(f"{what}: starts and counts must be int32, got {rows.dtype}")
+        if rows.get_device() != index:
+            _elsewhere(what, q, "starts or counts", rows)
+    if starts is not None:
+        starts = starts.contiguous()
+        starts_at = starts.data_ptr()
+    if counts is not None:
+        counts = counts.contiguous()
+        counts_at = counts.data_ptr()
+    packed = _PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), pool[0], pool[2], step[0], step[1], step[2], v_step[0], v_step[1], v_step[2], table.data_ptr(), table.stride(0), columns,
+                         lengths.data_ptr(), starts_at, counts_at, seqs)
     return packed, (table, lengths, starts, counts)
 
 
@@ -1634,15 +1660,9 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Ten
                  sin: Optional[torch.Tensor] = None, scaling: float = 1.0, interleaved: bool = False, q_norm: Optional[torch.Tensor] = None,
                  k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> tuple:
     """(q, k) with their heads normed and turned (`attention.rotate` says how), as [..., Hq, D] and [..., Hkv, D]."""
-    code, shape, q, k, _ = _heads_operands("rotate", q, k, None)
-    rows, Hkv, D = k.shape
-    if inv_freq is not None and positions is None:
-        raise ValueError("rotate: frequencies need positions")
-    Hq = q.shape[1] if q.dim() == 3 else q.shape[1] * q.shape[2]
-    q_out, k_out = q.new_empty((rows, Hq, D)), q.new_empty((rows, Hkv, D))
-    packed, keep = _pack_heads("rotate", q, k, None, q_out, k_out, shape, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
-    _launch("tpamd_rotate_heads", lib().tpamd_rotate_heads, q.get_device(), packed, rows, Hq, Hkv, D, code)
-    return q_out.view(*shape, Hq, D), k_out.view(*shape, Hkv, D)
+    packed, keep, q_out, k_out, sizes, index = _heads("rotate", q, k, None, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
+    _launch("tpamd_rotate_heads", lib().tpamd_rotate_heads, index, packed, *sizes)
+    return q_out, k_out
 
 
 def append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -1650,14 +1670,10 @@ def append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, scaling: float = 1.0, interleaved: bool = False, q_norm: Optional[torch.Tensor] = None,
                  k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """k and v of the new rows into their pages, k (and q, which is returned) normed and turned (`paged.append` says how)."""
-    code, shape, q, k, v = _heads_operands("append", q, k, v)
-    rows, Hkv, D = k.shape
-    Hq = q.shape[1] if q.dim() == 3 else q.shape[1] * q.shape[2]
-    pages, keep_pages = _pack_pages("append", q, rows, Hkv, D, k_pages, v_pages, table, lengths, starts, counts)
-    q_out = q.new_empty((rows, Hq, D))
-    packed, keep = _pack_heads("append", q, k, v, q_out, None, shape, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
-    _launch("tpamd_append_paged", lib().tpamd_append_paged, q.get_device(), packed, pages, rows, Hq, Hkv, D, code)
-    return q_out.view(*shape, Hq, D)
+    packed, keep, q_out, _, sizes, index = _heads("append", q, k, v, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
+    pages, keep_pages = _pages("append", q, index, sizes[2], sizes[3], k_pages, v_pages, table, lengths, starts, counts)
+    _launch("tpamd_append_paged", lib().tpamd_append_paged, index, packed, pages, *sizes)
+    return q_out
 
 
 def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
@@ -1666,41 +1682,55 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Causal attention of the new rows q [..., Hq, D] on their sequences' pages (`paged.attend` says how)."""
     if not q.is_cuda:
         require_device(q, "attend")
-    code = _HALF_CODES.get(q.dtype)
+    code, index = _HALF_CODES.get(q.dtype), q.get_device()
     if code is None:
         raise TypeError(f"attend: q must be bfloat16 or float16, got {q.dtype}")
-    if q.dim() < 2 or k_pages.dim() != 4:
-        raise ValueError(f"attend: q must be [..., heads, head_dim] and the pools [pages, heads, positions, head_dim], got {tuple(q.shape)} and {tuple(k_pages.shape)}")
     shape = q.shape
-    q = _one_axis(q, q.dim() - 2)
+    if len(shape) < 2 or k_pages.dim() != 4:
+        raise ValueError(f"attend: q must be [..., heads, head_dim] and the pools [pages, heads, positions, head_dim], got {tuple(shape)} and {tuple(k_pages.shape)}")
+    if len(shape) != 3:
+        q = _one_axis(q, len(shape) - 2)
     rows, Hq, D = q.shape
-    Hkv = k_pages.shape[1]
-    if q.stride(2) != 1:
+    pool = k_pages.shape
+    Hkv = pool[1]
+    step = q.stride()
+    if step[2] != 1:
         q = q.contiguous()
+        step = q.stride()
     if out is None:
         rows_out = q.new_empty((rows, Hq, D))
-        out = rows_out.view(shape)
+        out = rows_out if len(shape) == 3 else rows_out.view(shape)
+        out_step = (Hq * D, D)
     else:
         if out.shape != shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1:
             raise ValueError(f"attend: out must be a {tuple(shape)} {q.dtype} tensor on {q.device} with contiguous heads")
         rows_out = _one_axis(out, out.dim() - 2)
         if rows_out.numel() and rows_out.data_ptr() != out.data_ptr():
             raise ValueError("attend: the rows of out must follow one another")
-    pages, keep = _pack_pages("attend", q, rows, Hkv, D, k_pages, v_pages, table, lengths, starts, counts)
+        out_step = rows_out.stride()
+    pages, keep = _pages("attend", q, index, Hkv, D, k_pages, v_pages, table, lengths, starts, counts)
     if max_new is None:
         max_new = rows
     if max_length is None:
-        max_length = table.shape[1] * k_pages.shape[2]
-    index, need = q.get_device(), ctypes.c_uint64()
+        max_length = table.shape[1] * pool[2]
+    need = ctypes.c_uint64()
+    _launch_free("tpamd_attention_paged_workspace", lib().tpamd_attention_paged_workspace, index, pages, rows, Hq, Hkv, D, max_new, max_length, ctypes.byref(need))
+    size = need.value
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
+    _launch("tpamd_attention_paged", lib().tpamd_attention_paged, index, q.data_ptr(), step[0], step[1], pages, rows_out.data_ptr(), out_step[0], out_step[1], rows, Hq, Hkv, D, max_new,
+            max_length, D ** -0.5 if scale is None else float(scale), code, 0 if work is None else work.data_ptr(), size)
+    return out
+
+
+def _launch_free(what: str, call, index: int, *args) -> None:
+    """call(*args) with HIP device `index` as the current one: for calls that take no stream."""
     prev = _device_of_thread()
     if prev != index:
         torch.cuda.set_device(index)
     try:
-        _check(lib().tpamd_attention_paged_workspace(pages, rows, Hq, Hkv, D, max_new, max_length, ctypes.byref(need)), "tpamd_attention_paged_workspace")
+        rc = call(*args)
     finally:
         if prev != index:
             torch.cuda.set_device(prev)
-    work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
-    _launch("tpamd_attention_paged", lib().tpamd_attention_paged, index, q.data_ptr(), q.stride(0), q.stride(1), pages, rows_out.data_ptr(), rows_out.stride(0), rows_out.stride(1),
-            rows, Hq, Hkv, D, max_new, max_length, float(scale if scale is not None else D ** -0.5), code, 0 if work is None else work.data_ptr(), need.value)
-    return out
+    if rc != 0:
+        _check(rc, what)

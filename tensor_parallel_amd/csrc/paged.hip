@@ -9,7 +9,6 @@
 // Both load K and V straight into LDS, 16 positions by 16 positions: those lie in one page (pages have 16 positions or more, a power of two), so that a page is looked
 // up once for them and the loads have one descriptor and fixed offsets. A piece (16 bytes) c of a staged row r is in slot c ^ turned(r): rows are read as MFMA operands
 // (16 or 32 rows, one piece each) and through the transposing read (4 consecutive rows, 2 or 4 neighbouring pieces) without bank conflicts.
-#include "attention_model.h"
 #include "gemm_tile.h"
 #include "paged.h"
 
@@ -21,6 +20,7 @@ namespace {
 constexpr int FEW = 16;    // rows of a paged_few_kernel item
 constexpr int GROUP = 16;  // positions that lie in one page
 constexpr int UNIT = 64;   // positions of a piece of paged_few_kernel's work: a group for each of its wavefronts
+constexpr int START = 3;   // units that the start and the end of an item cost about as much as
 
 struct PagedParams {
     const char *q;
@@ -30,8 +30,8 @@ struct PagedParams {
     float scale_log2;  // scale * log2(e)
     int Hkv, G, D;
     int few, many;     // which of the kernels run
-    int splits;        // paged_many_kernel: key ranges
-    int least;         // paged_few_kernel: units a block takes at least; 0: a block takes one item, whole
+    int spread;        // paged_many_kernel: blocks that its work is spread over; 0: a row tile is never cut
+    int least;         // paged_few_kernel: the least share of a block; 0: a block takes one item, whole
     PagesView pages;
 };
 
@@ -46,9 +46,11 @@ __device__ __forceinline__ constexpr int turned(int r) {
     else return (r & 3) << 2 | ((r >> 2) & 3);
 }
 
+template <int OFFSET>
 __device__ __forceinline__ u32x2 lds_transpose_read(uint32_t at) {  // ds_read_b64_tr_b16, unseen by the compiler (as lds_read16)
+    static_assert(OFFSET >= 0 && OFFSET < 65536, "ds offset field is 16 bits");
     u32x2 v;
-    asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(v) : "v"(at));
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(at), "n"(OFFSET));
     return v;
 }
 __device__ __forceinline__ void half_landed(u32x2 &r) { asm volatile("" : "+v"(r)); }
@@ -70,19 +72,22 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Values that some rows of a tile do not see may be infinite or NaN, and zero times those would reach the rows through the matrix product. They go in as zeros, and where there are any, two
-// more products with ones in the place of +inf and NaN, and of -inf and NaN, say which sums they belong to.
+// Values that some rows of a tile do not see may be infinite or NaN, and zero times those would reach the rows through the matrix product. They go in as zeros. Where there are any, two more
+// products, of the largest bf16 value in the place of every +inf and NaN (then of its negative in the place of -inf and NaN) and of every probability above zero, add what overflows to an
+// infinity where it belongs: through the same sums, which are touched by nothing but matrix instructions.
 template <int DT>
 struct Beyond {
-    static constexpr uint32_t E = DT == TPAMD_BF16 ? 0x7f80u : 0x7c00u, ONE = DT == TPAMD_BF16 ? 0x3f80u : 0x3c00u;
-    static __device__ __forceinline__ bool any(uint32_t two) { return (two & E) == E || (two & (E << 16)) == (E << 16); }
+    static constexpr uint32_t E = DT == TPAMD_BF16 ? 0x7f80u : 0x7c00u, LAST = DT == TPAMD_BF16 ? 0x0080u : 0x0400u, HUGE_BF16 = 0x7f7fu;
+    // a bit of 0x80008000 for either value whose exponent is all ones (adding the exponent's last bit carries out of it)
+    static __device__ __forceinline__ uint32_t carries(uint32_t two) { return (two & (E << 16 | E)) + (LAST << 16 | LAST); }
     static __device__ __forceinline__ uint32_t finite(uint32_t two) {
         return two & (((two & E) == E ? 0u : 0xffffu) | ((two & (E << 16)) == (E << 16) ? 0u : 0xffff0000u));
     }
-    static __device__ __forceinline__ uint32_t one(uint32_t h, uint32_t sign) {  // of the low half: ONE for NaN and for the infinity of this sign
-        return (h & E) == E && ((h & 0x7fffu) != E || (h & 0x8000u) == sign) ? ONE : 0u;
+    static __device__ __forceinline__ uint32_t huge_one(uint32_t h, uint32_t sign) {  // of the low half: NaN and the infinity of this sign
+        return (h & E) == E && ((h & 0x7fffu) != E || (h & 0x8000u) == sign) ? HUGE_BF16 | sign : 0u;
     }
-    static __device__ __forceinline__ uint32_t ones(uint32_t two, uint32_t sign) { return one(two & 0xffffu, sign) | one(two >> 16, sign) << 16; }
+    static __device__ __forceinline__ uint32_t huge(uint32_t two, uint32_t sign) { return huge_one(two & 0xffffu, sign) | huge_one(two >> 16, sign) << 16; }
+    static __device__ __forceinline__ uint32_t seen(uint32_t two) { return ((two & 0x7fffu) != 0 ? HUGE_BF16 : 0u) | ((two & 0x7fff0000u) != 0 ? HUGE_BF16 << 16 : 0u); }
 };
 
 // The descriptor of 16 rows that begin at `base`: nothing (loads give zeros) where there is no page.
@@ -92,14 +97,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t group_rsrc(const char *pool, i
     return make_rsrc(base, extent);
 }
 
-// rows_of, of a sequence that the whole wavefront asks for.
-__device__ __forceinline__ SeqRows same_rows_of(const PagesView &p, int b) {
-    SeqRows s = rows_of(p, b);
-    s.first = __builtin_amdgcn_readfirstlane(s.first);
-    s.count = __builtin_amdgcn_readfirstlane(s.count);
-    s.length = __builtin_amdgcn_readfirstlane(s.length);
-    return s;
-}
 // A value that was loaded is here from now on: the compiler would otherwise wait for it inside the loop that uses it, and with it for loads that the loop has requested.
 __device__ __forceinline__ void arrived(int &v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void arrived(u32x4 &v) { asm volatile("" : "+v"(v)); }
@@ -109,51 +106,107 @@ __device__ __forceinline__ bool is_few(const PagedParams &p, int count) { return
 __device__ __forceinline__ int units_of(const PagedParams &p, const SeqRows &s) {
     return is_few(p, s.count) ? max((s.length + UNIT - 1) / UNIT, 1) : 0;  // one for a sequence without positions too: its rows are zeros
 }
-// Row tiles of ROWS rows, 0 for the other kernel's sequences.
-template <int ROWS>
-__device__ __forceinline__ int tiles_of(const PagedParams &p, const SeqRows &s) {
-    return s.count > 0 && !is_few(p, s.count) ? (s.count * p.G + ROWS - 1) / ROWS : 0;
+// What it costs a block of paged_few_kernel: its units, behind START for getting there.
+__device__ __forceinline__ int cost_of(const PagedParams &p, const SeqRows &s) {
+    const int n = units_of(p, s);
+    return n == 0 ? 0 : n + START;
 }
-// The sum over all sequences of what `of` gives, and (where `at` is one of the units) the sequence it falls into with the sum before it. By all lanes of a wavefront.
-template <class F>
-__device__ __forceinline__ int sum_over(const PagedParams &p, F &&of) {
-    const int lane = threadIdx.x & 63;
-    int mine = 0;
-    for (int b0 = 0; b0 < p.pages.seqs; b0 += 64)
-        if (b0 + lane < p.pages.seqs) mine += of(rows_of(p.pages, b0 + lane));
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d);
-    return __builtin_amdgcn_readfirstlane(mine);
+// paged_many_kernel's share of a sequence: tiles of ROWS rows (0 for the other kernel's sequences), and the tiles of KT positions that its first and its last row tile see.
+struct Tiles {
+    int rows, first, last;
+};
+template <int ROWS, int KT>
+__device__ __forceinline__ Tiles tiles_of(const PagedParams &p, const SeqRows &s) {
+    if (s.count <= 0 || is_few(p, s.count)) return {0, 0, 0};
+    const int rows = s.count * p.G, before = s.length - s.count;
+    return {(rows + ROWS - 1) / ROWS, (max(before + (min(rows, ROWS) - 1) / p.G + 1, 0) + KT - 1) / KT, (s.length + KT - 1) / KT};
 }
+// 64 sequences, one in a lane: lengths and counts of a batch are loaded once and asked for by lane from then on.
+struct Lanes {
+    SeqRows mine;
+    int b0;
+};
+__device__ __forceinline__ Lanes lanes_from(const PagedParams &p, int b0) {
+    Lanes l{{0, 0, 0}, b0};
+    const int b = b0 + static_cast<int>(threadIdx.x & 63);
+    if (b < p.pages.seqs) l.mine = rows_of(p.pages, b);
+    return l;
+}
+__device__ __forceinline__ SeqRows pick(const PagedParams &p, Lanes &l, int b) {  // b: the same in all lanes
+    if (b - l.b0 >= 64 || b < l.b0) l = lanes_from(p, b & ~63);
+    const int at = b - l.b0;
+    return {__builtin_amdgcn_readlane(l.mine.first, at), __builtin_amdgcn_readlane(l.mine.count, at), __builtin_amdgcn_readlane(l.mine.length, at)};
+}
+// v of the lanes that a DPP control names, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_lanes(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lanes(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = from_lanes<CTRL, ROWS>(static_cast<int>(u)), hi = from_lanes<CTRL, ROWS>(static_cast<int>(u >> 32));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// The sum over this lane and those before it, by moves inside the vector unit (1, 2, 4, 8 lanes up in a row of 16, then the last lane of a row to the next, of 32 to the others): six trips through
+// LDS are 0.3 us, and every block has two or three such sums in front of its first load.
+template <class T>
+__device__ __forceinline__ T sums_to_lane(T v) {
+    v += from_lanes<0x111, 0xf>(v);
+    v += from_lanes<0x112, 0xf>(v);
+    v += from_lanes<0x114, 0xf>(v);
+    v += from_lanes<0x118, 0xf>(v);
+    v += from_lanes<0x142, 0xa>(v);
+    v += from_lanes<0x143, 0xc>(v);
+    return v;
+}
+// The sum over all sequences of what `of` gives; l holds the first 64.
 template <class F>
-__device__ __forceinline__ int find_in(const PagedParams &p, int at, int &before, F &&of) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ int sum_over(const PagedParams &p, const Lanes &l, F &&of) {
+    int mine = of(l.mine);
+    for (int b0 = 64; b0 < p.pages.seqs; b0 += 64) mine += of(lanes_from(p, b0).mine);
+    return __builtin_amdgcn_readlane(sums_to_lane(mine), 63);
+}
+// The sequence that the at-th of these falls into (0 <= at < their sum), and how many come before that sequence's; l ends up with it among its 64.
+template <class F>
+__device__ __forceinline__ int find_in(const PagedParams &p, Lanes &l, int at, int &before, F &&of) {
     int done = 0;
     for (int b0 = 0; b0 < p.pages.seqs; b0 += 64) {
-        const int mine = b0 + lane < p.pages.seqs ? of(rows_of(p.pages, b0 + lane)) : 0;
-        int sum = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
-        }
+        if (b0 != l.b0) l = lanes_from(p, b0);
+        const int mine = of(l.mine), sum = sums_to_lane(mine);
         const uint64_t hit = __ballot(done + sum > at);
         if (hit != 0) {
-            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-            before = __builtin_amdgcn_readfirstlane(done + __shfl(sum - mine, l));
-            return __builtin_amdgcn_readfirstlane(b0 + l);
+            const int lane = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            before = done + __builtin_amdgcn_readlane(sum, lane) - __builtin_amdgcn_readlane(mine, lane);
+            return b0 + lane;
         }
-        done += __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+        done += __builtin_amdgcn_readlane(sum, 63);
     }
     return -1;
 }
-// Units of work of one block of paged_few_kernel: alike for all, but `least` at least.
-__device__ __forceinline__ int share_of(const PagedParams &p, int units, int blocks) { return max(p.least, (units + blocks - 1) / blocks); }
+// The positions of a sequence's row tiles are cut into ranges where the tiles have more of them than an equal share of all work (in tiles of KT positions) on `spread` blocks, so that a few long
+// sequences in a batch do not keep a few blocks busy when all others have ended. Sums of whole numbers in 64 bits: exact. With R the share there are at most sum(1 + work / R) = row tiles +
+// spread ranges, and fewer than 2 spread of tiles that are cut.
+constexpr int LEAST_TILES = 4;
+template <int ROWS, int KT>
+__device__ __forceinline__ int range_tiles(const PagedParams &p, const Lanes &l) {
+    if (p.spread == 0) return 0;
+    auto work = [&](const SeqRows &s) {
+        const Tiles t = tiles_of<ROWS, KT>(p, s);
+        return static_cast<double>(t.rows) * (t.first + t.last);
+    };
+    double mine = work(l.mine);
+    for (int b0 = 64; b0 < p.pages.seqs; b0 += 64) mine += work(lanes_from(p, b0).mine);
+    const double share = ceil(__shfl(sums_to_lane(mine), 63) * p.Hkv / (2.0 * p.spread));
+    return __builtin_amdgcn_readfirstlane(share < 1.0e9 ? max(static_cast<int>(share), LEAST_TILES) : 1000000000);
+}
+__device__ __forceinline__ int ranges_of(const Tiles &t, int range) { return range == 0 ? 1 : max((t.first + t.last + 2 * range - 1) / (2 * range), 1); }
+
+// What a block of paged_few_kernel takes: alike for all, but `least` at least.
+__device__ __forceinline__ int share_of(const PagedParams &p, int cost, int blocks) { return max(p.least, (cost + blocks - 1) / blocks); }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------------------------------------------------
-// An item is one key/value head of one sequence, its work the sequence's positions in units of 64. The units of all items, one after another, are cut into equal shares,
-// one for a block, so that a batch of sequences of very different lengths keeps all blocks busy to the end; where a cut falls inside an item, both sides leave
-// (m, l, O) as partials, and paged_few_merge_kernel joins them. A block has at most two such pieces (its first and its last), so the partials' memory does not
+// An item is one key/value head of one sequence, its work the sequence's positions in units of 64. The costs of all items (their units, and START units in front of them), one after
+// another, are cut into equal shares, one for a block, so that a batch of sequences of very different lengths keeps all blocks busy to the end; where a cut falls inside an item, both sides
+// leave (m, l, O) as partials, and paged_few_merge_kernel joins them. A block has at most two such pieces (its first and its last), so the partials' memory does not
 // grow with the batch. `least` == 0: a block takes an item whole and nothing is merged.
 //
 // Inside a block the four wavefronts take every fourth 16 positions through LDS stages of their own and meet at the end of an item.
@@ -169,27 +222,30 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
     char *ring = smem + wave * RING;
 
     // ---- this block's share
-    int b, hkv, unit, left;  // where it begins, and how many units it has
+    int b, hkv, at, left;  // where it begins, inside an item's cost, and how much it has
     const int share_index = blockIdx.x;
-    auto units = [&](const SeqRows &s) { return units_of(p, s); };
+    auto costs = [&](const SeqRows &s) { return cost_of(p, s); };
+    Lanes seqs = lanes_from(p, p.least == 0 ? share_index / p.Hkv & ~63 : 0);
+    int first_pages = -1;  // of a whole item, asked for together with its length
     if (p.least == 0) {
         b = share_index / p.Hkv;
         hkv = share_index - b * p.Hkv;
-        unit = 0;
-        left = units_of(p, same_rows_of(p.pages, b));
+        at = 0;
+        const int position = (wave + 4 * lane) * GROUP;
+        if (position < p.pages.room) first_pages = page_of(p.pages, b, position);
+        left = cost_of(p, pick(p, seqs, b));
         if (left == 0) return;
     } else {
-        const int all = sum_over(p, units) * p.Hkv, share = share_of(p, all, gridDim.x);
+        const int all = sum_over(p, seqs, costs) * p.Hkv, share = share_of(p, all, gridDim.x);
         const int64_t from = static_cast<int64_t>(share_index) * share;
         if (from >= all) return;
         left = min(share, all - static_cast<int>(from));
-        // units of a sequence before all heads': the scan counts a sequence's units once
+        // costs of a sequence before all heads': the scan counts a sequence once
         int before;
-        b = find_in(p, static_cast<int>(from) / p.Hkv, before, units);
-        // (the sequence whose Hkv * units hold `from`)
-        const int u = units_of(p, same_rows_of(p.pages, b)), inside = static_cast<int>(from) - before * p.Hkv;
-        hkv = inside / u;
-        unit = inside - hkv * u;
+        b = find_in(p, seqs, static_cast<int>(from) / p.Hkv, before, costs);
+        const int cost = cost_of(p, pick(p, seqs, b)), inside = static_cast<int>(from) - before * p.Hkv;
+        hkv = inside / cost;
+        at = inside - hkv * cost;
     }
     // pieces of 1024 bytes of a group: which row and piece this lane loads
     uint32_t k_off[LK], v_off[LK];
@@ -204,15 +260,24 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
     const uint32_t v_rd = lds_addr_of(ring) + VAT + vkey * PITCH + (((l16 & 3) >> 1) ^ turned<D>(vkey)) * 16 + (l16 & 1) * 8;
 
     while (left > 0 && b < p.pages.seqs) {
-        const SeqRows s = same_rows_of(p.pages, b);
+        const SeqRows s = pick(p, seqs, b);
         const int n_units = units_of(p, s);
         if (n_units == 0) {  // the other kernel's, or empty
             ++b;
             continue;
         }
-        const int take = min(left, n_units - unit);
-        const int k_begin = unit * UNIT, k_end = min((unit + take) * UNIT, s.length);
-        const bool from_start = unit == 0, to_end = unit + take == n_units;
+        const int take = min(left, n_units + START - at), unit = max(at - START, 0), unit_end = max(at + take - START, 0);
+        const int item = hkv;
+        left -= take;
+        at = 0;
+        if (++hkv == p.Hkv) {
+            hkv = 0;
+            ++b;
+        }
+        if (unit_end == unit) continue;  // the share ends in front of the item's units
+        const int seq = item + 1 == p.Hkv ? b - 1 : b;
+        const int k_begin = unit * UNIT, k_end = min(unit_end * UNIT, s.length);
+        const bool from_start = unit == 0, to_end = unit_end == n_units;
         const int rows = s.count * p.G;
         const int groups = k_end > k_begin ? (k_end - k_begin + GROUP - 1) / GROUP : 0;
         const int n = (groups - wave + 3) / 4;  // of this wavefront: wave, wave + 4, ...
@@ -221,7 +286,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
         const int row = l16 < rows ? l16 : 0, place = row / p.G;
         const int last = s.length - s.count + place;  // position that the row sees last
         const int seen_by_all = s.length - s.count;
-        const char *qrow = p.q + (static_cast<int64_t>(s.first + place) * p.q_row + static_cast<int64_t>(hkv * p.G + row - place * p.G) * p.q_head) * 2;
+        const char *qrow = p.q + (static_cast<int64_t>(s.first + place) * p.q_row + static_cast<int64_t>(item * p.G + row - place * p.G) * p.q_head) * 2;
         u32x4 qf[DK];
 #pragma unroll
         for (int kk = 0; kk < DK; ++kk) qf[kk] = *reinterpret_cast<const u32x4 *>(qrow + (32 * kk + 8 * lq) * 2);
@@ -232,15 +297,14 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
         for (int dt = 0; dt < DT16; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (n > 0) {
             const int group0 = k_begin / GROUP + wave;  // of the sequence
-            const int64_t k_at = hkv * p.pages.k_head, v_at = hkv * p.pages.v_head;
+            const int64_t k_at = item * p.pages.k_head, v_at = item * p.pages.v_head;
             // the pages of this wavefront's next 64 groups, one in a lane
             auto pages_from = [&](int i) {
                 const int g = group0 + 4 * (i + lane);
-                return g * GROUP < s.length ? page_of(p.pages, b, g * GROUP) : -1;
+                return g * GROUP < s.length ? page_of(p.pages, seq, g * GROUP) : -1;
             };
-            int my_page = pages_from(0), base = 0;
+            int my_page = p.least == 0 ? first_pages : pages_from(0), base = 0;
             arrived(my_page);
-            unrolled<DK>([&](auto kc) { arrived(qf[decltype(kc)::value]); });
             auto load = [&](int stage_off, int i) __attribute__((always_inline)) {
                 if (i < n) {
                     if (i - base == 64) {
@@ -274,7 +338,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
                 });
                 unrolled<DT16>([&](auto dc) {
                     constexpr int dt = decltype(dc)::value;
-                    vf[dt] = lds_transpose_read(D == 96 ? ((v_rd + stage_off) ^ ((dt & 1) * 32)) + (dt >> 1) * 64 : (v_rd + stage_off) ^ (dt * 32));
+                    vf[dt] = lds_transpose_read<0>(D == 96 ? ((v_rd + stage_off) ^ ((dt & 1) * 32)) + (dt >> 1) * 64 : (v_rd + stage_off) ^ (dt * 32));
                 });
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 unrolled<DK>([&](auto kc) { already_landed(kf[decltype(kc)::value]); });
@@ -329,26 +393,23 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
                 // probabilities are rounded to the dtype (half a step of it each, as errors of either sign that the sum averages)
                 const u32x2 pf = {pack2_half<DT>(sc[0], sc[1]), pack2_half<DT>(sc[2], sc[3])};
                 u32x2 all[DT16];
-                bool apart = false;
+                uint32_t carried = 0;
                 if (partly && s.count > 1) {
 #pragma unroll
                     for (int dt = 0; dt < DT16; ++dt) {
-                        apart = apart || Beyond<DT>::any(vf[dt].x) || Beyond<DT>::any(vf[dt].y);
+                        carried |= Beyond<DT>::carries(vf[dt].x) | Beyond<DT>::carries(vf[dt].y);
                         all[dt] = vf[dt];
                         vf[dt] = u32x2{Beyond<DT>::finite(vf[dt].x), Beyond<DT>::finite(vf[dt].y)};
                     }
                 }
 #pragma unroll
                 for (int dt = 0; dt < DT16; ++dt) acc[dt] = mfma16_k16<DT>(vf[dt], pf, acc[dt]);
-                if (__any(apart)) {
+                if (__any((carried & 0x80008000u) != 0)) {
+                    const u32x2 seen = {Beyond<DT>::seen(pf.x), Beyond<DT>::seen(pf.y)};
 #pragma unroll
-                    for (int dt = 0; dt < DT16; ++dt) {
-                        const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-                        const f32x4 plus = mfma16_k16<DT>(u32x2{Beyond<DT>::ones(all[dt].x, 0), Beyond<DT>::ones(all[dt].y, 0)}, pf, zero);
-                        const f32x4 minus = mfma16_k16<DT>(u32x2{Beyond<DT>::ones(all[dt].x, 0x8000u), Beyond<DT>::ones(all[dt].y, 0x8000u)}, pf, zero);
+                    for (int dt = 0; dt < DT16; ++dt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[dt][j] += (plus[j] > 0.f ? INFINITY : 0.f) - (minus[j] > 0.f ? INFINITY : 0.f);
-                    }
+                        for (uint32_t sign : {0u, 0x8000u}) acc[dt] = mfma16_k16<TPAMD_BF16>(u32x2{Beyond<DT>::huge(all[dt].x, sign), Beyond<DT>::huge(all[dt].y, sign)}, seen, acc[dt]);
                 }
             }
         }
@@ -387,7 +448,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
             if (whole) {
                 const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // a sum of NaN stays one
                 const int at = r / p.G;
-                *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + at) * p.o_row + static_cast<int64_t>(hkv * p.G + r - at * p.G) * p.o_head + d4) * 2) =
+                *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + at) * p.o_row + static_cast<int64_t>(item * p.G + r - at * p.G) * p.o_head + d4) * 2) =
                     make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
             } else {
                 *reinterpret_cast<f32x4 *>(out_part + r * PW + d4) = f32x4{o[0], o[1], o[2], o[3]};
@@ -395,75 +456,85 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
             }
         }
         __syncthreads();  // read before the next item's loads
-        left -= take;
-        unit = 0;
-        if (++hkv == p.Hkv) {
-            hkv = 0;
-            ++b;
-        }
     }
 }
 
-// Joins the pieces of the items that paged_few_kernel's shares cut: a block an item.
+// Joins the pieces of the items that paged_few_kernel's shares cut. D / 4 lanes hold a row; a block has as many such groups as there are threads for. Of an item in a few pieces each group
+// takes a row; the pieces of a longer one (a single long sequence has one in every block: 64 of them, one after another, cost 13 us) are dealt out to the groups, row by row.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int blocks) {
-    constexpr int PW = D + 4, per_row = D / 4;
-    const int b = blockIdx.x / p.Hkv, hkv = blockIdx.x - b * p.Hkv, lane = threadIdx.x & 63;
-    const SeqRows s = rows_of(p.pages, b);
-    const int n = units_of(p, s);
-    if (n == 0) return;
-    int all = 0, before = 0;
+    constexpr int PW = D + 4, LANES = D / 4, TAKERS = 256 / LANES;
+    __shared__ __align__(16) f32x4 sums[TAKERS][LANES];
+    __shared__ float2 weights[TAKERS];
+    const int b = blockIdx.x / p.Hkv, hkv = blockIdx.x - b * p.Hkv;
+    Lanes seqs = lanes_from(p, 0);
+    int before = 0, done = 0;
+    SeqRows s{0, 0, 0};
     for (int b0 = 0; b0 < p.pages.seqs; b0 += 64) {
-        const int u = b0 + lane < p.pages.seqs ? units_of(p, rows_of(p.pages, b0 + lane)) : 0;
-        all += u;
-        before += b0 + lane < b ? u : 0;
+        if (b0 != 0) seqs = lanes_from(p, b0);
+        const int mine = cost_of(p, seqs.mine), sum = sums_to_lane(mine);
+        if (b >= b0 && b < b0 + 64) {
+            s = pick(p, seqs, b);
+            before = done + __builtin_amdgcn_readlane(sum, b - b0) - __builtin_amdgcn_readlane(mine, b - b0);
+        }
+        done += __builtin_amdgcn_readlane(sum, 63);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        all += __shfl_xor(all, d);
-        before += __shfl_xor(before, d);
-    }
-    const int share = share_of(p, all * p.Hkv, blocks);
-    const int from = before * p.Hkv + hkv * n, first = from / share, last = (from + n - 1) / share;
+    const int n = units_of(p, s), rows = s.count * p.G;
+    if (n == 0) return;
+    const int share = share_of(p, done * p.Hkv, blocks);
+    const int from = before * p.Hkv + hkv * (n + START) + START, first = from / share, last = (from + n - 1) / share;
     if (first == last) return;  // whole in one block, which has stored it
-    const int rows = s.count * p.G;
-    const int64_t pitch = 2 * FEW * PW;
-    for (int e = threadIdx.x; e < rows * per_row; e += 256) {
-        const int r = e / per_row, d4 = (e % per_row) * 4;
-        // the piece of block i: its odd slot where the item begins in it
-        const float *base = p.part + r * PW;
-        auto piece = [&](int i) { return base + i * pitch + (i == first ? FEW * PW : 0); };
-        float M = -INFINITY;
-        for (int i0 = first; i0 <= last; i0 += 8) {
-            float ms[8];
+    const bool dealt = last - first >= TAKERS;
+    const int taker = threadIdx.x / LANES, d4 = (threadIdx.x % LANES) * 4, at_once = dealt ? 1 : TAKERS;
+    for (int r0 = blockIdx.y * at_once; r0 < rows; r0 += gridDim.y * at_once) {
+        const int r = dealt ? r0 : r0 + taker, step = dealt ? TAKERS : 1;
+        const bool mine = taker < TAKERS && r < rows;
+        float M = -INFINITY, l = 0.f;
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (mine) {
+            for (int i0 = first + (dealt ? taker : 0); i0 <= last; i0 += 4 * step) {
+                float2 ml[4];
+                f32x4 ov[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ms[j] = piece(min(i0 + j, last))[D];
+                for (int j = 0; j < 4; ++j) {
+                    const int i = min(i0 + j * step, last);  // the piece of block i: its odd slot where the item begins in it
+                    const float *piece = p.part + (static_cast<int64_t>(2 * i + (i == first ? 1 : 0)) * FEW + r) * PW;
+                    ml[j] = *reinterpret_cast<const float2 *>(piece + D);
+                    ov[j] = *reinterpret_cast<const f32x4 *>(piece + d4);
+                }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) M = fmaxf(M, ms[j]);
-        }
-        const float m_use = M == -INFINITY ? 0.f : M;
-        float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-        for (int i0 = first; i0 <= last; i0 += 8) {
-            float2 ml[8];
-            f32x4 ov[8];
+                for (int j = 0; j < 4; ++j) {
+                    if (i0 + j * step > last) continue;
+                    const float m = fmaxf(M, ml[j].x), m_use = m == -INFINITY ? 0.f : m, old = exp2f(M - m_use), now = exp2f(ml[j].x - m_use);
+                    M = m;
+                    l = l * old + ml[j].y * now;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float *from_piece = piece(min(i0 + j, last));
-                ml[j] = *reinterpret_cast<const float2 *>(from_piece + D);
-                ov[j] = *reinterpret_cast<const f32x4 *>(from_piece + d4);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (i0 + j > last) continue;
-                const float weight = exp2f(ml[j].x - m_use);
-                l += weight * ml[j].y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += weight * ov[j][i];
+                    for (int e = 0; e < 4; ++e) o[e] = o[e] * old + ov[j][e] * now;
+                }
             }
         }
+        if (dealt) {
+            if (mine) {
+                sums[taker][d4 / 4] = o;
+                if (d4 == 0) weights[taker] = make_float2(M, l);
+            }
+            __syncthreads();
+            M = -INFINITY;
+            for (int t = 0; t < TAKERS; ++t) M = fmaxf(M, weights[t].x);
+            const float m_use = M == -INFINITY ? 0.f : M;
+            l = 0.f;
+            o = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < TAKERS; ++t) {
+                const float weight = exp2f(weights[t].x - m_use);
+                l += weight * weights[t].y;
+                for (int e = 0; e < 4; ++e) o[e] += weight * sums[t][d4 / 4][e];
+            }
+            __syncthreads();
+        }
+        if (!mine || (dealt && taker != 0)) continue;
         const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-        const int at = r / p.G;
-        *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + at) * p.o_row + static_cast<int64_t>(hkv * p.G + r - at * p.G) * p.o_head + d4) * 2) =
+        const int place = r / p.G;
+        *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + place) * p.o_row + static_cast<int64_t>(hkv * p.G + r - place * p.G) * p.o_head + d4) * 2) =
             make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
     }
 }
@@ -474,9 +545,9 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int
 // and that the stage before it is free.
 //   S^T = K Q^T   v_mfma_f32_32x32x16 with K rows as the first operand: a lane has, of ONE query row, 16 of 32 positions, and one exchange with lane ^ 32 finishes a row's maximum
 //   O^T += V^T P^T  the lane's probabilities are the second operand as they are (8 positions of each 16, in an order that the transposing read of V follows)
-// Blocks are given out with the longest key ranges first; of few blocks the positions are cut into `splits` ranges, joined by paged_many_merge_kernel.
+// Blocks are given out with the last row tiles first; ranges of a tile whose positions were cut (range_tiles) leave (m, l, O) to paged_many_merge_kernel.
 template <int DT, int D, int WAVES, int KT, int NST>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void paged_many_kernel(PagedParams p) {
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 64 && WAVES == 4 ? 3 : 2, D == 256 ? 1 : D == 64 && WAVES == 4 ? 3 : 2))) void paged_many_kernel(PagedParams p) {
     constexpr int MANY = WAVES * 32, PITCH = D * 2, PIECES = D / 8, KTILE = KT * PITCH, STAGE = 2 * KTILE, PW = D + 4;
     constexpr int NL = D / 32, KK = D / 16, DT32 = D / 32, T32 = KT / 32;
     static_assert(WAVES / 2 == KT / GROUP, "a wavefront loads 16 rows of K or V");
@@ -486,14 +557,20 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     const int l32 = lane & 31, h = lane >> 5;
 
     // ---- which rows: the last sequence's last tile first
-    auto tiles_in = [&](const SeqRows &s) { return tiles_of<MANY>(p, s); };
     const int hkv = blockIdx.x % p.Hkv, nth = blockIdx.x / p.Hkv;
-    const int all = sum_over(p, tiles_in);
+    Lanes seqs = lanes_from(p, 0);
+    const int range = range_tiles<MANY, KT>(p, seqs);
+    auto pieces_in = [&](const SeqRows &s) {
+        const Tiles t = tiles_of<MANY, KT>(p, s);
+        return t.rows * ranges_of(t, range);
+    };
+    const int all = sum_over(p, seqs, pieces_in);
     if (nth >= all) return;
     int before;
-    const int b = find_in(p, all - 1 - nth, before, tiles_in);
-    const int row0 = (all - 1 - nth - before) * MANY;
-    const SeqRows s = same_rows_of(p.pages, b);
+    const int b = find_in(p, seqs, all - 1 - nth, before, pieces_in);
+    const SeqRows s = pick(p, seqs, b);
+    const int cut = ranges_of(tiles_of<MANY, KT>(p, s), range), piece = all - 1 - nth - before, row_tile = piece / cut, nth_range = piece - row_tile * cut;
+    const int row0 = row_tile * MANY;
     const int rows = s.count * p.G, seen_before = s.length - s.count;
     // a wavefront's number fixes its SIMD: rows that end early share one with rows that end late
     const int wave_row0 = row0 + (wave < 4 ? wave : 11 - wave) * 32;
@@ -502,8 +579,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     const int wave_first = seen_before + (wave_row0 < rows ? wave_row0 : 0) / p.G;              // what every row of the wavefront sees ends here
     const int wave_last = wave_row0 < rows ? seen_before + min(wave_row0 + 31, rows - 1) / p.G : -1;  // and what some row sees here
     const int seen = max(seen_before + min(row0 + MANY - 1, rows - 1) / p.G + 1, 0);
-    const int range = ((seen + KT - 1) / KT + p.splits - 1) / p.splits * KT;
-    const int k_begin = min(static_cast<int>(blockIdx.y) * range, seen), k_end = min(k_begin + range, seen);
+    const int positions = ((seen + KT - 1) / KT + cut - 1) / cut * KT;
+    const int k_begin = min(nth_range * positions, seen), k_end = min(k_begin + positions, seen);
     const int tiles = (k_end - k_begin + KT - 1) / KT;
 
     const char *qrow = p.q + (static_cast<int64_t>(s.first + place) * p.q_row + static_cast<int64_t>(hkv * p.G + safe - place * p.G) * p.q_head) * 2;
@@ -605,7 +682,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
 #pragma unroll
             for (int j = 0; j < 16; ++j) sc[t][j] = fmaf(sc[t][j], p.scale_log2, neg_ref);
         if (partly) {
-            const int vis = last - k0 - 4 * h;
+            int vis = last - k0 - 4 * h;
+            asm volatile("" : "+v"(vis));  // a branch: as selects the masks cost every tile 64 instructions
 #pragma unroll
             for (int t = 0; t < T32; ++t)
 #pragma unroll
@@ -655,8 +733,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
             unrolled<DT32>([&](auto dc) {
                 constexpr int dt = decltype(dc)::value;
                 const uint32_t a0 = D == 96 ? v_rd0 + at + dt * 64 : (v_rd0 + at) ^ (dt * 64), a1 = D == 96 ? v_rd1 + at + dt * 64 : (v_rd1 + at) ^ (dt * 64);
-                lo[dt] = lds_transpose_read(a0 + u * GROUP * PITCH);
-                hi[dt] = lds_transpose_read(a1 + u * GROUP * PITCH);
+                lo[dt] = lds_transpose_read<u * GROUP * PITCH>(a0);
+                hi[dt] = lds_transpose_read<u * GROUP * PITCH>(a1);
             });
         };
         unrolled<2 * T32>([&](auto uc) {
@@ -681,18 +759,17 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
             const u32x2 m_hi = {more >= 2 ? 0xffffffffu : more == 1 ? 0xffffu : 0u, more >= 4 ? 0xffffffffu : more == 3 ? 0xffffu : 0u};
             unrolled<DT32>([&](auto dc) {
                 constexpr int dt = decltype(dc)::value;
-                const u32x4 v = u32x4{lo[dt].x, lo[dt].y, hi[dt].x, hi[dt].y} & u32x4{m_lo.x, m_lo.y, m_hi.x, m_hi.y};
-                acc[dt] = mfma32<DT>(u32x4{Beyond<DT>::finite(v.x), Beyond<DT>::finite(v.y), Beyond<DT>::finite(v.z), Beyond<DT>::finite(v.w)}, pf[u], acc[dt]);
-                if (!__any(Beyond<DT>::any(v.x) || Beyond<DT>::any(v.y) || Beyond<DT>::any(v.z) || Beyond<DT>::any(v.w))) return;
+                u32x4 w = u32x4{lo[dt].x, lo[dt].y, hi[dt].x, hi[dt].y} & u32x4{m_lo.x, m_lo.y, m_hi.x, m_hi.y};
+                if (__any(((Beyond<DT>::carries(w.x) | Beyond<DT>::carries(w.y) | Beyond<DT>::carries(w.z) | Beyond<DT>::carries(w.w)) & 0x80008000u) != 0)) {
+                    const u32x4 seen = {Beyond<DT>::seen(pf[u].x), Beyond<DT>::seen(pf[u].y), Beyond<DT>::seen(pf[u].z), Beyond<DT>::seen(pf[u].w)};
 #pragma unroll
-                for (uint32_t sign : {0u, 0x8000u}) {
-                    f32x16 found;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) found[j] = 0.f;
-                    found = mfma32<DT>(u32x4{Beyond<DT>::ones(v.x, sign), Beyond<DT>::ones(v.y, sign), Beyond<DT>::ones(v.z, sign), Beyond<DT>::ones(v.w, sign)}, pf[u], found);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[dt][j] += found[j] > 0.f ? (sign != 0 ? -INFINITY : INFINITY) : 0.f;
+                    for (uint32_t sign : {0u, 0x8000u}) {
+                        const u32x4 huge = {Beyond<DT>::huge(w.x, sign), Beyond<DT>::huge(w.y, sign), Beyond<DT>::huge(w.z, sign), Beyond<DT>::huge(w.w, sign)};
+                        acc[dt] = mfma32<TPAMD_BF16>(huge, seen, acc[dt]);
+                    }
+                    w = u32x4{Beyond<DT>::finite(w.x), Beyond<DT>::finite(w.y), Beyond<DT>::finite(w.z), Beyond<DT>::finite(w.w)};
                 }
+                acc[dt] = mfma32<DT>(w, pf[u], acc[dt]);
             });
         });
     }
@@ -700,10 +777,22 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     l_run += __shfl_xor(l_run, 32);
 
     // ---- acc[dt][i] = O[this lane's row][32 dt + 8 (i / 4) + 4 h + i % 4]
+    // (the rows of a tile that was cut go to its range's place among the partials: those of the ranges of sequences before it, then its own)
+    int64_t slot = 0;
+    if (cut > 1) {
+        int mine = 0;
+        for (int b0 = 0; b0 <= b; b0 += 64) {
+            const Lanes l = lanes_from(p, b0);
+            const Tiles t = tiles_of<MANY, KT>(p, l.mine);
+            const int ranges = ranges_of(t, range);
+            mine += b0 + lane < b && ranges > 1 ? t.rows * ranges : 0;
+        }
+        slot = static_cast<int64_t>(__builtin_amdgcn_readlane(sums_to_lane(mine), 63) + piece) * p.Hkv + hkv;
+    }
     if (row >= rows) return;
     const int64_t token = s.first + place;
     const int head = hkv * p.G + row - place * p.G;
-    if (p.splits == 1) {
+    if (cut == 1) {
         const float inv = l_run > 0.f ? 1.0f / l_run : l_run == 0.f ? 0.f : l_run;  // a sum of NaN stays one
         char *orow = p.o + (token * p.o_row + head * p.o_head) * 2;
 #pragma unroll
@@ -714,7 +803,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
                     make_uint2(pack2_half<DT>(acc[dt][j] * inv, acc[dt][j + 1] * inv), pack2_half<DT>(acc[dt][j + 2] * inv, acc[dt][j + 3] * inv));
         return;
     }
-    float *pr = p.part + ((static_cast<int64_t>(blockIdx.y) * p.pages.rows + token) * (p.Hkv * p.G) + head) * PW;
+    float *pr = p.part + (slot * MANY + row - row0) * PW;
 #pragma unroll
     for (int dt = 0; dt < DT32; ++dt)
 #pragma unroll
@@ -722,50 +811,63 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     if (h == 0) *reinterpret_cast<float2 *>(pr + D) = make_float2(m_run, l_run);
 }
 
-// Joins the key ranges of paged_many_kernel's rows: a block a new row, all its query heads.
-template <int DT, int D>
+// Joins the ranges of paged_many_kernel's row tiles that were cut: gridDim.y blocks a row tile.
+template <int DT, int D, int WAVES, int KT>
 __global__ __launch_bounds__(256) void paged_many_merge_kernel(PagedParams p) {
-    constexpr int PW = D + 4, per_row = D / 4;
-    const int token = blockIdx.x, Hq = p.Hkv * p.G;
-    int place;
-    const int b = seq_of_row(p.pages, token, place);
-    if (b < 0) return;
-    const SeqRows s = rows_of(p.pages, b);
-    if (place >= s.count || is_few(p, s.count)) return;
-    const int64_t pitch = static_cast<int64_t>(p.pages.rows) * Hq * PW;
-    for (int e = blockIdx.y * 256 + threadIdx.x; e < Hq * per_row; e += gridDim.y * 256) {
-        const int head = e / per_row, d4 = (e % per_row) * 4;
-        const float *pr = p.part + (static_cast<int64_t>(token) * Hq + head) * PW;
-        float M = -INFINITY;
-        for (int i0 = 0; i0 < p.splits; i0 += 8) {
-            float ms[8];
+    constexpr int MANY = WAVES * 32, PW = D + 4, per_row = D / 4;
+    const int hkv = blockIdx.x % p.Hkv, nth = blockIdx.x / p.Hkv;
+    Lanes seqs = lanes_from(p, 0);
+    const int range = range_tiles<MANY, KT>(p, seqs);
+    auto cut_tiles = [&](const SeqRows &s) {
+        const Tiles t = tiles_of<MANY, KT>(p, s);
+        return ranges_of(t, range) > 1 ? t.rows : 0;
+    };
+    auto slots_in = [&](const SeqRows &s) {
+        const Tiles t = tiles_of<MANY, KT>(p, s);
+        const int ranges = ranges_of(t, range);
+        return ranges > 1 ? t.rows * ranges : 0;
+    };
+    if (nth >= sum_over(p, seqs, cut_tiles)) return;
+    int before;
+    const int b = find_in(p, seqs, nth, before, cut_tiles);
+    const SeqRows s = pick(p, seqs, b);
+    const int cut = ranges_of(tiles_of<MANY, KT>(p, s), range), tile = nth - before;
+    int slots = 0;  // of the sequences before it
+    for (int b0 = 0; b0 <= b; b0 += 64) {
+        const Lanes l = lanes_from(p, b0);
+        slots += b0 + static_cast<int>(threadIdx.x & 63) < b ? slots_in(l.mine) : 0;
+    }
+    slots = __builtin_amdgcn_readlane(sums_to_lane(slots), 63);
+    const int rows = min(s.count * p.G - tile * MANY, MANY);
+    const int64_t pitch = static_cast<int64_t>(p.Hkv) * MANY * PW;
+    const float *base = p.part + ((static_cast<int64_t>(slots) + static_cast<int64_t>(tile) * cut) * p.Hkv + hkv) * MANY * PW;
+    for (int e = blockIdx.y * 256 + threadIdx.x; e < rows * per_row; e += gridDim.y * 256) {
+        const int r = e / per_row, d4 = (e % per_row) * 4;
+        const float *pr = base + r * PW;
+        float M = -INFINITY, l = 0.f;
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < cut; i0 += 4) {
+            float2 ml[4];
+            f32x4 ov[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ms[j] = pr[min(i0 + j, p.splits - 1) * pitch + D];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) M = fmaxf(M, ms[j]);
-        }
-        const float m_use = M == -INFINITY ? 0.f : M;
-        float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-        for (int i0 = 0; i0 < p.splits; i0 += 8) {
-            float2 ml[8];
-            f32x4 ov[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float *from = pr + min(i0 + j, p.splits - 1) * pitch;
+            for (int j = 0; j < 4; ++j) {
+                const float *from = pr + min(i0 + j, cut - 1) * pitch;
                 ml[j] = *reinterpret_cast<const float2 *>(from + D);
                 ov[j] = *reinterpret_cast<const f32x4 *>(from + d4);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (i0 + j >= p.splits) continue;
-                const float weight = exp2f(ml[j].x - m_use);
-                l += weight * ml[j].y;
+            for (int j = 0; j < 4; ++j) {
+                if (i0 + j >= cut) continue;
+                const float m = fmaxf(M, ml[j].x), m_use = m == -INFINITY ? 0.f : m, old = exp2f(M - m_use), now = exp2f(ml[j].x - m_use);
+                M = m;
+                l = l * old + ml[j].y * now;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += weight * ov[j][i];
+                for (int k = 0; k < 4; ++k) o[k] = o[k] * old + ov[j][k] * now;
             }
         }
         const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-        *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(token) * p.o_row + static_cast<int64_t>(head) * p.o_head + d4) * 2) =
+        const int row = tile * MANY + r, place = row / p.G;
+        *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + place) * p.o_row + static_cast<int64_t>(hkv * p.G + row - place * p.G) * p.o_head + d4) * 2) =
             make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
     }
 }
@@ -774,14 +876,13 @@ __global__ __launch_bounds__(256) void paged_many_merge_kernel(PagedParams p) {
 // How a call is laid out, from what the host knows: the number of rows and sequences, and bounds of their new rows and lengths.
 struct Plan {
     bool few, many;
-    int few_blocks, least;  // paged_few_kernel: blocks, and units a block takes at least (0: a block an item)
-    int64_t tiles;          // paged_many_kernel: row tiles of a key/value head, at most
-    int splits;
+    int few_blocks, least;  // paged_few_kernel: blocks, and the least share of one (0: a block an item)
+    int merge_y;            // blocks of an item in its merge
+    int waves;              // paged_many_kernel: wavefronts of a block
+    int64_t tiles;          // row tiles of a key/value head, at most
+    int spread;
     uint64_t bytes;         // of partials
 };
-
-// Heads of 256 elements need the registers of two wavefronts each.
-constexpr int waves_of(int64_t D) { return D == 256 ? 4 : 8; }
 
 Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, bool packed, bool counted, int64_t max_new, int64_t max_length, int64_t room, int cus) {
     const int64_t G = Hq / Hkv, each = packed ? 0 : rows / seqs;
@@ -791,30 +892,32 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
     p.many = most * G > FEW;
     if (p.few) {
         const int64_t items = seqs * Hkv;
-        const int per_cu = D <= 64 ? 5 : D <= 96 ? 3 : D <= 128 ? 2 : 1;
-        const bool cut = decode_splits(items, max_length > 0 ? max_length : 1, D <= 64 ? 64 : 128, cus) > 1 || (items < 4ll * per_cu * cus && max_length > 512);
-        if (cut && items * (room / UNIT + 1) < (1ll << 31)) {  // units are counted in 32 bits
+        const int per_cu = D <= 64 ? 4 : D <= 96 ? 3 : D <= 128 ? 2 : 1;  // blocks that a CU holds (registers; 64 KiB of LDS a block of heads of 128)
+        // Whole items take their block about 0.43 us a unit (heads of 64) or 0.6 us, cut ones the second launch.
+        const bool cut = max_length * (D <= 64 ? 43 : 60) > 64 * 700;
+        if (cut && items * (room / UNIT + 1 + START) < (1ll << 31)) {  // costs are counted in 32 bits
             p.few_blocks = per_cu * cus;
-            p.least = 4;
+            p.least = START + 2;
             p.bytes = static_cast<uint64_t>(2) * p.few_blocks * FEW * (D + 4) * sizeof(float);
+            const int few_rows = static_cast<int>(most * G < FEW ? most * G : FEW), at_once = static_cast<int>(1024 / D);
+            p.merge_y = items * few_rows <= 2ll * cus ? few_rows : (few_rows + at_once - 1) / at_once;
         } else {
             p.few_blocks = static_cast<int>(items);
         }
     }
     if (p.many) {
-        const int64_t MANY = waves_of(D) * 32;
+        // Blocks of 8 wavefronts load keys and values half as often, blocks of 4, two to a CU, leave less of the device idle at the end of a batch and have shorter tiles.
+        // tiles of 256 rows and 64 positions for a CU; of sequences that may differ, half of what the bounds allow
+        const double per_cu = static_cast<double>(rows) * Hq * (max_length - most / 2) / (256.0 * 64.0) / cus * (packed || counted ? 0.5 : 1.0);
+        const bool enough = rows * G / 256 * Hkv >= cus;  // row tiles of 256, none of which need be cut
+        p.waves = D == 256 || per_cu < 40 || (D == 64 && enough) ? 4 : 8;
+        const int64_t MANY = p.waves * 32;
         p.tiles = packed ? rows * G / MANY + seqs : seqs * ((each * G + MANY - 1) / MANY);
-        p.splits = 1;
-        const int64_t blocks = (rows * G + MANY - 1) / MANY * Hkv, keys = max_length > 0 ? max_length : 1;
-        if (blocks < cus) {
-            int64_t splits = cus / blocks;
-            if (splits > keys / 256) splits = keys / 256;  // a range has 256 positions or more
-            if (splits > 32) splits = 32;
-            if (splits < 1) splits = 1;
-            p.splits = static_cast<int>(splits);
-        }
-        if (p.splits > 1) {
-            const uint64_t more = static_cast<uint64_t>(p.splits) * rows * Hq * (D + 4) * sizeof(float);
+        // Of a single sequence with two row tiles and more for a CU nothing is cut, and there is no merge: a share is at least as long as its last tile (the average one has half of that or
+        // more). A few tiles of positions are not cut either.
+        if (!(seqs == 1 && p.tiles * Hkv >= 2ll * cus) && max_length > LEAST_TILES * p.waves * 8) {
+            p.spread = cus;
+            const uint64_t more = static_cast<uint64_t>(2) * p.spread * MANY * (D + 4) * sizeof(float);
             if (more > p.bytes) p.bytes = more;
         }
     }
@@ -827,35 +930,43 @@ int launch(const PagedParams &base, const Plan &plan, hipStream_t s) {
     int dev = 0;
     TPAMD_HIP(hipGetDevice(&dev));
     if (plan.many) {
-        constexpr int WAVES = waves_of(D), KT = WAVES * 8, NST = D >= 128 ? 4 : 3, LDS = NST * 2 * KT * D * 2;
-        static thread_local int configured = -1;
-        if (configured != dev) {
-            TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DT, D, WAVES, KT, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-            configured = dev;
-        }
-        p.splits = plan.splits;
-        const int64_t blocks = plan.tiles * p.Hkv;
-        TPAMD_REQUIRE(blocks * plan.splits < (1ll << 23), "tpamd_attention_paged: too many rows for one launch");
-        hipLaunchKernelGGL((paged_many_kernel<DT, D, WAVES, KT, NST>), dim3(static_cast<unsigned>(blocks), plan.splits), dim3(WAVES * 64), LDS, s, p);
-        TPAMD_HIP(hipGetLastError());
-        if (plan.splits > 1) {
-            const unsigned y = static_cast<unsigned>((static_cast<int64_t>(p.Hkv) * p.G * (D / 4) + 255) / 256);
-            hipLaunchKernelGGL((paged_many_merge_kernel<DT, D>), dim3(static_cast<unsigned>(p.pages.rows), y < 4 ? y : 4), dim3(256), 0, s, p);
+        p.spread = plan.spread;
+        auto run = [&](auto waves) -> int {
+            constexpr int WAVES = decltype(waves)::value, KT = WAVES * 8, NST = 4, LDS = NST * 2 * KT * D * 2;
+            static thread_local int configured = -1;
+            if (configured != dev) {
+                TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DT, D, WAVES, KT, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+                configured = dev;
+            }
+            const int64_t tiles = plan.tiles * p.Hkv, blocks = tiles + plan.spread;
+            TPAMD_REQUIRE(blocks < (1ll << 22), "tpamd_attention_paged: too many rows for one launch");
+            hipLaunchKernelGGL((paged_many_kernel<DT, D, WAVES, KT, NST>), dim3(static_cast<unsigned>((blocks + p.Hkv - 1) / p.Hkv * p.Hkv)), dim3(WAVES * 64), LDS, s, p);
             TPAMD_HIP(hipGetLastError());
-        }
+            if (plan.spread > 0) {
+                // (a cut tile has two ranges and more, fewer than 2 spread in all)
+                const int64_t cut = tiles < plan.spread ? tiles : plan.spread;
+                hipLaunchKernelGGL((paged_many_merge_kernel<DT, D, WAVES, KT>), dim3(static_cast<unsigned>((cut + p.Hkv - 1) / p.Hkv * p.Hkv), WAVES), dim3(256), 0, s, p);
+                TPAMD_HIP(hipGetLastError());
+            }
+            return TPAMD_OK;
+        };
+        int rc;
+        if constexpr (D == 256) rc = run(std::integral_constant<int, 4>{});  // (two wavefronts of a SIMD do not have the registers)
+        else rc = plan.waves == 8 ? run(std::integral_constant<int, 8>{}) : run(std::integral_constant<int, 4>{});
+        if (rc != TPAMD_OK) return rc;
     }
     if (plan.few) {  // behind the other: their partials share the memory
-        constexpr int NST = 2, LDS = 4 * NST * 2 * GROUP * D * 2;
+        p.least = plan.least;
+        constexpr int NST = 2, LDS = 4 * NST * 2 * GROUP * D * 2;  // more stages are no faster: a block starts later with more LDS
         static thread_local int configured = -1;
         if (configured != dev) {
             TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_few_kernel<DT, D, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
             configured = dev;
         }
-        p.least = plan.least;
         hipLaunchKernelGGL((paged_few_kernel<DT, D, NST>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(256), LDS, s, p);
         TPAMD_HIP(hipGetLastError());
         if (plan.least > 0) {
-            hipLaunchKernelGGL((paged_few_merge_kernel<DT, D>), dim3(static_cast<unsigned>(p.pages.seqs * p.Hkv)), dim3(256), 0, s, p, plan.few_blocks);
+            hipLaunchKernelGGL((paged_few_merge_kernel<DT, D>), dim3(static_cast<unsigned>(p.pages.seqs * p.Hkv), plan.merge_y), dim3(256), 0, s, p, plan.few_blocks);
             TPAMD_HIP(hipGetLastError());
         }
     }
@@ -951,7 +1062,6 @@ extern "C" int tpamd_attention_paged(const void *q_dev, int64_t q_row, int64_t q
     p.scale_log2 = scale * 1.4426950408889634f;
     p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv); p.D = static_cast<int>(D);
     p.few = plan.few; p.many = plan.many;
-    p.splits = 1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool bf = dtype == TPAMD_BF16;
     switch (D) {

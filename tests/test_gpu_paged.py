@@ -492,7 +492,7 @@ def test_no_backward():
 def test_short_of_workspace_is_refused():
     batch = Batch([1], [20000], 2, 2, 64, 16, F16, seed=32)
     d, q = batch.on(), batch.q.to(DEV)
-    packed, keep = _native._pack_pages("attend", q, 1, 2, 64, d["k_pages"], d["v_pages"], d["table"], d["lengths"], d["starts"], None)
+    packed, keep = _native._pages("attend", q, 0, 2, 64, d["k_pages"], d["v_pages"], d["table"], d["lengths"], d["starts"], None)
     need = ctypes.c_uint64()
     assert _native.lib().tpamd_attention_paged_workspace(packed, 1, 2, 2, 64, 1, 20000, ctypes.byref(need)) == 0 and need.value > 0
     out = torch.empty_like(q)
