@@ -14,7 +14,10 @@ head_dim other than 64 / 128 raises: there is no second implementation to fall b
 rotary position embeddings handed in as `position_embeddings`, a transformers cache object): their forward then runs the
 rotary embedding, the hand-over to the cache and the attention core on the library's kernels too (`tpamd_rope_append` +
 `tpamd_attention` at prefill, `tpamd_attention_decode_rope` for one new position), writing into buffers with room to grow
-that the cache layer's `keys` / `values` are views of. A call those kernels do not cover takes the module's own forward.
+that the cache layer's `keys` / `values` are views of. A call those kernels do not cover takes the module's own forward. On a `paged.PagedCache` the same modules run `tpamd_append_paged`
+and `tpamd_attention_paged`, on sequences that differ in length.
+
+`rotate` is the rotation alone, of halves or neighbours, with the norms of query and key heads that some models have in front of it.
 """
 from __future__ import annotations
 
@@ -25,6 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native, together
+from .paged import PagedCache
 from .shard_modules import _guard, returned
 
 IMPLEMENTATION_NAME = "tpamd"
@@ -341,7 +345,27 @@ def takes_rows(module: torch.nn.Module, forward, hidden_states: torch.Tensor, kw
     return _caches_for(module, hidden_states, more.pop("position_embeddings", None), more.pop("attention_mask", None), more.pop("past_key_values", None), more) != (None, None)
 
 
+PAGED_HEAD_DIMS = (64, 96, 128, 256)
+
+
+def _check_paged(self, hidden_states, position_embeddings, attention_mask, head_dim: int, output_attentions) -> None:
+    """A paged cache has no other way to go: what the fused forward does not take is refused."""
+    if (position_embeddings is None or self.training or output_attentions or not isinstance(hidden_states, torch.Tensor) or hidden_states.dim() != 3
+            or hidden_states.device.type != "cuda" or hidden_states.dtype not in (torch.bfloat16, torch.float16) or head_dim not in PAGED_HEAD_DIMS):
+        raise NotImplementedError(f"PagedCache: attention on pages is inference on 16-bit hidden states on a HIP device with rotary embeddings and heads of {PAGED_HEAD_DIMS} elements, "
+                                  "without attention weights")
+    if attention_mask is not None:
+        raise NotImplementedError("PagedCache: an attention mask was passed; rows of a batch are padded on the right and counted (prepare), without a mask")
+
+
 def _fused_rotary_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+    if isinstance(past_key_values, PagedCache):
+        _check_paged(self, hidden_states, position_embeddings, None if self.__dict__.get("_tp_no_padding", False) else attention_mask, getattr(self, "head_dim", None),
+                     kwargs.get("output_attentions"))
+        B, S, _ = hidden_states.shape
+        q, k, v = _project_qkv(self, hidden_states, self.head_dim)
+        out = past_key_values.attend(q, k, v, *position_embeddings, self.layer_idx, getattr(self, "scaling", None))
+        return returned(self, _fused_rotary_forward, self.o_proj, out.reshape(B, S, -1)), None
     # (hidden_states may be `QuantizedRows`, where takes_rows has said that this forward takes the call)
     layer, static = _caches_for(self, hidden_states, position_embeddings, attention_mask, past_key_values, kwargs)
     if layer is None and static is None:
@@ -364,6 +388,14 @@ def _fused_falcon_forward(self, hidden_states: torch.Tensor, alibi=None, attenti
     was told is right (the mask is then the causal pattern the kernels apply themselves)."""
     D = self.head_dim
     layer = static = None
+    if isinstance(layer_past, PagedCache):
+        if alibi is not None or not self.new_decoder_architecture:
+            raise NotImplementedError("PagedCache: attention on pages is that of rotary, grouped heads")
+        _check_paged(self, hidden_states, position_embeddings, None, D, output_attentions)  # (the mask that this module is always handed is the causal one: see below)
+        B, S, _ = hidden_states.shape
+        qkv = self.query_key_value(hidden_states).view(B, S, self.num_kv_heads, -1, D)
+        out = layer_past.attend(qkv[:, :, :, :-2], qkv[:, :, :, -2], qkv[:, :, :, -1], *position_embeddings, self.layer_idx, self.inv_norm_factor)
+        return returned(self, _fused_falcon_forward, self.dense, out.reshape(B, S, self.num_heads * D)), None
     usable = (alibi is None and position_embeddings is not None and layer_past is not None and not self.training and not output_attentions
               and self.new_decoder_architecture and hidden_states.dim() == 3 and hidden_states.device.type == "cuda"
               and hidden_states.dtype in (torch.bfloat16, torch.float16) and D in (64, 128))

@@ -15,12 +15,16 @@ back. A page outside of the pool (-1, say) holds zeros and takes nothing.
   append(...)   rotates q and k (and norms their heads before, where weights are given) and writes k and v to their pages; returns q          tpamd_append_paged
   attend(...)   softmax(scale q k^T) v of the new rows, each on the positions up to its own                                                  tpamd_attention_paged
 
+  PagedCache    pools, page table and lengths of a wrapped model's layers: handed to a model as `past_key_values` once `attention.fuse_rotary_` has given its attention modules their
+                fused forward, on one rank or on several
+
 Two calls that write to the same pages, or one that reads what another writes, are the caller's to order, as for any two kernels (calls on one stream are). Inference only: a backward
 pass through either raises.
 """
 from __future__ import annotations
 
-from typing import Optional
+import copy
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -47,3 +51,183 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
     max_new: no sequence has more new rows (rows of one that does may be left out); tell it where it is known, a step of single rows is then one or two launches. max_length: no sequence
     has more positions; only the time depends on it. Both have to hold for every replay where the call is captured."""
     return _guard(_native.attention_paged(q, k_pages, v_pages, table, lengths, starts, counts, scale, max_new, max_length, out), q)
+
+
+class _Book:
+    """What the caches of all ranks and layers have in common: which pages each sequence has, how many positions, and the rows of the step that is on its way."""
+
+    def __init__(self, sequences: int, pages: int, page: int, columns: int):
+        self.sequences, self.pages, self.page, self.columns = sequences, pages, page, columns
+        self.device_state: Optional[torch.Tensor] = None
+        self.reset()
+
+    def reset(self) -> None:
+        self.free: List[int] = list(range(self.pages - 1, -1, -1))
+        self.tables: List[List[int]] = [[] for _ in range(self.sequences)]
+        self.before = [0] * self.sequences  # positions without the step's rows
+        self.counts = [0] * self.sequences  # the step's rows
+        self.number, self.taken, self.hold = 0, True, False  # of the step (0: none yet); whether a forward has begun it; whether further forwards are the same step
+        self.uploaded = -1
+
+    def after(self) -> List[int]:
+        return [n + c for n, c in zip(self.before, self.counts)]
+
+    def begin(self, counts: Sequence[int], hold: bool) -> None:
+        counts = [int(c) for c in counts]
+        if len(counts) != self.sequences or min(counts, default=0) < 0:
+            raise ValueError(f"PagedCache: {self.sequences} counts of new rows, none below 0, are needed, got {counts}")
+        before = self.after() if self.taken else self.before
+        need = [-(-(n + c) // self.page) - len(t) for n, c, t in zip(before, counts, self.tables)]
+        if max((len(t) + max(n, 0) for n, t in zip(need, self.tables)), default=0) > self.columns:
+            raise RuntimeError(f"PagedCache: a sequence of {max(n + c for n, c in zip(before, counts))} positions needs more than {self.columns} pages of {self.page}")
+        if sum(max(n, 0) for n in need) > len(self.free):
+            raise RuntimeError(f"PagedCache: {sum(max(n, 0) for n in need)} more pages of {self.page} positions are needed, {len(self.free)} of {self.pages} are free")
+        for table, n in zip(self.tables, need):
+            table.extend(self.free.pop() for _ in range(n))
+        self.before, self.counts = before, counts
+        self.number, self.taken, self.hold = self.number + 1, hold, hold  # (replays of a captured forward do not come by here)
+
+    def release(self, sequence: int) -> None:
+        if not self.taken:
+            raise RuntimeError("PagedCache: a step was prepared that no forward has made yet")
+        self.before = self.after()
+        self.counts = [0] * self.sequences
+        self.free.extend(reversed(self.tables[sequence]))
+        self.tables[sequence], self.before[sequence] = [], 0
+
+    def on(self, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """table, lengths and counts of the step on the device: always the same memory, which a captured forward reads."""
+        n = self.sequences
+        if self.device_state is None or self.device_state.device != device:
+            self.device_state, self.uploaded = torch.zeros(n * (self.columns + 2), dtype=torch.int32, device=device), -1
+        state = self.device_state
+        if self.uploaded != self.number:
+            rows = torch.full((n, self.columns), -1, dtype=torch.int32)
+            for row, table in zip(rows, self.tables):
+                row[:len(table)] = torch.tensor(table, dtype=torch.int32)
+            state.copy_(torch.cat([rows.flatten(), torch.tensor(self.after() + self.counts, dtype=torch.int32)]))
+            self.uploaded = self.number
+        return state[:n * self.columns].view(n, self.columns), state[n * self.columns:n * (self.columns + 1)], state[n * (self.columns + 1):]
+
+
+class PagedCache:
+    """A key/value cache in pages for `sequences` sequences, which differ in length and come and go, as `past_key_values` of a model whose attention modules have the fused forward
+    (`attention.fuse_rotary_`; others raise). Each layer of each rank gets a pool of `pages` pages with `page` positions when it is first used; all of them share one page table, which has
+    room for `most_pages` pages of a sequence (`pages` by default).
+
+        cache = tp.paged.PagedCache(sequences=3, pages=512)
+        positions = cache.prepare([40, 7, 100])                           # rows of each sequence in the next forward
+        model(input_ids=padded, position_ids=positions, past_key_values=cache, use_cache=True)      # [3, 100], rows padded on the right; what stands behind a sequence's rows means nothing
+        positions = cache.prepare([1, 1, 1])
+        logits = model(input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True).logits
+        cache.release(1)                                                  # sequence 1 has ended: its pages are free, row 1 may begin another
+
+    A forward that nothing was prepared for has all of its rows new, in every sequence. Positions are the model's business: it counts from the longest sequence where it is given none, so
+    sequences of different lengths need `position_ids` (a forward without them is refused). Masks of padding are refused too: rows are padded on the right, and counted.
+
+    `prepare(counts, hold=True)`: all forwards up to the next `prepare` are the same step, which counts as made. A forward captured under it (`tp.graphs.capture`, with
+    `fuse_rotary_(model, assume_no_padding=True)`: transformers makes a mask, the causal one, where a forward is captured) reads table and lengths when it is replayed:
+
+        positions = cache.prepare([1] * 3, hold=True)
+        step = tp.graphs.capture(model, input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True)
+        positions = cache.prepare([1] * 3, hold=True)                     # every further token, the first of them with the step's own
+        logits = step(input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True).logits
+
+    Not thread-safe; beam search (which would have sequences share pages) is not supported."""
+
+    is_compileable = False
+
+    def __init__(self, sequences: int, pages: int, page: int = 64, most_pages: Optional[int] = None):
+        if sequences < 1 or pages < 1 or page < 16 or page & (page - 1) or (most_pages is not None and most_pages < 1):
+            raise ValueError(f"PagedCache: at least one sequence and one page are needed, and a power of two from 16 on of positions in it, got {sequences}, {pages}, {page}, {most_pages}")
+        self._book = _Book(sequences, pages, page, pages if most_pages is None else most_pages)
+        self._own()
+
+    def _own(self) -> None:
+        self._pools: dict = {}          # layer -> (keys, values)
+        self._number, self._seen = -1, set()  # the step that this rank's forward is in, and its layers that have been there
+
+    def __deepcopy__(self, memo) -> "PagedCache":
+        """Another rank's cache: pools of its own, the same sequences (kv_cache.rank_caches)."""
+        other = copy.copy(self)
+        other.__dict__ = {"_book": self._book}
+        other._own()
+        return other
+
+    def prepare(self, counts: Sequence[int], hold: bool = False) -> Optional[torch.Tensor]:
+        """The next forward has counts[b] new rows of sequence b (of as many rows as the largest count has, padded on the right). Takes their pages, or raises with nothing changed. Returns the
+        rows' positions [sequences, largest count] on the host: `position_ids`, once they are on the model's device."""
+        book = self._book
+        book.begin(counts, hold)
+        if book.device_state is not None:
+            book.on(book.device_state.device)  # where a captured forward looks for them
+        return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts))
+
+    def release(self, sequence: int) -> None:
+        """Sequence `sequence` has ended: its pages are free and its length is 0."""
+        self._book.release(sequence)
+
+    def lengths(self) -> List[int]:
+        """The positions of each sequence, those of a step that a forward has begun among them."""
+        return self._book.after() if self._book.taken else list(self._book.before)
+
+    def reset(self) -> None:
+        """All sequences have ended. The pools stay."""
+        self._book.reset()
+        self._number, self._seen = -1, set()
+
+    # ---- what transformers asks of a cache
+    def get_seq_length(self, layer_idx: int = 0) -> int:
+        """The longest sequence's positions, as this rank's forward sees them: with a step's rows from its first attention module on."""
+        book = self._book
+        return max(book.after() if book.taken and self._number == book.number else book.before)
+
+    def get_max_length(self, layer_idx: int = 0) -> int:
+        return self._book.columns * self._book.page
+
+    get_max_cache_shape = get_max_length
+
+    def get_mask_sizes(self, query_length: int, layer_idx: int = 0) -> Tuple[int, int]:
+        return query_length, 0  # of the forward's own rows: the plain causal mask, which is not made; what a row sees is the kernels' business
+
+    def get_query_offset(self, layer_idx: int = 0) -> int:
+        return 0
+
+    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
+        raise NotImplementedError("PagedCache: this attention module works on keys and values that lie one after another; tp.attention.fuse_rotary_(model) gives those of the Llama pattern and "
+                                  "rotary Falcon a forward that works on pages")
+
+    def reorder_cache(self, beam_idx):
+        raise NotImplementedError("PagedCache: sequences do not share pages, so there is no beam search on it")
+
+    # ---- the fused attention modules' side
+    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, layer_idx: int, scale: Optional[float] = None) -> torch.Tensor:
+        """One attention module's share of a forward: q [B, S, Hq, D] (or grouped by key/value head), k, v [B, S, Hkv, D], the rotary embedding's tables cos, sin [B or 1, S, part]; [B, S, Hq, D]."""
+        book = self._book
+        B, S, Hkv, D = k.shape
+        if B != book.sequences:
+            raise ValueError(f"PagedCache: {B} sequences in a forward on a cache for {book.sequences}")
+        first = self._number != book.number or (layer_idx in self._seen and not book.hold)  # this rank's first module in a forward
+        begins = first and book.number in (0, self._number)  # a step that nothing was prepared for
+        if begins and not book.taken:
+            raise RuntimeError("PagedCache: a rank is a forward ahead of the others")
+        counts, before = ([S] * B, book.after()) if begins else (book.counts, book.before)
+        if max(counts) > S or (max(counts) < S and not book.hold):
+            raise ValueError(f"PagedCache: {counts} new rows were prepared, the forward has {S}")
+        if B > 1 and cos.shape[0] == 1 and min(before) != max(before):
+            raise ValueError(f"PagedCache: sequences of {before} positions in one forward need position_ids of their own")
+        if begins:
+            book.begin(counts, False)
+        if first:
+            book.taken, self._number, self._seen = True, book.number, set()
+        self._seen.add(layer_idx)
+        lengths = book.after()
+        if layer_idx not in self._pools:
+            self._pools[layer_idx] = tuple(torch.zeros((book.pages, Hkv, book.page, D), dtype=k.dtype, device=k.device) for _ in "kv")
+        pools = self._pools[layer_idx]
+        table, lengths_there, counts_there = book.on(k.device)
+        whole = min(counts) == S and not book.hold
+        plan = {"table": table, "lengths": lengths_there, "counts": None if whole else counts_there}
+        half = cos.shape[-1] // 2  # (transformers' tables have each pair's value twice)
+        q = append(q, k, v, *pools, **plan, cos=cos[..., :half], sin=sin[..., :half])
+        return attend(q, *pools, **plan, scale=scale, max_new=S, max_length=None if book.hold else max(lengths), out=None if whole else torch.zeros_like(q))
