@@ -1546,23 +1546,30 @@ def _heads(what: str, q, k, v, positions, inv_freq, cos, sin, scaling, interleav
         raise TypeError(f"{what}: q, k and v must share bfloat16 or float16")
     qs, ks = q.shape, k.shape
     axes = len(ks) - 2
-    if axes < 0 or len(qs) - len(ks) not in (0, 1) or qs[:axes] != ks[:axes] or qs[-1] != ks[-1] or (v is not None and v.shape != ks) or (len(qs) > len(ks) and qs[axes] != ks[axes]):
+    if axes == 1 and len(qs) == 3:  # the way of most calls
+        rows, Hkv, D = ks
+        fit, Hq = qs[0] == rows and qs[2] == D, qs[1]
+    else:
+        fit = axes >= 0 and len(qs) - len(ks) in (0, 1) and qs[:axes] == ks[:axes] and qs[-1] == ks[-1] and (len(qs) == len(ks) or qs[axes] == ks[axes])
+    if not fit or (v is not None and v.shape != ks):
         raise ValueError(f"{what}: shapes q {tuple(qs)}, k {tuple(ks)}{'' if v is None else f', v {tuple(v.shape)}'} do not fit")
     if k.get_device() != index or (v is not None and v.get_device() != index):
         raise ValueError(f"{what}: q, k and v lie on different devices")
     axis = ks[:axes]
     if axes != 1:
         q, k, v = (None if t is None else _one_axis(t, axes) for t in (q, k, v))
-        qs, ks = q.shape, k.shape
-    rows, Hkv, D = ks
     q_step, k_step = q.stride(), k.stride()
     v_step = k_step if v is None else v.stride()
+    if len(q_step) == 4:
+        rows, Hkv, D = k.shape
+        Hq, q_head, q_group = q.shape[1] * q.shape[2], q_step[2], q_step[1]
+    else:
+        if axes != 1:
+            rows, Hkv, D = k.shape
+            Hq = q.shape[1]
+        q_head, q_group = q_step[1], q_step[1] * (Hq // Hkv if Hkv else 1)
     if D > 1 and (q_step[-1] != 1 or k_step[2] != 1 or v_step[2] != 1):
         raise ValueError(f"{what}: heads must be contiguous")
-    if len(qs) == 3:
-        Hq, q_head, q_group = qs[1], q_step[1], q_step[1] * (qs[1] // Hkv if Hkv else 1)
-    else:
-        Hq, q_head, q_group = qs[1] * qs[2], q_step[2], q_step[1]
     part = table_row = table_code = freq_at = cos_at = sin_at = pos_at = q_norm_at = k_norm_at = 0
     if inv_freq is not None:
         if cos is not None or sin is not None:
@@ -1603,7 +1610,7 @@ def _heads(what: str, q, k, v, positions, inv_freq, cos, sin, scaling, interleav
         k_norm = k_norm.contiguous()
         k_norm_at = k_norm.data_ptr()
     q_out = q.new_empty((rows, Hq, D))
-    k_out = q.new_empty(ks) if v is None else None
+    k_out = q.new_empty((rows, Hkv, D)) if v is None else None
     packed = _HEADS.pack(q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), q_step[0], q_group, q_head, k_step[0], k_step[1], v_step[0], v_step[1],
                          q_norm_at, k_norm_at, eps, scaling, freq_at, cos_at, sin_at, table_row, table_code, 1 if interleaved else 0, part, pos_at,
                          q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), Hq * D, D, Hkv * D, D)
@@ -1713,24 +1720,25 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         max_new = rows
     if max_length is None:
         max_length = table.shape[1] * pool[2]
-    need = ctypes.c_uint64()
-    _launch_free("tpamd_attention_paged_workspace", lib().tpamd_attention_paged_workspace, index, pages, rows, Hq, Hkv, D, max_new, max_length, ctypes.byref(need))
-    size = need.value
+    max_length = -(-max_length // 64) * 64  # (the size below is asked for once in 64 steps)
+    size = _paged_workspace(rows, table.shape[0], Hq, Hkv, D, pool[2], table.shape[1], starts is not None, counts is not None, max_new, max_length, index)
     work = q.new_empty(size, dtype=torch.uint8) if size else None
     _launch("tpamd_attention_paged", lib().tpamd_attention_paged, index, q.data_ptr(), step[0], step[1], pages, rows_out.data_ptr(), out_step[0], out_step[1], rows, Hq, Hkv, D, max_new,
             max_length, D ** -0.5 if scale is None else float(scale), code, 0 if work is None else work.data_ptr(), size)
     return out
 
 
-def _launch_free(what: str, call, index: int, *args) -> None:
-    """call(*args) with HIP device `index` as the current one: for calls that take no stream."""
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace(rows: int, seqs: int, Hq: int, Hkv: int, D: int, page: int, columns: int, packed: bool, counted: bool, max_new: int, max_length: int, index: int) -> int:
+    """Bytes of workspace of a call of these sizes on HIP device `index` (host arithmetic; no pointer is looked into, so any that is not NULL will do)."""
+    pages, need = _PAGES.pack(1, 1, 1, page, 0, 0, 0, 0, 0, 0, 1, 0, columns, 1, 1 if packed else 0, 1 if counted else 0, seqs), ctypes.c_uint64()
     prev = _device_of_thread()
     if prev != index:
         torch.cuda.set_device(index)
     try:
-        rc = call(*args)
+        rc = lib().tpamd_attention_paged_workspace(pages, rows, Hq, Hkv, D, max_new, max_length, ctypes.byref(need))
     finally:
         if prev != index:
             torch.cuda.set_device(prev)
-    if rc != 0:
-        _check(rc, what)
+    _check(rc, "tpamd_attention_paged_workspace")
+    return need.value
