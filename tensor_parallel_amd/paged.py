@@ -24,7 +24,8 @@ pass through either raises.
 from __future__ import annotations
 
 import copy
-from typing import List, Optional, Sequence, Tuple
+import threading
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -58,7 +59,9 @@ class _Book:
 
     def __init__(self, sequences: int, pages: int, page: int, columns: int):
         self.sequences, self.pages, self.page, self.columns = sequences, pages, page, columns
-        self.device_state: Optional[torch.Tensor] = None
+        self.states: Dict[torch.device, torch.Tensor] = {}
+        self.uploaded: Dict[torch.device, int] = {}  # the step that is there
+        self.lock = threading.Lock()  # ranks on different devices are threads
         self.reset()
 
     def reset(self) -> None:
@@ -67,7 +70,7 @@ class _Book:
         self.before = [0] * self.sequences  # positions without the step's rows
         self.counts = [0] * self.sequences  # the step's rows
         self.number, self.taken, self.hold = 0, True, False  # of the step (0: none yet); whether a forward has begun it; whether further forwards are the same step
-        self.uploaded = -1
+        self.uploaded.clear()
 
     def after(self) -> List[int]:
         return [n + c for n, c in zip(self.before, self.counts)]
@@ -98,15 +101,15 @@ class _Book:
     def on(self, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """table, lengths and counts of the step on the device: always the same memory, which a captured forward reads."""
         n = self.sequences
-        if self.device_state is None or self.device_state.device != device:
-            self.device_state, self.uploaded = torch.zeros(n * (self.columns + 2), dtype=torch.int32, device=device), -1
-        state = self.device_state
-        if self.uploaded != self.number:
+        state = self.states.get(device)
+        if state is None:
+            state = self.states[device] = torch.zeros(n * (self.columns + 2), dtype=torch.int32, device=device)
+        if self.uploaded.get(device) != self.number:
             rows = torch.full((n, self.columns), -1, dtype=torch.int32)
             for row, table in zip(rows, self.tables):
                 row[:len(table)] = torch.tensor(table, dtype=torch.int32)
             state.copy_(torch.cat([rows.flatten(), torch.tensor(self.after() + self.counts, dtype=torch.int32)]))
-            self.uploaded = self.number
+            self.uploaded[device] = self.number
         return state[:n * self.columns].view(n, self.columns), state[n * self.columns:n * (self.columns + 1)], state[n * (self.columns + 1):]
 
 
@@ -133,7 +136,7 @@ class PagedCache:
         positions = cache.prepare([1] * 3, hold=True)                     # every further token, the first of them with the step's own
         logits = step(input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True).logits
 
-    Not thread-safe; beam search (which would have sequences share pages) is not supported."""
+    One caller at a time (the ranks of its forward may be threads); beam search (which would have sequences share pages) is not supported."""
 
     is_compileable = False
 
@@ -159,8 +162,8 @@ class PagedCache:
         rows' positions [sequences, largest count] on the host: `position_ids`, once they are on the model's device."""
         book = self._book
         book.begin(counts, hold)
-        if book.device_state is not None:
-            book.on(book.device_state.device)  # where a captured forward looks for them
+        for device in book.states:
+            book.on(device)  # where a captured forward looks for them
         return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts))
 
     def release(self, sequence: int) -> None:
@@ -203,6 +206,15 @@ class PagedCache:
     # ---- the fused attention modules' side
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, layer_idx: int, scale: Optional[float] = None) -> torch.Tensor:
         """One attention module's share of a forward: q [B, S, Hq, D] (or grouped by key/value head), k, v [B, S, Hkv, D], the rotary embedding's tables cos, sin [B or 1, S, part]; [B, S, Hq, D]."""
+        with self._book.lock:
+            plan, whole, longest = self._step_of(k, cos, layer_idx)
+        pools = self._pools[layer_idx]
+        half = cos.shape[-1] // 2  # (transformers' tables have each pair's value twice)
+        q = append(q, k, v, *pools, **plan, cos=cos[..., :half], sin=sin[..., :half])
+        return attend(q, *pools, **plan, scale=scale, max_new=k.shape[1], max_length=longest, out=None if whole else torch.zeros_like(q))
+
+    def _step_of(self, k: torch.Tensor, cos: torch.Tensor, layer_idx: int) -> Tuple[dict, bool, Optional[int]]:
+        """Begins the step where this module is the first to come by. Where its rows are, whether all of them are new, and the longest sequence's positions (None: replays differ)."""
         book = self._book
         B, S, Hkv, D = k.shape
         if B != book.sequences:
@@ -224,10 +236,6 @@ class PagedCache:
         lengths = book.after()
         if layer_idx not in self._pools:
             self._pools[layer_idx] = tuple(torch.zeros((book.pages, Hkv, book.page, D), dtype=k.dtype, device=k.device) for _ in "kv")
-        pools = self._pools[layer_idx]
         table, lengths_there, counts_there = book.on(k.device)
         whole = min(counts) == S and not book.hold
-        plan = {"table": table, "lengths": lengths_there, "counts": None if whole else counts_there}
-        half = cos.shape[-1] // 2  # (transformers' tables have each pair's value twice)
-        q = append(q, k, v, *pools, **plan, cos=cos[..., :half], sin=sin[..., :half])
-        return attend(q, *pools, **plan, scale=scale, max_new=S, max_length=None if book.hold else max(lengths), out=None if whole else torch.zeros_like(q))
+        return {"table": table, "lengths": lengths_there, "counts": None if whole else counts_there}, whole, None if book.hold else max(lengths)

@@ -1,5 +1,7 @@
 """The bookkeeping of `tp.paged.PagedCache`: pages, lengths, steps and ranks. Nothing is computed, so no GPU is needed."""
 import copy
+import threading
+import time
 
 import pytest
 import torch
@@ -103,3 +105,70 @@ def test_modules_of_other_kinds_are_refused():
         cache.update(None, None, 0)
     with pytest.raises(NotImplementedError, match="beam"):
         cache.reorder_cache(None)
+
+
+def forward(cache, rows, layers=2):
+    """The attention modules' share of a rank's forward, without the kernels."""
+    for layer in range(layers):
+        q, kv, table = torch.zeros(1, rows, 2, 64), torch.zeros(1, rows, 1, 64), torch.zeros(1, rows, 64)
+        cache.attend(q, kv, kv, table, table, layer)
+
+
+@pytest.fixture
+def no_kernels(monkeypatch):
+    monkeypatch.setattr(paged, "append", lambda q, *args, **kwargs: q)
+    monkeypatch.setattr(paged, "attend", lambda q, *args, **kwargs: q)
+
+
+@pytest.mark.parametrize("prepared", [False, True])
+def test_ranks_that_are_threads_begin_a_step_once(no_kernels, monkeypatch, prepared):
+    after = paged._Book.after
+
+    def slowly(book):
+        counts = after(book)
+        time.sleep(0.02)  # the other rank comes by between reading the book and writing it
+        return counts
+
+    monkeypatch.setattr(paged._Book, "after", slowly)
+    cache = paged.PagedCache(sequences=1, pages=8, page=16)
+    ranks = kv_cache.rank_caches(cache, 3)
+    failed = []
+
+    def run(rank, barrier):
+        try:
+            barrier.wait(10)
+            forward(rank, 5)
+        except BaseException as e:
+            failed.append(e)
+
+    for n in (1, 2):
+        if prepared:
+            cache.prepare([5])
+        barrier = threading.Barrier(len(ranks))
+        threads = [threading.Thread(target=run, args=(r, barrier)) for r in ranks]
+        [t.start() for t in threads]
+        [t.join(30) for t in threads]
+        assert not failed and cache.lengths() == [5 * n]
+
+
+def test_a_cache_that_was_reset_begins_a_step_once(no_kernels):
+    cache = paged.PagedCache(sequences=1, pages=8, page=16)
+    ranks = kv_cache.rank_caches(cache, 2)
+    for _ in range(3):
+        for n in (1, 2):
+            [forward(r, 5) for r in ranks]
+            assert cache.lengths() == [5 * n]
+        cache.reset()
+        assert cache.lengths() == [0] and [r.get_seq_length() for r in ranks] == [0, 0]
+
+
+def test_devices_have_state_of_their_own():
+    cache = paged.PagedCache(sequences=1, pages=8, page=16)
+    cache.prepare([3])
+    devices = torch.device("cpu"), torch.device("meta")
+    first = [cache._book.on(d) for d in devices]
+    step(cache)
+    cache.prepare([1])  # (both are brought up to date: captured forwards on either read them)
+    assert first[0][1].tolist() == [4]
+    for device, state in zip(devices, first):
+        assert all(a is b or (a.device == device and a.untyped_storage()._cdata == b.untyped_storage()._cdata) for a, b in zip(cache._book.on(device), state))
