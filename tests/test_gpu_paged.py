@@ -266,6 +266,25 @@ def test_values_that_are_not_finite(counts, lengths, D):
     assert got[-1].isnan().all() and not got[:-1, :, 20:].isnan().any()
 
 
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("counts,lengths", [([1, 4], [70, 133]), ([50, 40], [50, 161])])
+def test_values_that_are_not_finite_in_half_precision(counts, lengths, D):
+    batch = Batch(counts, lengths, 4, 2, D, 16, F16, seed=15, spread=0.0)
+    b, n = 1, lengths[1]
+    for back, column, value in ((2, 3, math.inf), (1, 5, -math.inf), (3, 7, math.nan), (0, 11, math.inf), (2, 11, -math.inf), (counts[1] + 1, 13, -math.inf)):
+        j = n - 1 - back
+        batch.v[batch.table[b][j // 16], :, j % 16, column] = value
+    check_attend(batch)
+
+
+@pytest.mark.parametrize("max_length", [None, 1, 4040, 1 << 20])
+@pytest.mark.parametrize("counts,lengths,Hq,Hkv,D,page", [MIXED[0], MIXED[1], FEW[3], MANY[3],
+                                                          ([1] * 70 + [40] + [2] * 20 + [64, 1], [33] * 70 + [3100] + [70] * 20 + [1500, 900], 4, 2, 64, 16)])
+def test_bounds_change_nothing_but_the_time(counts, lengths, Hq, Hkv, D, page, max_length):
+    """Whatever max_length says (of a captured call, what it said then); max_new as it is."""
+    check_attend(Batch(counts, lengths, Hq, Hkv, D, page, BF16, seed=16, behind=2), max_length=max_length, max_new=max(counts))
+
+
 def test_pages_that_the_pool_does_not_have_hold_zeros():
     for counts, lengths in (([1, 2], [100, 90]), ([40, 1], [100, 90])):
         batch = Batch(counts, lengths, 4, 2, 64, 16, F16, seed=13)
