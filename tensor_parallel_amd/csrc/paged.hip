@@ -3,8 +3,8 @@
 // read by the kernels.
 //
 // A sequence whose rows (new rows times query heads of a key/value head) fill at most one MFMA tile of 16 goes to paged_few_kernel, which is bound by reading keys and
-// values once; any other to paged_many_kernel, bound by its matrix products and exponentials. A call that may have both kinds launches both; each leaves the
-// other's sequences alone.
+// values once; any other to paged_many_kernel, bound by its matrix products and exponentials. A call that may have both kinds runs both (with blocks of 4 wavefronts as one
+// launch, paged_both_kernel); each leaves the other's sequences alone. What was cut is joined by paged_merge_kernel.
 //
 // Both load K and V straight into LDS, 16 positions by 16 positions: those lie in one page (pages have 16 positions or more, a power of two), so that a page is looked
 // up once for them and the loads have one descriptor and fixed offsets. A piece (16 bytes) c of a staged row r is in slot c ^ turned(r): rows are read as MFMA operands
@@ -20,13 +20,13 @@ namespace {
 constexpr int FEW = 16;    // rows of a paged_few_kernel item
 constexpr int GROUP = 16;  // positions that lie in one page
 constexpr int UNIT = 64;   // positions of a piece of paged_few_kernel's work: a group for each of its wavefronts
-constexpr int START = 3;   // units that the start and the end of an item cost about as much as
+constexpr int START = 3;   // units that the start and the end of an item cost about as much as; 200 sequences of 100 positions and 4 of 8000, 32 heads on 8 of 128: 60, 51, 48, 52 us with 0, 1, 3, 6
 
 struct PagedParams {
     const char *q;
     char *o;
     int64_t q_row, q_head, o_row, o_head;  // elements
-    float *part;
+    float *many_part, *few_part;
     float scale_log2;  // scale * log2(e)
     int Hkv, G, D;
     int few, many;     // which of the kernels run
@@ -206,12 +206,15 @@ __device__ __forceinline__ int share_of(const PagedParams &p, int cost, int bloc
 // ---- few rows --------------------------------------------------------------------------------------------------------------------------------------------------------
 // An item is one key/value head of one sequence, its work the sequence's positions in units of 64. The costs of all items (their units, and START units in front of them), one after
 // another, are cut into equal shares, one for a block, so that a batch of sequences of very different lengths keeps all blocks busy to the end; where a cut falls inside an item, both sides
-// leave (m, l, O) as partials, and paged_few_merge_kernel joins them. A block has at most two such pieces (its first and its last), so the partials' memory does not
+// leave (m, l, O) as partials, and few_merge joins them. A block has at most two such pieces (its first and its last), so the partials' memory does not
 // grow with the batch. `least` == 0: a block takes an item whole and nothing is merged.
 //
 // Inside a block the four wavefronts take every fourth 16 positions through LDS stages of their own and meet at the end of an item.
+//
+// Bound by HBM where there is enough to read: 100000 positions of 8 key/value heads of 128 elements 76 us and their merge 5 (410 MB, 5.0 TB/s of the whole call); 64 sequences of 81 to
+// 7113 positions, 4 key/value heads of 64 elements: 27 and 6. Below that by the way to the first positions: 500 positions of 16 heads of 128 elements 9.8 us in a graph.
 template <int DT, int D, int NST>
-__global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
+__device__ __forceinline__ void few_rows(const PagedParams &p, const int share_index, const int blocks) {
     constexpr int PITCH = D * 2, LK = D / 32, LPS = 2 * LK, VAT = GROUP * PITCH, STAGE = 2 * VAT, RING = NST * STAGE;
     constexpr int DK = D / 32, DT16 = D / 16, PW = D + 4, PIECES = D / 8;
     static_assert(NST >= 2 && (NST - 1) * LPS < 64, "the count in s_waitcnt");
@@ -223,7 +226,6 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
 
     // ---- this block's share
     int b, hkv, at, left;  // where it begins, inside an item's cost, and how much it has
-    const int share_index = blockIdx.x;
     auto costs = [&](const SeqRows &s) { return cost_of(p, s); };
     Lanes seqs = lanes_from(p, p.least == 0 ? share_index / p.Hkv & ~63 : 0);
     int first_pages = -1;  // of a whole item, asked for together with its length
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
         left = cost_of(p, pick(p, seqs, b));
         if (left == 0) return;
     } else {
-        const int all = sum_over(p, seqs, costs) * p.Hkv, share = share_of(p, all, gridDim.x);
+        const int all = sum_over(p, seqs, costs) * p.Hkv, share = share_of(p, all, blocks);
         const int64_t from = static_cast<int64_t>(share_index) * share;
         if (from >= all) return;
         left = min(share, all - static_cast<int>(from));
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
         const float *parts = reinterpret_cast<const float *>(smem);
         const bool whole = from_start && to_end;
         // the block's first piece, where it continues an item, has its even slot, one that goes on behind the block its odd slot
-        float *out_part = p.part + (static_cast<int64_t>(2 * share_index) + (from_start ? 1 : 0)) * FEW * PW;
+        float *out_part = p.few_part + (static_cast<int64_t>(2 * share_index) + (from_start ? 1 : 0)) * FEW * PW;
         for (int e = tid; e < rows * per_row; e += 256) {
             const int r = e / per_row, d4 = (e % per_row) * 4;
             float M = -INFINITY;
@@ -459,14 +461,19 @@ __global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
     }
 }
 
-// Joins the pieces of the items that paged_few_kernel's shares cut. D / 4 lanes hold a row; a block has as many such groups as there are threads for. Of an item in a few pieces each group
+template <int DT, int D, int NST>
+__global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
+    few_rows<DT, D, NST>(p, blockIdx.x, gridDim.x);
+}
+
+// Joins the pieces of the items that paged_few_kernel's shares cut (ys blocks an item). D / 4 lanes hold a row; a block has as many such groups as there are threads for. Of an item in a few pieces each group
 // takes a row; the pieces of a longer one (a single long sequence has one in every block: 64 of them, one after another, cost 13 us) are dealt out to the groups, row by row.
 template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int blocks) {
+__device__ __forceinline__ void few_merge(const PagedParams &p, const int blocks, const int item, const int y, const int ys) {
     constexpr int PW = D + 4, LANES = D / 4, TAKERS = 256 / LANES;
     __shared__ __align__(16) f32x4 sums[TAKERS][LANES];
     __shared__ float2 weights[TAKERS];
-    const int b = blockIdx.x / p.Hkv, hkv = blockIdx.x - b * p.Hkv;
+    const int b = item / p.Hkv, hkv = item - b * p.Hkv;
     Lanes seqs = lanes_from(p, 0);
     int before = 0, done = 0;
     SeqRows s{0, 0, 0};
@@ -486,7 +493,7 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int
     if (first == last) return;  // whole in one block, which has stored it
     const bool dealt = last - first >= TAKERS;
     const int taker = threadIdx.x / LANES, d4 = (threadIdx.x % LANES) * 4, at_once = dealt ? 1 : TAKERS;
-    for (int r0 = blockIdx.y * at_once; r0 < rows; r0 += gridDim.y * at_once) {
+    for (int r0 = y * at_once; r0 < rows; r0 += ys * at_once) {
         const int r = dealt ? r0 : r0 + taker, step = dealt ? TAKERS : 1;
         const bool mine = taker < TAKERS && r < rows;
         float M = -INFINITY, l = 0.f;
@@ -498,7 +505,7 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int i = min(i0 + j * step, last);  // the piece of block i: its odd slot where the item begins in it
-                    const float *piece = p.part + (static_cast<int64_t>(2 * i + (i == first ? 1 : 0)) * FEW + r) * PW;
+                    const float *piece = p.few_part + (static_cast<int64_t>(2 * i + (i == first ? 1 : 0)) * FEW + r) * PW;
                     ml[j] = *reinterpret_cast<const float2 *>(piece + D);
                     ov[j] = *reinterpret_cast<const f32x4 *>(piece + d4);
                 }
@@ -540,14 +547,18 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedParams p, int
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------------------------------------------
-// A block has 32 rows of one key/value head of one sequence for each of its 8 wavefronts (4 where heads have 256 elements); row = new row * G + query head, so that the heads of a group meet the
+// A block has 32 rows of one key/value head of one sequence for each of its 8 or 4 wavefronts (plan_of says which); row = new row * G + query head, so that the heads of a group meet the
 // same keys. It walks the positions in tiles of KT through NST stages in LDS, each wavefront loading 16 rows of K or V; one barrier a tile says that the tile is there
 // and that the stage before it is free.
 //   S^T = K Q^T   v_mfma_f32_32x32x16 with K rows as the first operand: a lane has, of ONE query row, 16 of 32 positions, and one exchange with lane ^ 32 finishes a row's maximum
 //   O^T += V^T P^T  the lane's probabilities are the second operand as they are (8 positions of each 16, in an order that the transposing read of V follows)
-// Blocks are given out with the last row tiles first; ranges of a tile whose positions were cut (range_tiles) leave (m, l, O) to paged_many_merge_kernel.
+// Blocks are given out with the last row tiles first; ranges of a tile whose positions were cut (range_tiles) leave (m, l, O) to many_merge.
+//
+// A tile of 256 rows and 64 positions reads 256 KiB of fragments from LDS and has 2048 cycles of matrix instructions (heads of 128 elements), and the two do not hide behind one another: 4096 new
+// rows of 32 heads on themselves take 152 - 165 us (830 - 900 TFLOP/s of what is not masked, the library's product of 8192^3 reaches 1340), 149 without a softmax and 138 without loads and barriers.
+// 500 rows on 30000 positions, 16 heads: 144 us (860 TFLOP/s) and 13 for the merge of 34 MB of partials.
 template <int DT, int D, int WAVES, int KT, int NST>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 64 && WAVES == 4 ? 3 : 2, D == 256 ? 1 : D == 64 && WAVES == 4 ? 3 : 2))) void paged_many_kernel(PagedParams p) {
+__device__ __forceinline__ void many_rows(const PagedParams &p, const int block) {
     constexpr int MANY = WAVES * 32, PITCH = D * 2, PIECES = D / 8, KTILE = KT * PITCH, STAGE = 2 * KTILE, PW = D + 4;
     constexpr int NL = D / 32, KK = D / 16, DT32 = D / 32, T32 = KT / 32;
     static_assert(WAVES / 2 == KT / GROUP, "a wavefront loads 16 rows of K or V");
@@ -557,7 +568,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(D ==
     const int l32 = lane & 31, h = lane >> 5;
 
     // ---- which rows: the last sequence's last tile first
-    const int hkv = blockIdx.x % p.Hkv, nth = blockIdx.x / p.Hkv;
+    const int hkv = block % p.Hkv, nth = block / p.Hkv;
     Lanes seqs = lanes_from(p, 0);
     const int range = range_tiles<MANY, KT>(p, seqs);
     auto pieces_in = [&](const SeqRows &s) {
@@ -803,7 +814,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(D ==
                     make_uint2(pack2_half<DT>(acc[dt][j] * inv, acc[dt][j + 1] * inv), pack2_half<DT>(acc[dt][j + 2] * inv, acc[dt][j + 3] * inv));
         return;
     }
-    float *pr = p.part + (slot * MANY + row - row0) * PW;
+    float *pr = p.many_part + (slot * MANY + row - row0) * PW;
 #pragma unroll
     for (int dt = 0; dt < DT32; ++dt)
 #pragma unroll
@@ -811,11 +822,27 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(D ==
     if (h == 0) *reinterpret_cast<float2 *>(pr + D) = make_float2(m_run, l_run);
 }
 
-// Joins the ranges of paged_many_kernel's row tiles that were cut: gridDim.y blocks a row tile.
+constexpr int many_waves_per_eu(int D, int WAVES) { return D == 256 ? 1 : D == 64 && WAVES == 4 ? 3 : 2; }
+constexpr int MANY_STAGES = 4, FEW_STAGES = 2;  // more stages of few rows are no faster: a block starts later with more LDS
 template <int DT, int D, int WAVES, int KT>
-__global__ __launch_bounds__(256) void paged_many_merge_kernel(PagedParams p) {
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(many_waves_per_eu(D, WAVES), many_waves_per_eu(D, WAVES)))) void paged_many_kernel(PagedParams p) {
+    many_rows<DT, D, WAVES, KT, MANY_STAGES>(p, blockIdx.x);
+}
+// Both kinds of sequences in one launch: blocks that read run beside blocks that multiply, and in the places of those that have ended. The first `many` blocks are row tiles, which are the longer
+// ones. 18 sequences with a row each and 6 with 85 to 293, up to 5800 positions, 32 heads on 8 of 128: 75 us with the merge, as two launches and two merges one after another 103; with the few rows' blocks
+// first 93, with the kinds alternating 109.
+template <int DT, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(many_waves_per_eu(D, 4), many_waves_per_eu(D, 4)))) void paged_both_kernel(PagedParams p, int many) {
+    const int block = blockIdx.x;
+    if (block < many) many_rows<DT, D, 4, 32, MANY_STAGES>(p, block);
+    else few_rows<DT, D, FEW_STAGES>(p, block - many, gridDim.x - many);
+}
+
+// Joins the ranges of paged_many_kernel's row tiles that were cut: ys blocks a row tile.
+template <int DT, int D, int WAVES, int KT>
+__device__ __forceinline__ void many_merge(const PagedParams &p, const int block, const int y, const int ys) {
     constexpr int MANY = WAVES * 32, PW = D + 4, per_row = D / 4;
-    const int hkv = blockIdx.x % p.Hkv, nth = blockIdx.x / p.Hkv;
+    const int hkv = block % p.Hkv, nth = block / p.Hkv;
     Lanes seqs = lanes_from(p, 0);
     const int range = range_tiles<MANY, KT>(p, seqs);
     auto cut_tiles = [&](const SeqRows &s) {
@@ -840,8 +867,8 @@ __global__ __launch_bounds__(256) void paged_many_merge_kernel(PagedParams p) {
     slots = __builtin_amdgcn_readlane(sums_to_lane(slots), 63);
     const int rows = min(s.count * p.G - tile * MANY, MANY);
     const int64_t pitch = static_cast<int64_t>(p.Hkv) * MANY * PW;
-    const float *base = p.part + ((static_cast<int64_t>(slots) + static_cast<int64_t>(tile) * cut) * p.Hkv + hkv) * MANY * PW;
-    for (int e = blockIdx.y * 256 + threadIdx.x; e < rows * per_row; e += gridDim.y * 256) {
+    const float *base = p.many_part + ((static_cast<int64_t>(slots) + static_cast<int64_t>(tile) * cut) * p.Hkv + hkv) * MANY * PW;
+    for (int e = y * 256 + threadIdx.x; e < rows * per_row; e += ys * 256) {
         const int r = e / per_row, d4 = (e % per_row) * 4;
         const float *pr = base + r * PW;
         float M = -INFINITY, l = 0.f;
@@ -872,6 +899,15 @@ __global__ __launch_bounds__(256) void paged_many_merge_kernel(PagedParams p) {
     }
 }
 
+// The first WAVES * many blocks join row tiles, WAVES of them each, the others items of few rows, as many of them each as there are. Blocks of a tile lie `many` apart: with key/value heads a multiple
+// of the 8 XCDs a tile is joined on the one that left its ranges (16 heads, 512 rows: 20.1 us with paged_many_kernel, 25.7 with a tile's blocks side by side).
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p, int many, int few_blocks, int few_y) {
+    const int block = blockIdx.x, few = block - WAVES * many, items = p.pages.seqs * p.Hkv;
+    if (few < 0) many_merge<DT, D, WAVES, WAVES * 8>(p, block % many, block / many, WAVES);
+    else few_merge<DT, D>(p, few_blocks, few % items, few / items, few_y);
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------------------------------------------------
 // How a call is laid out, from what the host knows: the number of rows and sequences, and bounds of their new rows and lengths.
 struct Plan {
@@ -881,7 +917,7 @@ struct Plan {
     int waves;              // paged_many_kernel: wavefronts of a block
     int64_t tiles;          // row tiles of a key/value head, at most
     int spread;
-    uint64_t bytes;         // of partials
+    uint64_t bytes, many_bytes;  // of partials: all, and paged_many_kernel's, which come first
 };
 
 Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, bool packed, bool counted, int64_t max_new, int64_t max_length, int64_t room, int cus) {
@@ -893,7 +929,8 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
     if (p.few) {
         const int64_t items = seqs * Hkv;
         const int per_cu = D <= 64 ? 4 : D <= 96 ? 3 : D <= 128 ? 2 : 1;  // blocks that a CU holds (registers; 64 KiB of LDS a block of heads of 128)
-        // Whole items take their block about 0.43 us a unit (heads of 64) or 0.6 us, cut ones the second launch.
+        // Whole items take their block about 0.43 us a unit (heads of 64) or 0.6 us, cut ones the second launch (heads of 128, 16 of them, whole and cut: 500 positions 9.8 and 11.5 us, 2000
+        // 24 and 12.7; 64 sequences of 81 to 7113, 64 heads on 4 of 64: 65 and 31).
         const bool cut = max_length * (D <= 64 ? 43 : 60) > 64 * 700;
         if (cut && items * (room / UNIT + 1 + START) < (1ll << 31)) {  // costs are counted in 32 bits
             p.few_blocks = per_cu * cus;
@@ -906,7 +943,8 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
         }
     }
     if (p.many) {
-        // Blocks of 8 wavefronts load keys and values half as often, blocks of 4, two to a CU, leave less of the device idle at the end of a batch and have shorter tiles.
+        // Blocks of 8 wavefronts load keys and values half as often, blocks of 4, two to a CU, leave less of the device idle at the end of a batch and have shorter tiles. With 4 and 8, heads of
+        // 128: 4096 rows 164 and 154 us, 500 on 30000 203 and 151, 8 x 1024 (32 heads on 8) 120 and 131, 3 x 701 32 and 45; of 64: 4096 rows 103 and 114.
         // tiles of 256 rows and 64 positions for a CU; of sequences that may differ, half of what the bounds allow
         const double per_cu = static_cast<double>(rows) * Hq * (max_length - most / 2) / (256.0 * 64.0) / cus * (packed || counted ? 0.5 : 1.0);
         const bool enough = rows * G / 256 * Hkv >= cus;  // row tiles of 256, none of which need be cut
@@ -917,60 +955,66 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
         // more). A few tiles of positions are not cut either.
         if (!(seqs == 1 && p.tiles * Hkv >= 2ll * cus) && max_length > LEAST_TILES * p.waves * 8) {
             p.spread = cus;
-            const uint64_t more = static_cast<uint64_t>(2) * p.spread * MANY * (D + 4) * sizeof(float);
-            if (more > p.bytes) p.bytes = more;
+            p.many_bytes = static_cast<uint64_t>(2) * p.spread * MANY * (D + 4) * sizeof(float);
+            p.bytes += p.many_bytes;
         }
     }
     return p;
 }
 
-template <int DT, int D>
-int launch(const PagedParams &base, const Plan &plan, hipStream_t s) {
-    PagedParams p = base;
+template <auto KERNEL>
+struct Kernel {
+    static constexpr auto at = KERNEL;
+};
+
+template <int DT, int D, int WAVES>
+int launch(PagedParams p, const Plan &plan, hipStream_t s) {
+    constexpr int KT = WAVES * 8, MANY_LDS = MANY_STAGES * 2 * KT * D * 2, FEW_LDS = 4 * FEW_STAGES * 2 * GROUP * D * 2;
+    static_assert(WAVES != 4 || MANY_LDS == FEW_LDS, "one launch of both");
     int dev = 0;
     TPAMD_HIP(hipGetDevice(&dev));
-    if (plan.many) {
-        p.spread = plan.spread;
-        auto run = [&](auto waves) -> int {
-            constexpr int WAVES = decltype(waves)::value, KT = WAVES * 8, NST = 4, LDS = NST * 2 * KT * D * 2;
-            static thread_local int configured = -1;
-            if (configured != dev) {
-                TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DT, D, WAVES, KT, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-                configured = dev;
-            }
-            const int64_t tiles = plan.tiles * p.Hkv, blocks = tiles + plan.spread;
-            TPAMD_REQUIRE(blocks < (1ll << 22), "tpamd_attention_paged: too many rows for one launch");
-            hipLaunchKernelGGL((paged_many_kernel<DT, D, WAVES, KT, NST>), dim3(static_cast<unsigned>((blocks + p.Hkv - 1) / p.Hkv * p.Hkv)), dim3(WAVES * 64), LDS, s, p);
-            TPAMD_HIP(hipGetLastError());
-            if (plan.spread > 0) {
-                // (a cut tile has two ranges and more, fewer than 2 spread in all)
-                const int64_t cut = tiles < plan.spread ? tiles : plan.spread;
-                hipLaunchKernelGGL((paged_many_merge_kernel<DT, D, WAVES, KT>), dim3(static_cast<unsigned>((cut + p.Hkv - 1) / p.Hkv * p.Hkv), WAVES), dim3(256), 0, s, p);
-                TPAMD_HIP(hipGetLastError());
-            }
-            return TPAMD_OK;
-        };
-        int rc;
-        if constexpr (D == 256) rc = run(std::integral_constant<int, 4>{});  // (two wavefronts of a SIMD do not have the registers)
-        else rc = plan.waves == 8 ? run(std::integral_constant<int, 8>{}) : run(std::integral_constant<int, 4>{});
-        if (rc != TPAMD_OK) return rc;
-    }
-    if (plan.few) {  // behind the other: their partials share the memory
-        p.least = plan.least;
-        constexpr int NST = 2, LDS = 4 * NST * 2 * GROUP * D * 2;  // more stages are no faster: a block starts later with more LDS
-        static thread_local int configured = -1;
+    p.spread = plan.spread;
+    p.least = plan.least;
+    const int64_t tiles = plan.many ? plan.tiles * p.Hkv : 0;
+    // (a cut tile has two ranges and more, fewer than 2 spread in all)
+    const int64_t cut = tiles < plan.spread ? tiles : plan.spread;
+    const int64_t joins = (cut + p.Hkv - 1) / p.Hkv * p.Hkv, few_joins = plan.least > 0 ? static_cast<int64_t>(p.pages.seqs) * p.Hkv * plan.merge_y : 0;
+    TPAMD_REQUIRE(tiles + plan.spread < (1ll << 22) && tiles + plan.spread + p.Hkv + (plan.few ? plan.few_blocks : 0) < (1ll << 24) && WAVES * joins + few_joins < (1ll << 24),
+                  "tpamd_attention_paged: too many rows or sequences for one launch");
+    const unsigned many = static_cast<unsigned>(plan.many ? (tiles + plan.spread + p.Hkv - 1) / p.Hkv * p.Hkv : 0), few = static_cast<unsigned>(plan.few ? plan.few_blocks : 0);
+    auto run = [&](auto kernel, unsigned blocks, int threads, int lds, auto... more) -> int {
+        static thread_local int configured = -1;  // (one for each kernel and its call)
         if (configured != dev) {
-            TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_few_kernel<DT, D, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+            TPAMD_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(decltype(kernel)::at), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
             configured = dev;
         }
-        hipLaunchKernelGGL((paged_few_kernel<DT, D, NST>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(256), LDS, s, p);
+        hipLaunchKernelGGL(decltype(kernel)::at, dim3(blocks), dim3(threads), lds, s, p, more...);
         TPAMD_HIP(hipGetLastError());
-        if (plan.least > 0) {
-            hipLaunchKernelGGL((paged_few_merge_kernel<DT, D>), dim3(static_cast<unsigned>(p.pages.seqs * p.Hkv), plan.merge_y), dim3(256), 0, s, p, plan.few_blocks);
-            TPAMD_HIP(hipGetLastError());
+        return TPAMD_OK;
+    };
+    if (WAVES == 4 && many > 0 && few > 0) {
+        if (int rc = run(Kernel<paged_both_kernel<DT, D>>{}, many + few, 256, FEW_LDS, static_cast<int>(many)); rc != TPAMD_OK) return rc;
+    } else {
+        if (many > 0) {
+            if (int rc = run(Kernel<paged_many_kernel<DT, D, WAVES, KT>>{}, many, WAVES * 64, MANY_LDS); rc != TPAMD_OK) return rc;
+        }
+        if (few > 0) {
+            if (int rc = run(Kernel<paged_few_kernel<DT, D, FEW_STAGES>>{}, few, 256, FEW_LDS); rc != TPAMD_OK) return rc;
         }
     }
+    if (joins + few_joins > 0) {
+        hipLaunchKernelGGL((paged_merge_kernel<DT, D, WAVES>), dim3(static_cast<unsigned>(WAVES * joins + few_joins)), dim3(256), 0, s, p, static_cast<int>(joins), plan.few_blocks, plan.merge_y);
+        TPAMD_HIP(hipGetLastError());
+    }
     return TPAMD_OK;
+}
+
+template <int DT, int D>
+int launch(const PagedParams &p, const Plan &plan, hipStream_t s) {
+    if constexpr (D != 256) {  // (two wavefronts of a SIMD do not have the registers)
+        if (plan.waves == 8) return launch<DT, D, 8>(p, plan, s);
+    }
+    return launch<DT, D, 4>(p, plan, s);
 }
 
 }  // namespace
@@ -1058,7 +1102,8 @@ extern "C" int tpamd_attention_paged(const void *q_dev, int64_t q_row, int64_t q
     p.q = static_cast<const char *>(q_dev);
     p.o = static_cast<char *>(out_dev);
     p.q_row = q_row; p.q_head = q_head; p.o_row = o_row; p.o_head = o_head;
-    p.part = static_cast<float *>(workspace_dev);
+    p.many_part = static_cast<float *>(workspace_dev);
+    p.few_part = p.many_part + plan.many_bytes / sizeof(float);
     p.scale_log2 = scale * 1.4426950408889634f;
     p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv); p.D = static_cast<int>(D);
     p.few = plan.few; p.many = plan.many;
