@@ -209,11 +209,11 @@ __device__ __forceinline__ int share_of(const PagedParams &p, int cost, int bloc
 // leave (m, l, O) as partials, and few_merge joins them. A block has at most two such pieces (its first and its last), so the partials' memory does not
 // grow with the batch. `least` == 0: a block takes an item whole and nothing is merged.
 //
-// Inside a block the four wavefronts take every fourth 16 positions through LDS stages of their own and meet at the end of an item.
+// Inside a block each of the 4 wavefronts (8: plan_of) takes every fourth 16 positions through LDS stages of their own and meet at the end of an item.
 //
 // Bound by HBM where there is enough to read: 100000 positions of 8 key/value heads of 128 elements 76 us and their merge 5 (410 MB, 5.0 TB/s of the whole call); 64 sequences of 81 to
-// 7113 positions, 4 key/value heads of 64 elements: 27 and 6. Below that by the way to the first positions: 500 positions of 16 heads of 128 elements 9.8 us in a graph.
-template <int DT, int D, int NST>
+// 7113 positions, 4 key/value heads of 64 elements: 27 and 6. Below that by the way to the first positions: 500 positions of 16 heads of 128 elements 8.9 us in a graph.
+template <int DT, int D, int WAVES, int NST>
 __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_index, const int blocks) {
     constexpr int PITCH = D * 2, LK = D / 32, LPS = 2 * LK, VAT = GROUP * PITCH, STAGE = 2 * VAT, RING = NST * STAGE;
     constexpr int DK = D / 32, DT16 = D / 16, PW = D + 4, PIECES = D / 8;
@@ -233,7 +233,7 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
         b = share_index / p.Hkv;
         hkv = share_index - b * p.Hkv;
         at = 0;
-        const int position = (wave + 4 * lane) * GROUP;
+        const int position = (wave + WAVES * lane) * GROUP;
         if (position < p.pages.room) first_pages = page_of(p.pages, b, position);
         left = cost_of(p, pick(p, seqs, b));
         if (left == 0) return;
@@ -282,7 +282,7 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
         const bool from_start = unit == 0, to_end = unit_end == n_units;
         const int rows = s.count * p.G;
         const int groups = k_end > k_begin ? (k_end - k_begin + GROUP - 1) / GROUP : 0;
-        const int n = (groups - wave + 3) / 4;  // of this wavefront: wave, wave + 4, ...
+        const int n = (groups - wave + WAVES - 1) / WAVES;  // of this wavefront: wave, wave + WAVES, ...
 
         // ---- this lane's row (those past the last: row 0, never stored)
         const int row = l16 < rows ? l16 : 0, place = row / p.G;
@@ -302,7 +302,7 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
             const int64_t k_at = item * p.pages.k_head, v_at = item * p.pages.v_head;
             // the pages of this wavefront's next 64 groups, one in a lane
             auto pages_from = [&](int i) {
-                const int g = group0 + 4 * (i + lane);
+                const int g = group0 + WAVES * (i + lane);
                 return g * GROUP < s.length ? page_of(p.pages, seq, g * GROUP) : -1;
             };
             int my_page = p.least == 0 ? first_pages : pages_from(0), base = 0;
@@ -315,7 +315,7 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
                         arrived(my_page);
                     }
                     const int page = __builtin_amdgcn_readlane(my_page, i - base);
-                    const int slot = ((group0 + 4 * i) * GROUP) & ((1 << p.pages.shift) - 1);
+                    const int slot = ((group0 + WAVES * i) * GROUP) & ((1 << p.pages.shift) - 1);
                     const __amdgpu_buffer_rsrc_t kr = group_rsrc(p.pages.k, page, p.pages.k_page, k_at, slot, p.pages.k_pos, D);
                     const __amdgpu_buffer_rsrc_t vr = group_rsrc(p.pages.v, page, p.pages.v_page, v_at, slot, p.pages.v_pos, D);
 #pragma unroll
@@ -352,7 +352,7 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
                 f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < DK; ++kk) sc = mfma16<DT>(kf[kk], qf[kk], sc);
-                const int k0 = (group0 + 4 * i) * GROUP;
+                const int k0 = (group0 + WAVES * i) * GROUP;
                 const bool partly = k0 + GROUP - 1 > seen_by_all;  // some row does not see all of them
                 if (partly) {
                     // the values behind the sequence's end are whatever the page held
@@ -417,7 +417,7 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
         }
         l_run += __shfl_xor(l_run, 16);
         l_run += __shfl_xor(l_run, 32);
-        // ---- the four wavefronts' results meet in the place of the stages, once every load into them has landed
+        // ---- the wavefronts' results meet in the place of the stages, once every load into them has landed
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         float *mine = reinterpret_cast<float *>(smem) + (wave * FEW + l16) * PW;
@@ -432,15 +432,15 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
         const bool whole = from_start && to_end;
         // the block's first piece, where it continues an item, has its even slot, one that goes on behind the block its odd slot
         float *out_part = p.few_part + (static_cast<int64_t>(2 * share_index) + (from_start ? 1 : 0)) * FEW * PW;
-        for (int e = tid; e < rows * per_row; e += 256) {
+        for (int e = tid; e < rows * per_row; e += WAVES * 64) {
             const int r = e / per_row, d4 = (e % per_row) * 4;
             float M = -INFINITY;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) M = fmaxf(M, parts[(v * FEW + r) * PW + D]);
+            for (int v = 0; v < WAVES; ++v) M = fmaxf(M, parts[(v * FEW + r) * PW + D]);
             const float m_use = M == -INFINITY ? 0.f : M;
             float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int v = 0; v < WAVES; ++v) {
                 const float weight = exp2f(parts[(v * FEW + r) * PW + D] - m_use);
                 const f32x4 ov = *reinterpret_cast<const f32x4 *>(parts + (v * FEW + r) * PW + d4);
                 l += weight * parts[(v * FEW + r) * PW + D + 1];
@@ -461,9 +461,9 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
     }
 }
 
-template <int DT, int D, int NST>
-__global__ __launch_bounds__(256) void paged_few_kernel(PagedParams p) {
-    few_rows<DT, D, NST>(p, blockIdx.x, gridDim.x);
+template <int DT, int D, int WAVES, int NST>
+__global__ __launch_bounds__(WAVES * 64) void paged_few_kernel(PagedParams p) {
+    few_rows<DT, D, WAVES, NST>(p, blockIdx.x, gridDim.x);
 }
 
 // Joins the pieces of the items that paged_few_kernel's shares cut (ys blocks an item). D / 4 lanes hold a row; a block has as many such groups as there are threads for. Of an item in a few pieces each group
@@ -835,7 +835,7 @@ template <int DT, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(many_waves_per_eu(D, 4), many_waves_per_eu(D, 4)))) void paged_both_kernel(PagedParams p, int many) {
     const int block = blockIdx.x;
     if (block < many) many_rows<DT, D, 4, 32, MANY_STAGES>(p, block);
-    else few_rows<DT, D, FEW_STAGES>(p, block - many, gridDim.x - many);
+    else few_rows<DT, D, 4, FEW_STAGES>(p, block - many, gridDim.x - many);
 }
 
 // Joins the ranges of paged_many_kernel's row tiles that were cut: ys blocks a row tile.
@@ -913,6 +913,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p, int man
 struct Plan {
     bool few, many;
     int few_blocks, least;  // paged_few_kernel: blocks, and the least share of one (0: a block an item)
+    int few_waves;          // wavefronts of its blocks
     int merge_y;            // blocks of an item in its merge
     int waves;              // paged_many_kernel: wavefronts of a block
     int64_t tiles;          // row tiles of a key/value head, at most
@@ -928,10 +929,14 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
     p.many = most * G > FEW;
     if (p.few) {
         const int64_t items = seqs * Hkv;
+        p.few_waves = 4;
         const int per_cu = D <= 64 ? 4 : D <= 96 ? 3 : D <= 128 ? 2 : 1;  // blocks that a CU holds (registers; 64 KiB of LDS a block of heads of 128)
-        // Whole items take their block about 0.43 us a unit (heads of 64) or 0.6 us, cut ones the second launch (heads of 128, 16 of them, whole and cut: 500 positions 9.8 and 11.5 us, 2000
-        // 24 and 12.7; 64 sequences of 81 to 7113, 64 heads on 4 of 64: 65 and 31).
-        const bool cut = max_length * (D <= 64 ? 43 : 60) > 64 * 700;
+        // Where every whole item has a CU to itself its block has 8 wavefronts: 500 positions of 16 heads of 128 take 8.9 us, with 4 wavefronts 10.0; 700 9.7 and 12.0; of 4 heads of 64 6.8 and 7.8.
+        // Not for up to 4 units (128 positions 6.3 and 5.8), nor for items on most CUs (192: 500 12.7 and 12.4), nor beside row tiles, whose blocks have 4.
+        const bool wide = items <= cus / 2 && D <= 128 && !p.many;
+        // A whole item takes a time that grows with its units (a hundredth of a us each, at 4 wavefronts and 8), cut ones the second launch. Whole with 4, with 8 and cut, us: one sequence, 16 heads
+        // of 128: 500 10.0, 8.8, 11.6; 1000 15.3, 12.5, 12.0; 2000 25.4, 21.4, 13.1. 4 heads of 64: 1000 11.9, 8.8, 10.1; 2000 19.5, 12.4, 11.3.
+        const bool cut = max_length * (wide ? (D <= 64 ? 28 : 48) : (D <= 64 ? 43 : 60)) > 64 * 700;
         if (cut && items * (room / UNIT + 1 + START) < (1ll << 31)) {  // costs are counted in 32 bits
             p.few_blocks = per_cu * cus;
             p.least = START + 2;
@@ -940,6 +945,7 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
             p.merge_y = items * few_rows <= 2ll * cus ? few_rows : (few_rows + at_once - 1) / at_once;
         } else {
             p.few_blocks = static_cast<int>(items);
+            p.few_waves = wide && max_length > 4 * UNIT ? 8 : 4;
         }
     }
     if (p.many) {
@@ -999,7 +1005,10 @@ int launch(PagedParams p, const Plan &plan, hipStream_t s) {
             if (int rc = run(Kernel<paged_many_kernel<DT, D, WAVES, KT>>{}, many, WAVES * 64, MANY_LDS); rc != TPAMD_OK) return rc;
         }
         if (few > 0) {
-            if (int rc = run(Kernel<paged_few_kernel<DT, D, FEW_STAGES>>{}, few, 256, FEW_LDS); rc != TPAMD_OK) return rc;
+            int rc;
+            if constexpr (D <= 128) rc = plan.few_waves == 8 ? run(Kernel<paged_few_kernel<DT, D, 8, FEW_STAGES>>{}, few, 512, 2 * FEW_LDS) : run(Kernel<paged_few_kernel<DT, D, 4, FEW_STAGES>>{}, few, 256, FEW_LDS);
+            else rc = run(Kernel<paged_few_kernel<DT, D, 4, FEW_STAGES>>{}, few, 256, FEW_LDS);
+            if (rc != TPAMD_OK) return rc;
         }
     }
     if (joins + few_joins > 0) {

@@ -285,6 +285,21 @@ def test_bounds_change_nothing_but_the_time(counts, lengths, Hq, Hkv, D, page, m
     check_attend(Batch(counts, lengths, Hq, Hkv, D, page, BF16, seed=16, behind=2), max_length=max_length, max_new=max(counts))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("counts,lengths,max_length", [([1], [257], 257), ([1, 3, 2, 0], [260, 700, 13, 9], 700), ([4, 2, 1], [4, 2, 600], 700), ([1], [5], 500), ([3, 1], [1, 0], 300)])
+def test_short_steps_in_wide_blocks(dtype, D, counts, lengths, max_length):
+    """Few items of a few hundred positions: wavefronts without any, and those whose last positions some rows do not see."""
+    check_attend(Batch(counts, lengths, 4, 2, D, 16, dtype, seed=17, behind=1), max_length=max_length, max_new=max(counts))
+    batch = Batch(counts, lengths, 4, 2, D, 16, dtype, seed=18, spread=0.0)
+    b = max(range(len(lengths)), key=lambda i: lengths[i])
+    for back, column, value in ((0, 3, math.inf), (1, 5, math.nan), (2, 7, -math.inf)):
+        j = lengths[b] - 1 - back
+        if j >= 0:
+            batch.v[batch.table[b][j // 16], :, j % 16, column] = value
+    check_attend(batch, max_length=max_length, max_new=max(counts))
+
+
 def test_pages_that_the_pool_does_not_have_hold_zeros():
     for counts, lengths in (([1, 2], [100, 90]), ([40, 1], [100, 90])):
         batch = Batch(counts, lengths, 4, 2, 64, 16, F16, seed=13)
