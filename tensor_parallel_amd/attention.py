@@ -66,7 +66,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor] =
 
     q_norm, k_norm [D]: each head is x * rsqrt(mean(x^2) + eps) * weight first, in the same pass. All of it in fp32, rounded once. Inference only: a backward pass raises."""
     q_out, k_out = _native.rotate_heads(q, k, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps)
-    return (_guard(q_out, q, q_norm), _guard(k_out, k, k_norm)) if torch.is_grad_enabled() else (q_out, k_out)
+    return (_guard(q_out, q, q_norm, inv_freq, cos, sin), _guard(k_out, k, k_norm, inv_freq, cos, sin)) if torch.is_grad_enabled() else (q_out, k_out)
 
 
 # What the mask kernel stands in for: the names that `sdpa_mask` and the causal rule look up, their arguments and locals.

@@ -40,18 +40,19 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
     """The new rows q [..., Hq, D] (or [..., Hkv, Hq / Hkv, D]), k and v [..., Hkv, D], views of projection outputs: k and v go to their positions' pages, k and q rotated as
     `attention.rotate` does (frequencies or tables; neither: as they are). A row is rotated to its place in its sequence, or to `positions` [...]. Returns q as [..., Hq, D]; rows of no
     sequence are left as the memory was."""
-    return _guard(_native.append_paged(q, k, v, k_pages, v_pages, table, lengths, starts, counts, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps), q, k, v)
+    return _guard(_native.append_paged(q, k, v, k_pages, v_pages, table, lengths, starts, counts, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps), q, k, v,
+                  q_norm, k_norm, inv_freq, cos, sin)
 
 
 def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, starts: Optional[torch.Tensor] = None,
            counts: Optional[torch.Tensor] = None, scale: Optional[float] = None, max_new: Optional[int] = None, max_length: Optional[int] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of the new rows q [..., Hq, D] on their sequences' pages (which hold the new rows' keys and values already): [..., Hq, D], `out` if it is given. Hq a multiple of
-    Hkv, D 64, 96, 128 or 256; scale D ** -0.5 by default. Rows of no sequence are left as the memory was, a row in front of position 0 (more new rows than positions) is zeros.
+    Hkv, D 64, 96, 128 or 256, rows of q and of the pools on 16-byte boundaries (others are refused); scale D ** -0.5 by default. Rows of no sequence are left as the memory was, a row in front of position 0 (more new rows than positions) is zeros.
 
     max_new: no sequence has more new rows (rows of one that does may be left out); tell it where it is known, a step of single rows is then one or two launches. max_length: no sequence
     has more positions; only the time depends on it. Both have to hold for every replay where the call is captured."""
-    return _guard(_native.attention_paged(q, k_pages, v_pages, table, lengths, starts, counts, scale, max_new, max_length, out), q)
+    return _guard(_native.attention_paged(q, k_pages, v_pages, table, lengths, starts, counts, scale, max_new, max_length, out), q, k_pages, v_pages)
 
 
 class _Book:

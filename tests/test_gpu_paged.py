@@ -523,6 +523,28 @@ def test_no_backward():
             out.float().sum().backward()
 
 
+def test_no_backward_to_norms_tables_and_pools():
+    """What is learned beside q, k and v gets no gradient in silence either."""
+    batch = Batch([1, 2], [20, 9], 2, 2, 64, 16, F16, seed=33)
+    d, q = batch.on(), batch.q.to(DEV)
+    positions = torch.arange(batch.rows, device=DEV)
+
+    def learned(*shape, dtype=F16):
+        return torch.ones(*shape, dtype=dtype, device=DEV, requires_grad=True)
+
+    calls = [lambda: paged.append(q, q, q, **d, q_norm=learned(64)), lambda: paged.append(q, q, q, **d, k_norm=learned(64)), lambda: paged.append(q, q, q, **d, inv_freq=learned(32, dtype=torch.float32)),
+             lambda: paged.append(q, q, q, **d, cos=learned(batch.rows, 32), sin=learned(batch.rows, 32)), lambda: paged.attend(q, **{**d, "k_pages": d["k_pages"].clone().requires_grad_()}),
+             lambda: paged.attend(q, **{**d, "v_pages": d["v_pages"].clone().requires_grad_()}), lambda: attention.rotate(q, q, positions, inv_freq=learned(32, dtype=torch.float32))[0],
+             lambda: attention.rotate(q, q, positions, inv_freq=learned(32, dtype=torch.float32))[1], lambda: attention.rotate(q, q, cos=learned(batch.rows, 32), sin=learned(batch.rows, 32))[1]]
+    for call in calls:
+        out = call()
+        assert out.requires_grad
+        with pytest.raises(NotImplementedError, match="backward"):
+            out.float().sum().backward()
+        with torch.no_grad():
+            assert not call().requires_grad
+
+
 def test_short_of_workspace_is_refused():
     batch = Batch([1], [20000], 2, 2, 64, 16, F16, seed=32)
     d, q = batch.on(), batch.q.to(DEV)
