@@ -185,7 +185,7 @@ __device__ __forceinline__ int find_in(const PagedParams &p, Lanes &l, int at, i
 // The positions of a sequence's row tiles are cut into ranges where the tiles have more of them than an equal share of all work (in tiles of KT positions) on `spread` blocks, so that a few long
 // sequences in a batch do not keep a few blocks busy when all others have ended. Sums of whole numbers in 64 bits: exact. With R the share there are at most sum(1 + work / R) = row tiles +
 // spread ranges, and fewer than 2 spread of tiles that are cut.
-constexpr int LEAST_TILES = 4;
+constexpr int LEAST_TILES = 4;  // of a range: with 8 512 rows of 16 heads of 128 take 22.7 us instead of 20.7, 32 rows on 500 14.4 instead of 13.2
 template <int ROWS, int KT>
 __device__ __forceinline__ int range_tiles(const PagedParams &p, const Lanes &l) {
     if (p.spread == 0) return 0;
@@ -957,9 +957,11 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
         p.waves = D == 256 || per_cu < 40 || (D == 64 && enough) ? 4 : 8;
         const int64_t MANY = p.waves * 32;
         p.tiles = packed ? rows * G / MANY + seqs : seqs * ((each * G + MANY - 1) / MANY);
-        // Of a single sequence with two row tiles and more for a CU nothing is cut, and there is no merge: a share is at least as long as its last tile (the average one has half of that or
-        // more). A few tiles of positions are not cut either.
-        if (!(seqs == 1 && p.tiles * Hkv >= 2ll * cus) && max_length > LEAST_TILES * p.waves * 8) {
+        // Nothing is cut, and there is no merge, of a single sequence with two row tiles and more for a CU (a share is at least as long as its last tile: the average one has half of that or more), of
+        // sequences with a row tile for each CU that differ in length by twice at most (uncut and cut, us: 3 x 701 rows of 16 heads of 128 26.6 and 29.8, 8 x 1024 of 32 on 8 111 and 115, of 64 71
+        // and 77), and of few tiles of positions (250 rows 14.7 and 18.5, 8 x 256 21.3 and 24.7; 512 rows 21.0 and 20.7).
+        const bool alike = !packed && !counted && max_length <= 2 * each && p.tiles * Hkv >= cus;
+        if (!alike && !(seqs == 1 && p.tiles * Hkv >= 2ll * cus) && max_length > 2 * LEAST_TILES * p.waves * 8) {
             p.spread = cus;
             p.many_bytes = static_cast<uint64_t>(2) * p.spread * MANY * (D + 4) * sizeof(float);
             p.bytes += p.many_bytes;
