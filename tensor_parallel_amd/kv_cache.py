@@ -36,7 +36,12 @@ def rank_caches(cache: Any, world_size: int) -> List[Any]:
         raise NotImplementedError(
             "a cache that already holds keys and values for all heads cannot be handed to rank shards; start from an empty cache"
         )
-    siblings = [copy.deepcopy(cache) for _ in range(world_size - 1)]
+    make = getattr(cache, "rank_sibling", None)  # (a cache whose copies are caches of their own says itself what another rank's is)
+    return [cache] + link(cache, [make() if make is not None else copy.deepcopy(cache) for _ in range(world_size - 1)])
+
+
+def link(cache: Any, siblings: List[Any]) -> List[Any]:
+    """Makes these the caches of the other ranks: batch-level operations on `cache` are repeated on them."""
     for name in _BATCH_LEVEL:
         original = getattr(cache, name, None)
         if original is None:
@@ -50,4 +55,4 @@ def rank_caches(cache: Any, world_size: int) -> List[Any]:
 
         setattr(cache, name, functools.wraps(original)(both))
     cache.__dict__["_tp_rank_siblings"] = siblings
-    return [cache] + siblings
+    return siblings

@@ -29,7 +29,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
-from . import _native
+from . import _native, kv_cache
 from .shard_modules import _guard
 
 
@@ -72,6 +72,14 @@ class _Book:
         self.counts = [0] * self.sequences  # the step's rows
         self.number, self.taken, self.hold = 0, True, False  # of the step (0: none yet); whether a forward has begun it; whether further forwards are the same step
         self.uploaded.clear()
+
+    def __deepcopy__(self, memo) -> "_Book":
+        with self.lock:
+            other = _Book(self.sequences, self.pages, self.page, self.columns)
+            for name, value in self.__dict__.items():
+                if name not in ("states", "uploaded", "lock"):  # (what a device was told is told anew)
+                    setattr(other, name, copy.deepcopy(value, memo))
+        return other
 
     def after(self) -> List[int]:
         return [n + c for n, c in zip(self.before, self.counts)]
@@ -137,6 +145,8 @@ class PagedCache:
         positions = cache.prepare([1] * 3, hold=True)                     # every further token, the first of them with the step's own
         logits = step(input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True).logits
 
+    `copy.deepcopy(cache)` is a cache of its own, with the same sequences in pages of its own; a shallow copy is refused.
+
     One caller at a time (the ranks of its forward may be threads); beam search (which would have sequences share pages) is not supported."""
 
     is_compileable = False
@@ -151,12 +161,31 @@ class PagedCache:
         self._pools: dict = {}          # layer -> (keys, values)
         self._number, self._seen = -1, set()  # the step that this rank's forward is in, and its layers that have been there
 
-    def __deepcopy__(self, memo) -> "PagedCache":
+    def rank_sibling(self) -> "PagedCache":
         """Another rank's cache: pools of its own, the same sequences (kv_cache.rank_caches)."""
-        other = copy.copy(self)
-        other.__dict__ = {"_book": self._book}
+        return self._with(self._book)
+
+    def _with(self, book: _Book) -> "PagedCache":
+        other = type(self).__new__(type(self))
+        other._book = book
         other._own()
         return other
+
+    def __deepcopy__(self, memo) -> "PagedCache":
+        """A cache of its own that holds the same sequences (a prefix to go on from in two ways, say): its pages and those of its ranks are copied, the two know nothing of each other."""
+        book = copy.deepcopy(self._book, memo)
+        others = []
+        for one in [self] + self.__dict__.get("_tp_rank_siblings", []):
+            other = memo[id(one)] = self._with(book)
+            other._pools = {layer: tuple(pool.clone() for pool in pools) for layer, pools in one._pools.items()}
+            other._number, other._seen = one._number, set(one._seen)
+            others.append(other)
+        if "_tp_rank_siblings" in self.__dict__:
+            kv_cache.link(others[0], others[1:])
+        return others[0]
+
+    def __copy__(self):
+        raise NotImplementedError("PagedCache: a copy that shares its pages would write to them too; copy.deepcopy copies them")
 
     def prepare(self, counts: Sequence[int], hold: bool = False) -> Optional[torch.Tensor]:
         """The next forward has counts[b] new rows of sequence b (of as many rows as the largest count has, padded on the right). Takes their pages, or raises with nothing changed. Returns the

@@ -1,0 +1,77 @@
+"""What a `tp.paged.PagedCache` does between steps: copies, steps that are held, taken back or ended, and ranks. Nothing is computed, so no GPU is needed."""
+import copy
+
+import pytest
+import torch
+
+from tensor_parallel_amd import kv_cache, paged
+
+
+@pytest.fixture
+def written(monkeypatch):
+    """attend and append without kernels: the new rows of each sequence are written to its pages, as the kernels do."""
+    def append(q, k, v, k_pages, v_pages, table, lengths, counts=None, **kwargs):
+        page = k_pages.shape[2]
+        for b in range(k.shape[0]):
+            n = k.shape[1] if counts is None else min(int(counts[b]), k.shape[1])
+            for i in range(n):
+                at = int(lengths[b]) - n + i
+                k_pages[int(table[b, at // page]), :, at % page], v_pages[int(table[b, at // page]), :, at % page] = k[b, i], v[b, i]
+        return q
+
+    monkeypatch.setattr(paged, "append", append)
+    monkeypatch.setattr(paged, "attend", lambda q, *args, **kwargs: q)
+
+
+def forward(cache, rows, layers=2, value=1.0):
+    """The attention modules' share of a rank's forward."""
+    B = cache._book.sequences
+    for layer in range(layers):
+        q, kv, table = torch.zeros(B, rows, 2, 64), torch.full((B, rows, 1, 64), value), torch.zeros(B, rows, 64)
+        cache.attend(q, kv, kv, table, table, layer)
+
+
+def keys(cache, layer=0):
+    """The keys of each sequence, by the page table, one value a position."""
+    book = cache._book
+    pool = cache._pools[layer][0]
+    return [[float(pool[book.tables[b][j // book.page], 0, j % book.page, 0]) for j in range(n)] for b, n in enumerate(cache.lengths())]
+
+
+# ---- copies ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("ranks", [1, 2])
+def test_a_copy_of_a_filled_cache_is_a_cache_of_its_own(written, ranks):
+    cache = paged.PagedCache(sequences=1, pages=8, page=16)
+    of_ranks = kv_cache.rank_caches(cache, ranks)
+    for rank in of_ranks:
+        forward(rank, 20, value=3.0)
+    other = copy.deepcopy(cache)
+    of_others = kv_cache.rank_caches(other, ranks)
+    assert other.lengths() == [20] and [keys(c) for c in of_others] == [[[3.0] * 20]] * ranks
+    for rank in of_others:
+        forward(rank, 1, value=5.0)  # (a step that nothing was prepared for)
+    assert cache.lengths() == [20] and other.lengths() == [21]
+    cache.prepare([2])
+    for rank in of_ranks:
+        forward(rank, 2, value=7.0)
+    assert [keys(c) for c in of_ranks] == [[[3.0] * 20 + [7.0] * 2]] * ranks
+    assert [keys(c) for c in of_others] == [[[3.0] * 20 + [5.0]]] * ranks
+    other.reset()
+    assert other.lengths() == [0] == of_others[-1].lengths() and cache.lengths() == [22] == of_ranks[-1].lengths()
+    cache.reset()
+    assert cache.lengths() == [0]
+
+
+def test_a_copy_has_the_step_that_was_prepared(written):
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    cache.prepare([3, 1])
+    other = copy.deepcopy(cache)
+    forward(other, 3)
+    assert other.lengths() == [3, 1] and cache.lengths() == [0, 0]
+    forward(cache, 3)
+    assert cache.lengths() == [3, 1]
+
+
+def test_a_shallow_copy_is_refused():
+    with pytest.raises(NotImplementedError, match="deepcopy"):
+        copy.copy(paged.PagedCache(1, 1))
