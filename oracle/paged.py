@@ -70,7 +70,7 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table,
             kv = h * Hkv // Hq
             s = (q[first:first + n, h].double() @ k[kv].T) * scale
             unseen = torch.arange(length) > (torch.arange(n) + length - n)[:, None]
-            p = torch.softmax(s.masked_fill(unseen, -math.inf), 1).nan_to_num(0.0) if length else torch.zeros(n, 0, dtype=torch.float64)
+            p = torch.softmax(s.masked_fill(unseen, -math.inf), 1).masked_fill(unseen.all(1, keepdim=True), 0.0) if length else torch.zeros(n, 0, dtype=torch.float64)
             if finite:
                 out[first:first + n, h], weight[first:first + n, h] = p @ v[kv], p @ v[kv].abs()
             else:

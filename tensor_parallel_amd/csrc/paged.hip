@@ -101,6 +101,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t group_rsrc(const char *pool, i
 __device__ __forceinline__ void arrived(int &v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void arrived(u32x4 &v) { asm volatile("" : "+v"(v)); }
 
+// What the sum of a row's products is multiplied by, l its probabilities' sum and `last` the last position it sees: nothing for a row in front of position 0. A row all of whose scores are -inf has no
+// softmax: its sums are zeros, and zero times 1 / 0 the NaN that it is by definition.
+__device__ __forceinline__ float factor_of(float l, int last) { return last >= 0 ? 1.0f / l : 0.f; }
+
 // ---- which rows go where ---------------------------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ bool is_few(const PagedParams &p, int count) { return p.few && count > 0 && count * p.G <= FEW; }
 __device__ __forceinline__ int units_of(const PagedParams &p, const SeqRows &s) {
@@ -448,8 +452,8 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
                 for (int j = 0; j < 4; ++j) o[j] += weight * ov[j];
             }
             if (whole) {
-                const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // a sum of NaN stays one
                 const int at = r / p.G;
+                const float inv = factor_of(l, seen_by_all + at);
                 *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + at) * p.o_row + static_cast<int64_t>(item * p.G + r - at * p.G) * p.o_head + d4) * 2) =
                     make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
             } else {
@@ -539,8 +543,8 @@ __device__ __forceinline__ void few_merge(const PagedParams &p, const int blocks
             __syncthreads();
         }
         if (!mine || (dealt && taker != 0)) continue;
-        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
         const int place = r / p.G;
+        const float inv = factor_of(l, s.length - s.count + place);
         *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + place) * p.o_row + static_cast<int64_t>(hkv * p.G + r - place * p.G) * p.o_head + d4) * 2) =
             make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
     }
@@ -804,7 +808,7 @@ __device__ __forceinline__ void many_rows(const PagedParams &p, const int block)
     const int64_t token = s.first + place;
     const int head = hkv * p.G + row - place * p.G;
     if (cut == 1) {
-        const float inv = l_run > 0.f ? 1.0f / l_run : l_run == 0.f ? 0.f : l_run;  // a sum of NaN stays one
+        const float inv = factor_of(l_run, last);
         char *orow = p.o + (token * p.o_row + head * p.o_head) * 2;
 #pragma unroll
         for (int dt = 0; dt < DT32; ++dt)
@@ -892,8 +896,8 @@ __device__ __forceinline__ void many_merge(const PagedParams &p, const int block
                 for (int k = 0; k < 4; ++k) o[k] = o[k] * old + ov[j][k] * now;
             }
         }
-        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
         const int row = tile * MANY + r, place = row / p.G;
+        const float inv = factor_of(l, s.length - s.count + place);
         *reinterpret_cast<uint2 *>(p.o + (static_cast<int64_t>(s.first + place) * p.o_row + static_cast<int64_t>(hkv * p.G + row - place * p.G) * p.o_head + d4) * 2) =
             make_uint2(pack2_half<DT>(o[0] * inv, o[1] * inv), pack2_half<DT>(o[2] * inv, o[3] * inv));
     }
