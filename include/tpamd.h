@@ -520,7 +520,8 @@ typedef struct {
 int tpamd_append_paged(const tpamd_heads *heads, const tpamd_pages *pages, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int dtype, void *stream);
 
 /* out [rows, Hq, D] = softmax(scale q k^T) v of the new rows on the pages, a row on the positions up to its own; zeros for a row before position 0 (a sequence with fewer positions than new
- * rows), NaN for one whose scores all are -inf. What stands at positions a row does not see, infinities and NaN too, does not reach it. Scores, softmax and sums in fp32, probabilities rounded to dtype in front of the
+ * rows), NaN for one whose scores all are -inf. What stands at positions a row does not see, infinities and NaN too, does not reach it; an infinite value that it
+ * sees gives it that infinity, or NaN where its probability is too small for the dtype. Scores, softmax and sums in fp32, probabilities rounded to dtype in front of the
  * second product, the result once. D 64, 96, 128 or 256, BF16 or F16; rows of q and of the pools on 16-byte boundaries, of out on 8.
  * max_new: no sequence has more new rows (rows of one that does may be left out); max_length: none has more positions (a hint: only the time depends on it). Bounds that hold for every
  * replay, where the call is captured. workspace_dev: tpamd_attention_paged_workspace() bytes, 16-byte aligned, for the call alone until it has run; out overlaps nothing else. */

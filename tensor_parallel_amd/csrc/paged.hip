@@ -73,8 +73,8 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // Values that some rows of a tile do not see may be infinite or NaN, and zero times those would reach the rows through the matrix product. They go in as zeros. Where there are any, two more
-// products, of the largest bf16 value in the place of every +inf and NaN (then of its negative in the place of -inf and NaN) and of every probability above zero, add what overflows to an
-// infinity where it belongs: through the same sums, which are touched by nothing but matrix instructions.
+// products, of the largest bf16 value in the place of every +inf and NaN (then of its negative in the place of -inf and NaN) and of every probability of a position that the row sees (which may be
+// too small for the dtype, and is not zero for that), add what overflows to an infinity where it belongs: through the same sums, which are touched by nothing but matrix instructions.
 template <int DT>
 struct Beyond {
     static constexpr uint32_t E = DT == TPAMD_BF16 ? 0x7f80u : 0x7c00u, LAST = DT == TPAMD_BF16 ? 0x0080u : 0x0400u, HUGE_BF16 = 0x7f7fu;
@@ -87,7 +87,7 @@ struct Beyond {
         return (h & E) == E && ((h & 0x7fffu) != E || (h & 0x8000u) == sign) ? HUGE_BF16 | sign : 0u;
     }
     static __device__ __forceinline__ uint32_t huge(uint32_t two, uint32_t sign) { return huge_one(two & 0xffffu, sign) | huge_one(two >> 16, sign) << 16; }
-    static __device__ __forceinline__ uint32_t seen(uint32_t two) { return ((two & 0x7fffu) != 0 ? HUGE_BF16 : 0u) | ((two & 0x7fff0000u) != 0 ? HUGE_BF16 << 16 : 0u); }
+    static __device__ __forceinline__ uint32_t seen(int most) { return (most >= 0 ? HUGE_BF16 : 0u) | (most >= 1 ? HUGE_BF16 << 16 : 0u); }  // of two positions, where those up to the most-th are seen
 };
 
 // The descriptor of 16 rows that begin at `base`: nothing (loads give zeros) where there is no page.
@@ -411,7 +411,8 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
 #pragma unroll
                 for (int dt = 0; dt < DT16; ++dt) acc[dt] = mfma16_k16<DT>(vf[dt], pf, acc[dt]);
                 if (__any((carried & 0x80008000u) != 0)) {
-                    const u32x2 seen = {Beyond<DT>::seen(pf.x), Beyond<DT>::seen(pf.y)};
+                    const int most = last - k0 - 4 * lq;
+                    const u32x2 seen = {Beyond<DT>::seen(most), Beyond<DT>::seen(most - 2)};
 #pragma unroll
                     for (int dt = 0; dt < DT16; ++dt)
 #pragma unroll
@@ -776,7 +777,8 @@ __device__ __forceinline__ void many_rows(const PagedParams &p, const int block)
                 constexpr int dt = decltype(dc)::value;
                 u32x4 w = u32x4{lo[dt].x, lo[dt].y, hi[dt].x, hi[dt].y} & u32x4{m_lo.x, m_lo.y, m_hi.x, m_hi.y};
                 if (__any(((Beyond<DT>::carries(w.x) | Beyond<DT>::carries(w.y) | Beyond<DT>::carries(w.z) | Beyond<DT>::carries(w.w)) & 0x80008000u) != 0)) {
-                    const u32x4 seen = {Beyond<DT>::seen(pf[u].x), Beyond<DT>::seen(pf[u].y), Beyond<DT>::seen(pf[u].z), Beyond<DT>::seen(pf[u].w)};
+                    const int most = last - k0 - 16 * u - 4 * h;
+                    const u32x4 seen = {Beyond<DT>::seen(most), Beyond<DT>::seen(most - 2), Beyond<DT>::seen(most - 8), Beyond<DT>::seen(most - 10)};
 #pragma unroll
                     for (uint32_t sign : {0u, 0x8000u}) {
                         const u32x4 huge = {Beyond<DT>::huge(w.x, sign), Beyond<DT>::huge(w.y, sign), Beyond<DT>::huge(w.z, sign), Beyond<DT>::huge(w.w, sign)};

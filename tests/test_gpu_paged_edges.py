@@ -44,3 +44,29 @@ def test_rows_before_position_zero_are_zeros_beside_scores_of_minus_infinity():
         got = check_attend(batch)
         before = counts[0] - lengths[0]
         assert (got[:before] == 0).all() and got[before].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("counts,lengths", [([1, 4], [70, 133]), ([1], [600]), ([50, 40], [50, 161]), ([3], [9000]), ([40], [5000])])
+def test_infinite_values_of_small_probability_do_not_vanish(dtype, D, counts, lengths):
+    """Values that are not finite at positions whose probability is below what the dtype holds (e^-200 and less, but not zero): the rows that see them are not finite in their columns (the value itself,
+    or the NaN of zero times it), and no other row or column is touched."""
+    batch = Batch(counts, lengths, 4, 2, D, 16, dtype, seed=42, spread=0.1)
+    b, n, new = len(counts) - 1, lengths[-1], counts[-1]
+    batch.q[:, :, 0] = 16.0
+    placed = {3: (n - 1, math.inf), 5: (max(n - 2, 0), -math.inf), 7: (n - 1 - new // 2, math.nan), 11: (n - new, math.inf), 13: (n // 2, -math.inf)}
+    for column, (j, value) in placed.items():
+        batch.k[batch.table[b][j // 16], :, j % 16, 0] = -15.0 * D**0.5
+        batch.v[batch.table[b][j // 16], :, j % 16, column] = value
+    got = paged.attend(batch.q.to(DEV), **batch.on(), max_new=max(counts), max_length=max(lengths)).cpu().double()
+    want, weight = batch.want(D**-0.5)
+    tol = batch.tolerance(want, weight, D**-0.5)
+    finite = torch.isfinite(want)
+    first, count, length = batch.seqs[b]
+    for column, (j, value) in placed.items():
+        for i in range(count):
+            sees = j <= length - count + i
+            assert bool(torch.isfinite(got[first + i, :, column]).any()) != sees, (column, i)
+    assert torch.equal(torch.isfinite(got), finite)
+    assert ((got - want).abs() - tol)[finite].max() <= 0
