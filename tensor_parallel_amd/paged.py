@@ -211,9 +211,9 @@ class PagedCache:
 
     # ---- what transformers asks of a cache
     def get_seq_length(self, layer_idx: int = 0) -> int:
-        """The longest sequence's positions, as this rank's forward sees them: with a step's rows from its first attention module on."""
+        """The longest sequence's positions, as this rank's forward sees them: with a step's rows from its first attention module on, but for a step that is held: its next forward is the same one."""
         book = self._book
-        return max(book.after() if book.taken and self._number == book.number else book.before)
+        return max(book.after() if book.taken and not book.hold and self._number == book.number else book.before)
 
     def get_max_length(self, layer_idx: int = 0) -> int:
         return self._book.columns * self._book.page

@@ -75,3 +75,21 @@ def test_a_copy_has_the_step_that_was_prepared(written):
 def test_a_shallow_copy_is_refused():
     with pytest.raises(NotImplementedError, match="deepcopy"):
         copy.copy(paged.PagedCache(1, 1))
+
+
+# ---- steps that are held -----------------------------------------------------------------------------------------------
+def test_forwards_of_a_held_step_begin_at_the_same_position(written):
+    """A model that is given no positions counts from this."""
+    cache = paged.PagedCache(sequences=1, pages=8, page=16)
+    forward(cache, 5)
+    assert cache.get_seq_length() == 5
+    for before in (5, 6):
+        cache.prepare([1], hold=True)
+        for _ in range(3):
+            assert cache.get_seq_length() == before
+            forward(cache, 1)
+        assert cache.get_seq_length() == before and cache.lengths() == [before + 1]
+    cache.prepare([1])
+    assert cache.get_seq_length() == 7
+    forward(cache, 1)
+    assert cache.get_seq_length() == 8
