@@ -25,7 +25,7 @@ from __future__ import annotations
 
 import copy
 import threading
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Set, Tuple
 
 import torch
 
@@ -55,6 +55,10 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
     return _guard(_native.attention_paged(q, k_pages, v_pages, table, lengths, starts, counts, scale, max_new, max_length, out), q, k_pages, v_pages)
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class _Book:
     """What the caches of all ranks and layers have in common: which pages each sequence has, how many positions, and the rows of the step that is on its way."""
 
@@ -63,6 +67,7 @@ class _Book:
         self.states: Dict[torch.device, torch.Tensor] = {}
         self.uploaded: Dict[torch.device, int] = {}  # the step that is there
         self.lock = threading.Lock()  # ranks on different devices are threads
+        self.captured: Set[int] = set()  # rows (of each sequence) of the forwards that were captured
         self.reset()
 
     def reset(self) -> None:
@@ -71,23 +76,29 @@ class _Book:
         self.before = [0] * self.sequences  # positions without the step's rows
         self.counts = [0] * self.sequences  # the step's rows
         self.number, self.taken, self.hold = 0, True, False  # of the step (0: none yet); whether a forward has begun it; whether further forwards are the same step
+        self.rows: Optional[int] = None  # of a held step's forwards, where the caller has said it
         self.uploaded.clear()
 
     def __deepcopy__(self, memo) -> "_Book":
         with self.lock:
             other = _Book(self.sequences, self.pages, self.page, self.columns)
             for name, value in self.__dict__.items():
-                if name not in ("states", "uploaded", "lock"):  # (what a device was told is told anew)
+                if name not in ("states", "uploaded", "lock", "captured"):  # (what a device was told is told anew, and what was captured reads the original's)
                     setattr(other, name, copy.deepcopy(value, memo))
         return other
 
     def after(self) -> List[int]:
         return [n + c for n, c in zip(self.before, self.counts)]
 
-    def begin(self, counts: Sequence[int], hold: bool) -> None:
+    def begin(self, counts: Sequence[int], hold: bool, rows: Optional[int] = None) -> None:
         counts = [int(c) for c in counts]
         if len(counts) != self.sequences or min(counts, default=0) < 0:
             raise ValueError(f"PagedCache: {self.sequences} counts of new rows, none below 0, are needed, got {counts}")
+        if rows is not None and (not hold or rows < 1):
+            raise ValueError(f"PagedCache: rows says how many rows of each sequence the forwards of a held step have, got {rows}{'' if hold else ' for a step that is not held'}")
+        most = rows if rows is not None else min(self.captured) if hold and self.captured else None
+        if most is not None and max(counts) > most:
+            raise ValueError(f"PagedCache: {counts} new rows for a forward of {most} rows a sequence" + ("" if rows is not None else ", as was captured; rows= says which one will be replayed"))
         before = self.after() if self.taken else self.before
         need = [-(-(n + c) // self.page) - len(t) for n, c, t in zip(before, counts, self.tables)]
         if max((len(t) + max(n, 0) for n, t in zip(need, self.tables)), default=0) > self.columns:
@@ -96,7 +107,7 @@ class _Book:
             raise RuntimeError(f"PagedCache: {sum(max(n, 0) for n in need)} more pages of {self.page} positions are needed, {len(self.free)} of {self.pages} are free")
         for table, n in zip(self.tables, need):
             table.extend(self.free.pop() for _ in range(n))
-        self.before, self.counts = before, counts
+        self.before, self.counts, self.rows = before, counts, rows
         self.number, self.taken, self.hold = self.number + 1, hold, hold  # (replays of a captured forward do not come by here)
 
     def release(self, sequence: int) -> None:
@@ -187,14 +198,17 @@ class PagedCache:
     def __copy__(self):
         raise NotImplementedError("PagedCache: a copy that shares its pages would write to them too; copy.deepcopy copies them")
 
-    def prepare(self, counts: Sequence[int], hold: bool = False) -> Optional[torch.Tensor]:
+    def prepare(self, counts: Sequence[int], hold: bool = False, rows: Optional[int] = None) -> torch.Tensor:
         """The next forward has counts[b] new rows of sequence b (of as many rows as the largest count has, padded on the right). Takes their pages, or raises with nothing changed. Returns the
-        rows' positions [sequences, largest count] on the host: `position_ids`, once they are on the model's device."""
+        rows' positions [sequences, largest count] on the host: `position_ids`, once they are on the model's device.
+
+        rows: how many rows of each sequence the forwards of a held step have (and the positions returned). A replay cannot have more rows than it was captured with, so larger counts raise; with
+        captured forwards of several widths those larger than the narrowest one's have to be told which one is meant."""
         book = self._book
-        book.begin(counts, hold)
+        book.begin(counts, hold, rows)
         for device in book.states:
             book.on(device)  # where a captured forward looks for them
-        return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts))
+        return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts) if rows is None else rows)
 
     def release(self, sequence: int) -> None:
         """Sequence `sequence` has ended: its pages are free and its length is 0."""
@@ -256,6 +270,8 @@ class PagedCache:
         counts, before = ([S] * B, book.after()) if begins else (book.counts, book.before)
         if max(counts) > S or (max(counts) < S and not book.hold):
             raise ValueError(f"PagedCache: {counts} new rows were prepared, the forward has {S}")
+        if book.hold and book.rows not in (None, S):
+            raise ValueError(f"PagedCache: forwards of {book.rows} rows a sequence were prepared, this one has {S}")
         if B > 1 and cos.shape[0] == 1 and min(before) != max(before):
             raise ValueError(f"PagedCache: sequences of {before} positions in one forward need position_ids of their own")
         if begins:
@@ -263,6 +279,8 @@ class PagedCache:
         if first:
             book.taken, self._number, self._seen = True, book.number, set()
         self._seen.add(layer_idx)
+        if book.hold and _capturing(k):
+            book.captured.add(S)
         lengths = book.after()
         if layer_idx not in self._pools:
             self._pools[layer_idx] = tuple(torch.zeros((book.pages, Hkv, book.page, D), dtype=k.dtype, device=k.device) for _ in "kv")

@@ -93,3 +93,49 @@ def test_forwards_of_a_held_step_begin_at_the_same_position(written):
     assert cache.get_seq_length() == 7
     forward(cache, 1)
     assert cache.get_seq_length() == 8
+
+
+def captured(monkeypatch, cache, width, **how):
+    """A held forward while a stream is captured, and the replay of it: what the kernels read."""
+    cache.prepare([1] * cache._book.sequences, hold=True, **how)
+    with monkeypatch.context() as m:
+        m.setattr(paged, "_capturing", lambda t: True)
+        forward(cache, width)
+
+
+def test_a_step_of_more_rows_than_were_captured_is_refused(written, monkeypatch):
+    """A replay has the rows it was captured with: counted beyond them, positions would be attended to that nothing was written to."""
+    cache = paged.PagedCache(sequences=2, pages=16, page=16)
+    forward(cache, 5)
+    cache.prepare([3, 1], hold=True)  # (nothing is captured yet: a forward says by itself that it has fewer)
+    with pytest.raises(ValueError, match="prepared"):
+        forward(cache, 1)
+    captured(monkeypatch, cache, 1)
+    lengths = cache.lengths()
+    state = [t.clone() for t in cache._book.on(torch.device("cpu"))]
+    for how in ({}, {"rows": 2}):
+        with pytest.raises(ValueError, match="rows"):
+            cache.prepare([3, 1], hold=True, **how)
+        assert cache.lengths() == lengths and all(torch.equal(a, b) for a, b in zip(state, cache._book.on(torch.device("cpu"))))
+    cache.prepare([3, 1])  # forwards that are not held are not captured ones
+    forward(cache, 3)
+    cache.reset()
+    with pytest.raises(ValueError, match="rows"):
+        cache.prepare([2, 1], hold=True)
+
+
+def test_captured_forwards_of_several_widths(written, monkeypatch):
+    cache = paged.PagedCache(sequences=1, pages=16, page=16)
+    captured(monkeypatch, cache, 4, rows=4)
+    cache.prepare([3], hold=True)
+    captured(monkeypatch, cache, 1)
+    with pytest.raises(ValueError, match="rows"):
+        cache.prepare([3], hold=True)  # which of the two will be replayed is not known
+    assert cache.prepare([3], hold=True, rows=4).shape == (1, 4)
+    with pytest.raises(ValueError, match="4"):
+        forward(cache, 3)
+    forward(cache, 4)
+    with pytest.raises(ValueError):
+        cache.prepare([1], rows=4)  # of steps that are held
+    other = copy.deepcopy(cache)
+    other.prepare([9], hold=True)  # what was captured works on the original
