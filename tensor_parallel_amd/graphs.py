@@ -29,12 +29,14 @@ memory are.
 from __future__ import annotations
 
 import importlib
+import inspect
 from typing import Any, List, Sequence, Tuple
 
 import torch
 from torch import nn
 
 from . import _native
+from .paged import PagedCache
 
 
 def _walk(value: Any, leaves: List[Tuple[str, Any]], path: str) -> None:
@@ -76,6 +78,19 @@ def _count_tensors(cache) -> list:
     return out
 
 
+def _check_paged(module: nn.Module, args: tuple, kwargs: dict, leaves) -> None:
+    """What a captured forward on a `paged.PagedCache` needs: positions among its arguments (those that a model counts on the host would be the captured step's in every replay)."""
+    if not any(isinstance(value, PagedCache) for _, value in leaves):
+        return
+    model = getattr(module, "wrapped_model", module)
+    model = (getattr(model, "module_shards", None) or [model])[0]
+    signature = inspect.signature(model.forward)
+    if "position_ids" not in signature.parameters:
+        return  # it has positions of its own
+    if not isinstance(signature.bind_partial(*args, **kwargs).arguments.get("position_ids"), torch.Tensor):
+        raise ValueError("graphs.capture: a forward on a PagedCache needs position_ids among its tensors (prepare returns them); without them it would replay the positions it was captured at")
+
+
 class GraphedForward:
     """`module(*args, **kwargs)` captured once; calls replay it on new values of the same tensors."""
 
@@ -84,6 +99,7 @@ class GraphedForward:
         tp_module = importlib.import_module(__package__ + ".tensor_parallel")
 
         self.module = module
+        _check_paged(module, args, kwargs, self._leaves(args, kwargs))
         devices = {t.device for _, t in self._leaves(args, kwargs) if isinstance(t, torch.Tensor)}
         devices |= {p.device for p in module.parameters()}
         if len(devices) != 1 or next(iter(devices)).type != "cuda":

@@ -4,7 +4,7 @@ import copy
 import pytest
 import torch
 
-from tensor_parallel_amd import kv_cache, paged
+from tensor_parallel_amd import graphs, kv_cache, paged
 
 
 @pytest.fixture
@@ -139,3 +139,38 @@ def test_captured_forwards_of_several_widths(written, monkeypatch):
         cache.prepare([1], rows=4)  # of steps that are held
     other = copy.deepcopy(cache)
     other.prepare([9], hold=True)  # what was captured works on the original
+
+
+class Model(torch.nn.Module):
+    """Takes positions as a transformers model does, by name or in their place."""
+
+    def __init__(self):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.zeros(1))
+
+    def forward(self, input_ids, attention_mask=None, position_ids=None, past_key_values=None, **kwargs):
+        raise AssertionError("the capture was not refused")
+
+
+class OwnPositions(Model):
+    def forward(self, input_ids, past_key_values=None):
+        raise AssertionError("the capture was not refused")
+
+
+def test_a_capture_without_positions_is_refused():
+    """Positions that the model counts on the host would be the captured step's in every replay."""
+    ids = torch.zeros(2, 1, dtype=torch.int64)
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    positions = cache.prepare([1, 1], hold=True)
+    nested = torch.nn.Module()
+    nested.module_shards = [Model()]
+    outer = torch.nn.Module()
+    outer.wrapped_model = nested
+    for model in (Model(), nested, outer):
+        with pytest.raises(ValueError, match="position_ids"):
+            graphs.capture(model, input_ids=ids, past_key_values=cache)
+    # (these get as far as the devices, of which there are none here)
+    for call in (lambda: graphs.capture(Model(), input_ids=ids, position_ids=positions, past_key_values=cache), lambda: graphs.capture(Model(), ids, None, positions, past_key_values=cache),
+                 lambda: graphs.capture(OwnPositions(), ids, past_key_values=cache)):
+        with pytest.raises(ValueError, match="HIP device"):
+            call()
