@@ -79,9 +79,13 @@ def _count_tensors(cache) -> list:
 
 
 def _check_paged(module: nn.Module, args: tuple, kwargs: dict, leaves) -> None:
-    """What a captured forward on a `paged.PagedCache` needs: positions among its arguments (those that a model counts on the host would be the captured step's in every replay)."""
-    if not any(isinstance(value, PagedCache) for _, value in leaves):
+    """What a captured forward on a `paged.PagedCache` needs: a step that is held (the forwards that a capture runs would each be counted as another), and positions among its arguments (those that a
+    model counts on the host would be the captured step's in every replay)."""
+    caches = [value for _, value in leaves if isinstance(value, PagedCache)]
+    if not caches:
         return
+    if not all(cache.held for cache in caches):
+        raise ValueError("graphs.capture: a forward on a PagedCache is captured under a step that is held (prepare(counts, hold=True))")
     model = getattr(module, "wrapped_model", module)
     model = (getattr(model, "module_shards", None) or [model])[0]
     signature = inspect.signature(model.forward)

@@ -210,6 +210,11 @@ class PagedCache:
             book.on(device)  # where a captured forward looks for them
         return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts) if rows is None else rows)
 
+    @property
+    def held(self) -> bool:
+        """Whether all forwards up to the next `prepare` are the same step."""
+        return self._book.hold
+
     def release(self, sequence: int) -> None:
         """Sequence `sequence` has ended: its pages are free and its length is 0."""
         self._book.release(sequence)
@@ -263,6 +268,8 @@ class PagedCache:
         B, S, Hkv, D = k.shape
         if B != book.sequences:
             raise ValueError(f"PagedCache: {B} sequences in a forward on a cache for {book.sequences}")
+        if not book.hold and _capturing(k):
+            raise RuntimeError("PagedCache: a forward is captured under a step that is held (prepare(counts, hold=True))")
         first = self._number != book.number or (layer_idx in self._seen and not book.hold)  # this rank's first module in a forward
         begins = first and book.number in (0, self._number)  # a step that nothing was prepared for
         if begins and not book.taken:

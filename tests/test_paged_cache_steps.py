@@ -174,3 +174,20 @@ def test_a_capture_without_positions_is_refused():
                  lambda: graphs.capture(OwnPositions(), ids, past_key_values=cache)):
         with pytest.raises(ValueError, match="HIP device"):
             call()
+
+
+def test_a_capture_of_a_step_that_is_not_held_is_refused(written, monkeypatch):
+    """Each of a capture's own forwards would be counted as a step, and no replay."""
+    ids = torch.zeros(2, 1, dtype=torch.int64)
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    forward(cache, 3)
+    for prepared in (False, True):
+        positions = cache.prepare([1, 1]) if prepared else torch.tensor([[3], [3]])
+        with pytest.raises(ValueError, match="hold"):
+            graphs.capture(Model(), input_ids=ids, position_ids=positions, past_key_values=cache)
+        assert cache.lengths() == [3, 3]
+        with monkeypatch.context() as m:  # by torch's own means
+            m.setattr(paged, "_capturing", lambda t: True)
+            with pytest.raises(RuntimeError, match="hold"):
+                forward(cache, 1)
+        assert cache.lengths() == [3, 3]
