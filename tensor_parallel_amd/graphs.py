@@ -91,8 +91,11 @@ def _check_paged(module: nn.Module, args: tuple, kwargs: dict, leaves) -> None:
     signature = inspect.signature(model.forward)
     if "position_ids" not in signature.parameters:
         return  # it has positions of its own
-    if not isinstance(signature.bind_partial(*args, **kwargs).arguments.get("position_ids"), torch.Tensor):
+    positions = signature.bind_partial(*args, **kwargs).arguments.get("position_ids")
+    if not isinstance(positions, torch.Tensor):
         raise ValueError("graphs.capture: a forward on a PagedCache needs position_ids among its tensors (prepare returns them); without them it would replay the positions it was captured at")
+    if positions.dim() == 2 and positions.shape[0] == 1 and any(cache.sequences > 1 for cache in caches):
+        raise ValueError("graphs.capture: a forward on a PagedCache needs a row of position_ids for each sequence, since they may differ in length when it is replayed")
 
 
 class GraphedForward:

@@ -211,6 +211,10 @@ class PagedCache:
         return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts) if rows is None else rows)
 
     @property
+    def sequences(self) -> int:
+        return self._book.sequences
+
+    @property
     def held(self) -> bool:
         """Whether all forwards up to the next `prepare` are the same step."""
         return self._book.hold
@@ -279,7 +283,7 @@ class PagedCache:
             raise ValueError(f"PagedCache: {counts} new rows were prepared, the forward has {S}")
         if book.hold and book.rows not in (None, S):
             raise ValueError(f"PagedCache: forwards of {book.rows} rows a sequence were prepared, this one has {S}")
-        if B > 1 and cos.shape[0] == 1 and min(before) != max(before):
+        if B > 1 and cos.shape[0] == 1 and (min(before) != max(before) or _capturing(k)):  # (of a captured forward they may differ in any replay)
             raise ValueError(f"PagedCache: sequences of {before} positions in one forward need position_ids of their own")
         if begins:
             book.begin(counts, False)

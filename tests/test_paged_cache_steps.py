@@ -191,3 +191,19 @@ def test_a_capture_of_a_step_that_is_not_held_is_refused(written, monkeypatch):
             with pytest.raises(RuntimeError, match="hold"):
                 forward(cache, 1)
         assert cache.lengths() == [3, 3]
+
+
+def test_a_capture_with_one_row_of_positions_for_several_sequences_is_refused(written, monkeypatch):
+    """They may be as long as one another now; replays would turn them alike when they no longer are."""
+    ids = torch.zeros(2, 1, dtype=torch.int64)
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    cache.prepare([1, 1], hold=True)
+    with pytest.raises(ValueError, match="each"):
+        graphs.capture(Model(), input_ids=ids, position_ids=torch.zeros(1, 1, dtype=torch.int64), past_key_values=cache)
+    q, kv = torch.zeros(2, 1, 2, 64), torch.zeros(2, 1, 1, 64)
+    tables = {rows: torch.zeros(rows, 1, 64) for rows in (1, 2)}
+    cache.attend(q, kv, kv, tables[1], tables[1], 0)  # (an eager forward is told when they no longer fit)
+    monkeypatch.setattr(paged, "_capturing", lambda t: True)
+    with pytest.raises(ValueError, match="of their own"):
+        cache.attend(q, kv, kv, tables[1], tables[1], 0)
+    cache.attend(q, kv, kv, tables[2], tables[2], 0)
