@@ -24,6 +24,7 @@ pass through either raises.
 from __future__ import annotations
 
 import copy
+import operator
 import threading
 from typing import Dict, List, Optional, Sequence, Set, Tuple
 
@@ -111,6 +112,9 @@ class _Book:
         self.number, self.taken, self.hold = self.number + 1, hold, hold  # (replays of a captured forward do not come by here)
 
     def release(self, sequence: int) -> None:
+        sequence = operator.index(sequence)
+        if not 0 <= sequence < self.sequences:
+            raise IndexError(f"PagedCache: there is no sequence {sequence} among {self.sequences}")
         if not self.taken:
             raise RuntimeError("PagedCache: a step was prepared that no forward has made yet")
         self.before = self.after()

@@ -207,3 +207,15 @@ def test_a_capture_with_one_row_of_positions_for_several_sequences_is_refused(wr
     with pytest.raises(ValueError, match="of their own"):
         cache.attend(q, kv, kv, tables[1], tables[1], 0)
     cache.attend(q, kv, kv, tables[2], tables[2], 0)
+
+
+# ---- sequences that end ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("sequence", [-1, 2, 1.0, None])
+def test_a_sequence_that_there_is_not_is_not_released(written, sequence):
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    forward(cache, 20)
+    with pytest.raises((IndexError, TypeError)):
+        cache.release(sequence)
+    assert cache.lengths() == [20, 20] and len(cache._book.free) == 4
+    cache.release(1)
+    assert cache.lengths() == [20, 0]
