@@ -66,19 +66,24 @@ class _Book:
     def __init__(self, sequences: int, pages: int, page: int, columns: int):
         self.sequences, self.pages, self.page, self.columns = sequences, pages, page, columns
         self.states: Dict[torch.device, torch.Tensor] = {}
-        self.uploaded: Dict[torch.device, int] = {}  # the step that is there
+        self.uploaded: Dict[torch.device, int] = {}  # the version of it that is there
         self.lock = threading.Lock()  # ranks on different devices are threads
         self.captured: Set[int] = set()  # rows (of each sequence) of the forwards that were captured
+        self.number = self.version = 0  # of the step and of what devices are told, never given twice
         self.reset()
 
     def reset(self) -> None:
         self.free: List[int] = list(range(self.pages - 1, -1, -1))
         self.tables: List[List[int]] = [[] for _ in range(self.sequences)]
         self.before = [0] * self.sequences  # positions without the step's rows
+        self.end()
+
+    def end(self) -> None:
+        """No step is on its way: the next forward, of whichever rank, begins another, and replays have no new rows."""
         self.counts = [0] * self.sequences  # the step's rows
-        self.number, self.taken, self.hold = 0, True, False  # of the step (0: none yet); whether a forward has begun it; whether further forwards are the same step
+        self.taken, self.hold, self.over = True, False, True  # whether a forward has begun the step; whether further forwards are the same step; whether it has ended for all
         self.rows: Optional[int] = None  # of a held step's forwards, where the caller has said it
-        self.uploaded.clear()
+        self.version += 1
 
     def __deepcopy__(self, memo) -> "_Book":
         with self.lock:
@@ -109,7 +114,8 @@ class _Book:
         for table, n in zip(self.tables, need):
             table.extend(self.free.pop() for _ in range(n))
         self.before, self.counts, self.rows = before, counts, rows
-        self.number, self.taken, self.hold = self.number + 1, hold, hold  # (replays of a captured forward do not come by here)
+        self.number, self.version = self.number + 1, self.version + 1
+        self.taken, self.hold, self.over = hold, hold, False  # (replays of a captured forward do not come by here)
 
     def release(self, sequence: int) -> None:
         sequence = operator.index(sequence)
@@ -118,7 +124,7 @@ class _Book:
         if not self.taken:
             raise RuntimeError("PagedCache: a step was prepared that no forward has made yet")
         self.before = self.after()
-        self.counts = [0] * self.sequences
+        self.end()
         self.free.extend(reversed(self.tables[sequence]))
         self.tables[sequence], self.before[sequence] = [], 0
 
@@ -128,13 +134,18 @@ class _Book:
         state = self.states.get(device)
         if state is None:
             state = self.states[device] = torch.zeros(n * (self.columns + 2), dtype=torch.int32, device=device)
-        if self.uploaded.get(device) != self.number:
+        if self.uploaded.get(device) != self.version:
             rows = torch.full((n, self.columns), -1, dtype=torch.int32)
             for row, table in zip(rows, self.tables):
                 row[:len(table)] = torch.tensor(table, dtype=torch.int32)
             state.copy_(torch.cat([rows.flatten(), torch.tensor(self.after() + self.counts, dtype=torch.int32)]))
-            self.uploaded[device] = self.number
+            self.uploaded[device] = self.version
         return state[:n * self.columns].view(n, self.columns), state[n * self.columns:n * (self.columns + 1)], state[n * (self.columns + 1):]
+
+    def tell(self) -> None:
+        """Brings the devices' state up to date, where captured forwards look for it."""
+        for device in self.states:
+            self.on(device)
 
 
 class PagedCache:
@@ -210,8 +221,7 @@ class PagedCache:
         captured forwards of several widths those larger than the narrowest one's have to be told which one is meant."""
         book = self._book
         book.begin(counts, hold, rows)
-        for device in book.states:
-            book.on(device)  # where a captured forward looks for them
+        book.tell()
         return torch.tensor(book.before)[:, None] + torch.arange(max(book.counts) if rows is None else rows)
 
     @property
@@ -224,17 +234,18 @@ class PagedCache:
         return self._book.hold
 
     def release(self, sequence: int) -> None:
-        """Sequence `sequence` has ended: its pages are free and its length is 0."""
+        """Sequence `sequence` has ended: its pages are free and its length is 0. A step that was held has ended too: a replay before the next `prepare` has no new rows."""
         self._book.release(sequence)
+        self._book.tell()
 
     def lengths(self) -> List[int]:
         """The positions of each sequence, those of a step that a forward has begun among them."""
         return self._book.after() if self._book.taken else list(self._book.before)
 
     def reset(self) -> None:
-        """All sequences have ended. The pools stay."""
+        """All sequences have ended, and a step that was held. The pools stay."""
         self._book.reset()
-        self._number, self._seen = -1, set()
+        self._book.tell()
 
     # ---- what transformers asks of a cache
     def get_seq_length(self, layer_idx: int = 0) -> int:
@@ -278,8 +289,8 @@ class PagedCache:
             raise ValueError(f"PagedCache: {B} sequences in a forward on a cache for {book.sequences}")
         if not book.hold and _capturing(k):
             raise RuntimeError("PagedCache: a forward is captured under a step that is held (prepare(counts, hold=True))")
-        first = self._number != book.number or (layer_idx in self._seen and not book.hold)  # this rank's first module in a forward
-        begins = first and book.number in (0, self._number)  # a step that nothing was prepared for
+        first = book.over or self._number != book.number or (layer_idx in self._seen and not book.hold)  # this rank's first module in a forward
+        begins = book.over or (first and book.number == self._number)  # a step that nothing was prepared for
         if begins and not book.taken:
             raise RuntimeError("PagedCache: a rank is a forward ahead of the others")
         counts, before = ([S] * B, book.after()) if begins else (book.counts, book.before)

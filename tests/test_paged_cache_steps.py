@@ -219,3 +219,27 @@ def test_a_sequence_that_there_is_not_is_not_released(written, sequence):
     assert cache.lengths() == [20, 20] and len(cache._book.free) == 4
     cache.release(1)
     assert cache.lengths() == [20, 0]
+
+
+@pytest.mark.parametrize("end", ["release", "reset"])
+def test_replays_after_a_sequence_has_ended_write_nothing_to_its_pages(written, monkeypatch, end):
+    """What a captured forward reads is told that there are no new rows, and that the pages are another's, before the next step is prepared."""
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    forward(cache, 20)
+    captured(monkeypatch, cache, 1)
+    table, lengths, counts = (t for t in cache._book.on(torch.device("cpu")))  # what the captured forward reads
+    assert lengths.tolist() == [21, 21] and counts.tolist() == [1, 1]
+    cache.release(0) if end == "release" else cache.reset()
+    assert counts.tolist() == [0, 0] and lengths.tolist() == ([0, 21] if end == "release" else [0, 0])
+    assert (table[0] == -1).all() and (end == "release" or (table == -1).all())
+    if end == "release":
+        assert table[1, :2].tolist() == pages_of(cache)[1]
+    # the held step has ended with it: an eager forward that nothing was prepared for is a step of its own
+    before = cache.lengths()
+    forward(cache, 2)
+    assert cache.lengths() == [n + 2 for n in before] and counts.tolist() == [2, 2]
+    assert not cache.held
+
+
+def pages_of(cache):
+    return cache._book.tables
