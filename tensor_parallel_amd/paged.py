@@ -133,7 +133,8 @@ class _Book:
         n = self.sequences
         state = self.states.get(device)
         if state is None:
-            state = self.states[device] = torch.zeros(n * (self.columns + 2), dtype=torch.int32, device=device)
+            with torch.inference_mode(False):  # (written outside of that mode too)
+                state = self.states[device] = torch.zeros(n * (self.columns + 2), dtype=torch.int32, device=device)
         if self.uploaded.get(device) != self.version:
             rows = torch.full((n, self.columns), -1, dtype=torch.int32)
             for row, table in zip(rows, self.tables):
@@ -203,7 +204,8 @@ class PagedCache:
         others = []
         for one in [self] + self.__dict__.get("_tp_rank_siblings", []):
             other = memo[id(one)] = self._with(book)
-            other._pools = {layer: tuple(pool.clone() for pool in pools) for layer, pools in one._pools.items()}
+            with torch.inference_mode(False):
+                other._pools = {layer: tuple(pool.clone() for pool in pools) for layer, pools in one._pools.items()}
             other._number, other._seen = one._number, set(one._seen)
             others.append(other)
         if "_tp_rank_siblings" in self.__dict__:
@@ -309,7 +311,8 @@ class PagedCache:
             book.captured.add(S)
         lengths = book.after()
         if layer_idx not in self._pools:
-            self._pools[layer_idx] = tuple(torch.zeros((book.pages, Hkv, book.page, D), dtype=k.dtype, device=k.device) for _ in "kv")
+            with torch.inference_mode(False):
+                self._pools[layer_idx] = tuple(torch.zeros((book.pages, Hkv, book.page, D), dtype=k.dtype, device=k.device) for _ in "kv")
         table, lengths_there, counts_there = book.on(k.device)
         whole = min(counts) == S and not book.hold
         return {"table": table, "lengths": lengths_there, "counts": None if whole else counts_there}, whole, None if book.hold else max(lengths)

@@ -243,3 +243,20 @@ def test_replays_after_a_sequence_has_ended_write_nothing_to_its_pages(written, 
 
 def pages_of(cache):
     return cache._book.tables
+
+
+# ---- modes of torch ----------------------------------------------------------------------------------------------------
+def test_forwards_in_inference_mode_and_steps_outside_of_it(written):
+    cache = paged.PagedCache(sequences=1, pages=8, page=16)
+    with torch.inference_mode():
+        forward(cache, 5)
+    cache.prepare([2])
+    forward(cache, 2)
+    with torch.inference_mode():
+        cache.prepare([1])
+        forward(cache, 1)
+        other = copy.deepcopy(cache)
+    other.prepare([1])
+    forward(other, 1)
+    cache.release(0)
+    assert other.lengths() == [9] and cache.lengths() == [0]
