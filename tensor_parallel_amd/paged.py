@@ -174,6 +174,8 @@ class PagedCache:
 
     `copy.deepcopy(cache)` is a cache of its own, with the same sequences in pages of its own; a shallow copy is refused.
 
+    A forward that failed has to be taken back with `abandon()` before it is made again.
+
     One caller at a time (the ranks of its forward may be threads); beam search (which would have sequences share pages) is not supported."""
 
     is_compileable = False
@@ -243,6 +245,12 @@ class PagedCache:
     def lengths(self) -> List[int]:
         """The positions of each sequence, those of a step that a forward has begun among them."""
         return self._book.after() if self._book.taken else list(self._book.before)
+
+    def abandon(self) -> None:
+        """The last step is taken back, prepared, held or begun as it is: a forward that failed on its way (behind its first attention module the step counts as made) is made again after this, as if
+        it had not been begun. Sequences keep the pages that were taken for it."""
+        self._book.end()
+        self._book.tell()
 
     def reset(self) -> None:
         """All sequences have ended, and a step that was held. The pools stay."""

@@ -260,3 +260,46 @@ def test_forwards_in_inference_mode_and_steps_outside_of_it(written):
     forward(other, 1)
     cache.release(0)
     assert other.lengths() == [9] and cache.lengths() == [0]
+
+
+# ---- forwards that fail ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("prepared", [False, True])
+@pytest.mark.parametrize("came_by", [(1, 0), (2, 0), (2, 1), (0, 1)])
+def test_a_step_that_failed_is_taken_back_and_made_again(written, prepared, came_by):
+    """Some modules of some ranks have come by when a forward fails; made again, whichever rank is first, it counts once and fills every layer."""
+    cache = paged.PagedCache(sequences=2, pages=12, page=16)
+    ranks = kv_cache.rank_caches(cache, 2)
+    for rank in ranks:
+        forward(rank, 15, value=1.0)
+    if prepared:
+        cache.prepare([3, 2])
+    for rank, layers in zip(ranks, came_by):
+        forward(rank, 3, layers=layers, value=9.0)
+    cache.abandon()
+    assert cache.lengths() == [15, 15] and [r.get_seq_length() for r in ranks] == [15, 15]
+    if prepared:
+        assert cache.prepare([3, 2])[:, 0].tolist() == [15, 15]
+    for rank in ranks[::-1]:
+        forward(rank, 3, value=2.0)
+    assert cache.lengths() == [18, 17 if prepared else 18]
+    for rank in ranks:
+        for layer in (0, 1):
+            assert [k[15:] for k in keys(rank, layer)] == [[2.0] * (n - 15) for n in cache.lengths()]
+    used = [p for t in pages_of(cache) for p in t]
+    assert len(set(used)) == len(used) == 12 - len(cache._book.free)
+
+
+def test_a_prepared_and_a_held_step_are_taken_back(written, monkeypatch):
+    cache = paged.PagedCache(sequences=1, pages=4, page=16)
+    cache.abandon()  # there is nothing to take back
+    cache.prepare([40])
+    cache.abandon()
+    cache.release(0)  # (a step that no forward has made would be in its way)
+    forward(cache, 5)
+    captured(monkeypatch, cache, 1)
+    _, lengths, counts = cache._book.on(torch.device("cpu"))
+    cache.prepare([1], hold=True)
+    assert lengths.tolist() == [7]
+    cache.abandon()
+    assert cache.lengths() == [6] == lengths.tolist() and counts.tolist() == [0] and not cache.held
+    assert cache.prepare([1], hold=True).tolist() == [[6]] and lengths.tolist() == [7] and counts.tolist() == [1]
