@@ -482,7 +482,7 @@ int tpamd_rows_q8_ranks(int n, const tpamd_q8_rank *ranks, int64_t rows, int64_t
  *   x' = x * rsqrt(mean(x^2) + eps) * norm                                           where q_norm / k_norm ([D], in dtype) is not NULL,
  *   (a, b) -> (a c - b s, b c + a s)                                                  for the pairs of its first `part` elements: neighbours (2 i, 2 i + 1) where `interleaved`, else (i, i + part / 2),
  * c and s = scaling times cos and sin of position * inv_freq[i] (fp32 [part / 2]; the angle in 64 bits), or scaling times the tables cos / sin [rows, part / 2] (table_dtype; table_row
- * elements between rows, 0 where all rows share one). Everything in fp32, rounded once. part = 0: nothing is turned. positions: int64 [rows].
+ * elements between rows, 0 where all rows share one). Everything in fp32, rounded once. part = 0: nothing is turned. positions: int64 [rows], not beside tables.
  * Any even D up to 512, any alignment; fewer than 2^24 rows. Rows, sizes and strides of whole 16-byte pieces (part too: a multiple of 16 elements) are fastest, of 8-byte ones next; any others
  * are read by single elements. Outputs overlap no input. */
 typedef struct {

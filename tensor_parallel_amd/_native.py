@@ -1595,6 +1595,8 @@ def _heads(what: str, q, k, v, positions, inv_freq, cos, sin, scaling, interleav
             table_row = cos.stride(0)
         part, cos_at, sin_at = 2 * half, cos.data_ptr(), sin.data_ptr()
     if positions is not None:
+        if cos is not None:
+            raise ValueError(f"{what}: positions go with frequencies; tables of cos and sin have a row for each of the call's rows, or one for all")
         if positions.dtype not in (torch.int64, torch.int32) or positions.shape != axis or positions.get_device() != index:
             raise ValueError(f"{what}: positions must be int64 or int32 {tuple(axis)} on {q.device}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
         if positions.dtype != torch.int64 or not positions.is_contiguous():

@@ -61,7 +61,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor] =
     both, contiguous, as [..., H, D]. Any even D up to 512.
 
     Pairs (a, b) become (a c - b s, b c + a s), c and s `scaling` times cos and sin of position * inv_freq[i], angles in 64 bits: positions [...] (int64 or int32) and inv_freq [part / 2]; or
-    `scaling` times the tables cos and sin [..., part / 2] (16 or 32 bits, one value a pair). Of a head's first `part` elements the pairs are (i, i + part / 2), or with `interleaved`
+    `scaling` times the tables cos and sin [..., part / 2] (16 or 32 bits, one value a pair; a row of them for each row of the call, whose positions are in them, or one for all). Of a head's first `part` elements the pairs are (i, i + part / 2), or with `interleaved`
     neighbours (2 i, 2 i + 1); the others stay as they are. Frequencies and scaling are those that a model's rotary embedding has for long contexts, too.
 
     q_norm, k_norm [D]: each head is x * rsqrt(mean(x^2) + eps) * weight first, in the same pass. All of it in fp32, rounded once. Inference only: a backward pass raises."""

@@ -234,6 +234,7 @@ int heads_entry(const char *who, const tpamd_heads *h, const tpamd_pages *pages,
     TPAMD_REQUIRE(h->part == 0 || (h->inv_freq != nullptr) != (h->cos != nullptr && h->sin != nullptr), "%s: frequencies or tables are needed, and not both", who);
     TPAMD_REQUIRE(h->part == 0 || h->inv_freq == nullptr || h->positions != nullptr || pages != nullptr, "%s: positions are needed", who);
     TPAMD_REQUIRE(h->cos == nullptr || h->table_dtype == TPAMD_BF16 || h->table_dtype == TPAMD_F16 || h->table_dtype == TPAMD_F32, "%s: unknown dtype of tables", who);
+    TPAMD_REQUIRE(h->part == 0 || h->cos == nullptr || h->positions == nullptr, "%s: tables have a row for each of the call's rows: positions go with frequencies", who);
     HeadsParams p{};
     p.paged = pages != nullptr;
     if (pages != nullptr) {

@@ -39,7 +39,8 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
            cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, scaling: float = 1.0, interleaved: bool = False, q_norm: Optional[torch.Tensor] = None,
            k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """The new rows q [..., Hq, D] (or [..., Hkv, Hq / Hkv, D]), k and v [..., Hkv, D], views of projection outputs: k and v go to their positions' pages, k and q rotated as
-    `attention.rotate` does (frequencies or tables; neither: as they are). A row is rotated to its place in its sequence, or to `positions` [...]. Returns q as [..., Hq, D]; rows of no
+    `attention.rotate` does (frequencies or tables; neither: as they are). By frequencies a row is rotated to its place in its sequence, or to
+    `positions` [...]; tables have its position in them, and positions beside them are refused. Returns q as [..., Hq, D]; rows of no
     sequence are left as the memory was."""
     return _guard(_native.append_paged(q, k, v, k_pages, v_pages, table, lengths, starts, counts, positions, inv_freq, cos, sin, scaling, interleaved, q_norm, k_norm, eps), q, k, v,
                   q_norm, k_norm, inv_freq, cos, sin)

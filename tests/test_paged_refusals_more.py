@@ -1,0 +1,24 @@
+"""Further calls on heads and paged caches that are refused: nothing is launched, so no GPU is needed."""
+import ctypes
+
+import pytest
+import torch
+
+from tensor_parallel_amd import _native, attention, paged
+from test_paged_refusals import AT, HEADS, INVALID, PAGES, append, attend_c, checks, needs_library, packed, refused, rotate, z  # noqa: F401 (checks is a fixture)
+
+
+def test_positions_beside_tables(checks):
+    """Tables have a row for each of the call's rows: positions would be ignored."""
+    tables = {"inv_freq": None, "cos": torch.zeros(2, 32), "sin": torch.zeros(2, 32)}
+    with pytest.raises(ValueError, match="positions"):
+        rotate(**tables)
+    with pytest.raises(ValueError, match="positions"):
+        append(**tables, positions=torch.zeros(2, dtype=torch.int64))
+
+
+@needs_library
+def test_positions_beside_tables_at_the_entry_points():
+    heads = packed(_native._HEADS, HEADS, inv_freq=0, cos=AT, sin=AT)
+    refused(_native.lib().tpamd_rotate_heads(heads, 2, 4, 2, 64, 1, 0), INVALID, "positions")
+    refused(_native.lib().tpamd_append_paged(heads, packed(_native._PAGES, PAGES), 2, 4, 2, 64, 1, 0), INVALID, "positions")
