@@ -350,6 +350,8 @@ PAGED_HEAD_DIMS = (64, 96, 128, 256)
 
 def _check_paged(self, hidden_states, position_embeddings, attention_mask, head_dim: int, output_attentions) -> None:
     """A paged cache has no other way to go: what the fused forward does not take is refused."""
+    if not getattr(self, "is_causal", True):
+        raise NotImplementedError("PagedCache: attention on pages is causal, and this module's is not")
     if (position_embeddings is None or self.training or output_attentions or not isinstance(hidden_states, torch.Tensor) or hidden_states.dim() != 3
             or hidden_states.device.type != "cuda" or hidden_states.dtype not in (torch.bfloat16, torch.float16) or head_dim not in PAGED_HEAD_DIMS):
         raise NotImplementedError(f"PagedCache: attention on pages is inference on 16-bit hidden states on a HIP device with rotary embeddings and heads of {PAGED_HEAD_DIMS} elements, "
