@@ -502,7 +502,7 @@ typedef struct {
 /* q_out [rows, Hq, D], k_out [rows, Hkv, D] (v is ignored). */
 int tpamd_rotate_heads(const tpamd_heads *heads, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int dtype, void *stream);
 
-/* A cache whose positions lie in pages: k_pages, v_pages [pages, Hkv, page, D] by strides (elements; D contiguous), `page` a power of two from 16 on. Position j of sequence b is in slot
+/* A cache whose positions lie in pages: k_pages, v_pages [pages, Hkv, page, D] by strides (elements; D contiguous), `page` a power of two from 16 on, columns * page up to 2^31 - 2^16. Position j of sequence b is in slot
  * j % page of page table[b][j / page] (int32 [seqs, columns], table_row elements between rows). lengths (int32 [seqs]) count a sequence's positions WITH its new rows, which are the last ones.
  * The new rows of all sequences follow one another: those of b are rows starts[b] .. starts[b + 1] - 1 (int32 [seqs + 1], not decreasing), or, with starts NULL, the first counts[b] (int32; NULL: all) of the
  * rows / seqs rows from b * rows / seqs on. Rows of no sequence are neither read nor written.

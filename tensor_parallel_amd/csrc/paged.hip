@@ -1039,7 +1039,8 @@ int launch(const PagedParams &p, const Plan &plan, hipStream_t s) {
 int take_pages(const char *who, const tpamd_pages *g, int64_t rows, int64_t Hkv, int64_t D, PagesView *out) {
     TPAMD_REQUIRE(g->seqs >= 0 && g->seqs < (1ll << 24) && g->columns >= 0 && g->pages >= 0 && g->pages < (1ll << 31), "%s: bad dimension", who);
     TPAMD_REQUIRE(g->page >= GROUP && g->page < (1ll << 30) && (g->page & (g->page - 1)) == 0, "%s: a page has %lld positions: a power of two from %d on is needed", who, (long long)g->page, GROUP);
-    TPAMD_REQUIRE(g->columns * g->page < (1ll << 31), "%s: %lld pages of %lld positions a sequence are too many", who, (long long)g->columns, (long long)g->page);
+    // (positions are counted in 32 bits, and some behind a sequence's last: whole tiles, ranges of up to 512 x 64, the pages of the next 64 tiles of 128)
+    TPAMD_REQUIRE(g->columns <= ((1ll << 31) - (1 << 16)) / g->page, "%s: %lld pages of %lld positions a sequence are too many", who, (long long)g->columns, (long long)g->page);
     TPAMD_REQUIRE(g->starts == nullptr || g->counts == nullptr, "%s: starts (packed rows) or counts (padded rows), not both", who);
     TPAMD_REQUIRE(g->seqs == 0 || g->starts != nullptr || rows % g->seqs == 0, "%s: %lld rows are not the same number for each of %lld sequences", who, (long long)rows, (long long)g->seqs);
     for (int64_t s : {g->k_page, g->k_head, g->k_pos, g->v_page, g->v_head, g->v_pos, g->table_row}) TPAMD_REQUIRE(s >= 0, "%s: a negative stride", who);
