@@ -149,6 +149,10 @@ class _Book:
         for device in self.states:
             self.on(device)
 
+    def tell_captured(self) -> None:
+        if self.captured:  # (eager forwards ask by themselves)
+            self.tell()
+
 
 class PagedCache:
     """A key/value cache in pages for `sequences` sequences, which differ in length and come and go, as `past_key_values` of a model whose attention modules have the fused forward
@@ -241,7 +245,7 @@ class PagedCache:
     def release(self, sequence: int) -> None:
         """Sequence `sequence` has ended: its pages are free and its length is 0. A step that was held has ended too: a replay before the next `prepare` has no new rows."""
         self._book.release(sequence)
-        self._book.tell()
+        self._book.tell_captured()
 
     def lengths(self) -> List[int]:
         """The positions of each sequence, those of a step that a forward has begun among them."""
@@ -251,12 +255,12 @@ class PagedCache:
         """The last step is taken back, prepared, held or begun as it is: a forward that failed on its way (behind its first attention module the step counts as made) is made again after this, as if
         it had not been begun. Sequences keep the pages that were taken for it."""
         self._book.end()
-        self._book.tell()
+        self._book.tell_captured()
 
     def reset(self) -> None:
         """All sequences have ended, and a step that was held. The pools stay."""
         self._book.reset()
-        self._book.tell()
+        self._book.tell_captured()
 
     # ---- what transformers asks of a cache
     def get_seq_length(self, layer_idx: int = 0) -> int:

@@ -303,3 +303,19 @@ def test_a_prepared_and_a_held_step_are_taken_back(written, monkeypatch):
     cache.abandon()
     assert cache.lengths() == [6] == lengths.tolist() and counts.tolist() == [0] and not cache.held
     assert cache.prepare([1], hold=True).tolist() == [[6]] and lengths.tolist() == [7] and counts.tolist() == [1]
+
+
+def test_nothing_is_uploaded_at_the_end_of_a_sequence_where_nothing_was_captured(written, monkeypatch):
+    """A server's sequences end many at a time, and its next step brings the state up to date anyway."""
+    cache = paged.PagedCache(sequences=2, pages=8, page=16)
+    forward(cache, 5)
+    uploads = []
+    on = paged._Book.on
+    monkeypatch.setattr(paged._Book, "on", lambda book, device: uploads.append(device) or on(book, device))
+    cache.release(0)
+    cache.release(1)
+    cache.abandon()
+    cache.reset()
+    assert not uploads
+    forward(cache, 5, layers=1)
+    assert len(uploads) == 1 and on(cache._book, torch.device("cpu"))[1].tolist() == [5, 5]
