@@ -4,7 +4,7 @@
 //   x' = x * rsqrt(mean(x^2) + eps) * w                                   (where there is a weight)
 //   (a, b) -> (a cos t - b sin t, b cos t + a sin t), t = position * inv_freq, cos and sin times `scaling`,
 // for the pairs of the first `part` elements of a head: neighbours (2 i, 2 i + 1), or (i, i + part / 2); the others stay. Everything in fp32 and rounded once, at the
-// store. An angle is a product in 64 bits, reduced to one turn before it is 32 bits: at position 10^6 an angle in 32 bits is off by up to 0.06.
+// store. An angle is a product in 64 bits, reduced to one turn before it is 32 bits: at position 10^6 an angle in 32 bits is off by up to 0.03 (half of 2^-4).
 //
 // Bound: HBM (every byte once), or the launch: 4096 rows of 32 + 32 heads of 128, normed, 27 us (134 MB, 5.0 TB/s); 2103 rows of 64 + 4 heads of 64 10.8 (37 MB, 3.4 TB/s); one row 2.8. A block takes
 // all heads of one row (or, of few rows, as many as its lanes hold), so that the row's angles are computed once, into LDS. A lane holds 2 VEC elements of a head: the VEC pairs, in either layout,
@@ -238,7 +238,7 @@ int heads_entry(const char *who, const tpamd_heads *h, const tpamd_pages *pages,
     HeadsParams p{};
     p.paged = pages != nullptr;
     if (pages != nullptr) {
-        if (int rc = take_pages(who, pages, rows, Hkv, D, &p.pages); rc != TPAMD_OK) return rc;
+        if (int rc = take_pages(who, pages, rows, &p.pages); rc != TPAMD_OK) return rc;
         if (p.pages.seqs == 0) return TPAMD_OK;
     }
     TPAMD_REQUIRE(h->q && h->k && h->q_out && (pages != nullptr ? h->v != nullptr : h->k_out != nullptr), "%s: null pointer", who);

@@ -64,6 +64,6 @@ __device__ __forceinline__ int seq_of_row(const PagesView &p, int row, int &plac
 }
 
 // Host side (paged.hip): checks a tpamd_pages for `rows` rows and fills in the view.
-int take_pages(const char *who, const tpamd_pages *pages, int64_t rows, int64_t Hkv, int64_t D, PagesView *out);
+int take_pages(const char *who, const tpamd_pages *pages, int64_t rows, PagesView *out);
 
 }  // namespace tpamd

@@ -28,7 +28,7 @@ struct PagedParams {
     int64_t q_row, q_head, o_row, o_head;  // elements
     float *many_part, *few_part;
     float scale_log2;  // scale * log2(e)
-    int Hkv, G, D;
+    int Hkv, G;
     int few, many;     // which of the kernels run
     int spread;        // paged_many_kernel: blocks that its work is spread over; 0: a row tile is never cut
     int least;         // paged_few_kernel: the least share of a block; 0: a block takes one item, whole
@@ -215,8 +215,9 @@ __device__ __forceinline__ int share_of(const PagedParams &p, int cost, int bloc
 //
 // Inside a block each of the 4 wavefronts (8: plan_of) takes every fourth 16 positions through LDS stages of their own and meet at the end of an item.
 //
-// Bound by HBM where there is enough to read: 100000 positions of 8 key/value heads of 128 elements 76 us and their merge 5 (410 MB, 5.0 TB/s of the whole call); 64 sequences of 81 to
-// 7113 positions, 4 key/value heads of 64 elements: 27 and 6. Below that by the way to the first positions: 500 positions of 16 heads of 128 elements 8.9 us in a graph.
+// Bound by HBM where there is enough to read: 100000 positions of 8 key/value heads of 128 elements 66 us and their merge 5 (410 MB, 5.7 TB/s of the whole call); 64 sequences of 81 to
+// 7113 positions, 4 key/value heads of 64 elements: 27 and 6. Below that by the way to the first positions: 500 positions of 16 heads of 128 elements 8.0 us in a graph on three pools in turn,
+// 8.8 on so many that they come from HBM.
 template <int DT, int D, int WAVES, int NST>
 __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_index, const int blocks) {
     constexpr int PITCH = D * 2, LK = D / 32, LPS = 2 * LK, VAT = GROUP * PITCH, STAGE = 2 * VAT, RING = NST * STAGE;
@@ -396,7 +397,8 @@ __device__ __forceinline__ void few_rows(const PagedParams &p, const int share_i
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sc[j] = __builtin_amdgcn_exp2f(sc[j]);
                 l_run += (sc[0] + sc[1]) + (sc[2] + sc[3]);
-                // probabilities are rounded to the dtype (half a step of it each, as errors of either sign that the sum averages)
+                // probabilities are rounded to the dtype, as the matrix instruction takes them: half a step each, errors of either sign that the sum averages. Against 64 bits results of bf16 are off by
+                // 0.0021 of their size on average and of fp16 by 0.00026, where the rounding of the result alone is 0.0016 and 0.00021.
                 const u32x2 pf = {pack2_half<DT>(sc[0], sc[1]), pack2_half<DT>(sc[2], sc[3])};
                 u32x2 all[DT16];
                 uint32_t carried = 0;
@@ -735,7 +737,7 @@ __device__ __forceinline__ void many_rows(const PagedParams &p, const int block)
 #pragma unroll
             for (int j = 0; j < 16; ++j) sc[t][j] = __builtin_amdgcn_exp2f(sc[t][j]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < 2; ++u) {  // (rounded to the dtype, as there)
                 pf[2 * t + u] = u32x4{pack2_half<DT>(sc[t][8 * u], sc[t][8 * u + 1]), pack2_half<DT>(sc[t][8 * u + 2], sc[t][8 * u + 3]), pack2_half<DT>(sc[t][8 * u + 4], sc[t][8 * u + 5]),
                                       pack2_half<DT>(sc[t][8 * u + 6], sc[t][8 * u + 7])};
             }
@@ -940,8 +942,11 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
         // Where every whole item has a CU to itself its block has 8 wavefronts: 500 positions of 16 heads of 128 take 8.9 us, with 4 wavefronts 10.0; 700 9.7 and 12.0; of 4 heads of 64 6.8 and 7.8.
         // Not for up to 4 units (128 positions 6.3 and 5.8), nor for items on most CUs (192: 500 12.7 and 12.4), nor beside row tiles, whose blocks have 4.
         const bool wide = items <= cus / 2 && D <= 128 && !p.many;
-        // A whole item takes a time that grows with its units (a hundredth of a us each, at 4 wavefronts and 8), cut ones the second launch. Whole with 4, with 8 and cut, us: one sequence, 16 heads
-        // of 128: 500 10.0, 8.8, 11.6; 1000 15.3, 12.5, 12.0; 2000 25.4, 21.4, 13.1. 4 heads of 64: 1000 11.9, 8.8, 10.1; 2000 19.5, 12.4, 11.3.
+        // A whole item takes a time that grows with its units of 64 positions (in hundredths of a us each, 60 with 4 wavefronts and 48 with 8, up to 64 elements 43 and 28), cut ones the second launch:
+        // whole up to 7 us. Whole with 4, with 8 and cut, us: one sequence, 16 heads of 128: 500 10.2, 8.9, 11.7; 1000 15.6, 12.2, 12.0; 2000 25.9, 21.5, 13.3. 4 heads of 64: 1000 11.8, 8.5, 9.7;
+        // 2000 19.6, 12.5, 10.7. 16 of 96: 500 9.1, 8.0, 10.8; 1000 13.7, 10.2, 11.0; 2000 22.9, 17.1, 12.0. 16 of 256 (with 4, and cut): 500 15.2, 15.9; 700 18.9, 16.2; 1000 24.5, 16.4.
+        // Of many sequences the longest says it, since how they differ is not known here. 24 of 32 heads on 8 of 96, 128 and 256 elements between 100 and 3000 positions, whole and cut: 30.1 and 21.9,
+        // 33.7 and 25.0, 57.7 and 37.3; all of 1000: 16.9 and 21.0, 19.9 and 25.2, 35.6 and 39.9; 200 of 100 and 4 of 8000 108 and 49.
         const bool cut = max_length * (wide ? (D <= 64 ? 28 : 48) : (D <= 64 ? 43 : 60)) > 64 * 700;
         if (cut && items * (room / UNIT + 1 + START) < (1ll << 31)) {  // costs are counted in 32 bits
             p.few_blocks = per_cu * cus;
@@ -956,7 +961,8 @@ Plan plan_of(int64_t rows, int64_t seqs, int64_t Hq, int64_t Hkv, int64_t D, boo
     }
     if (p.many) {
         // Blocks of 8 wavefronts load keys and values half as often, blocks of 4, two to a CU, leave less of the device idle at the end of a batch and have shorter tiles. With 4 and 8, heads of
-        // 128: 4096 rows 164 and 154 us, 500 on 30000 203 and 151, 8 x 1024 (32 heads on 8) 120 and 131, 3 x 701 32 and 45; of 64: 4096 rows 103 and 114.
+        // 128: 4096 rows 164 and 154 us, 500 on 30000 203 and 151, 8 x 1024 (32 heads on 8) 120 and 131, 3 x 701 32 and 45; of 64: 4096 rows 103 and 114;
+        // of 96: 250 rows 12.9 and 16.3, 512 17.8 and 22.1, 3 x 701 23.6 and 37.1, 4096 136 and 124, 500 on 30000 189 and 120.
         // tiles of 256 rows and 64 positions for a CU; of sequences that may differ, half of what the bounds allow
         const double per_cu = static_cast<double>(rows) * Hq * (max_length - most / 2) / (256.0 * 64.0) / cus * (packed || counted ? 0.5 : 1.0);
         const bool enough = rows * G / 256 * Hkv >= cus;  // row tiles of 256, none of which need be cut
@@ -1036,7 +1042,7 @@ int launch(const PagedParams &p, const Plan &plan, hipStream_t s) {
 
 }  // namespace
 
-int take_pages(const char *who, const tpamd_pages *g, int64_t rows, int64_t Hkv, int64_t D, PagesView *out) {
+int take_pages(const char *who, const tpamd_pages *g, int64_t rows, PagesView *out) {
     TPAMD_REQUIRE(g->seqs >= 0 && g->seqs < (1ll << 24) && g->columns >= 0 && g->pages >= 0 && g->pages < (1ll << 31), "%s: bad dimension", who);
     TPAMD_REQUIRE(g->page >= GROUP && g->page < (1ll << 30) && (g->page & (g->page - 1)) == 0, "%s: a page has %lld positions: a power of two from %d on is needed", who, (long long)g->page, GROUP);
     // (positions are counted in 32 bits, and some behind a sequence's last: whole tiles, ranges of up to 512 x 64, the pages of the next 64 tiles of 128)
@@ -1085,7 +1091,7 @@ extern "C" int tpamd_attention_paged_workspace(const tpamd_pages *pages, int64_t
     TPAMD_REQUIRE(bytes_out != nullptr && max_new >= 0 && max_length >= 0, "%s: bad argument", who);
     *bytes_out = 0;
     PagesView view;
-    if (int rc = take_pages(who, pages, rows, Hkv, D, &view); rc != TPAMD_OK) return rc;
+    if (int rc = take_pages(who, pages, rows, &view); rc != TPAMD_OK) return rc;
     if (rows == 0 || view.seqs == 0) return TPAMD_OK;
     int dev = 0, cus = 256;
     TPAMD_HIP(hipGetDevice(&dev));
@@ -1101,7 +1107,7 @@ extern "C" int tpamd_attention_paged(const void *q_dev, int64_t q_row, int64_t q
     if (int rc = check_sizes(who, pages, rows, Hq, Hkv, D); rc != TPAMD_OK) return rc;
     TPAMD_REQUIRE(max_new >= 0 && max_length >= 0 && q_row >= 0 && q_head >= 0 && o_row >= 0 && o_head >= 0, "%s: bad argument", who);
     PagedParams p{};
-    if (int rc = take_pages(who, pages, rows, Hkv, D, &p.pages); rc != TPAMD_OK) return rc;
+    if (int rc = take_pages(who, pages, rows, &p.pages); rc != TPAMD_OK) return rc;
     if (rows == 0 || p.pages.seqs == 0) return TPAMD_OK;
     TPAMD_REQUIRE(q_dev != nullptr && out_dev != nullptr, "%s: null pointer", who);
     bool ok = aligned(q_dev, 16) && q_row % 8 == 0 && q_head % 8 == 0 && aligned(out_dev, 8) && o_row % 4 == 0 && o_head % 4 == 0 && aligned(p.pages.k, 16) && aligned(p.pages.v, 16);
@@ -1123,7 +1129,7 @@ extern "C" int tpamd_attention_paged(const void *q_dev, int64_t q_row, int64_t q
     p.many_part = static_cast<float *>(workspace_dev);
     p.few_part = p.many_part + plan.many_bytes / sizeof(float);
     p.scale_log2 = scale * 1.4426950408889634f;
-    p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv); p.D = static_cast<int>(D);
+    p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv);
     p.few = plan.few; p.many = plan.many;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool bf = dtype == TPAMD_BF16;
