@@ -18,6 +18,9 @@ read that count on the device, which `tp.attention.fuse_rotary_(model, assume_no
     step = tp.graphs.capture(model, input_ids=token, past_key_values=cache, use_cache=True)
     logits = step(input_ids=next_token, past_key_values=cache, use_cache=True).logits   # every further token: one replay
 
+A forward on a `paged.PagedCache` is captured under a step that is held, with a row of `position_ids` for each sequence among its arguments; anything else would replay the captured step's
+positions, or count each of the capture's own forwards as a step, and is refused.
+
 The forwards that a capture runs beforehand (to let first uses happen outside it) advance such a cache like any other
 forward: the counts of static caches among the arguments, and the tensors named in `restore`, are put back to what
 they were before `capture` returns; what those forwards wrote behind the count is overwritten by the steps that follow.

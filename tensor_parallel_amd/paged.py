@@ -49,8 +49,11 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
 def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, starts: Optional[torch.Tensor] = None,
            counts: Optional[torch.Tensor] = None, scale: Optional[float] = None, max_new: Optional[int] = None, max_length: Optional[int] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Causal attention of the new rows q [..., Hq, D] on their sequences' pages (which hold the new rows' keys and values already): [..., Hq, D], `out` if it is given. Hq a multiple of
-    Hkv, D 64, 96, 128 or 256, rows of q and of the pools on 16-byte boundaries (others are refused); scale D ** -0.5 by default. Rows of no sequence are left as the memory was, a row in front of position 0 (more new rows than positions) is zeros.
+    """Causal attention of the new rows q [..., Hq, D] on their sequences' pages (which hold the new rows' keys and values already): [..., Hq, D], `out` if it is given (which overlaps no
+    operand). Hq a multiple of Hkv, D 64, 96, 128 or 256, rows of q and of the pools on 16-byte boundaries (others are refused); scale D ** -0.5 by default. Rows of no
+    sequence are left as the memory was, a row in front of position 0 (more new rows than positions) is zeros, one whose scores all are -inf is NaN. What stands at positions that a row does not see does
+    not reach it; an infinite value that it sees gives it that infinity, or NaN where its probability is too small for the dtype. Probabilities are rounded to the dtype in front of the product with v,
+    sums are in 32 bits.
 
     max_new: no sequence has more new rows (rows of one that does may be left out); tell it where it is known, a step of single rows is then one or two launches. max_length: no sequence
     has more positions; only the time depends on it. Both have to hold for every replay where the call is captured."""
@@ -167,15 +170,20 @@ class PagedCache:
         cache.release(1)                                                  # sequence 1 has ended: its pages are free, row 1 may begin another
 
     A forward that nothing was prepared for has all of its rows new, in every sequence. Positions are the model's business: it counts from the longest sequence where it is given none, so
-    sequences of different lengths need `position_ids` (a forward without them is refused). Masks of padding are refused too: rows are padded on the right, and counted.
+    sequences of different lengths need `position_ids` (a forward without them is refused). Masks of padding are refused too (rows are padded on the right, and counted) where an attention module can
+    tell them: with `fuse_rotary_(model, assume_no_padding=True)`, which Falcon always needs, any mask is the causal one by the caller's word, and is ignored. Rotations are by the model's own tables of
+    cos and sin, in the model's dtype.
 
     `prepare(counts, hold=True)`: all forwards up to the next `prepare` are the same step, which counts as made. A forward captured under it (`tp.graphs.capture`, with
     `fuse_rotary_(model, assume_no_padding=True)`: transformers makes a mask, the causal one, where a forward is captured) reads table and lengths when it is replayed:
 
-        positions = cache.prepare([1] * 3, hold=True)
+        positions = cache.prepare([1] * 3, hold=True).to(device)
         step = tp.graphs.capture(model, input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True)
-        positions = cache.prepare([1] * 3, hold=True)                     # every further token, the first of them with the step's own
+        positions = cache.prepare([1] * 3, hold=True).to(device)          # every further token, the first of them with the step's own
         logits = step(input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True).logits
+
+    A capture needs a step that is held, and a row of position_ids for each sequence; any other is refused. `prepare`, and `release`, `reset` and `abandon` where a forward was captured, write the state
+    that captured forwards read on the current streams of their devices: replays on other streams are the caller's to order.
 
     `copy.deepcopy(cache)` is a cache of its own, with the same sequences in pages of its own; a shallow copy is refused.
 
